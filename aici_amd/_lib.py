@@ -77,6 +77,10 @@ _ERR_FUNCS = {
     "hipattn_mha_varlen_fwd": [TP, TP, TP, TP, TP, TP, c_int, c_int, c_float, c_float, c_bool, c_bool, c_int, c_int,
                                TP, TP, c_void_p],
     "hipattn_mha_varlen_fwd_paged": [TP, TP, TP, TP, TP, TP, c_int, c_int, c_float, c_bool, TP, TP, c_void_p],
+    "hipattn_mha_varlen_fwd_paged_window": [TP, TP, TP, TP, TP, TP, c_int, c_int, c_float, c_int, c_int, TP, TP, c_void_p],
+    "hipattn_paged_attention_window": [TP, TP, TP, TP, c_int, c_float, TP, TP, c_int, c_int, c_int, c_int, TP, TP, c_void_p],
+    "hipattn_paged_attention_window_workspace_size": [c_int64, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int32,
+                                                      POINTER(c_int64)],
     "hipattn_paged_attention_v1": [TP, TP, TP, TP, c_int, c_float, TP, TP, c_int, c_int, TP, c_void_p],
     "hipattn_paged_attention_v1_ws": [TP, TP, TP, TP, c_int, c_float, TP, TP, c_int, c_int, TP, c_void_p, c_int64,
                                       c_void_p],
@@ -107,6 +111,8 @@ _ERR_FUNCS = {
     "hipattn_gelu_fast": [TP, TP, c_void_p],
     "hipattn_bias_argmax": [TP, TP, TP, TP, TP, TP, c_void_p],
     "hipattn_bias_sample": [TP, TP, TP, TP, TP, TP, TP, TP, c_void_p],
+    "hipattn_penalize_logits": [TP, TP, TP, TP, TP, TP, TP, TP, TP, TP, TP, c_void_p],
+    "hipattn_step_blocks": [TP, TP, TP, TP, TP, c_int, c_int, c_int, c_int, TP, TP, TP, TP, TP, TP, TP, TP, TP, TP, c_void_p],
     "hipattn_reset_peak_memory_stats": [c_int],
     "hipattn_empty_cache": [],
     "hipattn_get_stats_allocated_bytes": [c_int, POINTER(MemStats)],
@@ -164,6 +170,8 @@ _ERR_FUNCS = {
                             TP, TP, TP, c_void_p],
     "hipattn_varlen_attn_paged": [TP, TP, TP, TP, TP, TP, TP, TP, TP, c_int64, c_int, c_int, TP, TP, c_int, c_int,
                                   c_float, TP, c_void_p],
+    "hipattn_varlen_attn_paged_window": [TP, TP, TP, TP, TP, TP, TP, TP, TP, c_int64, c_int, c_int, TP, TP, c_int, c_int,
+                                         c_float, c_int, c_int, TP, c_void_p],
 }
 
 # name -> (restype, argtypes) for the few calls that do not return an error string.

@@ -79,7 +79,8 @@ def _reads_through_tables(q: torch.Tensor, k: torch.Tensor, batch_info: BatchInf
 
 def varlen_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch_info: BatchInfo, key_cache: torch.Tensor,
                 value_cache: torch.Tensor, softmax_scale: Optional[float] = None,
-                paged_prefill: bool = False, cached: bool = False) -> torch.Tensor:
+                paged_prefill: bool = False, cached: bool = False, window_size_left: Optional[int] = None,
+                sink_tokens: int = 0) -> torch.Tensor:
     """mod.rs:318-354: q [T,Hq,d], k/v [T,Hkv,d] -> [T, Hq*d].  `cached`: the new K/V are in the cache
     already (kernels.rotary_embedding_and_cache) and the scatter is skipped.
 
@@ -87,12 +88,28 @@ def varlen_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch_info: B
     varlen prefill rows, paged decode rows) is one C-ABI call.  The multi-token
     rows read their context from the cache through block tables, or, where the
     caches are not what that takes, from a gathered copy; with `paged_prefill`
-    always through the tables (needs the builder's multi_block_tables)."""
+    always through the tables (needs the builder's multi_block_tables).
+
+    window_size_left: a token sees that many tokens before it, itself and the first sink_tokens of its sequence
+    (None: all of them); multi-token rows then always read through the tables."""
     T, Hq, d = q.shape
     Hkv = k.size(1)
     if softmax_scale is None:
         softmax_scale = 1.0 / math.sqrt(d)
     y = torch.empty((T, Hq, d), dtype=q.dtype, device=q.device)
+    if window_size_left is not None:
+        has_m, has_p = batch_info.q_multi > 0, batch_info.q_multi < T
+        if has_m and batch_info.multi_block_tables is None:
+            raise ValueError("a window needs batch_info.multi_block_tables (slots must follow the blocks in order)")
+        _native.varlen_attn_paged_window(q, k, v, key_cache, value_cache, None if cached else batch_info.slot_mapping,
+                                         batch_info.multi_block_tables if has_m else None, batch_info.seqlens_q if has_m else None,
+                                         batch_info.multi_context_lens if has_m else None, batch_info.q_multi, batch_info.max_seqlen_q,
+                                         batch_info.max_seqlen_k, batch_info.paged_block_tables if has_p else None,
+                                         batch_info.paged_context_lens if has_p else None, batch_info.paged_block_size,
+                                         batch_info.paged_max_context_len, softmax_scale, window_size_left, sink_tokens, y)
+        return y.reshape(T, Hq * d)
+    if sink_tokens != 0:
+        raise ValueError("sink_tokens needs a window")
     if paged_prefill or _reads_through_tables(q, k, batch_info, key_cache, value_cache):
         if batch_info.multi_block_tables is None:
             raise ValueError("paged_prefill needs batch_info.multi_block_tables (slots must follow the blocks in order)")

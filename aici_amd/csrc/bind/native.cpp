@@ -335,6 +335,10 @@ PyMethodDef g_methods[] = {
                          "zero_tensors,causal,window_left,window_right,out,lse"),
     BIND(mha_varlen_fwd_paged, "q,key_cache,value_cache,block_tables,cu_seqlens_q,context_lens,max_seqlen_q,max_seqlen_k,"
                                "softmax_scale,causal,out,lse"),
+    BIND(mha_varlen_fwd_paged_window, "q,key_cache,value_cache,block_tables,cu_seqlens_q,context_lens,max_seqlen_q,max_seqlen_k,"
+                                      "softmax_scale,window_size_left,sink_tokens,out,lse"),
+    BIND(paged_attention_window, "out,query,key_cache,value_cache,num_kv_heads,scale,block_tables,context_lens,block_size,"
+                                 "max_context_len,window_size_left,sink_tokens,alibi,workspace"),
     BIND(paged_attention_v1, "out,query,key_cache,value_cache,num_kv_heads,scale,block_tables,context_lens,block_size,"
                              "max_context_len,alibi"),
     BIND(paged_attention_v1_static, "out,query,key_cache,value_cache,num_kv_heads,scale,block_tables,context_lens,"
@@ -360,12 +364,18 @@ PyMethodDef g_methods[] = {
     BIND(gelu_fast, "out,input"),
     BIND(bias_argmax, "logits,bias,mask,bias_rows,out_tokens,out_logits"),
     BIND(bias_sample, "logits,bias,mask,bias_rows,temperature,top_p,uniforms,out_tokens"),
+    BIND(penalize_logits, "out,logits,history,history_offsets,prompt_lens,repetition,frequency,presence,bias,mask,bias_rows"),
+    BIND(step_blocks, "new_lens,state,block_tables,free_ring,ring_ends,block_size,rows_per_request,window_size_left,sink_tokens,"
+                      "state_out,ring_ends_out,served,context_lens,seqlens_q,logit_idxs,positions,slot_mapping,totals,workspace"),
     BIND(varlen_attn, "q,k,v,key_cache,value_cache,slot_mapping,gather_mapping,seqlens_q,seqlens_k,q_multi,max_seqlen_q,"
                       "max_seqlen_k,paged_block_tables,paged_context_lens,paged_block_size,paged_max_context_len,"
                       "softmax_scale,gather_k,gather_v,y"),
     BIND(varlen_attn_paged, "q,k,v,key_cache,value_cache,slot_mapping,multi_block_tables,seqlens_q,multi_context_lens,"
                             "q_multi,max_seqlen_q,max_seqlen_k,paged_block_tables,paged_context_lens,paged_block_size,"
                             "paged_max_context_len,softmax_scale,y"),
+    BIND(varlen_attn_paged_window, "q,k,v,key_cache,value_cache,slot_mapping,multi_block_tables,seqlens_q,multi_context_lens,"
+                                   "q_multi,max_seqlen_q,max_seqlen_k,paged_block_tables,paged_context_lens,paged_block_size,"
+                                   "paged_max_context_len,softmax_scale,window_size_left,sink_tokens,y"),
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_native", "Bindings of libhipattn.so's hot entry points.", -1, g_methods,

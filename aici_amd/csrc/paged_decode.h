@@ -41,6 +41,31 @@ struct DecodeParams {
   int *flat_prefix;  // [S + 1] block pairs before each sequence, written by workgroup 0
   int flat_waves;    // wavefronts of the main launch
   int flat_cols;   // query-head columns kept per partial slot: min(G, 16)
+  // WindowKeys only: the token at position ctx - 1 sees the window_left tokens before it and the first `sinks` ones.
+  int window_left, sinks;
+};
+
+// Which keys of its context a sequence's token sees: all of them, or a window and the sinks (window_decode.hip).
+struct AllKeys {
+  static constexpr bool window = false;
+};
+struct WindowKeys {
+  static constexpr bool window = true;
+};
+
+// The block pairs (32 tokens) of a context that hold a key the token sees, numbered one after the other: pairs [0, sink_pairs) of the
+// context and then those from pair sink_pairs + skip on.  Key t is seen iff t < ctx and (t >= first or t < sink_end).
+struct SeenKeys {
+  int first, sink_end, sink_pairs, skip;
+  __device__ __forceinline__ SeenKeys(const DecodeParams &p, int ctx) {
+    first = max(ctx - 1 - p.window_left, 0);
+    sink_end = min(p.sinks, first);
+    sink_pairs = (sink_end + 2 * 16 - 1) / (2 * 16);
+    skip = max(first / (2 * 16) - sink_pairs, 0);
+  }
+  // The context's column (tables of BS-token blocks) and run of 16 tokens behind a number among those that are seen.
+  __device__ __forceinline__ int column(int c, int bs) const { return c < sink_pairs * (32 / bs) ? c : c + skip * (32 / bs); }
+  __device__ __forceinline__ int run(int r) const { return r < 2 * sink_pairs ? r : r + 2 * skip; }
 };
 
 // What hipattn_paged_attention_v1 checks of its arguments and makes of them; false: nothing to do.
@@ -64,6 +89,19 @@ struct FlatScratch {
 };
 FlatScratch flat_scratch(int64_t S, int G, int head_size, int workgroups);
 void flat_scratch_set(DecodeParams &p, const FlatScratch &f, int workgroups, int head_size, char *ws);
+// How a call is carried out and what scratch memory it needs: computed from the shapes alone, so that
+// hipattn_paged_attention_workspace_size and the launch agree.
+struct DecodePlan {
+  bool generic = false, flat = false;
+  int part_blocks = 0;  // partitioned launch: KV blocks per partition
+  int num_parts = 1;    // partitioned / generic launch
+  int waves = 4;        // partitioned launch: wavefronts per partition
+  int flat_wgs = 0;
+  FlatScratch flat_scratch = {};
+  size_t slots = 0;          // partitioned / generic launch: partial results (each head_size + 2 floats)
+  size_t bytes = 0;          // scratch memory in all
+};
+DecodePlan plan_decode(int64_t S, int Hq, int Hkv, int head_size, int block_size, int dtype, int max_context_len);
 // Block pairs of all sequences and kv heads at most, and whether the flat split can count them.
 int64_t flat_units(int64_t S, int heads, int max_context_len);
 bool flat_split_counts(int64_t S, int heads, int max_context_len);
@@ -203,9 +241,11 @@ __device__ __forceinline__ void pair_load_bs(const DecodeParams &p, const T *kba
 // Folds a loaded block pair -- blocks `blk` and `blk + 1` of the context, the
 // second absent when !has_b -- into the running softmax state (m_run, l_run,
 // acc).  qreg: lane (kg, col) holds q[head col][32*step + 8*kg .. +8].
-template <typename T, int HD>
+// KEYS::window: keys from sink_end on and below `first` are not seen; what the cache holds there (a block that has been given to
+// another sequence, anything) has no say in the result.
+template <typename T, int HD, typename KEYS = AllKeys>
 __device__ __forceinline__ void pair_compute(const DecodeParams &p, PairRegs<HD> &r, int blk, bool has_b, int ctx,
-                                             float slope, const typename Vec8<T>::type (&qreg)[(HD + 31) / 32],
+                                             int first, int sink_end, float slope, const typename Vec8<T>::type (&qreg)[(HD + 31) / 32],
                                              float &m_run, float &l_run, f32x4_t (&acc)[HD / 16]) {
   typedef typename Vec8<T>::type vec8;
   constexpr int NSTEP = (HD + 31) / 32;
@@ -235,6 +275,10 @@ __device__ __forceinline__ void pair_compute(const DecodeParams &p, PairRegs<HD>
     x[4 + i] = sb[i] * p.scale_log2 + slope * (float)(tok_b + i - ctx + 1);
     if (tok_a + i >= ctx) x[i] = -INFINITY;
     if (tok_b + i >= ctx) x[4 + i] = -INFINITY;
+    if constexpr (KEYS::window) {
+      if (tok_a + i >= sink_end && tok_a + i < first) x[i] = -INFINITY;
+      if (tok_b + i >= sink_end && tok_b + i < first) x[4 + i] = -INFINITY;
+    }
   }
   float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
   mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
@@ -268,6 +312,21 @@ __device__ __forceinline__ void pair_compute(const DecodeParams &p, PairRegs<HD>
       for (int i = 0; i < 4; i++) {
         if (tok_a + i >= ctx) ea[i] = 0;
         if (tok_b + i >= ctx) eb[i] = 0;
+      }
+    }
+  }
+
+  if constexpr (KEYS::window) {
+    if (blk * kBlockSize < first && (blk + 2) * kBlockSize > sink_end) {  // wave-uniform: the last pair of the sinks, the first of the window
+#pragma unroll
+      for (int dt = 0; dt < NDT; dt++) {
+        uint16_t *ea = reinterpret_cast<uint16_t *>(&vra[dt]);
+        uint16_t *eb = reinterpret_cast<uint16_t *>(&vrb[dt]);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          if (tok_a + i >= sink_end && tok_a + i < first) ea[i] = 0;
+          if (tok_b + i >= sink_end && tok_b + i < first) eb[i] = 0;
+        }
       }
     }
   }
@@ -326,7 +385,7 @@ struct FlatLds {
   float park_ml[4][2][64];
 };
 
-template <typename T, int HD, int BS>
+template <typename T, int HD, int BS, typename KEYS = AllKeys>
 __device__ __forceinline__ void decode_flat(const DecodeParams &p, const int wg, FlatLds<HD> &lds) {
   typedef typename Vec8<T>::type vec8;
   constexpr int NCH = HD / 8;
@@ -353,6 +412,7 @@ __device__ __forceinline__ void decode_flat(const DecodeParams &p, const int wg,
       const int s = 4 * tid + j;
       c[j] = s < S ? min(p.context_lens[s], p.max_ctx) : 0;
       n[j] = ctx_pairs(c[j]);
+      if constexpr (KEYS::window) n[j] -= SeenKeys(p, c[j]).skip;
       tsum += n[j];
     }
     int inc = tsum;
@@ -411,7 +471,8 @@ __device__ __forceinline__ void decode_flat(const DecodeParams &p, const int wg,
       continue;
     }
     const int ctx = uniform(s_ctx[seq]);
-    const int nblk = (ctx + kBlockSize - 1) / kBlockSize;
+    const SeenKeys seen(p, KEYS::window ? ctx : 0);
+    const int nblk = (ctx + kBlockSize - 1) / kBlockSize - (KEYS::window ? 2 * seen.skip : 0);
     const int r = u - hk * before;
     const int h = r / pairs;
     const int pr0 = r - h * pairs;
@@ -447,11 +508,12 @@ __device__ __forceinline__ void decode_flat(const DecodeParams &p, const int wg,
       const int nsub = min(32, n - sp);
       const int b_first = 2 * (pr0 + sp);             // in runs of 16 tokens
       const int t_first = b_first * kBlockSize / BS;  // the table column of the first of them
+      auto column = [&](int c) { return KEYS::window ? seen.column(c, BS) : c; };
       int tbl = 0;
-      if (lane < 64 * kBlockSize / BS && t_first + lane < p.table_cols)
-        tbl = p.block_tables[seq * p.max_blocks + t_first + lane];
+      if (lane < 64 * kBlockSize / BS && column(t_first + lane) < p.table_cols)
+        tbl = p.block_tables[seq * p.max_blocks + column(t_first + lane)];
       int tbl_hi = 0;  // 8-token blocks: 32 pairs span 128 columns
-      if (BS == 8 && t_first + 64 + lane < p.table_cols) tbl_hi = p.block_tables[seq * p.max_blocks + t_first + 64 + lane];
+      if (BS == 8 && column(t_first + 64 + lane) < p.table_cols) tbl_hi = p.block_tables[seq * p.max_blocks + column(t_first + 64 + lane)];
       // Two register sets (heads up to 128 elements): the next pair's loads are
       // in flight while the current pair is folded in.
       auto issue = [&](int it, PairRegs<HD> &r) {
@@ -471,7 +533,8 @@ __device__ __forceinline__ void decode_flat(const DecodeParams &p, const int wg,
       };
       auto fold = [&](int it, PairRegs<HD> &r) {
         const int blk = b_first + 2 * it;
-        pair_compute<T, HD>(p, r, blk, blk + 1 < nblk, ctx, slope, qreg, m_run, l_run, acc);
+        pair_compute<T, HD, KEYS>(p, r, KEYS::window ? seen.run(blk) : blk, blk + 1 < nblk, ctx, seen.first, seen.sink_end, slope, qreg, m_run,
+                                  l_run, acc);
       };
       // The pairs of a batch are visited in bit-reversed order (of 32: 0, 16, 8, 24, 4, ...), not in the order of
       // the table; in a batch of fewer than 32 the largest power of two of them is, the rest follow in table order.

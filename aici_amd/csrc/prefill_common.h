@@ -27,7 +27,7 @@ struct PrefillParams {
   int causal;  // win_left < 0 && win_right == 0
   // Query row i (0-based in its sequence) sees key j iff i + off - win_left <= j <= i + off + win_right,
   // off = Lk - Lq; a negative bound is no bound (flash_attn/softmax.h:142-179, flash_api.cpp:113-120).
-  // Only prefill_varlen_kernel reads these; the eight-wavefront kernel takes causal or unmasked launches.
+  // Only prefill_varlen_kernel and the windowed forms of the eight-wavefront kernel read these; it takes causal or unmasked launches else.
   int win_left, win_right;
   // K/V read straight from the paged cache (prefill_varlen_w8_kernel<..., W8_PAGED or W8_PAGED_DMA>): k and v are
   // the caches, position p of sequence b lives in block block_tables[b][p / 16] at offset p % 16.
@@ -46,6 +46,7 @@ struct PrefillParams {
   // A workgroup of W wavefronts covers 2^wg_heads_log2 query heads of one kv group and 32 W >> wg_heads_log2
   // query rows of each (wavefront w: head w % heads, row group w / heads).
   int wg_heads_log2;
+  int sinks;  // windows with sinks: the first keys of a sequence that stay visible (kernels with STEP::window or SINKS)
 };
 
 template <typename T>
@@ -111,10 +112,14 @@ struct PagedPrefillCall {
   int max_q, max_k;
   float scale;
   bool causal;
+  const char *op = "mha_varlen_fwd_paged";
 };
 bool paged_prefill_params(const PagedPrefillCall &c, hipattn_tensor *out, hipattn_tensor *lse, PrefillParams &p);
 // Whether the blocks of the caches can go into LDS as they are (16-token blocks, 16-byte aligned images, and no switch against it).
 bool paged_prefill_copies_images(const PrefillParams &p);
+
+// The four-wavefront kernel with p.win_left and p.sinks (prefill_varlen.hip): any block size and head size.
+void launch_staged_window(const PrefillParams &p, int dtype, hipStream_t stream);
 
 // Launches the kernel that rotates three groups of wavefronts through the matrix pipe (prefill_r3.hip) when it
 // covers the shapes in p; returns false, having done nothing, when it does not.

@@ -67,8 +67,11 @@ typedef __attribute__((address_space(3))) s16x4_t lds_s16x4;
 // PAGED: K and V are the paged caches, read through the block table (p.block_tables, p.context_lens); tiles
 // are staged in the caches' own order -- 16-byte runs of K go to the rows they belong to, 16-byte runs of V (8
 // tokens of one head element) to rows of a V^T tile, whose operands plain 8-byte LDS reads deliver.
-template <typename T, int HDP, int QT, bool PAGED = false>
+// SINKS (paged, causal, win_left >= 0): the first p.sinks keys of a sequence are seen beside the window; tiles are numbered without the
+// gap between them, as in prefill_varlen_w8_kernel.
+template <typename T, int HDP, int QT, bool PAGED = false, bool SINKS = false>
 __global__ __launch_bounds__(256) void prefill_varlen_kernel(PrefillParams p) {
+  static_assert(PAGED || !SINKS, "sinks: the paged form alone");
   typedef typename Vec8<T>::type vec8;
   typedef Tile<HDP> TL;
   constexpr int KSTEPS = HDP / 16;  // contraction steps of S^T = K.Q^T
@@ -103,14 +106,26 @@ __global__ __launch_bounds__(256) void prefill_varlen_kernel(PrefillParams p) {
   if (!PAGED && p.seqused_k) Lk = min(Lk, p.seqused_k[b]);
   const int wg_row0 = qb * BM;
   if (wg_row0 >= Lq) return;
-  const int off = Lk - Lq;  // bottom-right alignment of the mask
+  int off = Lk - Lq;  // bottom-right alignment of the mask
   const int wg_last_row = min(wg_row0 + BM, Lq) - 1;
   const bool bound_hi = p.win_right >= 0, bound_lo = p.win_left >= 0;
   int kmax = bound_hi ? min((int64_t)Lk, (int64_t)wg_last_row + off + p.win_right + 1) : Lk;
   if (kmax < 0) kmax = 0;
-  const int n_tiles = (kmax + BN - 1) / BN;
+  int n_tiles = (kmax + BN - 1) / BN;
+  // SINKS: tile t is the context's tile t, from gap_tile on tile t + skip; Lk, off and keys are counted that way, and keys from p.sinks to
+  // seen_from are seen by no row of the workgroup.
+  int gap_tile = 0, skip = 0, seen_from = 0;
+  if constexpr (SINKS) {
+    seen_from = max(wg_row0 + off - p.win_left, 0);
+    gap_tile = (min(p.sinks, seen_from) + BN - 1) / BN;
+    skip = max(seen_from / BN - gap_tile, 0);
+    n_tiles -= skip;
+    Lk -= skip * BN;
+    off -= skip * BN;
+    seen_from -= skip * BN;
+  }
   // first tile that any row of the workgroup can see
-  const int first_tile = bound_lo ? (int)max((int64_t)0, ((int64_t)wg_row0 + off - p.win_left)) / BN : 0;
+  const int first_tile = SINKS ? 0 : bound_lo ? (int)max((int64_t)0, ((int64_t)wg_row0 + off - p.win_left)) / BN : 0;
 
   const int wave_row0 = wg_row0 + wave * (QT * 32);
   const int wave_last_row = wave_row0 + QT * 32 - 1;
@@ -159,14 +174,15 @@ __global__ __launch_bounds__(256) void prefill_varlen_kernel(PrefillParams p) {
       // (block r, chunk, token), V unit (block r, head element, half of the block's tokens).  Blocks past the
       // context re-read its last one (their keys are masked, their V runs cleared before they reach LDS).
       staged_k0 = k0;
+      const int past = SINKS && tile >= gap_tile ? skip * BN : 0;  // keys of the gap in front of this tile
       if (p.block_log2 != 4) {
         // Caches of 8- or 32-token blocks: the same units -- a 16-byte run of K is (chunk, token) and one of V
         // (head element, 8 tokens) at any block size -- each finding its own block: the id comes from the
         // table row per unit, and the block's pitch takes the place of the 16.
         const int bl = p.block_log2, bs = 1 << bl;
-        const int last_col = max(min((Lk - 1) >> bl, p.table_cols - 1), 0);
+        const int last_col = max(min((Lk - 1 + past) >> bl, p.table_cols - 1), 0);
         auto block_of = [&](int pos) -> int64_t {
-          const int id = table_row[min(pos >> bl, last_col)];
+          const int id = table_row[min((pos + past) >> bl, last_col)];
           return id < 0 ? 0 : (id >= p.num_blocks ? p.num_blocks - 1 : (int64_t)id);
         };
         constexpr int K_PER_16 = CPR * 16, V_PER_16 = HDP * 2;
@@ -186,11 +202,11 @@ __global__ __launch_bounds__(256) void prefill_varlen_kernel(PrefillParams p) {
         }
         return;
       }
-      const int last_col = max(min((Lk - 1) >> 4, p.table_cols - 1), 0);
+      const int last_col = max(min((Lk - 1 + past) >> 4, p.table_cols - 1), 0);
       int64_t blk[4];
 #pragma unroll
       for (int r = 0; r < 4; r++) {
-        const int id = table_row[min((k0 >> 4) + r, last_col)];
+        const int id = table_row[min(((k0 + past) >> 4) + r, last_col)];
         blk[r] = id < 0 ? 0 : (id >= p.num_blocks ? p.num_blocks - 1 : (int64_t)id);
       }
       constexpr int K_PER_BLOCK = CPR * 16, V_PER_BLOCK = HDP * 2;
@@ -250,6 +266,13 @@ __global__ __launch_bounds__(256) void prefill_varlen_kernel(PrefillParams p) {
               o[w] &= a2 <= 0 ? 0u : (a2 == 1 ? 0xffffu : 0xffffffffu);
             }
           }
+          if (SINKS && staged_k0 < seen_from && staged_k0 + BN > p.sinks) {  // ... and those between the sinks and the window
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+              const int t = staged_k0 + r * 16 + half * 8 + 2 * w;
+              o[w] &= (t >= p.sinks && t < seen_from ? 0u : 0xffffu) | (t + 1 >= p.sinks && t + 1 < seen_from ? 0u : 0xffff0000u);
+            }
+          }
           *reinterpret_cast<u32x4_t *>(vs + drow * TL::VTSTR + r * 16 + half * 8) = o;
         }
       }
@@ -284,9 +307,9 @@ __global__ __launch_bounds__(256) void prefill_varlen_kernel(PrefillParams p) {
     const int k0 = j * BN;
     // Wave-level view of this tile: skip it if it lies entirely outside the
     // window of every row this wave owns.
-    const bool skip = (wave_row0 >= Lq) || (bound_hi && k0 > (int64_t)wave_last_row + off + p.win_right) ||
-                      (bound_lo && k0 + BN - 1 < (int64_t)wave_row0 + off - p.win_left);
-    if (!skip) {
+    const bool unseen = (wave_row0 >= Lq) || (bound_hi && k0 > (int64_t)wave_last_row + off + p.win_right) ||
+                      (bound_lo && k0 + BN - 1 < (int64_t)wave_row0 + off - p.win_left && (!SINKS || k0 >= p.sinks));
+    if (!unseen) {
       const T *ks_base = smem + cur * TL::STAGE_ELEMS;
       const T *vs_base = ks_base + TL::K_ELEMS;
       const bool need_mask = (k0 + BN > Lk) || (bound_hi && k0 + BN - 1 > (int64_t)wave_row0 + off + p.win_right) ||
@@ -316,7 +339,7 @@ __global__ __launch_bounds__(256) void prefill_varlen_kernel(PrefillParams p) {
 #pragma unroll
             for (int i = 0; i < 16; i++) {
               const int key = k0 + hf * 32 + (i >> 2) * 8 + g * 4 + (i & 3);
-              if (key > limit || key < first) s[qt][i] = -INFINITY;
+              if (key > limit || (key < first && (!SINKS || key >= p.sinks))) s[qt][i] = -INFINITY;
             }
           }
           float mx = s[qt][0];
@@ -502,11 +525,11 @@ void launch_prefill_w8(const PrefillParams &p, hipStream_t stream) {
   }
 }
 
-template <typename T, int HDP, int QT, bool PAGED = false>
+template <typename T, int HDP, int QT, bool PAGED = false, bool SINKS = false>
 void launch_prefill(PrefillParams p, hipStream_t stream) {
   constexpr int BM = 4 * QT * 32;
   static bool attr_set = false;  // benign race: setting twice is harmless
-  auto kernel = prefill_varlen_kernel<T, HDP, QT, PAGED>;
+  auto kernel = prefill_varlen_kernel<T, HDP, QT, PAGED, SINKS>;
   if (!attr_set) {
     HA_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
                                (int)Tile<HDP>::LDS_BYTES));
@@ -689,6 +712,21 @@ void mha_varlen_fwd_impl(const hipattn_tensor *q, const hipattn_tensor *k, const
   else dispatch_hd<bf16_t>(p, total_q, stream);
 }
 
+template <typename T>
+void dispatch_staged_window(const PrefillParams &p, hipStream_t stream) {
+  switch ((p.d + 31) / 32 * 32) {
+    case 32: launch_prefill<T, 32, 1, true, true>(p, stream); break;
+    case 64: launch_prefill<T, 64, 1, true, true>(p, stream); break;
+    case 96: launch_prefill<T, 96, 1, true, true>(p, stream); break;
+    case 128: launch_prefill<T, 128, 1, true, true>(p, stream); break;
+    case 160: launch_prefill<T, 160, 1, true, true>(p, stream); break;
+    case 192: launch_prefill<T, 192, 1, true, true>(p, stream); break;
+    case 224: launch_prefill<T, 224, 1, true, true>(p, stream); break;
+    case 256: launch_prefill<T, 256, 1, true, true>(p, stream); break;
+    default: fail("mha_varlen_fwd_paged_window: head size %d not supported (at most 256)", p.d);
+  }
+}
+
 // Varlen prefill whose keys and values are read from the paged cache through block tables: what
 // rLLM composes from gather_cached_kv -> repeat_kv -> flash_attn_varlen (llm/mod.rs:181-238) without
 // the two copies.  Eight-wavefront kernel for head sizes up to 128, four-wavefront kernel above.
@@ -737,7 +775,7 @@ void dispatch_paged(const PrefillParams &p, hipStream_t stream) {
 }  // namespace
 
 bool paged_prefill_params(const PagedPrefillCall &c, hipattn_tensor *out, hipattn_tensor *lse, PrefillParams &p) {
-  const char *op = "mha_varlen_fwd_paged";
+  const char *op = c.op;
   const hipattn_tensor *q = c.q, *key_cache = c.key_cache, *value_cache = c.value_cache, *block_tables = c.block_tables, *cu_q = c.cu_q,
                        *context_lens = c.context_lens;
   const int max_q = c.max_q, max_k = c.max_k;
@@ -839,6 +877,11 @@ bool paged_prefill_params(const PagedPrefillCall &c, hipattn_tensor *out, hipatt
   p.vc_head = value_cache->strides[1];
   p.block_log2 = bs == 8 ? 3 : (bs == 16 ? 4 : 5);
   return true;
+}
+
+void launch_staged_window(const PrefillParams &p, int dtype, hipStream_t stream) {
+  if (dtype == HIPATTN_F16) dispatch_staged_window<half_t>(p, stream);
+  else dispatch_staged_window<bf16_t>(p, stream);
 }
 
 bool paged_prefill_copies_images(const PrefillParams &p) {

@@ -39,9 +39,12 @@ enum { W8_ROWS = 0, W8_PAGED = 1, W8_PAGED_DMA = 2, W8_PAGED_DMA_PART = 3 };
 // STEP: what else a launch holds.  Nothing, or (step_attn.hip) workgroups of paged decode in front or behind, and a row block's keys dealt out to up
 // to n_parts workgroups: piece i takes tiles [i part_tiles, (i + 1) part_tiles), the last one the rest, and where a row block has more
 // than one they leave sums, maximum and accumulators for the launch behind to merge.
+// Or (prefill_window.hip) its rows see a window of keys and the sinks, and their keys may be dealt out the same way.
 struct PrefillAlone {
   typedef PrefillParams Params;
-  static constexpr bool value = false;
+  static constexpr bool value = false;   // decode rows beside it
+  static constexpr bool parts = false;   // keys dealt out
+  static constexpr bool window = false;  // a window and sinks
 };
 
 // Wavefronts per SIMD and places for tiles in LDS of the forms with eight and four wavefronts.
@@ -123,7 +126,7 @@ __global__ __launch_bounds__(NW * 64, STEP::value ? 2 : w8_wavefronts(HDP, NW)) 
   const int n_slots = p.Hq >> hl;
   const int slot = id % n_slots;
   id /= n_slots;
-  if constexpr (STEP::value) {
+  if constexpr (STEP::parts) {
     part = id % p.n_parts;
     id /= p.n_parts;
   }
@@ -146,8 +149,23 @@ __global__ __launch_bounds__(NW * 64, STEP::value ? 2 : w8_wavefronts(HDP, NW)) 
   if (kmax < 0) kmax = 0;
   int n_tiles = (kmax + BN - 1) / BN;
   int first_tile = 0;
+  // Window: the tiles that hold a key some row sees are numbered without the gap -- tile t is the context's tile t, from gap_tile on tile
+  // t + skip -- and Lk, off and the keys of the masks are counted that way: key j is seen by row r iff j <= r + off and
+  // (j >= r + off - win_left or j < sinks), for tiles on either side of the gap (in front of it nothing but the sinks is within
+  // reach of either rule, behind it no sink is).  Keys from `sinks` to seen_from are seen by no row of the workgroup.
+  int gap_tile = 0, skip = 0, sinks = 0, seen_from = 0;
+  if constexpr (STEP::window) {
+    sinks = p.sinks;
+    seen_from = max(wg_row0 + off - p.win_left, 0);
+    gap_tile = (min(sinks, seen_from) + BN - 1) / BN;
+    skip = max(seen_from / BN - gap_tile, 0);
+    n_tiles -= skip;
+    Lk -= skip * BN;
+    off -= skip * BN;
+    seen_from -= skip * BN;
+  }
   bool whole = true;  // this workgroup sees all keys of its rows
-  if constexpr (STEP::value) {
+  if constexpr (STEP::parts) {
     whole = p.n_parts == 1 || n_tiles <= p.part_tiles;
     first_tile = part * p.part_tiles;
     if (part > 0 && first_tile >= n_tiles) return;
@@ -155,6 +173,10 @@ __global__ __launch_bounds__(NW * 64, STEP::value ? 2 : w8_wavefronts(HDP, NW)) 
     if (part < p.n_parts - 1) n_tiles = min(n_tiles, p.part_tiles);  // (the last piece: whatever lies beyond the caller's bound, too)
     Lk -= first_tile * BN;  // keys are counted from the piece's first one on
     off -= first_tile * BN;
+    if constexpr (STEP::window) {
+      sinks -= first_tile * BN;
+      seen_from -= first_tile * BN;
+    }
   }
   // Wavefronts w and w + 4 share a SIMD.  Under the causal mask a wavefront's work grows with its rows'
   // position in the block, so with one head per workgroup the two of a SIMD take row groups (w, 7 - w):
@@ -269,13 +291,17 @@ __global__ __launch_bounds__(NW * 64, STEP::value ? 2 : w8_wavefronts(HDP, NW)) 
   u32x4_t vstp[PAGED ? NLOADVP : 1];
   int staged_k0 = 0;  // first key of the tile held in the staging registers
   const int32_t *table_row = PAGED ? p.block_tables + (int64_t)b * p.table_stride : nullptr;
-  if constexpr (STEP::value) table_row += first_tile * (BN / 16);
+  if constexpr (STEP::parts && !STEP::window) table_row += first_tile * (BN / 16);
   // The block ids of 64 table columns (16 tiles) sit one per lane (columns past the context repeat its
   // last one), and a tile's four ids are lane reads into scalar registers: no tile waits for a table
   // read.  The next group is asked for one tile before it is needed and the ids are clamped to the cache
   // where they are used, so that nothing waits for the read where it is issued.
   int tbl_cur = 0, tbl_nxt = 0;
   auto load_ids = [&](int group) -> int {
+    if constexpr (STEP::window) {
+      const int col = first_tile * (BN / 16) + min(group * 64 + lane, (Lk - 1) >> 4);
+      return table_row[max(min(col >= gap_tile * (BN / 16) ? col + skip * (BN / 16) : col, p.table_cols - 1), 0)];
+    }
     const int last_col = min((Lk - 1) >> 4, p.table_cols - first_tile * (BN / 16) - 1);
     return table_row[max(min(group * 64 + lane, last_col), 0)];
   };
@@ -436,6 +462,24 @@ __global__ __launch_bounds__(NW * 64, STEP::value ? 2 : w8_wavefronts(HDP, NW)) 
           for (int w = 0; w < 4; w++) {
             const int a2 = alive - 2 * w;
             o[w] &= a2 <= 0 ? 0u : (a2 == 1 ? 0xffffu : 0xffffffffu);
+          }
+          *run = o;
+        }
+      }
+    }
+    if constexpr (STEP::window) {
+      // ... and the tokens between the sinks and what the first row sees, in whose blocks anything may lie by now.
+      if (dma_v(IMG - 1) && tile * BN < seen_from && tile * BN + BN > sinks) {
+        T *vs = smem + (tile % NST) * STAGE_ELEMS + K_ELEMS + dma_r * BLK_ELEMS;
+        const int tok = tile * BN + dma_r * 16 + g * 8;  // the first of this lane's runs
+#pragma unroll
+        for (int i = 0; i < NDMA; i++) {
+          u32x4_t *run = reinterpret_cast<u32x4_t *>(vs + i * 512 + lane * 8);
+          u32x4_t o = *run;
+#pragma unroll
+          for (int w = 0; w < 4; w++) {
+            const int t = tok + 2 * w;
+            o[w] &= (t >= sinks && t < seen_from ? 0u : 0xffffu) | (t + 1 >= sinks && t + 1 < seen_from ? 0u : 0xffff0000u);
           }
           *run = o;
         }
@@ -698,7 +742,12 @@ __global__ __launch_bounds__(NW * 64, STEP::value ? 2 : w8_wavefronts(HDP, NW)) 
     }
   };
   // Tiles entirely past the diagonal of every row of this wavefront are skipped.
-  auto skip_tile = [&](int j) { return (wave_row0 >= Lq) || (p.causal && j * BN > wave_last_row + off); };
+  // (and those in front of the window of every row, sinks aside)
+  auto skip_tile = [&](int j) {
+    if constexpr (STEP::window)
+      if (j * BN + BN - 1 < wave_row0 + off - p.win_left && j * BN >= sinks) return true;
+    return (wave_row0 >= Lq) || (p.causal && j * BN > wave_last_row + off);
+  };
 
   // ---- the pipelined tile loop (staged tiles; block images run the alternating blocks further down) ----
   // Iteration j of a wavefront: the matrix pipe computes S(j+1) = K(j+1).Q^T while
@@ -734,7 +783,8 @@ __global__ __launch_bounds__(NW * 64, STEP::value ? 2 : w8_wavefronts(HDP, NW)) 
       }
     };
 
-    const bool need_mask = (k0 + BN > Lk) || (p.causal && k0 + BN - 1 > wave_row0 + off);
+    bool need_mask = (k0 + BN > Lk) || (p.causal && k0 + BN - 1 > wave_row0 + off);
+    if constexpr (STEP::window) need_mask = need_mask || (k0 < wave_last_row + off - p.win_left && k0 + BN > sinks);
     if (need_mask) {
       const int row = wave_row0 + c;
       int limit = p.causal ? row + off : Lk - 1;
@@ -746,6 +796,8 @@ __global__ __launch_bounds__(NW * 64, STEP::value ? 2 : w8_wavefronts(HDP, NW)) 
           const int key = KIMG ? k0 + kt * 32 + ((i >> 3) & 1) * 16 + g * 8 + ((i >> 2) & 1) * 4 + (i & 3)
                                : k0 + kt * 32 + (i >> 2) * 8 + g * 4 + (i & 3);
           if (key > limit) s[kt][i] = -INFINITY;
+          if constexpr (STEP::window)
+            if (key < row + off - p.win_left && key >= sinks) s[kt][i] = -INFINITY;
         }
     }
     // row maximum in the shadow of the first MAXS MFMAs
@@ -1018,7 +1070,7 @@ __global__ __launch_bounds__(NW * 64, STEP::value ? 2 : w8_wavefronts(HDP, NW)) 
   const int h_e = head0 + (wave_e & ((1 << hl_e) - 1));
   T *op = static_cast<T *>(p.out) + (int64_t)q_begin * p.o_row + (int64_t)h_e * p.o_head;
   T *ost = smem + wave_e * (32 * OSTR);
-  if constexpr (STEP::value) {
+  if constexpr (STEP::parts) {
     if (!whole) {
       const int row = wave_row0_e + c_e;
       if (row < Lq) {

@@ -20,15 +20,13 @@
 #include <algorithm>
 
 #include "paged_decode.h"
+#include "prefill_parts.h"
 #include "prefill_w8.h"
 #include "step_attn.h"
 
 namespace hipattn {
 
 namespace {
-
-constexpr int kMostParts = 16;
-constexpr int kMergeHeads = 8;  // query heads of a row per workgroup of the merge
 
 template <typename T, int HD>
 struct StepDecode {
@@ -38,7 +36,7 @@ struct StepDecode {
     int n_parts, part_tiles;   // pieces of a row block's keys at most, and 64-key tiles in each
     float *part_acc, *part_ml;  // of piece i of row r and head h, at (i * total_q + r) * Hq + h: d sums; maximum and sum
   };
-  static constexpr bool value = true;
+  static constexpr bool value = true, parts = true, window = false;
   static __device__ __forceinline__ void decode(const Params &p, int wg, unsigned char *lds) {
     decode_flat<T, HD, kBlockSize>(p.decode, wg, *reinterpret_cast<FlatLds<HD> *>(lds));
   }
@@ -67,44 +65,7 @@ __global__ __launch_bounds__(128) void step_merge_kernel(typename StepDecode<T, 
   const int tiles = (max(p.causal ? min(Lk, last_row + Lk - Lq + 1) : Lk, 0) + BN - 1) / BN;
   if (tiles <= p.part_tiles) return;  // whole, and written
   const int parts = min((tiles + p.part_tiles - 1) / p.part_tiles, p.n_parts);
-  constexpr int QUADS = HD / 4;
-  for (int i = threadIdx.x; i < kMergeHeads * QUADS; i += 128) {
-    const int h = h0 + i / QUADS, e = i % QUADS * 4;
-    if (h >= p.Hq) break;
-    float m[kMostParts], l[kMostParts];
-    f32x4_t a[kMostParts];
-#pragma unroll
-    for (int k = 0; k < kMostParts; k++) {
-      m[k] = -INFINITY;
-      l[k] = 0.f;
-      a[k] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-      if (k < parts) {
-        const int64_t at = ((int64_t)k * p.total_q + r) * p.Hq + h;
-        const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + 2 * at);
-        m[k] = ml.x;
-        l[k] = ml.y;
-        a[k] = *reinterpret_cast<const f32x4_t *>(p.part_acc + at * HD + e);
-      }
-    }
-    float most = m[0];
-#pragma unroll
-    for (int k = 1; k < kMostParts; k++) most = fmaxf(most, m[k]);
-    const float base = most == -INFINITY ? 0.f : most;
-    float sum = 0.f;
-    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int k = 0; k < kMostParts; k++) {
-      const float w = fast_exp2(m[k] - base);
-      sum += w * l[k];
-#pragma unroll
-      for (int j = 0; j < 4; j++) o[j] += w * a[k][j];
-    }
-    const float inv = sum > 0.f ? 1.0f / sum : 0.f;
-    T out[4];
-#pragma unroll
-    for (int j = 0; j < 4; j++) out[j] = from_float<T>(o[j] * inv);
-    *reinterpret_cast<u32x2_t *>(static_cast<T *>(p.out) + (int64_t)r * p.o_row + (int64_t)h * p.o_head + e) = *reinterpret_cast<u32x2_t *>(out);
-  }
+  merge_parts<T, HD>(p, r, h0, parts);
 }
 
 // A stream's buffer, allocated once (buffers that grow with the batch are all kept): the flat split's partial results, 17 MB at most, and

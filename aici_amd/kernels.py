@@ -10,7 +10,7 @@ the CPU are rejected.
 from __future__ import annotations
 
 import ctypes
-from typing import Dict, List, Optional, Sequence
+from typing import Dict, List, NamedTuple, Optional, Sequence
 
 import torch
 
@@ -93,6 +93,41 @@ def flash_attn_varlen_paged(q: torch.Tensor, key_cache: torch.Tensor, value_cach
     _native.mha_varlen_fwd_paged(q, key_cache, value_cache, block_tables, seqlens_q, context_lens, max_seqlen_q,
                                  max_seqlen_k, softmax_scale, causal, out, lse)
     return (out, lse) if return_lse else out
+
+
+def flash_attn_varlen_paged_window(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, block_tables: torch.Tensor,
+                                   seqlens_q: torch.Tensor, context_lens: torch.Tensor, max_seqlen_q: int, max_seqlen_k: int,
+                                   softmax_scale: float, window_size_left: int, sink_tokens: int = 0, return_lse: bool = False,
+                                   out_dtype: Optional[torch.dtype] = None):
+    """`flash_attn_varlen_paged`, causal, with a sliding window and sinks: the query at position p of its sequence sees key j iff j <= p
+    and (j >= p - window_size_left or j < sink_tokens).  Blocks of keys that none of a sequence's new tokens sees may be gone."""
+    out = torch.empty_like(q, dtype=out_dtype or q.dtype)
+    lse = None
+    if return_lse:
+        lse = torch.empty((context_lens.numel(), q.size(1), max(int(max_seqlen_q), 1)), dtype=torch.float32, device=q.device)
+    _native.mha_varlen_fwd_paged_window(q, key_cache, value_cache, block_tables, seqlens_q, context_lens, max_seqlen_q, max_seqlen_k,
+                                        softmax_scale, window_size_left, sink_tokens, out, lse)
+    return (out, lse) if return_lse else out
+
+
+def paged_attention_window(out: torch.Tensor, query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                           num_kv_heads: int, scale: float, block_tables: torch.Tensor, context_lens: torch.Tensor, block_size: int,
+                           max_context_len: int, window_size_left: int, sink_tokens: int = 0,
+                           alibi_slopes: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> None:
+    """`paged_attention_v1` with a sliding window and sinks: the token of a sequence of ctx tokens sees key t iff
+    t >= ctx - 1 - window_size_left or t < sink_tokens.  Blocks between the two may be gone.  workspace: uint8,
+    `paged_attention_window_workspace_size` bytes; None: a buffer that the library keeps per stream."""
+    _native.paged_attention_window(out, query, key_cache, value_cache, num_kv_heads, scale, block_tables, context_lens, block_size,
+                                   max_context_len, window_size_left, sink_tokens, alibi_slopes, workspace)
+
+
+def paged_attention_window_workspace_size(num_seqs: int, num_heads: int, num_kv_heads: int, head_size: int, block_size: int,
+                                          max_context_len: int, window_size_left: int, sink_tokens: int, dtype: torch.dtype) -> int:
+    """Bytes of scratch memory paged_attention_window needs for these shapes on the current device."""
+    n = ctypes.c_int64(0)
+    call("hipattn_paged_attention_window_workspace_size", int(num_seqs), int(num_heads), int(num_kv_heads), int(head_size),
+         int(block_size), int(max_context_len), int(window_size_left), int(sink_tokens), _DTYPES[dtype], ctypes.byref(n))
+    return int(n.value)
 
 
 def paged_attention_v1(out: torch.Tensor, query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
@@ -388,6 +423,64 @@ def bias_sample(logits: torch.Tensor, temperature: torch.Tensor, top_p: torch.Te
     tokens = torch.empty((S,), dtype=torch.int32, device=logits.device)
     _native.bias_sample(logits, bias, mask, bias_rows, temperature, top_p, uniforms, tokens)
     return tokens
+
+
+def penalize_logits(logits: torch.Tensor, history: torch.Tensor, history_offsets: torch.Tensor,
+                    prompt_lens: Optional[torch.Tensor] = None, repetition: Optional[torch.Tensor] = None,
+                    frequency: Optional[torch.Tensor] = None, presence: Optional[torch.Tensor] = None,
+                    bias: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None, bias_rows: Optional[torch.Tensor] = None,
+                    out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """Penalties for what every row's sequence has said, bias and allow-mask on the logits [S, V], in front of `bias_argmax` /
+    `bias_sample`.  history int32 [N]: the sequences' tokens one after the other, from history_offsets [S + 1] on, the first
+    prompt_lens [S] of each its prompt.  A token that the sequence holds: x / repetition where x > 0, else x * repetition; then
+    - frequency * count - presence * (count > 0), counted behind the prompt; + bias; -inf where the mask bars it.  Returns `out`, by
+    default a new tensor of out_dtype (that of logits, or float32); out=logits works in place."""
+    if out is None:
+        out = torch.empty(logits.shape, dtype=out_dtype or logits.dtype, device=logits.device)
+    _native.penalize_logits(out, logits, history, history_offsets, prompt_lens, repetition, frequency, presence, bias, mask, bias_rows)
+    return out
+
+
+# --------------------------------------------------------------------------- a step's blocks on the device
+
+class StepBlocks(NamedTuple):
+    """What `step_blocks` makes of a step."""
+    state: torch.Tensor         # int32 [R, 2]: tokens in the cache, columns gone
+    ends: torch.Tensor          # int64 [2]: head and tail of the ring of free blocks
+    served: torch.Tensor        # int32 [R]: tokens given; -1: no blocks or rows left, -2: does not fit its table or its rows
+    context_lens: torch.Tensor  # int32 [R]: keys of a request that is served, else 0
+    seqlens_q: torch.Tensor     # int32 [R + 1]: sums of the tokens given
+    logit_idxs: torch.Tensor    # int32 [R]: a served request's last row, else 0
+    positions: torch.Tensor     # int64 [T]
+    slot_mapping: torch.Tensor  # int32 [T], -1: no token
+    totals: torch.Tensor        # int32 [4]: tokens given, requests not served, blocks free, blocks taken
+
+
+STEP_BLOCKS_MAX_REQUESTS = 4096
+
+
+def step_blocks(new_lens: torch.Tensor, state: torch.Tensor, block_tables: torch.Tensor, free_ring: torch.Tensor, ring_ends: torch.Tensor,
+                block_size: int, num_rows: int, rows_per_request: int = 0, window_size_left: int = -1, sink_tokens: int = 0,
+                state_out: Optional[torch.Tensor] = None, ring_ends_out: Optional[torch.Tensor] = None) -> StepBlocks:
+    """A step's block bookkeeping on the device (hipattn_step_blocks in hipattn.h): new_lens int32 [R] tokens per request (0: idle,
+    negative: ended); blocks that ended requests and windows let go return to free_ring, blocks that are needed come from it into
+    block_tables, both updated in place, and num_rows rows get their positions and slots.  state_out / ring_ends_out default to new
+    tensors; they may be state / ring_ends themselves."""
+    R, dev = new_lens.size(0), new_lens.device
+    # (one allocation for what a step hands out: the host's time per call is what a small step waits for)
+    words = [4 * (R + 1), 2 * R if state_out is None else 0, R, R, R + 1, R, int(num_rows), 4]
+    padded = [(w + 3) & ~3 for w in words]
+    wide = [2 * int(num_rows), 4 if ring_ends_out is None else 0]
+    pool = torch.empty((sum(padded) + sum(wide),), dtype=torch.int32, device=dev)
+    parts = pool.split(padded + wide)
+    work, new_state, served, context_lens, seqlens_q, logit_idxs, slots, totals = (
+        p if p.numel() == w else p[:w] for p, w in zip(parts, words))
+    positions = parts[8].view(torch.int64)
+    state_out = new_state.view(R, 2) if state_out is None else state_out
+    ring_ends_out = parts[9].view(torch.int64) if ring_ends_out is None else ring_ends_out
+    _native.step_blocks(new_lens, state, block_tables, free_ring, ring_ends, block_size, rows_per_request, window_size_left, sink_tokens,
+                        state_out, ring_ends_out, served, context_lens, seqlens_q, logit_idxs, positions, slots, totals, work.view(R + 1, 4))
+    return StepBlocks(state_out, ring_ends_out, served, context_lens, seqlens_q, logit_idxs, positions, slots, totals)
 
 
 # --------------------------------------------------------------------------- runtime plumbing

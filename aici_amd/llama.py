@@ -18,7 +18,7 @@ data path, not a language model.
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Dict, List, Tuple
+from typing import Dict, List, Optional, Tuple
 
 import torch
 
@@ -40,6 +40,8 @@ class LlamaConfig:
     max_position_embeddings: int = 8192
     rope_theta: float = 10000.0
     dtype: torch.dtype = torch.bfloat16
+    sliding_window: Optional[int] = None  # tokens a token sees, with itself (None: all); no field of the reference's
+    attention_sinks: int = 0              # the first tokens of a sequence, which stay visible beside the window
 
     @property
     def head_dim(self) -> int:
@@ -178,6 +180,7 @@ class Llama:
         bits."""
         cfg = self.cfg
         Hq, Hkv, d = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
+        window = {} if cfg.sliding_window is None else {"window_size_left": cfg.sliding_window - 1, "sink_tokens": cfg.attention_sinks}
         x = _rows(self.wte, batch_info.tokens)                                   # llama.rs:203
         T = x.size(0)
         # h: the normalised rows, None where the projection that takes them does it
@@ -200,11 +203,11 @@ class Llama:
                 if not rotated:
                     self.rotary.forward_and_cache(batch_info.positions, q, k, v, kc, vc, batch_info.slot_mapping)
                 y = varlen_attn(q.view(T, Hq, d), k.view(T, Hkv, d), v, batch_info, kc, vc,
-                                paged_prefill=paged_prefill, cached=True)      # :93
+                                paged_prefill=paged_prefill, cached=True, **window)  # :93
             else:
                 q, k, v = (t.contiguous() for t in qkv.split([Hq * d, Hkv * d, Hkv * d], dim=1))
                 q, k = self.rotary.forward(batch_info.positions, q, k)          # :85 (in place on the copies)
-                y = varlen_attn(q, k, v.reshape(T, Hkv, d), batch_info, kc, vc, paged_prefill=paged_prefill)  # :93
+                y = varlen_attn(q, k, v.reshape(T, Hkv, d), batch_info, kc, vc, paged_prefill=paged_prefill, **window)  # :93
             x, h = self._proj_add_norm(y, layer["o"], x, layer["rms_2"], layer["gate_up"])  # :96, :166, :169
             if h is None:
                 act = kernels.rms_norm_linear(x, layer["rms_2"], cfg.rms_norm_eps, layer["gate_up"], silu_and_mul=True)
@@ -218,21 +221,41 @@ class Llama:
         return self._proj(sel, self.lm_head)                                    # :210
 
 
-def aici_greedy(logits: torch.Tensor, allow_masks: torch.Tensor) -> torch.Tensor:
+@dataclass
+class Penalties:
+    """What `kernels.penalize_logits` takes of a batch beside its logits."""
+    history: torch.Tensor          # int32 [N]: every sequence's tokens, one after the other
+    history_offsets: torch.Tensor  # int64 or int32 [S + 1]
+    prompt_lens: Optional[torch.Tensor] = None  # int32 [S]
+    repetition: Optional[torch.Tensor] = None   # f32 [S]
+    frequency: Optional[torch.Tensor] = None    # f32 [S]
+    presence: Optional[torch.Tensor] = None     # f32 [S]
+
+    def apply(self, logits: torch.Tensor) -> torch.Tensor:
+        return kernels.penalize_logits(logits, self.history, self.history_offsets, self.prompt_lens, self.repetition, self.frequency,
+                                       self.presence)
+
+
+def aici_greedy(logits: torch.Tensor, allow_masks: torch.Tensor, penalties: Optional[Penalties] = None) -> torch.Tensor:
     """The sampling half of a constrained step: every sequence's packed allow-mask (u8
     [S, 4*ceil(V/32)], bit k of byte i <-> token 8i+k; aicirt/src/api.rs:278-292) is applied
     as a 0/-inf bias and the arg-max taken (tmodel.rs:277-283, 234-236), all rows in one
-    launch and without materialising f32 bias rows.  Returns int32 [S]."""
+    launch and without materialising f32 bias rows; `penalties` go first, in a launch of their own.  Returns int32 [S]."""
+    if penalties is not None:
+        logits = penalties.apply(logits)
     return kernels.bias_argmax(logits, mask=allow_masks)
 
 
 def aici_sample(logits: torch.Tensor, allow_masks: torch.Tensor, temperature: torch.Tensor, top_p: torch.Tensor,
-                uniforms: torch.Tensor = None, generator: torch.Generator = None) -> torch.Tensor:
+                uniforms: torch.Tensor = None, generator: torch.Generator = None,
+                penalties: Optional[Penalties] = None) -> torch.Tensor:
     """The sampling half with temperature and top-p (tmodel.rs:172-194, 236-268) under the same packed
     allow-masks: rows with temperature < 1e-5 are greedy, the others are drawn with one uniform number per
     row in [0, 1) -- the caller's, or drawn here from `generator` (a seeded torch.Generator on the CPU stands
     in for the reference's per-sequence `StdRng`: the same seed gives the same tokens).  All rows in one
-    call, no host round trip.  Returns int32 [S]."""
+    call, no host round trip; `penalties` go first.  Returns int32 [S]."""
+    if penalties is not None:
+        logits = penalties.apply(logits)
     if uniforms is None:
         uniforms = torch.rand((logits.size(0),), generator=generator, dtype=torch.float32).to(logits.device)
     return kernels.bias_sample(logits, temperature, top_p, uniforms, mask=allow_masks)

@@ -366,6 +366,50 @@ class DecodeBatch:
         return _batch_info(bi)
 
 
+class DeviceBlocks:
+    """The blocks of a paged cache on the device (`kernels.step_blocks`), for up to max_requests requests that share none: every step's block
+    tables, slots and positions come from how many tokens each request brings, without the host knowing a length, so that a step can be
+    captured into a graph.  With a window (window_size_left >= 0, as in `attn.varlen_attn`) blocks that it has passed, sinks aside,
+    go back to the pool.  A request is a row of the tables; the row is free again when its request has ended."""
+
+    def __init__(self, block_size: int, num_blocks: int, max_requests: int, max_model_len: int, device, window_size_left: int = -1,
+                 sink_tokens: int = 0):
+        self.block_size = int(block_size)
+        self.window_size_left, self.sink_tokens = int(window_size_left), int(sink_tokens)
+        columns = (int(max_model_len) + self.block_size - 1) // self.block_size
+        self.max_context_len = columns * self.block_size
+        self.state = torch.zeros((max_requests, 2), dtype=torch.int32, device=device)
+        self.block_tables = torch.zeros((max_requests, columns), dtype=torch.int32, device=device)
+        self.free_ring = torch.arange(num_blocks, dtype=torch.int32, device=device)
+        self.ring_ends = torch.tensor([0, num_blocks], dtype=torch.int64, device=device)
+
+    def step(self, new_lens: torch.Tensor, num_rows: int, rows_per_request: int = 0):
+        """int32 [max_requests] tokens that every request brings (0: idle, negative: ended) -> `kernels.StepBlocks` of num_rows rows."""
+        from . import kernels
+
+        return kernels.step_blocks(new_lens, self.state, self.block_tables, self.free_ring, self.ring_ends, self.block_size, num_rows,
+                                   rows_per_request, self.window_size_left, self.sink_tokens, state_out=self.state,
+                                   ring_ends_out=self.ring_ends)
+
+    def batch_info(self, step, tokens: torch.Tensor, max_new: Optional[int] = None) -> BatchInfo:
+        """The batch of a step whose rows hold `tokens` [num_rows].  max_new None: decode rows, of a step with rows_per_request=1 and a row for
+        every request; else chunks of at most max_new tokens, of a step with rows_per_request=0, read through the block tables."""
+        rows, requests = step.positions.numel(), self.state.size(0)
+        decode = max_new is None
+        if decode and rows != requests:
+            raise ValueError(f"decode rows: {rows} rows for {requests} requests")
+        none = self.free_ring.new_zeros((0,))
+        return BatchInfo(
+            tokens=tokens, positions=step.positions, seqlens_q=none if decode else step.seqlens_q, seqlens_k=none, gather_mapping=none,
+            slot_mapping=step.slot_mapping, logit_idxs=step.logit_idxs, max_seqlen_q=0 if decode else int(max_new),
+            max_seqlen_k=0 if decode else self.max_context_len, seq_ids=list(range(requests)),
+            paged_block_tables=self.block_tables if decode else none.view(0, 0),
+            paged_context_lens=step.context_lens if decode else none, paged_block_size=self.block_size,
+            paged_max_context_len=self.max_context_len if decode else 0, seqlen_multi=0 if decode else requests,
+            q_multi=0 if decode else rows, multi_block_tables=None if decode else self.block_tables,
+            multi_context_lens=None if decode else step.context_lens)
+
+
 def _batch_info(bi) -> BatchInfo:
     """Copies a `hipattn_batch_info` (arrays owned by the C++ side) into host tensors."""
     nm = int(bi.num_multi)

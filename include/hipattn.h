@@ -110,6 +110,20 @@ char *hipattn_mha_varlen_fwd_paged(const hipattn_tensor *q, const hipattn_tensor
                                    int max_seqlen_q, int max_seqlen_k, float softmax_scale, bool is_causal,
                                    hipattn_tensor *out, hipattn_tensor *softmax_lse, void *stream);
 
+/* hipattn_mha_varlen_fwd_paged with a sliding window and sinks: always causal, and the query at position p of its sequence sees key j
+ * iff j <= p and (j >= p - window_size_left or j < sink_tokens) -- window_size_left + 1 tokens with its own, as the window of
+ * hipattn_mha_varlen_fwd counts them, and the first sink_tokens of the sequence.  No counterpart in tch-cuda (its windows have no sinks
+ * and read rows of k / v).  window_size_left >= 0, sink_tokens >= 0; everything else as there, any of its types, head and block sizes.
+ * Keys that no new token of a sequence sees may be gone: table columns that hold only such keys may name any block or none (a negative
+ * or large number), and their blocks may hold anything.  Values of a key that some of a sequence's new tokens see are taken to be finite,
+ * also where others do not see it.  A row that sees nothing (its position is negative) is zero, its LSE +inf. */
+char *hipattn_mha_varlen_fwd_paged_window(const hipattn_tensor *q, const hipattn_tensor *key_cache,
+                                          const hipattn_tensor *value_cache, const hipattn_tensor *block_tables,
+                                          const hipattn_tensor *cu_seqlens_q, const hipattn_tensor *context_lens,
+                                          int max_seqlen_q, int max_seqlen_k, float softmax_scale,
+                                          int window_size_left, int sink_tokens, hipattn_tensor *out,
+                                          hipattn_tensor *softmax_lse, void *stream);
+
 /* Replaces paged_attention_v1_C (lib.rs:107-120; attention_kernels.cu:679-700).
  * out/query [S, Hq, d]; key_cache [nb, Hkv, d/x, BS, x]; value_cache
  * [nb, Hkv, d, BS]; block_tables int32 [S, max_blocks]; context_lens int32 [S].
@@ -192,6 +206,24 @@ char *hipattn_paged_attention_workspace_size(int64_t num_seqs, int num_heads,
                                              int block_size,
                                              int max_context_len, int32_t dtype,
                                              int64_t *bytes);
+
+/* hipattn_paged_attention_v1 with a sliding window and sinks: the token of a sequence of ctx tokens sees key t iff t < ctx and
+ * (t >= ctx - 1 - window_size_left or t < sink_tokens).  No counterpart in tch-cuda.  Reads those keys alone: table columns between the
+ * sinks and the window may name any block or none, and their blocks hold anything.  f16 and bf16 caches, head sizes 64, 80, 96, 112, 128
+ * and 256, block sizes 8, 16 and 32; window_size_left >= 0, sink_tokens >= 0; arguments else as for hipattn_paged_attention_v1.
+ * workspace: u8, 256-byte aligned, hipattn_paged_attention_window_workspace_size bytes -- a function of the shapes, max_context_len, the
+ * window and the sinks -- or NULL for a buffer that the library keeps per stream, with what hipattn_paged_attention_v1 says about captures
+ * and overlapping calls. */
+char *hipattn_paged_attention_window(hipattn_tensor *out, const hipattn_tensor *query,
+                                     const hipattn_tensor *key_cache, const hipattn_tensor *value_cache,
+                                     int num_kv_heads, float scale, const hipattn_tensor *block_tables,
+                                     const hipattn_tensor *context_lens, int block_size, int max_context_len,
+                                     int window_size_left, int sink_tokens, const hipattn_tensor *alibi_slopes,
+                                     const hipattn_tensor *workspace, void *stream);
+char *hipattn_paged_attention_window_workspace_size(int64_t num_seqs, int num_heads, int num_kv_heads,
+                                                    int head_size, int block_size, int max_context_len,
+                                                    int window_size_left, int sink_tokens, int32_t dtype,
+                                                    int64_t *bytes);
 
 /* Replaces paged_attention_v2_C (lib.rs:122-137; attention_kernels.cu:421-546,
  * 729-874).  Same as v1 with caller-provided split-K workspaces: exp_sums and
@@ -436,6 +468,20 @@ char *hipattn_bias_argmax(const hipattn_tensor *logits,
                           const hipattn_tensor *bias_rows,
                           hipattn_tensor *out_tokens,
                           hipattn_tensor *out_logits, void *stream);
+
+/* Penalties for what a sequence has said, bias and allow-mask on the logits of all rows, in front of hipattn_bias_argmax /
+ * hipattn_bias_sample (rLLM applies the bias alone, tmodel.rs:277-283):
+ *   x = logits; a token that the sequence holds: x = x > 0 ? x / repetition : x * repetition;
+ *   x -= frequency * count + presence * (count > 0), count: how often the token stands behind the prompt; x += bias; not allowed: x = -inf.
+ * history int32 [N]: the tokens of all sequences one after the other, sequence s those from history_offsets[s] (int64 or int32 [S + 1]) on,
+ * the first prompt_lens[s] (int32 [S] or NULL: none) of them its prompt; tokens outside the vocabulary count for nothing.  repetition,
+ * frequency, presence f32 [S], NULL: 1, 0, 0.  bias f32 rows, mask packed allow-bits and bias_rows as for hipattn_bias_argmax, but any of
+ * them, both or none.  out [S, V] in the type of logits or f32, rounded once from fp32; it may be logits itself (same type and strides). */
+char *hipattn_penalize_logits(hipattn_tensor *out, const hipattn_tensor *logits, const hipattn_tensor *history,
+                              const hipattn_tensor *history_offsets, const hipattn_tensor *prompt_lens,
+                              const hipattn_tensor *repetition, const hipattn_tensor *frequency,
+                              const hipattn_tensor *presence, const hipattn_tensor *bias,
+                              const hipattn_tensor *mask, const hipattn_tensor *bias_rows, void *stream);
 
 /* Bias + temperature + nucleus (top-p) sampling for all rows in one call:
  * `TchAiciBias::apply` followed by `TModel::sample` / `sample_topp` /
@@ -813,6 +859,33 @@ char *hipattn_block_space_step_generation(
     int64_t max_copy_pairs, int64_t *n_copy_pairs, int64_t *swap_out_pairs,
     int64_t max_swap_pairs, int64_t *n_swap_pairs);
 
+/* The block bookkeeping of a step on the device, for sequences that share no blocks: what append_slots and the batch builder give on the
+ * host, from device arrays alone, so that a step can be captured and replayed.  R requests (at most 4096), a pool of nb blocks.
+ *   new_lens int32 [R]: tokens that request r brings; 0: it idles; negative: it has ended and its blocks go back.
+ *   state int32 [R, 2]: its tokens in the cache, and the table columns in front of which everything but the sinks is gone.  state_out may
+ *     be the same memory.
+ *   block_tables int32 [R, cols] (rows may lie apart), updated in place: columns of blocks that are taken; the others stay as they are.
+ *   free_ring int32 [nb]: the free blocks, in a ring: the next to be taken is free_ring[ring_ends[0] % nb], the place of the next that comes
+ *     back free_ring[ring_ends[1] % nb] (int64 [2], both only grow; ring_ends_out may be the same memory).
+ * Blocks go back first: those of ended requests and, with window_size_left >= 0, columns that hold only tokens in front of the window of
+ * a request's next token and behind its sink_tokens; in the order of requests and columns.  Then requests are served in their order, as long
+ * as the pool and the rows last: one that does not get all it needs gets nothing, nor do those behind it (served -1).  One whose tokens
+ * exceed its table row, its rows or all rows is passed over (served -2).
+ * rows_per_request 0: the rows of the T = positions' length lie one request behind the other, from seqlens_q[r] on; q > 0: request r has
+ * rows q r .. q r + q - 1 whether it uses them or not (R q <= T).
+ * Outputs: served int32 [R], the tokens given or the codes above; context_lens int32 [R]: keys of a request that is served, else 0;
+ * seqlens_q int32 [R + 1]: sums of the tokens given; logit_idxs int32 [R]: a served request's last row, else 0; positions int64 [T] and
+ * slot_mapping int32 [T], of rows without a token 0 and -1; totals int32 [4]: tokens given, requests not served (-1 and -2), blocks
+ * free afterwards, blocks taken.  workspace int32 [R + 1, 4], 16-byte aligned. */
+char *hipattn_step_blocks(const hipattn_tensor *new_lens, const hipattn_tensor *state,
+                          hipattn_tensor *block_tables, hipattn_tensor *free_ring,
+                          const hipattn_tensor *ring_ends, int block_size, int rows_per_request,
+                          int window_size_left, int sink_tokens, hipattn_tensor *state_out,
+                          hipattn_tensor *ring_ends_out, hipattn_tensor *served, hipattn_tensor *context_lens,
+                          hipattn_tensor *seqlens_q, hipattn_tensor *logit_idxs, hipattn_tensor *positions,
+                          hipattn_tensor *slot_mapping, hipattn_tensor *totals, hipattn_tensor *workspace,
+                          void *stream);
+
 /* Cache geometry (`CacheEngine`, cache_engine.rs:81-100,165-175):
  * x = 16 / elt_size; key block [Hkv, d/x, BS, x], value block [Hkv, d, BS];
  * bytes per block over all layers = 2*BS*Hkv*d*elt*layers. */
@@ -871,6 +944,19 @@ char *hipattn_varlen_attn_paged(
     const hipattn_tensor *paged_context_lens, int paged_block_size,
     int paged_max_context_len, float softmax_scale, hipattn_tensor *y,
     void *stream);
+
+/* The same for a model with a sliding window and sinks: hipattn_reshape_and_cache (slot_mapping not NULL),
+ * hipattn_mha_varlen_fwd_paged_window for the first q_multi rows, hipattn_paged_attention_window for the rest. */
+char *hipattn_varlen_attn_paged_window(
+    const hipattn_tensor *q, const hipattn_tensor *k, const hipattn_tensor *v,
+    hipattn_tensor *key_cache, hipattn_tensor *value_cache,
+    const hipattn_tensor *slot_mapping, const hipattn_tensor *multi_block_tables,
+    const hipattn_tensor *seqlens_q, const hipattn_tensor *multi_context_lens,
+    int64_t q_multi, int max_seqlen_q, int max_seqlen_k,
+    const hipattn_tensor *paged_block_tables,
+    const hipattn_tensor *paged_context_lens, int paged_block_size,
+    int paged_max_context_len, float softmax_scale, int window_size_left,
+    int sink_tokens, hipattn_tensor *y, void *stream);
 
 #ifdef __cplusplus
 }

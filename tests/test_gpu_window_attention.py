@@ -1,0 +1,291 @@
+"""Attention with a sliding window and sinks over the paged cache, decode rows and chunks, against a row-by-row restatement in 64 bits over
+the keys that are seen and no others.  Everything else in the cache is NaN -- blocks of columns that the window has passed, tokens behind
+the context, tokens between the sinks and the window -- and table columns of passed blocks hold numbers that name no block.
+
+Tolerance, per element: the output's own rounding, half a step of |out|; the probabilities, rounded to the cache's type as operands of
+the second product, half a step of sum p |v|; and 1e-4 of sum p |v| for scores and sums in fp32 (128 products of up to 6 x 6 x scale, 2^-24 each,
+in the exponent; some thousand terms in the sums)."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from aici_amd import attn, kernels as K
+from aici_amd import workloads as W
+from aici_amd._lib import HipAttnError
+from aici_amd.kernels import _native
+from oracle import steps
+from tests.common import make_cache
+
+pytestmark = pytest.mark.gpu
+NAN = float("nan")
+
+
+def bound(out, mass, dtype, rounded=True):
+    half = torch.finfo(dtype).eps / 2
+    return 1.01 * half * (mass + (out.abs() if rounded else 0)) + 1e-4 * mass + 1e-6
+
+
+def case(seed, lens_q, ctx, heads, dtype, window, sinks, bs=16):
+    """A cache that holds what some new token sees, and NaN in every other place; columns of blocks with nothing to see name no block."""
+    hq, hkv, d = heads
+    g = torch.Generator().manual_seed(seed)
+    width = max(1, max(-(-c // bs) for c in ctx))
+    blocks = sum(-(-c // bs) for c in ctx) + 3
+    perm = torch.randperm(blocks, generator=g).tolist()
+    kc, vc = make_cache(blocks, hkv, d, bs, dtype, fill=NAN)
+    tables = torch.zeros((len(ctx), width), dtype=torch.int32)
+    junk = [-1, blocks, 2 ** 31 - 1, -(2 ** 31), blocks + 7]
+    for b, (lq, lk) in enumerate(zip(lens_q, ctx)):
+        first = max(lk - lq, 0) - window  # what the first new token still sees
+        used = [j for j in range(lk) if j >= first or j < sinks] if lq else []
+        cols = {j // bs for j in used}
+        for c in range(-(-lk // bs)):
+            tables[b, c] = perm.pop() if c in cols else junk[c % len(junk)]
+        for j in used:
+            block = int(tables[b, j // bs])
+            kc[block, :, :, j % bs, :] = torch.randn((hkv, d // 8, 8), generator=g).to(dtype)
+            vc[block, :, :, j % bs] = torch.randn((hkv, d), generator=g).to(dtype)
+    q = torch.randn((sum(lens_q), hq, d), generator=g).to(dtype)
+    return dict(q=q, kc=kc, vc=vc, tables=tables, lens_q=lens_q, ctx=ctx, scale=1.0 / math.sqrt(d), window=window, sinks=sinks, bs=bs,
+                heads=heads, dtype=dtype)
+
+
+def want(c, alibi=None):
+    return steps.window_attention(c["q"], c["kc"], c["vc"], c["tables"], c["lens_q"], c["ctx"], c["scale"], c["window"], c["sinks"], alibi)
+
+
+def decode(c, device, alibi=None, workspace=None, out=None, q=None):
+    q = c["q"].to(device) if q is None else q
+    out = torch.full_like(q, NAN) if out is None else out
+    K.paged_attention_window(out, q, c["kc"].to(device), c["vc"].to(device), c["heads"][1], c["scale"], c["tables"].to(device),
+                             torch.tensor(c["ctx"], dtype=torch.int32, device=device), c["bs"], c["tables"].size(1) * c["bs"], c["window"],
+                             c["sinks"], None if alibi is None else alibi.to(device), workspace)
+    return out
+
+
+def chunk(c, device, **kw):
+    return K.flash_attn_varlen_paged_window(c["q"].to(device), c["kc"].to(device), c["vc"].to(device), c["tables"].to(device),
+                                            W.offsets(c["lens_q"]).to(device), torch.tensor(c["ctx"], dtype=torch.int32, device=device),
+                                            max(c["lens_q"]), max(c["ctx"]), c["scale"], c["window"], c["sinks"], **kw)
+
+
+def check(got, c, expect, rounded=True):
+    out, mass, _ = expect
+    got = got.cpu().double()
+    assert not torch.isnan(got).any()
+    over = (got - out).abs() - bound(out, mass, c["dtype"], rounded)
+    assert float(over.max()) <= 0, f"largest excess {float(over.max()):.3g}"
+
+
+CTX = [1, 0, 2, 15, 16, 17, 31, 33, 64, 100, 129, 257, 300, 511]
+
+
+@pytest.mark.parametrize("heads", [(8, 2, 64), (4, 4, 80), (6, 1, 96), (12, 4, 112), (32, 8, 128), (34, 2, 128), (4, 2, 256)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("bs", [8, 16, 32])
+def test_decode(device, heads, dtype, bs):
+    for n, (window, sinks) in enumerate([(0, 0), (0, 1), (30, 4), (127, 0), (100, 33), (200, 64), (1000, 5), (31, 600)]):
+        c = case(100 + n, [1] * len(CTX), CTX, heads, dtype, window, sinks, bs)
+        if n % 2:  # a context of no tokens has a row all the same
+            c["q"] = c["q"]
+        check(decode(c, device), c, want(c))
+
+
+@pytest.mark.parametrize("launch", ["flat", "partitioned", "partitions of two blocks"])
+def test_decode_launches(device, tuning, launch):
+    """Long windows in every launch strategy, with many partitions and few."""
+    tuning("decode_flat", 1 if launch == "flat" else 0)
+    if launch == "partitions of two blocks":
+        tuning("decode_part_blocks", 2)
+    for dtype, heads, bs in ((torch.bfloat16, (8, 2, 128), 16), (torch.float16, (12, 4, 112), 8), (torch.bfloat16, (4, 2, 64), 32)):
+        c = case(7, [1] * 6, [700, 1, 2500, 33, 0, 1999], heads, dtype, 1100, 37, bs)
+        check(decode(c, device), c, want(c))
+
+
+def test_decode_takes_the_same_keys_whatever_the_block_size(device):
+    outs = []
+    for bs in (8, 16, 32):
+        c = case(11, [1] * 3, [900, 64, 333], (8, 2, 128), torch.bfloat16, 250, 20, 16)
+        # the same tokens moved into blocks of bs
+        kc, vc = make_cache(200, 2, 128, bs, torch.bfloat16, fill=NAN)
+        tables = torch.full((3, -(-900 // bs)), -1, dtype=torch.int32)
+        nxt = 0
+        for b, n in enumerate(c["ctx"]):
+            for j in steps.seen(n - 1, 250, 20):
+                if tables[b, j // bs] < 0:
+                    tables[b, j // bs] = nxt
+                    nxt += 1
+                kc[tables[b, j // bs], :, :, j % bs] = c["kc"][c["tables"][b, j // 16], :, :, j % 16]
+                vc[tables[b, j // bs], :, :, j % bs] = c["vc"][c["tables"][b, j // 16], :, :, j % 16]
+        c.update(kc=kc, vc=vc, tables=tables, bs=bs)
+        outs.append(decode(c, device))
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[1], outs[2])
+
+
+def test_decode_alibi_and_strides_and_unwritten_rows(device):
+    c = case(12, [1] * 4, [40, 300, 17, 129], (8, 2, 128), torch.float16, 60, 5)
+    alibi = torch.linspace(-0.3, -0.01, 8)
+    wide = torch.full((4, 3 * 8 * 128), NAN, dtype=torch.float16, device=device)
+    q = wide[:, 1024:2048].view(4, 8, 128)
+    q.copy_(c["q"])
+    frame = torch.full((6, 8, 128), 7.0, dtype=torch.float16, device=device)
+    out = decode(c, device, alibi=alibi, q=q, out=frame[1:5])
+    check(out, c, want(c, alibi))
+    assert bool((frame[0] == 7).all()) and bool((frame[5] == 7).all())
+
+
+def test_a_window_over_everything_is_paged_attention(device):
+    d = W.decode_inputs(5, 5, 1, 700, 8, 2, 128, torch.bfloat16, 300).to(device)
+    args = (d.q, d.key_cache, d.value_cache, 2, d.scale, d.block_tables, d.context_lens, 16, d.max_ctx)
+    a, b = torch.empty_like(d.q), torch.empty_like(d.q)
+    K.paged_attention_v1(a, *args)
+    K.paged_attention_window(b, *args, 5000, 3)
+    assert torch.equal(a, b)
+
+
+SEQS = [(5, 5), (64, 64), (33, 133), (0, 20), (1, 18), (200, 200), (65, 700), (16, 31), (130, 400), (9, 5)]
+
+
+@pytest.mark.parametrize("heads", [(4, 2, 8), (4, 4, 32), (4, 2, 40), (8, 2, 64), (4, 4, 80), (6, 1, 96), (12, 4, 112), (16, 2, 128), (4, 2, 160),
+                                   (2, 1, 256)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("bs", [16, 8, 32])
+def test_chunks(device, tuning, heads, dtype, bs):
+    for n, (window, sinks) in enumerate([(0, 0), (30, 4), (63, 64), (100, 33), (255, 100), (2000, 5)]):
+        c = case(200 + n, [a for a, _ in SEQS], [b for _, b in SEQS], heads, dtype, window, sinks, bs)
+        expect = want(c)
+        for kernel in ((5, 1) if bs == 16 and 32 <= heads[2] <= 128 else (0,)):
+            tuning("prefill_kernel", kernel)
+            check(chunk(c, device), c, expect)
+
+
+@pytest.mark.parametrize("heads", [(8, 2, 64), (4, 2, 96), (8, 2, 128)])
+def test_long_chunks(device, heads):
+    """Windows of many tiles with sinks of more than one, and the staged route."""
+    for window, sinks, lens_q, ctx in ((700, 70, [100, 300], [2100, 1300]), (1023, 4, [40], [1800]), (64, 200, [257], [900])):
+        c = case(31, lens_q, ctx, heads, torch.bfloat16, window, sinks)
+        expect = want(c)
+        check(chunk(c, device), c, expect)
+
+
+def test_chunk_outputs_in_fp32_lse_and_rows_behind_the_last(device):
+    c = case(41, [70, 1, 0, 9], [300, 40, 12, 5], (8, 2, 128), torch.bfloat16, 90, 10)
+    expect = want(c)
+    out, lse = chunk(c, device, return_lse=True, out_dtype=torch.float32)
+    check(out, c, expect, rounded=False)
+    row = 0
+    for b, n in enumerate(c["lens_q"]):
+        got, ref = lse[b, :, :n].cpu().double(), expect[2][row:row + n].T
+        assert torch.equal(torch.isinf(got), torch.isinf(ref))
+        fin = ~torch.isinf(ref)
+        assert n == 0 or float((got - ref)[fin].abs().max()) < 2e-3  # (the top probability's rounding, half a step of bf16, is in the sum)
+        row += n
+    assert bool((out[row - 9:row - 5] == 0).all())  # positions before the first key see nothing
+    # strided q and out with rows that no sequence owns
+    T = c["q"].size(0)
+    wide = torch.full((T + 5, 10, 128), NAN, dtype=torch.bfloat16, device=device)
+    wide[:T, 1:9] = c["q"].to(device)
+    frame = torch.full((T + 5, 12, 128), 7.0, dtype=torch.bfloat16, device=device)
+    _native.mha_varlen_fwd_paged_window(wide[:, 1:9], c["kc"].to(device), c["vc"].to(device), c["tables"].to(device),
+                                        W.offsets(c["lens_q"]).to(device), torch.tensor(c["ctx"], dtype=torch.int32, device=device), 70, 300,
+                                        c["scale"], 90, 10, frame[:, 2:10], None)
+    check(frame[:T, 2:10], c, expect)
+    assert bool((frame[T:] == 7).all()) and bool((frame[:, :2] == 7).all()) and bool((frame[:, 10:] == 7).all())
+
+
+def test_a_window_over_everything_is_causal_attention(device):
+    c = case(51, [100, 64], [500, 64], (8, 2, 128), torch.float16, 10000, 0)
+    whole = K.flash_attn_varlen_paged(c["q"].to(device), c["kc"].to(device), c["vc"].to(device), c["tables"].to(device),
+                                      W.offsets(c["lens_q"]).to(device), torch.tensor(c["ctx"], dtype=torch.int32, device=device), 100, 500,
+                                      c["scale"], True)
+    assert torch.equal(chunk(c, device), whole)
+
+
+def test_composition(device):
+    """attn.varlen_attn with a window: chunks and decode rows of one batch, their keys written to the cache by the call."""
+    dtype, heads, window, sinks, bs = torch.bfloat16, (8, 2, 128), 50, 6, 16
+    lens_q, ctx = [40, 3, 1, 1], [90, 3, 200, 1]
+    c = case(61, lens_q, ctx, heads, dtype, window, sinks)
+    q, kc, vc = c["q"], c["kc"].clone(), c["vc"].clone()
+    new_k, new_v, slots = [], [], []
+    for b, (n, lk) in enumerate(zip(lens_q, ctx)):
+        for j in range(lk - n, lk):
+            block = int(c["tables"][b, j // bs])
+            new_k.append(c["kc"][block, :, :, j % bs].reshape(2, 128))
+            new_v.append(c["vc"][block, :, :, j % bs])
+            slots.append(block * bs + j % bs)
+            kc[block, :, :, j % bs] = NAN
+            vc[block, :, :, j % bs] = NAN
+
+    class Batch:
+        q_multi, max_seqlen_q, max_seqlen_k, paged_block_size, paged_max_context_len = 43, 40, 90, bs, 200
+        slot_mapping = torch.tensor(slots, dtype=torch.int32, device=device)
+        multi_block_tables, multi_context_lens = c["tables"][:2].to(device), torch.tensor(ctx[:2], dtype=torch.int32, device=device)
+        seqlens_q = W.offsets(lens_q[:2]).to(device)
+        paged_block_tables, paged_context_lens = c["tables"][2:].to(device), torch.tensor(ctx[2:], dtype=torch.int32, device=device)
+
+    y = attn.varlen_attn(q.to(device), torch.stack(new_k).to(device), torch.stack(new_v).to(device), Batch, kc.to(device), vc.to(device),
+                         window_size_left=window, sink_tokens=sinks)
+    check(y.view(-1, 8, 128), c, want(c))
+
+
+def test_streams_workspaces_and_replays(device):
+    """Decode on a side stream with a workspace of its own, captured and replayed over new inputs beside eager calls."""
+    c = case(71, [1] * 3, [2000, 900, 1500], (8, 2, 128), torch.bfloat16, 1200, 20)
+    other = case(72, [1] * 3, [2000, 900, 1500], (8, 2, 128), torch.bfloat16, 1200, 20)
+    need = K.paged_attention_window_workspace_size(3, 8, 2, 128, 16, c["tables"].size(1) * 16, 1200, 20, torch.bfloat16)
+    assert need > 0
+    ws = torch.empty((need,), dtype=torch.uint8, device=device)
+    with pytest.raises(HipAttnError, match="too small"):
+        decode(c, device, workspace=ws[:need - 256])
+    eager = [decode(x, device) for x in (c, other)]
+    q, kc, vc, tables = (c[k].to(device) for k in ("q", "kc", "vc", "tables"))
+    ctx = torch.tensor(c["ctx"], dtype=torch.int32, device=device)
+    out, chunk_out = torch.empty_like(q), torch.empty_like(q)
+    cu = W.offsets([1, 1, 1]).to(device)
+
+    def step():
+        K.paged_attention_window(out, q, kc, vc, 2, c["scale"], tables, ctx, 16, tables.size(1) * 16, 1200, 20, None, ws)
+        chunk_out.copy_(K.flash_attn_varlen_paged_window(q, kc, vc, tables, cu, ctx, 1, 2000, c["scale"], 1200, 20))
+
+    torch.cuda.synchronize()
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    assert torch.equal(out, eager[0])
+    with torch.cuda.graph(graph, stream=side):
+        step()
+    for k in range(4):
+        x = (other, c)[k % 2]
+        for t, n in ((q, "q"), (kc, "kc"), (vc, "vc"), (tables, "tables")):
+            t.copy_(x[n])
+        out.fill_(NAN)
+        chunk_out.fill_(NAN)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager[(k + 1) % 2])
+        check(chunk_out, x, want(x))
+        assert torch.equal(decode(x, device), out)
+
+
+def test_far_blocks(device):
+    """Blocks beyond 2^31 elements of the cache."""
+    hkv, d, bs = 8, 128, 16
+    blocks = (1 << 31) // (hkv * d * bs) + 40  # 4.3 GB of keys, as much of values
+    c = case(81, [1, 1], [300, 90], (16, 8, 128), torch.bfloat16, 100, 5)
+    small = c["kc"].size(0)
+    kc = torch.zeros((blocks, hkv, d // 8, bs, 8), dtype=torch.bfloat16, device=device)
+    vc = torch.zeros((blocks, hkv, d, bs), dtype=torch.bfloat16, device=device)
+    kc[blocks - small:] = c["kc"].to(device)
+    vc[blocks - small:] = c["vc"].to(device)
+    tables = torch.where((c["tables"] >= 0) & (c["tables"] < small), c["tables"] + (blocks - small), c["tables"]).to(device)
+    ctx = torch.tensor(c["ctx"], dtype=torch.int32, device=device)
+    out = torch.full_like(c["q"], NAN).to(device)
+    K.paged_attention_window(out, c["q"].to(device), kc, vc, 8, c["scale"], tables, ctx, 16, tables.size(1) * 16, 100, 5)
+    expect = want(c)
+    check(out, c, expect)
+    out = K.flash_attn_varlen_paged_window(c["q"].to(device), kc, vc, tables, W.offsets([1, 1]).to(device), ctx, 1, 300, c["scale"], 100, 5)
+    check(out, c, expect)
