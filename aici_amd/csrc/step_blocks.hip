@@ -8,9 +8,13 @@
 //   the order of requests and columns; a request is served as long as the sums of `need` and of `new` up to it stay within what is free
 //   and within the rows.
 //
-// It is bound by latency: three running sums over the requests, and a few words per request, row and block.  step_requests_kernel, one
-// workgroup, does the sums and what is said of each request; step_rows, spread over the launch's threads, moves the blocks and fills the
-// rows, each finding its request by a search in the sums.  Small steps have both in the one workgroup.
+// It is bound by latency: running sums over the requests, and a few words per request, row and block.  step_requests_kernel, one workgroup,
+// does the sums in one round and what is said of each request; step_work, spread over a launch's threads, moves the blocks and fills the
+// rows, each item finding its request by a search in the sums.  Small steps have both in the one workgroup; larger ones a launch of workgroups
+// that each do the sums for themselves, or, where the state is updated in place, two launches.
+// us on the device (a call from Python 10.5, what the host takes to make its outputs): 64 requests, a row each, 5.4 (13.2 with a round of sums
+// each for what comes back, is wanted, needed and given, and the three kinds of items one after the other); 301 requests, 8192 rows 6.9 in one
+// launch, 4.2 + 4.4 in two; 2048 requests, 131072 rows 8.2, 6.4 + 8.1 in two.
 #include "common.h"
 #include "device_types.h"
 
@@ -31,32 +35,8 @@ struct StepParams {
   int32_t *served, *context_lens, *cu, *logit_idxs;
   int64_t *positions;
   int32_t *slots, *totals;
-  int4 *moves;  // [R + 1]: blocks given back and taken by the requests in front, columns [0, z) and from w on that are given back
+  int4 *moves;  // [R + 1]: blocks given back and taken by the requests in front, columns [0, z) and those from w on are given back
 };
-
-// Sums in front of each thread's value, over the workgroup's wavefronts; `total` is all of them.  Order and result do not depend on anything
-// but the values.
-template <typename V>
-__device__ __forceinline__ V sums_before(V v, V *s_wave, V &total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-  V inc = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const V t = __shfl_up(inc, o, 64);
-    if (lane >= o) inc += t;
-  }
-  __syncthreads();  // s_wave may still be read from the sums before
-  if (lane == 63) s_wave[wave] = inc;
-  __syncthreads();
-  V before = inc - v;
-  total = 0;
-  for (int w = 0; w < waves; w++) {
-    const V x = s_wave[w];
-    before += w < wave ? x : 0;
-    total += x;
-  }
-  return before;
-}
 
 // The last request whose sum is at most i; sums[0] = 0 and i < sums[n].
 __device__ __forceinline__ int owner_of(const int *sums, int n, int i) {
@@ -69,172 +49,260 @@ __device__ __forceinline__ int owner_of(const int *sums, int n, int i) {
   return lo;
 }
 
-// Blocks back to the ring, blocks out of it into the tables, and the rows.  back, taken, cu: [R + 1] sums.  Nothing that is read here is
-// written here: what is given back lies in columns that are held, what is taken goes to columns behind them, and what is read of the
-// ring are the blocks that were free -- where a step needs more, it finds those that come back in the table they come from.
-__device__ __forceinline__ void step_rows(const StepParams &p, const int *back, const int *taken, const int *cu, int first, int stride) {
+// What goes back of a request: columns [0, in_sinks) and [behind, ..), as many as its part of the sums says.
+struct Columns {
+  int in_sinks, behind;
+};
+
+// Blocks back to the ring, blocks out of it into the tables, and the rows.  back, taken, cu: [R + 1] sums; kv(r), columns(r): a request's
+// tokens before the step and what goes back of it.  Nothing that is read here is written here: what is given back lies in columns that
+// are held, what is taken goes to columns behind them, and what is read of the ring are the blocks that were free -- where a step needs
+// more, it finds those that come back in the table they come from.
+template <typename KV, typename COLS>
+__device__ __forceinline__ void step_work(const StepParams &p, const int *back, const int *taken, const int *cu, KV kv_of, COLS columns_of,
+                                          int64_t head, int64_t tail, int first, int stride) {
   const int n_back = back[p.R], n_taken = taken[p.R], bs = 1 << p.log2_bs;
-  const int64_t head = p.ends_out[0] - n_taken, tail = p.ends_out[1] - n_back;
   const int64_t free_before = tail - head;
   const unsigned nb = (unsigned)p.nb, head_at = (unsigned)((head % p.nb + p.nb) % p.nb), tail_at = (unsigned)((tail % p.nb + p.nb) % p.nb);
   auto given_back = [&](int i) -> int32_t {
     const int r = owner_of(back, p.R, i);
     const int j = i - back[r];
-    const int4 m = p.moves[r];
-    return p.tables[r * p.table_stride + (j < m.z ? j : m.w + (j - m.z))];
+    const Columns c = columns_of(r);
+    return p.tables[r * p.table_stride + (j < c.in_sinks ? j : c.behind + (j - c.in_sinks))];
   };
   auto taken_block = [&](int i) -> int32_t {
     return i < free_before ? p.ring[(head_at + (unsigned)i) % nb] : given_back((int)(i - free_before));
   };
-  for (int i = first; i < n_back; i += stride) p.ring[(tail_at + (unsigned)i) % nb] = given_back(i);
-  auto held_before = [&](int r) -> int {  // tokens that were in the cache
-    return p.state_out[r].x - (cu[r + 1] - cu[r]);
-  };
-  for (int i = first; i < n_taken; i += stride) {
-    const int r = owner_of(taken, p.R, i);
-    const int held = (held_before(r) + bs - 1) >> p.log2_bs;
-    p.tables[r * p.table_stride + held + (i - taken[r])] = taken_block(i);
-  }
   const int rows = p.per_request > 0 ? p.R * p.per_request : cu[p.R];
-  for (int t = first; t < p.T; t += stride) {
-    int64_t pos = 0;
-    int slot = -1;
-    if (t < rows) {
-      const int r = p.per_request > 0 ? t / p.per_request : owner_of(cu, p.R, t);
-      const int at = t - (p.per_request > 0 ? r * p.per_request : cu[r]);
-      if (at < cu[r + 1] - cu[r]) {
-        const int kv = held_before(r), held = (kv + bs - 1) >> p.log2_bs;
-        pos = kv + at;
-        const int col = (kv + at) >> p.log2_bs;
-        const int block = col < held ? p.tables[r * p.table_stride + col] : taken_block(taken[r] + col - held);
-        slot = block * bs + ((kv + at) & (bs - 1));
+  // One run over all items: a thread's next one does not wait for the stores of the last.
+  const int64_t items = (int64_t)p.T + n_taken + n_back;
+  for (int64_t item = first; item < items; item += stride) {
+    if (item < p.T) {
+      const int t = (int)item;
+      int64_t pos = 0;
+      int slot = -1;
+      if (t < rows) {
+        const int r = p.per_request > 0 ? t / p.per_request : owner_of(cu, p.R, t);
+        const int at = t - (p.per_request > 0 ? r * p.per_request : cu[r]);
+        if (at < cu[r + 1] - cu[r]) {
+          const int kv = kv_of(r), held = (kv + bs - 1) >> p.log2_bs;
+          pos = kv + at;
+          const int col = (kv + at) >> p.log2_bs;
+          const int block = col < held ? p.tables[r * p.table_stride + col] : taken_block(taken[r] + col - held);
+          slot = block * bs + ((kv + at) & (bs - 1));
+        }
       }
+      p.positions[t] = pos;
+      p.slots[t] = slot;
+    } else if (item < (int64_t)p.T + n_taken) {
+      const int i = (int)(item - p.T);
+      const int r = owner_of(taken, p.R, i);
+      const int held = (kv_of(r) + bs - 1) >> p.log2_bs;
+      p.tables[r * p.table_stride + held + (i - taken[r])] = taken_block(i);
+    } else {
+      const int i = (int)(item - p.T - n_taken);
+      p.ring[(tail_at + (unsigned)i) % nb] = given_back(i);
     }
-    p.positions[t] = pos;
-    p.slots[t] = slot;
   }
 }
 
-constexpr int kFusedRequests = 1024;  // what the one workgroup keeps the sums of in LDS
+constexpr int kThreads = 1024;
 
-// FUSED: at most kFusedRequests requests, and the blocks and rows as well.
-template <bool FUSED>
-__global__ __launch_bounds__(1024) void step_requests_kernel(StepParams p) {
-  __shared__ int64_t s_wide[16];
-  __shared__ int s_wave[16];
-  __shared__ int s_back[FUSED ? kFusedRequests + 1 : 1], s_taken[FUSED ? kFusedRequests + 1 : 1], s_cu[FUSED ? kFusedRequests + 1 : 1];
-  __shared__ int s_refused;
-  const int tid = threadIdx.x, N = blockDim.x, bs = 1 << p.log2_bs;
+// SUMS: one workgroup, the sums and what is said of each request, for step_work_kernel behind it.  ONE: the blocks and rows as well.  MANY: the
+// same in several workgroups, each of which does the sums for itself; only the first writes what is said of the requests, which must not lie
+// over what the others still read (state_out, ring_ends_out apart from state, ring_ends).
+enum { STEP_SUMS, STEP_ONE, STEP_MANY };
+
+// A thread has PER consecutive requests (PER * kThreads >= R).
+template <int MODE, int PER>
+__global__ __launch_bounds__(kThreads) void step_requests_kernel(StepParams p) {
+  constexpr bool FUSED = MODE != STEP_SUMS;
+  constexpr int WAVES = kThreads / 64, KEPT = FUSED ? PER * kThreads : 0;
+  __shared__ int64_t s_want[WAVES];
+  __shared__ int s_need[WAVES], s_came[WAVES];
+  __shared__ int s_back[KEPT + 1], s_taken[KEPT + 1], s_cu[KEPT + 1];
+  __shared__ int s_kv[PER == 1 ? KEPT + 1 : 1];  // (more of them are worked out again where they are asked for)
+  __shared__ Columns s_columns[PER == 1 ? KEPT + 1 : 1];
+  const bool says = MODE != STEP_MANY || blockIdx.x == 0;
+  __shared__ int s_refused, s_rows, s_blocks;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, bs = 1 << p.log2_bs;
   const int64_t head = p.ends[0], tail = p.ends[1];
   const int sunk = p.window_left >= 0 ? (p.sinks + bs - 1) >> p.log2_bs : 0;
-  if (tid == 0) s_refused = 0;
+  if (tid == 0) s_refused = s_rows = s_blocks = 0;
 
   struct Request {
-    int kv, gone, added, held, dead;
+    int added, kv, held, gone, dead;
+    Columns columns;
   };
   auto request = [&](int r) -> Request {
-    Request q = {0, 0, 0, 0, 0};
-    if (r < p.R) {
-      const int2 s = p.state[r];
-      q.added = p.new_lens[r];
-      q.kv = min(max(s.x, 0), p.cols << p.log2_bs);  // (a state that is none reads a wrong column, never outside)
-      q.held = (q.kv + bs - 1) >> p.log2_bs;
-      q.gone = min(max(s.y, 0), q.held);
-      q.dead = p.window_left >= 0 ? max(q.gone, max(q.kv - p.window_left, 0) >> p.log2_bs) : q.gone;
-    }
+    const int2 s = p.state[r];
+    Request q;
+    q.added = p.new_lens[r];
+    q.kv = min(max(s.x, 0), p.cols << p.log2_bs);  // (a state that is none reads a wrong column, never outside)
+    q.held = (q.kv + bs - 1) >> p.log2_bs;
+    q.gone = min(max(s.y, 0), q.held);
+    q.dead = p.window_left >= 0 ? max(q.gone, max(q.kv - p.window_left, 0) >> p.log2_bs) : q.gone;
+    q.columns.in_sinks = q.added < 0 ? min(sunk, q.held) : 0;
+    q.columns.behind = max(q.gone, sunk);
     return q;
   };
-
-  // What goes back.
-  int n_back = 0;
-  for (int r0 = 0; r0 < p.R; r0 += N) {
-    const int r = r0 + tid;
-    const Request q = request(r);
-    const bool ended = q.added < 0;
-    // columns [0, in_sinks) and [behind, end)
-    const int in_sinks = ended ? min(sunk, q.held) : 0, behind = max(q.gone, sunk), end = ended ? q.held : q.dead;
-    int total;
-    const int before = n_back + sums_before(in_sinks + max(end - behind, 0), s_wave, total);
-    if (r < p.R) {
-      p.moves[r] = make_int4(before, 0, in_sinks, behind);
-      if (FUSED) s_back[r] = before;
-    }
-    n_back += total;
+  Request req[PER];
+  int came[PER], want[PER], need[PER];
+  bool fits[PER];
+  int sum_came = 0, sum_need = 0;
+  int64_t sum_want = 0;
+#pragma unroll
+  for (int j = 0; j < PER; j++) {
+    const int r = tid * PER + j;
+    req[j] = Request{0, 0, 0, 0, 0, {0, 0}};
+    if (r < p.R) req[j] = request(r);
+    const Request &q = req[j];
+    came[j] = q.columns.in_sinks + max((q.added < 0 ? q.held : q.dead) - q.columns.behind, 0);
+    fits[j] = (int64_t)q.kv + q.added <= ((int64_t)p.cols << p.log2_bs) && q.added <= (p.per_request > 0 ? p.per_request : p.T);
+    want[j] = q.added > 0 && fits[j] ? q.added : 0;
+    need[j] = want[j] > 0 ? ((q.kv + want[j] + bs - 1) >> p.log2_bs) - q.held : 0;
+    sum_came += came[j];
+    sum_need += need[j];
+    sum_want += want[j];
   }
-  const int64_t free_blocks = tail - head + n_back;
-
-  // Who is served.  The sums run over everyone who could be, so that nobody overtakes a request that has to wait.
-  int64_t want_before = 0, need_before = 0;
-  int n_rows = 0, n_taken = 0;
-  for (int r0 = 0; r0 < p.R; r0 += N) {
-    const int r = r0 + tid;
-    const Request q = request(r);
-    const bool fits = (int64_t)q.kv + q.added <= ((int64_t)p.cols << p.log2_bs) && q.added <= (p.per_request > 0 ? p.per_request : p.T);
-    const int want = q.added > 0 && fits ? q.added : 0;
-    const int need = want > 0 ? ((q.kv + want + bs - 1) >> p.log2_bs) - q.held : 0;
-    int64_t want_total, need_total;
-    const int64_t want_to = want_before + sums_before<int64_t>(want, s_wide, want_total) + want;
-    const int64_t need_to = need_before + sums_before<int64_t>(need, s_wide, need_total) + need;
-    want_before += want_total;
-    need_before += need_total;
-    const bool lasts = need_to <= free_blocks && (p.per_request > 0 || want_to <= p.T);
-    const int given = lasts ? want : 0, taken = lasts ? need : 0;
-    int rows_total, taken_total;
-    const int row = n_rows + sums_before(given, s_wave, rows_total);
-    const int block = n_taken + sums_before(taken, s_wave, taken_total);
-    n_rows += rows_total;
-    n_taken += taken_total;
-    if (r < p.R) {
-      const bool ended = q.added < 0;
-      const int served = q.added > 0 && !fits ? -2 : (want > 0 && !lasts ? -1 : given);
-      if (served < 0) atomicAdd(&s_refused, 1);
-      p.state_out[r] = ended ? make_int2(0, 0) : make_int2(q.kv + given, q.dead);
-      p.served[r] = served;
-      p.context_lens[r] = given > 0 ? q.kv + given : 0;
-      p.cu[r] = row;
-      p.logit_idxs[r] = given > 0 ? (p.per_request > 0 ? r * p.per_request : row) + given - 1 : 0;
-      p.moves[r].y = block;
-      if (FUSED) {
-        s_cu[r] = row;
-        s_taken[r] = block;
-      }
+  // The three sums in front of the thread's requests.
+  int to_came = sum_came, to_need = sum_need;
+  int64_t to_want = sum_want;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int a = __shfl_up(to_came, o, 64), b = __shfl_up(to_need, o, 64);
+    const int64_t c = __shfl_up(to_want, o, 64);
+    if (lane >= o) {
+      to_came += a;
+      to_need += b;
+      to_want += c;
     }
+  }
+  if (lane == 63) {
+    s_came[wave] = to_came;
+    s_need[wave] = to_need;
+    s_want[wave] = to_want;
   }
   __syncthreads();
-  if (tid == 0) {
+  int back_before = to_came - sum_came, need_before = to_need - sum_need, n_back = 0, all_need = 0;
+  int64_t want_before = to_want - sum_want, all_want = 0;
+  const int waves = min((p.R + 64 * PER - 1) / (64 * PER), WAVES);  // (behind them nothing is wanted)
+  for (int w = 0; w < waves; w++) {
+    if (w == wave) {
+      back_before += n_back;
+      need_before += all_need;
+      want_before += all_want;
+    }
+    n_back += s_came[w];
+    all_need += s_need[w];
+    all_want += s_want[w];
+  }
+  // Who is served: the sums run over everyone who could be, so that nobody overtakes a request that has to wait, and those served are the
+  // first of them.
+  const int64_t free_blocks = tail - head + n_back;
+  auto lasts = [&](int64_t want_to, int need_to) { return need_to <= free_blocks && (p.per_request > 0 || want_to <= p.T); };
+  int n_rows = (int)all_want, n_taken = all_need;
+  if (!lasts(all_want, all_need)) {  // uniform
+    int64_t to_w = want_before;
+    int to_n = need_before;
+    int rows = 0, blocks = 0;
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+      to_w += want[j];
+      to_n += need[j];
+      if (lasts(to_w, to_n)) {
+        rows = (int)to_w;
+        blocks = to_n;
+      }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      rows = max(rows, __shfl_xor(rows, o, 64));
+      blocks = max(blocks, __shfl_xor(blocks, o, 64));
+    }
+    if (lane == 0) {
+      atomicMax(&s_rows, rows);
+      atomicMax(&s_blocks, blocks);
+    }
+    __syncthreads();
+    n_rows = s_rows;
+    n_taken = s_blocks;
+  }
+  int refused = 0;
+#pragma unroll
+  for (int j = 0; j < PER; j++) {
+    const int r = tid * PER + j;
+    const int row = (int)min(want_before, (int64_t)n_rows), block = min(need_before, n_taken);
+    want_before += want[j];
+    need_before += need[j];
+    const bool given_all = want[j] > 0 && lasts(want_before, need_before);
+    const int given = given_all ? want[j] : 0;
+    const Request &q = req[j];
+    const int served = q.added > 0 && !fits[j] ? -2 : (want[j] > 0 && !given_all ? -1 : given);
+    if (r < p.R) {
+      refused += served < 0;
+      if (says) {
+        p.state_out[r] = q.added < 0 ? make_int2(0, 0) : make_int2(q.kv + given, q.dead);
+        p.served[r] = served;
+        p.context_lens[r] = given > 0 ? q.kv + given : 0;
+        p.cu[r] = row;
+        p.logit_idxs[r] = given > 0 ? (p.per_request > 0 ? r * p.per_request : row) + given - 1 : 0;
+      }
+      if (FUSED) {
+        s_back[r] = back_before;
+        s_taken[r] = block;
+        s_cu[r] = row;
+        if (PER == 1) {
+          s_kv[r] = q.kv;
+          s_columns[r] = q.columns;
+        }
+      } else {
+        p.moves[r] = make_int4(back_before, block, q.columns.in_sinks, q.columns.behind);
+      }
+    }
+    back_before += came[j];
+  }
+  if (refused > 0) atomicAdd(&s_refused, refused);
+  if (FUSED && tid == 0) {
+    s_back[p.R] = n_back;
+    s_taken[p.R] = n_taken;
+    s_cu[p.R] = n_rows;
+  }
+  __syncthreads();
+  if (tid == 0 && says) {
     p.cu[p.R] = n_rows;
-    p.moves[p.R] = make_int4(n_back, n_taken, 0, 0);
+    if (!FUSED) p.moves[p.R] = make_int4(n_back, n_taken, 0, 0);
     p.ends_out[0] = head + n_taken;
     p.ends_out[1] = tail + n_back;
     p.totals[0] = n_rows;
     p.totals[1] = s_refused;
     p.totals[2] = (int)(tail + n_back - head - n_taken);
     p.totals[3] = n_taken;
-    if (FUSED) {
-      s_cu[p.R] = n_rows;
-      s_back[p.R] = n_back;
-      s_taken[p.R] = n_taken;
-    }
   }
-  if constexpr (FUSED) {
-    __syncthreads();
-    step_rows(p, s_back, s_taken, s_cu, tid, N);
-  }
+  if constexpr (FUSED)
+    step_work(p, s_back, s_taken, s_cu, [&](int r) { return PER == 1 ? s_kv[r] : request(r).kv; },
+              [&](int r) { return PER == 1 ? s_columns[r] : request(r).columns; }, head, tail, blockIdx.x * kThreads + tid,
+              gridDim.x * kThreads);
 }
 
-constexpr int kSearchRequests = 4096;  // more are searched in memory
+constexpr int kMostRequests = 4096;
 
-__global__ __launch_bounds__(256) void step_rows_kernel(StepParams p) {
-  __shared__ int s_back[kSearchRequests + 1], s_taken[kSearchRequests + 1], s_cu[kSearchRequests + 1];
-  // (the sums of back and taken lie four words apart in `moves`)
+__global__ __launch_bounds__(256) void step_work_kernel(StepParams p) {
+  __shared__ int s_back[kMostRequests + 1], s_taken[kMostRequests + 1], s_cu[kMostRequests + 1];
   for (int r = threadIdx.x; r <= p.R; r += 256) {
     const int4 m = p.moves[r];
     s_back[r] = m.x;
     s_taken[r] = m.y;
     s_cu[r] = p.cu[r];
   }
+  const int64_t head_out = p.ends_out[0], tail_out = p.ends_out[1];
   __syncthreads();
-  step_rows(p, s_back, s_taken, s_cu, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
+  step_work(p, s_back, s_taken, s_cu, [&](int r) { return p.state_out[r].x - (s_cu[r + 1] - s_cu[r]); },
+            [&](int r) {
+              const int4 m = p.moves[r];
+              return Columns{m.z, m.w};
+            },
+            head_out - s_taken[p.R], tail_out - s_back[p.R], blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
 }
 
 void check_i32(const hipattn_tensor *t, const char *name, int ndim, int64_t a, int64_t b = 0) {
@@ -261,7 +329,7 @@ void step_blocks_impl(const hipattn_tensor *new_lens, const hipattn_tensor *stat
   check_tensor(new_lens, "new_lens", 1);
   const int64_t R = new_lens->sizes[0];
   HA_CHECK(R >= 1, "step_blocks: no requests");
-  HA_CHECK(R <= kSearchRequests, "step_blocks: %lld requests, at most %d", (long long)R, kSearchRequests);
+  HA_CHECK(R <= kMostRequests, "step_blocks: %lld requests, at most %d", (long long)R, kMostRequests);
   HA_CHECK(block_size == 8 || block_size == 16 || block_size == 32, "step_blocks: unsupported block size %d (supported: 8, 16, 32)",
            block_size);
   HA_CHECK(sinks >= 0, "step_blocks: sink_tokens must not be negative, got %d", sinks);
@@ -297,7 +365,7 @@ void step_blocks_impl(const hipattn_tensor *new_lens, const hipattn_tensor *stat
   check_i64(positions, "positions", T);
   check_i32(slots, "slot_mapping", 1, T);
   check_i32(totals, "totals", 1, 4);
-  check_i32(moves, "workspace", 2, R + 1, 4);
+  check_i32(moves, "workspace", 1, 4 * (R + 1));
   HA_CHECK((reinterpret_cast<uintptr_t>(moves->data) & 15) == 0, "step_blocks: workspace must be 16-byte aligned");
   StepParams p;
   p.new_lens = static_cast<const int32_t *>(new_lens->data);
@@ -325,15 +393,29 @@ void step_blocks_impl(const hipattn_tensor *new_lens, const hipattn_tensor *stat
   p.totals = static_cast<int32_t *>(totals->data);
   p.moves = static_cast<int4 *>(moves->data);
   hipStream_t stream = resolve_stream(stream_arg);
-  if (R <= kFusedRequests && T <= 4096) {
-    step_requests_kernel<true><<<1, R <= 256 && T <= 256 ? 256 : 1024, 0, stream>>>(p);
+  if (R <= kThreads && T <= 4096) {
+    step_requests_kernel<STEP_ONE, 1><<<1, kThreads, 0, stream>>>(p);
     check_launch("step_blocks");
     return;
   }
-  step_requests_kernel<false><<<1, 1024, 0, stream>>>(p);
+  auto apart = [](const hipattn_tensor *a, const hipattn_tensor *b) {
+    const char *x = static_cast<const char *>(a->data), *y = static_cast<const char *>(b->data);
+    const int64_t n = numel(a) * dtype_size(a->dtype);
+    return x + n <= y || y + n <= x;
+  };
+  if (apart(state, state_out) && apart(ends, ends_out)) {
+    const int64_t wgs = (T + 511) / 512;
+    const dim3 grid((unsigned)(wgs < 64 ? 64 : (wgs > 256 ? 256 : wgs)));
+    if (R <= kThreads) step_requests_kernel<STEP_MANY, 1><<<grid, kThreads, 0, stream>>>(p);
+    else step_requests_kernel<STEP_MANY, 4><<<grid, kThreads, 0, stream>>>(p);
+    check_launch("step_blocks");
+    return;
+  }
+  if (R <= kThreads) step_requests_kernel<STEP_SUMS, 1><<<1, kThreads, 0, stream>>>(p);
+  else step_requests_kernel<STEP_SUMS, 4><<<1, kThreads, 0, stream>>>(p);
   check_launch("step_blocks");
   const int64_t wgs = (T + 255) / 256;
-  step_rows_kernel<<<dim3((unsigned)(wgs < 256 ? 256 : (wgs > 1024 ? 1024 : wgs))), 256, 0, stream>>>(p);
+  step_work_kernel<<<dim3((unsigned)(wgs < 256 ? 256 : (wgs > 1024 ? 1024 : wgs))), 256, 0, stream>>>(p);
   check_launch("step_blocks (rows)");
 }
 

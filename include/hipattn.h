@@ -876,7 +876,7 @@ char *hipattn_block_space_step_generation(
  * Outputs: served int32 [R], the tokens given or the codes above; context_lens int32 [R]: keys of a request that is served, else 0;
  * seqlens_q int32 [R + 1]: sums of the tokens given; logit_idxs int32 [R]: a served request's last row, else 0; positions int64 [T] and
  * slot_mapping int32 [T], of rows without a token 0 and -1; totals int32 [4]: tokens given, requests not served (-1 and -2), blocks
- * free afterwards, blocks taken.  workspace int32 [R + 1, 4], 16-byte aligned. */
+ * free afterwards, blocks taken.  workspace int32 [4 (R + 1)], 16-byte aligned. */
 char *hipattn_step_blocks(const hipattn_tensor *new_lens, const hipattn_tensor *state,
                           hipattn_tensor *block_tables, hipattn_tensor *free_ring,
                           const hipattn_tensor *ring_ends, int block_size, int rows_per_request,

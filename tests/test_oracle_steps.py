@@ -164,7 +164,7 @@ def _step_args(**over):
     i, w = dict(dtype=_lib.I32), dict(dtype=_lib.I64)
     a = dict(new=_t(5, **i), state=_t(5, 2, **i), tables=_t(5, 8, **i), ring=_t(30, **i), ends=_t(2, **w), bs=16, per=0, window=-1, sinks=0,
              state_out=_t(5, 2, **i), ends_out=_t(2, **w), served=_t(5, **i), ctx=_t(5, **i), cu=_t(6, **i), last=_t(5, **i), pos=_t(9, **w),
-             slots=_t(9, **i), totals=_t(4, **i), work=_t(6, 4, **i))
+             slots=_t(9, **i), totals=_t(4, **i), work=_t(24, **i))
     a.update(over)
     return [*a.values(), None]
 
@@ -176,7 +176,7 @@ def _step_args(**over):
     (dict(ring=_t(0, dtype=_lib.I32)), "there are none"), (dict(ring=_t(1 << 28, dtype=_lib.I32)), "do not fit 32 bits"),
     (dict(ends=_t(2, dtype=_lib.I32)), "must be int64"), (dict(cu=_t(5, dtype=_lib.I32)), "seqlens_q has the wrong shape"),
     (dict(slots=_t(8, dtype=_lib.I32)), "slot_mapping has the wrong shape"), (dict(pos=_t(0, dtype=_lib.I64)), "0 rows"),
-    (dict(work=_t(5, 4, dtype=_lib.I32)), "workspace has the wrong shape"), (dict(state_out=_t(5, 2, dtype=_lib.I32, data=260)), "8-byte aligned"),
+    (dict(work=_t(20, dtype=_lib.I32)), "workspace has the wrong shape"), (dict(state_out=_t(5, 2, dtype=_lib.I32, data=260)), "8-byte aligned"),
 ])
 def test_step_blocks_refuses(over, message):
     with pytest.raises(_lib.HipAttnError, match=message):
