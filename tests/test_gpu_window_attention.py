@@ -170,6 +170,18 @@ def test_long_chunks(device, heads):
         check(chunk(c, device), c, expect)
 
 
+@pytest.mark.parametrize("heads", [(8, 2, 64), (4, 4, 80), (6, 1, 96), (12, 4, 112), (8, 2, 128)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_chunks_whose_keys_are_dealt_out(device, heads, dtype):
+    """Few rows over long windows: several workgroups share a row block's keys, others of the same batch have too few for that."""
+    for n, (window, sinks, lens_q, ctx) in enumerate([(2500, 70, [16], [4000]), (1300, 0, [1, 40, 3, 0, 5], [2000, 1700, 40, 9, 3]),
+                                                      (900, 130, [150, 2], [1500, 901])]):
+        c = case(300 + n, lens_q, ctx, heads, dtype, window, sinks)
+        expect = want(c)
+        check(chunk(c, device), c, expect)
+        check(chunk(c, device, out_dtype=torch.float32), c, expect, rounded=False)
+
+
 def test_chunk_outputs_in_fp32_lse_and_rows_behind_the_last(device):
     c = case(41, [70, 1, 0, 9], [300, 40, 12, 5], (8, 2, 128), torch.bfloat16, 90, 10)
     expect = want(c)
@@ -195,7 +207,8 @@ def test_chunk_outputs_in_fp32_lse_and_rows_behind_the_last(device):
     assert bool((frame[T:] == 7).all()) and bool((frame[:, :2] == 7).all()) and bool((frame[:, 10:] == 7).all())
 
 
-def test_a_window_over_everything_is_causal_attention(device):
+def test_a_window_over_everything_is_causal_attention(device, tuning):
+    tuning("prefill_kernel", 5)  # (keys that are not dealt out: the same bits)
     c = case(51, [100, 64], [500, 64], (8, 2, 128), torch.float16, 10000, 0)
     whole = K.flash_attn_varlen_paged(c["q"].to(device), c["kc"].to(device), c["vc"].to(device), c["tables"].to(device),
                                       W.offsets(c["lens_q"]).to(device), torch.tensor(c["ctx"], dtype=torch.int32, device=device), 100, 500,
