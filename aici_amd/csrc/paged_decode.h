@@ -53,12 +53,19 @@ struct WindowKeys {
   static constexpr bool window = true;
 };
 
-// The block pairs (32 tokens) of a context that hold a key the token sees, numbered one after the other: pairs [0, sink_pairs) of the
-// context and then those from pair sink_pairs + skip on.  Key t is seen iff t < ctx and (t >= first or t < sink_end).
-struct SeenKeys {
-  int first, sink_end, sink_pairs, skip;
-  __device__ __forceinline__ SeenKeys(const DecodeParams &p, int ctx) {
-    first = max(ctx - 1 - p.window_left, 0);
+// Key t is seen iff t < ctx and (t >= first or t < sink_end).
+struct KeyRange {
+  int ctx, first, sink_end;
+};
+
+// The block pairs (32 tokens) of a context that hold a key that is seen, numbered one after the other: pairs [0, sink_pairs) of the
+// context and then those from pair sink_pairs + skip on.  Seen by the token at position ctx - 1, or (window_rows.hip) by one of the
+// `rows` tokens up to there.
+struct SeenKeys : KeyRange {
+  int sink_pairs, skip;
+  __device__ __forceinline__ SeenKeys(const DecodeParams &p, int ctx_, int rows = 1) {
+    ctx = ctx_;
+    first = max(ctx - rows - p.window_left, 0);
     sink_end = min(p.sinks, first);
     sink_pairs = (sink_end + 2 * 16 - 1) / (2 * 16);
     skip = max(first / (2 * 16) - sink_pairs, 0);
@@ -130,8 +137,10 @@ struct Mfma16<bf16_t> {
 // A load of cache bytes.  Every byte of K and V is read once per launch and never again: the loads carry the
 // non-temporal hint, so the lines are not kept in L2 and the memory-side cache at the expense of each other.
 // Measured on MI355X, 64 sequences of 512..4096 tokens, 8 kv heads x 128: 120.8 -> 107.2 us per step.
-template <typename V>
+// ONCE false: bytes that other workgroups read too (window_rows.hip).
+template <bool ONCE = true, typename V>
 __device__ __forceinline__ V stream_load(const V *p) {
+  if constexpr (!ONCE) return *p;
   return __builtin_nontemporal_load(p);
 }
 
@@ -143,7 +152,7 @@ struct PairRegs {
 };
 
 // Issues the loads of the block pair (pa, pb) of one kv head.
-template <typename T, int HD>
+template <typename T, int HD, bool ONCE = true>
 __device__ __forceinline__ void pair_load(const DecodeParams &p, const T *kbase, const T *vbase, int64_t pa, int64_t pb,
                                           PairRegs<HD> &r) {
   constexpr int NCH = HD / 8;
@@ -166,16 +175,16 @@ __device__ __forceinline__ void pair_load(const DecodeParams &p, const T *kbase,
     r.kra[s] = u32x4_t{0u, 0u, 0u, 0u};
     r.krb[s] = u32x4_t{0u, 0u, 0u, 0u};
     if (NCH % 4 == 0 || ch < NCH) {
-      r.kra[s] = stream_load(reinterpret_cast<const u32x4_t *>(ka + (ch * kBlockSize + col) * 8));
-      r.krb[s] = stream_load(reinterpret_cast<const u32x4_t *>(kb + (ch * kBlockSize + col) * 8));
+      r.kra[s] = stream_load<ONCE>(reinterpret_cast<const u32x4_t *>(ka + (ch * kBlockSize + col) * 8));
+      r.krb[s] = stream_load<ONCE>(reinterpret_cast<const u32x4_t *>(kb + (ch * kBlockSize + col) * 8));
     }
   }
   // V: tile dt of a block is the contiguous 512 B run of rows 16dt..16dt+15;
   // lane (kg, row) takes tokens 4kg..4kg+3 of its row.
 #pragma unroll
   for (int dt = 0; dt < NDT; dt++) {
-    r.vra[dt] = stream_load(reinterpret_cast<const u32x2_t *>(va + (dt * 16 + col) * kBlockSize + kg * 4));
-    r.vrb[dt] = stream_load(reinterpret_cast<const u32x2_t *>(vb + (dt * 16 + col) * kBlockSize + kg * 4));
+    r.vra[dt] = stream_load<ONCE>(reinterpret_cast<const u32x2_t *>(va + (dt * 16 + col) * kBlockSize + kg * 4));
+    r.vrb[dt] = stream_load<ONCE>(reinterpret_cast<const u32x2_t *>(vb + (dt * 16 + col) * kBlockSize + kg * 4));
   }
 }
 
@@ -184,12 +193,12 @@ __device__ __forceinline__ void pair_load(const DecodeParams &p, const T *kbase,
 // 32-token block of the cache (id i0; its two halves) or four 8-token blocks (ids i0..i3; a lane's token
 // says which one it reads).  Ids are clamped like those of pair_load: a pair's trailing ids may lie past
 // the context, where the table holds anything; the tokens read through them are masked by the caller.
-template <typename T, int HD, int BS>
+template <typename T, int HD, int BS, bool ONCE = true>
 __device__ __forceinline__ void pair_load_bs(const DecodeParams &p, const T *kbase, const T *vbase, int64_t i0, int64_t i1,
                                              int64_t i2, int64_t i3, PairRegs<HD> &r) {
   static_assert(BS == 8 || BS == 16 || BS == 32, "block sizes of the reference's support matrix");
   if constexpr (BS == 16) {
-    pair_load<T, HD>(p, kbase, vbase, i0, i1, r);
+    pair_load<T, HD, ONCE>(p, kbase, vbase, i0, i1, r);
   } else {
     constexpr int NCH = HD / 8;
     constexpr int NSTEP = (HD + 31) / 32;
@@ -226,14 +235,14 @@ __device__ __forceinline__ void pair_load_bs(const DecodeParams &p, const T *kba
       r.kra[s] = u32x4_t{0u, 0u, 0u, 0u};
       r.krb[s] = u32x4_t{0u, 0u, 0u, 0u};
       if (NCH % 4 == 0 || ch < NCH) {
-        r.kra[s] = stream_load(reinterpret_cast<const u32x4_t *>(kal + (4 * s * BS * 8 - BIAS)));
-        r.krb[s] = stream_load(reinterpret_cast<const u32x4_t *>(kbl + (4 * s * BS * 8 - BIAS)));
+        r.kra[s] = stream_load<ONCE>(reinterpret_cast<const u32x4_t *>(kal + (4 * s * BS * 8 - BIAS)));
+        r.krb[s] = stream_load<ONCE>(reinterpret_cast<const u32x4_t *>(kbl + (4 * s * BS * 8 - BIAS)));
       }
     }
 #pragma unroll
     for (int dt = 0; dt < NDT; dt++) {
-      r.vra[dt] = stream_load(reinterpret_cast<const u32x2_t *>(val + (dt * 16 * BS - BIAS)));
-      r.vrb[dt] = stream_load(reinterpret_cast<const u32x2_t *>(vbl + (dt * 16 * BS - BIAS)));
+      r.vra[dt] = stream_load<ONCE>(reinterpret_cast<const u32x2_t *>(val + (dt * 16 * BS - BIAS)));
+      r.vrb[dt] = stream_load<ONCE>(reinterpret_cast<const u32x2_t *>(vbl + (dt * 16 * BS - BIAS)));
     }
   }
 }
@@ -241,11 +250,11 @@ __device__ __forceinline__ void pair_load_bs(const DecodeParams &p, const T *kba
 // Folds a loaded block pair -- blocks `blk` and `blk + 1` of the context, the
 // second absent when !has_b -- into the running softmax state (m_run, l_run,
 // acc).  qreg: lane (kg, col) holds q[head col][32*step + 8*kg .. +8].
-// KEYS::window: keys from sink_end on and below `first` are not seen; what the cache holds there (a block that has been given to
-// another sequence, anything) has no say in the result.
+// mine: the keys that this lane's column sees; seen: those that some column does, the same in every lane.  What the cache holds elsewhere (a block
+// that has been given to another sequence, anything) has no say in the result.  Without KEYS::window all below ctx are seen.
 template <typename T, int HD, typename KEYS = AllKeys>
-__device__ __forceinline__ void pair_compute(const DecodeParams &p, PairRegs<HD> &r, int blk, bool has_b, int ctx,
-                                             int first, int sink_end, float slope, const typename Vec8<T>::type (&qreg)[(HD + 31) / 32],
+__device__ __forceinline__ void pair_compute(const DecodeParams &p, PairRegs<HD> &r, int blk, bool has_b, const KeyRange &mine,
+                                             const KeyRange &seen, float slope, const typename Vec8<T>::type (&qreg)[(HD + 31) / 32],
                                              float &m_run, float &l_run, f32x4_t (&acc)[HD / 16]) {
   typedef typename Vec8<T>::type vec8;
   constexpr int NSTEP = (HD + 31) / 32;
@@ -271,13 +280,13 @@ __device__ __forceinline__ void pair_compute(const DecodeParams &p, PairRegs<HD>
   float x[8];
 #pragma unroll
   for (int i = 0; i < 4; i++) {
-    x[i] = sa[i] * p.scale_log2 + slope * (float)(tok_a + i - ctx + 1);
-    x[4 + i] = sb[i] * p.scale_log2 + slope * (float)(tok_b + i - ctx + 1);
-    if (tok_a + i >= ctx) x[i] = -INFINITY;
-    if (tok_b + i >= ctx) x[4 + i] = -INFINITY;
+    x[i] = sa[i] * p.scale_log2 + slope * (float)(tok_a + i - mine.ctx + 1);
+    x[4 + i] = sb[i] * p.scale_log2 + slope * (float)(tok_b + i - mine.ctx + 1);
+    if (tok_a + i >= mine.ctx) x[i] = -INFINITY;
+    if (tok_b + i >= mine.ctx) x[4 + i] = -INFINITY;
     if constexpr (KEYS::window) {
-      if (tok_a + i >= sink_end && tok_a + i < first) x[i] = -INFINITY;
-      if (tok_b + i >= sink_end && tok_b + i < first) x[4 + i] = -INFINITY;
+      if (tok_a + i >= mine.sink_end && tok_a + i < mine.first) x[i] = -INFINITY;
+      if (tok_b + i >= mine.sink_end && tok_b + i < mine.first) x[4 + i] = -INFINITY;
     }
   }
   float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
@@ -303,29 +312,29 @@ __device__ __forceinline__ void pair_compute(const DecodeParams &p, PairRegs<HD>
 
   // Tokens past the context hold whatever the cache held before; a zero
   // probability does not neutralise a NaN, so clear those V entries.
-  if ((blk + 2) * kBlockSize > ctx || !has_b) {  // wave-uniform: only the context's last pair
+  if ((blk + 2) * kBlockSize > seen.ctx || !has_b) {  // wave-uniform: only the context's last pair
 #pragma unroll
     for (int dt = 0; dt < NDT; dt++) {
       uint16_t *ea = reinterpret_cast<uint16_t *>(&vra[dt]);
       uint16_t *eb = reinterpret_cast<uint16_t *>(&vrb[dt]);
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        if (tok_a + i >= ctx) ea[i] = 0;
-        if (tok_b + i >= ctx) eb[i] = 0;
+        if (tok_a + i >= seen.ctx) ea[i] = 0;
+        if (tok_b + i >= seen.ctx) eb[i] = 0;
       }
     }
   }
 
   if constexpr (KEYS::window) {
-    if (blk * kBlockSize < first && (blk + 2) * kBlockSize > sink_end) {  // wave-uniform: the last pair of the sinks, the first of the window
+    if (blk * kBlockSize < seen.first && (blk + 2) * kBlockSize > seen.sink_end) {  // wave-uniform: the last pair of the sinks, the first of the window
 #pragma unroll
       for (int dt = 0; dt < NDT; dt++) {
         uint16_t *ea = reinterpret_cast<uint16_t *>(&vra[dt]);
         uint16_t *eb = reinterpret_cast<uint16_t *>(&vrb[dt]);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          if (tok_a + i >= sink_end && tok_a + i < first) ea[i] = 0;
-          if (tok_b + i >= sink_end && tok_b + i < first) eb[i] = 0;
+          if (tok_a + i >= seen.sink_end && tok_a + i < seen.first) ea[i] = 0;
+          if (tok_b + i >= seen.sink_end && tok_b + i < seen.first) eb[i] = 0;
         }
       }
     }
@@ -471,7 +480,7 @@ __device__ __forceinline__ void decode_flat(const DecodeParams &p, const int wg,
       continue;
     }
     const int ctx = uniform(s_ctx[seq]);
-    const SeenKeys seen(p, KEYS::window ? ctx : 0);
+    const SeenKeys seen(p, ctx);
     const int nblk = (ctx + kBlockSize - 1) / kBlockSize - (KEYS::window ? 2 * seen.skip : 0);
     const int r = u - hk * before;
     const int h = r / pairs;
@@ -533,8 +542,7 @@ __device__ __forceinline__ void decode_flat(const DecodeParams &p, const int wg,
       };
       auto fold = [&](int it, PairRegs<HD> &r) {
         const int blk = b_first + 2 * it;
-        pair_compute<T, HD, KEYS>(p, r, KEYS::window ? seen.run(blk) : blk, blk + 1 < nblk, ctx, seen.first, seen.sink_end, slope, qreg, m_run,
-                                  l_run, acc);
+        pair_compute<T, HD, KEYS>(p, r, KEYS::window ? seen.run(blk) : blk, blk + 1 < nblk, seen, seen, slope, qreg, m_run, l_run, acc);
       };
       // The pairs of a batch are visited in bit-reversed order (of 32: 0, 16, 8, 24, 4, ...), not in the order of
       // the table; in a batch of fewer than 32 the largest power of two of them is, the rest follow in table order.

@@ -46,7 +46,7 @@ __global__ __launch_bounds__(WAVES * 64) void paged_decode_kernel(DecodeParams p
   };
   if constexpr (!KEYS::window) load_table([](int c) { return c; });
   const int ctx = min(p.context_lens[seq], p.max_ctx);
-  const SeenKeys seen(p, KEYS::window ? ctx : 0);
+  const SeenKeys seen(p, ctx);
   if constexpr (KEYS::window) load_table([&](int c) { return seen.column(c, BS); });
   const int nblk = (ctx + kBlockSize - 1) / kBlockSize - (KEYS::window ? 2 * seen.skip : 0);
   const int g_idx = cg * 16 + col;  // query head within the GQA group
@@ -109,8 +109,7 @@ __global__ __launch_bounds__(WAVES * 64) void paged_decode_kernel(DecodeParams p
     pair_load_bs<T, HD, BS>(p, kbase, vbase, i0, i1, i2, i3, r);
   };
   auto fold = [&](int it, PairRegs<HD> &r) {
-    pair_compute<T, HD, KEYS>(p, r, KEYS::window ? seen.run(b0 + it) : b0 + it, it + 1 < nb, ctx, seen.first, seen.sink_end, slope, qreg, m_run,
-                              l_run, acc);
+    pair_compute<T, HD, KEYS>(p, r, KEYS::window ? seen.run(b0 + it) : b0 + it, it + 1 < nb, seen, seen, slope, qreg, m_run, l_run, acc);
   };
   constexpr int STEP = 2 * WAVES;
   if constexpr (WAVES == 4) {

@@ -11,6 +11,17 @@ namespace {
 constexpr int kMostParts = 16;
 constexpr int kMergeHeads = 8;  // query heads of a row per workgroup of the merge
 
+// The sequence that holds row r of all sequences' rows, -1: none; by a whole wavefront.
+__device__ __forceinline__ int sequence_of_row(const int32_t *cu_q, int batch, int r) {
+  const int lane = threadIdx.x & 63;
+  if (r < cu_q[0]) return -1;
+  for (int s0 = 0; s0 < batch; s0 += 64) {
+    const unsigned long long past = __ballot(s0 + lane < batch && cu_q[min(s0 + lane, batch - 1) + 1] > r);
+    if (past != 0) return s0 + __builtin_ctzll(past);
+  }
+  return -1;
+}
+
 // Adds up the `parts` pieces of row r (of all sequences) for the kMergeHeads heads from h0 on, a workgroup of 128 threads.
 template <typename T, int HD, typename P>
 __device__ __forceinline__ void merge_parts(const P &p, const int r, const int h0, const int parts) {

@@ -45,6 +45,7 @@ struct PrefillAlone {
   static constexpr bool value = false;   // decode rows beside it
   static constexpr bool parts = false;   // keys dealt out
   static constexpr bool window = false;  // a window and sinks
+  static constexpr int block = 16;       // tokens per block of the cache (block images; staged tiles know 16)
 };
 
 // Wavefronts per SIMD and places for tiles in LDS of the forms with eight and four wavefronts.
@@ -290,17 +291,20 @@ __global__ __launch_bounds__(NW * 64, STEP::value ? 2 : w8_wavefronts(HDP, NW)) 
   constexpr int NLOADVP = (4 * V_PER_BLOCK + 511) / 512;
   u32x4_t vstp[PAGED ? NLOADVP : 1];
   int staged_k0 = 0;  // first key of the tile held in the staging registers
+  constexpr int BS = STEP::block, TILE_COLS = BN / BS;  // table columns of a tile
+  constexpr int TILES_HELD = 64 / TILE_COLS;            // tiles whose ids the lanes hold
+  static_assert(BS == 16 || DMA, "other blocks: images");
   const int32_t *table_row = PAGED ? p.block_tables + (int64_t)b * p.table_stride : nullptr;
   if constexpr (STEP::parts && !STEP::window) table_row += first_tile * (BN / 16);
-  // The block ids of 64 table columns (16 tiles) sit one per lane (columns past the context repeat its
+  // The block ids of 64 table columns (16 tiles of 16-token blocks) sit one per lane (columns past the context repeat its
   // last one), and a tile's four ids are lane reads into scalar registers: no tile waits for a table
   // read.  The next group is asked for one tile before it is needed and the ids are clamped to the cache
   // where they are used, so that nothing waits for the read where it is issued.
   int tbl_cur = 0, tbl_nxt = 0;
   auto load_ids = [&](int group) -> int {
     if constexpr (STEP::window) {
-      const int col = first_tile * (BN / 16) + min(group * 64 + lane, (Lk - 1) >> 4);
-      return table_row[max(min(col >= gap_tile * (BN / 16) ? col + skip * (BN / 16) : col, p.table_cols - 1), 0)];
+      const int col = first_tile * TILE_COLS + min(group * 64 + lane, (Lk - 1) / BS);
+      return table_row[max(min(col >= gap_tile * TILE_COLS ? col + skip * TILE_COLS : col, p.table_cols - 1), 0)];
     }
     const int last_col = min((Lk - 1) >> 4, p.table_cols - first_tile * (BN / 16) - 1);
     return table_row[max(min(group * 64 + lane, last_col), 0)];
@@ -366,7 +370,12 @@ __global__ __launch_bounds__(NW * 64, STEP::value ? 2 : w8_wavefronts(HDP, NW)) 
   int64_t tbl_off[IMG];
 #pragma unroll
   for (int im = 0; im < IMG; im++) {
-    dma_lane[im] = dma_v(im) ? c * 32 + g * 16 : lane * 16;
+    if constexpr (BS == 16)
+      dma_lane[im] = dma_v(im) ? c * 32 + g * 16 : lane * 16;
+    else if constexpr (BS == 32)
+      dma_lane[im] = dma_v(im) ? c * 64 + (dma_r & 1) * 32 + g * 16 : (lane >> 4) * 512 + (dma_r & 1) * 256 + (lane & 15) * 16;
+    else
+      dma_lane[im] = dma_v(im) ? c * 16 : (lane >> 4) * 128 + (lane & 7) * 16;
     dma_base[im] = reinterpret_cast<const char *>(dma_v(im) ? vp : kp);
     dma_blk_bytes[im] = (dma_v(im) ? p.vc_block : p.kc_block) * (int64_t)sizeof(T);
     dma_last_ok[im] = !DMA_PART || (dma_v(im) ? c < dma_tail : lane < 2 * dma_tail);
@@ -376,39 +385,69 @@ __global__ __launch_bounds__(NW * 64, STEP::value ? 2 : w8_wavefronts(HDP, NW)) 
     const int64_t bid = blk < 0 ? 0 : (blk >= p.num_blocks ? p.num_blocks - 1 : (int64_t)blk);
     return bid * dma_blk_bytes[im];
   };
-  auto dma_piece = [&](int tile, int i, int im) {
-    const int idx = (tile & 15) * 4 + dma_r;
-    const unsigned lo = __builtin_amdgcn_readlane((int)(uint32_t)tbl_off[im], idx);
-    const unsigned hi = __builtin_amdgcn_readlane((int)(uint32_t)(tbl_off[im] >> 32), idx);
-    // (an "s" operand is not made a scalar for the asm when the compiler holds the value in vector registers)
-    const uint64_t src_v = reinterpret_cast<uint64_t>(dma_base[im]) + (((uint64_t)hi << 32) | lo);
-    const char *src = reinterpret_cast<const char *>(
-        ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(src_v >> 32)) << 32) |
-        (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)src_v));
-    // the instruction's offset field moves both ends of the copy: the address in memory and the one in LDS
+  // The same images out of caches with other blocks: a run of 16 tokens is half of a 32-token block, whose runs of K and rows of V lie twice as
+  // far apart, or two 8-token blocks, of which a lane's token says which one it reads.
+  auto dma_piece_bs = [&](int tile, int i, int im) {
     const unsigned dst = (unsigned)__builtin_amdgcn_readfirstlane(
-        (int)(lds0 + (unsigned)(((tile % NST) * STAGE_ELEMS + dma_v(im) * K_ELEMS + dma_r * BLK_ELEMS) * (int)sizeof(T))));
+        (int)(lds0 + (unsigned)(((tile % NST) * STAGE_ELEMS + dma_v(im) * K_ELEMS + dma_r * BLK_ELEMS) * (int)sizeof(T) + i * 1024)));
+    auto offset_of = [&](int idx) -> uint64_t {
+      const unsigned lo = __builtin_amdgcn_readlane((int)(uint32_t)tbl_off[im], idx);
+      const unsigned hi = __builtin_amdgcn_readlane((int)(uint32_t)(tbl_off[im] >> 32), idx);
+      return ((uint64_t)hi << 32) | lo;
+    };
+    const int col0 = (tile & (TILES_HELD - 1)) * TILE_COLS;
+    if (!DMA_PART || i < NDMA - 1 || dma_last_ok[im]) {
+      if constexpr (BS == 32) {
+        const char *src = uniform_ptr(dma_base[im] + offset_of(col0 + (dma_r >> 1)) + i * 2048);
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                     :
+                     : "s"(dst), "v"(dma_lane[im]), "s"(src)
+                     : "memory", "m0");
+      } else {
+        const uint64_t first = offset_of(col0 + 2 * dma_r), second = offset_of(col0 + 2 * dma_r + 1);
+        const char *src = dma_base[im] + ((dma_v(im) ? g != 0 : (lane & 8) != 0) ? second : first) + i * 512 + dma_lane[im];
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(dst), "v"(src) : "memory", "m0");
+      }
+    }
+  };
+  auto dma_piece = [&](int tile, int i, int im) {
+    if constexpr (BS != 16) {
+      dma_piece_bs(tile, i, im);
+    } else {
+      const int idx = (tile & 15) * 4 + dma_r;
+      const unsigned lo = __builtin_amdgcn_readlane((int)(uint32_t)tbl_off[im], idx);
+      const unsigned hi = __builtin_amdgcn_readlane((int)(uint32_t)(tbl_off[im] >> 32), idx);
+      // (an "s" operand is not made a scalar for the asm when the compiler holds the value in vector registers)
+      const uint64_t src_v = reinterpret_cast<uint64_t>(dma_base[im]) + (((uint64_t)hi << 32) | lo);
+      const char *src = reinterpret_cast<const char *>(
+          ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(src_v >> 32)) << 32) |
+          (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)src_v));
+      // the instruction's offset field moves both ends of the copy: the address in memory and the one in LDS
+      const unsigned dst = (unsigned)__builtin_amdgcn_readfirstlane(
+          (int)(lds0 + (unsigned)(((tile % NST) * STAGE_ELEMS + dma_v(im) * K_ELEMS + dma_r * BLK_ELEMS) * (int)sizeof(T))));
 #define HA_DMA_PIECE(OFF)                                                                          \
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:" #OFF \
                :                                                                                   \
                : "s"(dst), "v"(dma_lane[im]), "s"(src)                                                 \
                : "memory", "m0")
-    if (!DMA_PART || i < NDMA - 1 || dma_last_ok[im]) {
-      switch (i) {
-        case 0: HA_DMA_PIECE(0); break;
-        case 1: HA_DMA_PIECE(1024); break;
-        case 2: HA_DMA_PIECE(2048); break;
-        default: HA_DMA_PIECE(3072); break;
+      if (!DMA_PART || i < NDMA - 1 || dma_last_ok[im]) {
+        switch (i) {
+          case 0: HA_DMA_PIECE(0); break;
+          case 1: HA_DMA_PIECE(1024); break;
+          case 2: HA_DMA_PIECE(2048); break;
+          default: HA_DMA_PIECE(3072); break;
+        }
       }
-    }
 #undef HA_DMA_PIECE
+    }
+    constexpr int LAST = TILES_HELD - 1;  // of the tiles whose ids are held
     if (NST == 2 && i == NDMA - 1) {
       // (K's image is one tile ahead of V's: the ids that are asked for with the one are still there when the other turns to them)
-      if (im == 0 && (tile & 15) == 14) tbl_nxt = load_ids((tile >> 4) + 1);
-      if ((tile & 15) == 15) tbl_off[im] = id_to_offset(tbl_nxt, im);
+      if (im == 0 && (tile & LAST) == LAST - 1) tbl_nxt = load_ids(tile / TILES_HELD + 1);
+      if ((tile & LAST) == LAST) tbl_off[im] = id_to_offset(tbl_nxt, im);
     } else if (NST > 2 && i == NDMA - 1 && im == IMG - 1) {
-      if ((tile & 15) == 14) tbl_nxt = load_ids((tile >> 4) + 1);
-      if ((tile & 15) == 15) {
+      if ((tile & LAST) == LAST - 1) tbl_nxt = load_ids(tile / TILES_HELD + 1);
+      if ((tile & LAST) == LAST) {
 #pragma unroll
         for (int m = 0; m < IMG; m++) tbl_off[m] = id_to_offset(tbl_nxt, m);
       }

@@ -12,76 +12,18 @@
 
 #include "paged_decode.h"
 #include "prefill_parts.h"
-#include "prefill_w8.h"
+#include "prefill_window_params.h"
+#include "window_rows.h"
 
 namespace hipattn {
 
 namespace {
 
-struct PrefillWindow {
-  struct Params : PrefillParams {
-    int block_rows;             // rows of a row block
-    int n_parts, part_tiles;    // pieces of a row block's keys at most, and 64-key tiles in each
-    float *part_acc, *part_ml;  // of piece i of row r and head h, at (i * total_q + r) * Hq + h: d sums; maximum and sum
-  };
-  static constexpr bool value = false, parts = true, window = true;
-};
-
-// The merge of row blocks whose keys were dealt out, a workgroup per (row, kMergeHeads heads).
-template <typename T, int HD>
-__global__ __launch_bounds__(128) void window_merge_kernel(PrefillWindow::Params p) {
-  const int groups = (p.Hq + kMergeHeads - 1) / kMergeHeads, lane = threadIdx.x & 63;
-  const int r = blockIdx.x / groups, h0 = blockIdx.x % groups * kMergeHeads;
-  int b = -1;
-  for (int s0 = 0; s0 < p.batch && b < 0; s0 += 64) {
-    const unsigned long long past = __ballot(s0 + lane < p.batch && p.cu_q[min(s0 + lane, p.batch - 1) + 1] > r);
-    if (past != 0) b = s0 + __builtin_ctzll(past);
-  }
-  if (b < 0) return;
-  const int q_begin = p.cu_q[b], Lq = p.cu_q[b + 1] - q_begin, Lk = p.context_lens[b];
-  if (r < q_begin) return;
-  const int first_row = (r - q_begin) / p.block_rows * p.block_rows, last_row = min(first_row + p.block_rows, Lq) - 1;  // of the row's block
-  int tiles = (max(min(Lk, last_row + Lk - Lq + 1), 0) + BN - 1) / BN;
-  const int seen_from = max(first_row + Lk - Lq - p.win_left, 0);  // (the kernel's arithmetic)
-  tiles -= max(seen_from / BN - (min(p.sinks, seen_from) + BN - 1) / BN, 0);
-  if (tiles <= p.part_tiles) return;  // whole, and written
-  merge_parts<T, HD>(p, r, h0, min((tiles + p.part_tiles - 1) / p.part_tiles, p.n_parts));
-}
-
-template <typename T, int HDP, int MODE, int NW>
-void launch_window_nw(PrefillWindow::Params p, int hl, hipStream_t stream) {
-  static bool attr_set = false;  // benign race: setting twice is harmless
-  auto kernel = prefill_varlen_w8_kernel<T, HDP, MODE, PrefillWindow, NW>;
-  constexpr size_t lds_bytes = (size_t)w8_stages(HDP, NW) * 2 * BN * HDP * 2;
-  if (!attr_set) {
-    HA_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_bytes));
-    attr_set = true;
-  }
-  p.wg_heads_log2 = hl;
-  const int bm = p.block_rows = (NW * 32) >> hl;
-  p.n_qblocks = (p.max_q + bm - 1) / bm;
-  const int64_t n_wg = (int64_t)p.n_qblocks * p.batch * (p.Hq >> hl) * p.n_parts;
-  HA_CHECK(n_wg <= 0x7fffffff, "mha_varlen_fwd_paged_window: too many workgroups");
-  kernel<<<dim3((unsigned)n_wg), NW * 64, lds_bytes, stream>>>(p);
-  check_launch("mha_varlen_fwd_paged_window");
-  if (p.n_parts > 1) {
-    const int64_t merges = p.total_q * ((p.Hq + kMergeHeads - 1) / kMergeHeads);
-    HA_CHECK(merges <= 0x7fffffff, "mha_varlen_fwd_paged_window: too many rows");
-    switch (p.d) {
-      case 64: window_merge_kernel<T, 64><<<dim3((unsigned)merges), 128, 0, stream>>>(p); break;
-      case 80: window_merge_kernel<T, 80><<<dim3((unsigned)merges), 128, 0, stream>>>(p); break;
-      case 96: window_merge_kernel<T, 96><<<dim3((unsigned)merges), 128, 0, stream>>>(p); break;
-      case 112: window_merge_kernel<T, 112><<<dim3((unsigned)merges), 128, 0, stream>>>(p); break;
-      case 128: window_merge_kernel<T, 128><<<dim3((unsigned)merges), 128, 0, stream>>>(p); break;
-      default: fail("mha_varlen_fwd_paged_window: no merge for head size %d", p.d);
-    }
-    check_launch("mha_varlen_fwd_paged_window (merge)");
-  }
-}
+constexpr int kTileKeys = 64;
 
 // Tiles of the longest chain: what a row block of `rows` rows sees at most.
 int64_t most_tiles(const PrefillParams &p, int rows) {
-  return std::min<int64_t>(((int64_t)p.max_k + BN - 1) / BN, ((int64_t)p.sinks + BN - 1) / BN + ((int64_t)p.win_left + rows + BN - 1) / BN + 1);
+  return std::min<int64_t>(((int64_t)p.max_k + kTileKeys - 1) / kTileKeys, ((int64_t)p.sinks + kTileKeys - 1) / kTileKeys + ((int64_t)p.win_left + rows + kTileKeys - 1) / kTileKeys + 1);
 }
 
 // Workgroups of `waves` wavefronts with work to do, about.
@@ -107,70 +49,39 @@ bool eight_wavefronts_pay(const PrefillParams &p) {
 // x 4 new tokens to 2 x 4096, windows of 100 to 4096) the choice among 1, 2, 3, 4, 6, 10 and 16, which asks for a tenth before it cuts, is 0.7 % off the best on average.  us, whole / best:
 // 32 / 8 x 128, 1 x 16 over 4096 keys 102 / 25 (16 pieces), 1 x 300 106 / 47 (6), 4 x 64 over 2048 62 / 33 (4), 16 x 20 over 4096 104 / 63 (4);
 // 16 / 2 x 64, 1 x 45 over 256 17.5 / 11.1 (7); 32 / 8 x 128, 4 x 8 over 100 10.5 / 10.5 (1; in 2 13.7).
-int choose_parts(const PrefillParams &p) {
+// At most `most`; us: about what the launch takes then.
+int choose_parts(const PrefillParams &p, int most, double &us) {
   const int hl = prefill_heads_log2(p, 2);
   const int64_t tiles = most_tiles(p, 128 >> hl), wgs = busy_workgroups(p, 4, hl);
   const double tile = p.d > 96 ? 1.45 : (p.d > 64 ? 1.55 : 1.25), share = (p.d > 96 ? 0.6 : 0.4) / compute_units();
   const double piece = (double)p.total_q * p.Hq * (p.d + 2) * 2e-6;
-  double best = 0;
+  double best = 0, whole = 0;
   int parts = 1;
-  for (int n = 1; n <= kMostParts && n <= tiles; n++) {
+  for (int n = 1; n <= most && n <= tiles; n++) {
     const int64_t part_tiles = (tiles + n - 1) / n;
     if ((tiles + part_tiles - 1) / part_tiles != n) continue;
     const double t = (double)part_tiles * tile * std::max(1.0, share * (double)(wgs * n)) + (n > 1 ? 3.0 + n * piece : 0.0);
-    if (n == 1) {
-      best = 0.9 * t;
-    } else if (t < best) {
-      best = t;
-      parts = n;
+    if (n == 1 || t < 0.9 * whole) {
+      if (n == 1) whole = t;
+      if (n == 1 || t < best) {
+        best = t;
+        parts = n;
+      }
     }
   }
+  us = 1.4 * best + (p.d > 96 ? 7.7 : (p.d > 64 ? 8.5 : 4.5));
   return parts;
 }
 
-// A stream's buffer, allocated once; row blocks whose pieces do not fit go whole.
+// What the staged form takes: workgroups of 128 rows of one head, about 3.5 us a tile of a head size of 256 (us, 8 / 2 x 256: 1 x 8 over 1024 69, 1 x
+// 300 over 4096 268, 4 x 64 over 2048 156).
+double staged_us(const PrefillParams &p) {
+  const int64_t wgs = std::max<int64_t>(p.total_q / 128 + (p.batch + 1) / 2, 1) * p.Hq;
+  return 10 + (double)most_tiles(p, 128) * 3.5 * std::max(p.d, 128) / 256 * std::max(1.0, 0.6 * (double)wgs / compute_units());
+}
+
+// A stream's buffer, allocated once.
 constexpr size_t kWindowScratchBytes = (size_t)64 << 20;
-
-template <typename T, int HDP, int MODE>
-void launch_window(PrefillWindow::Params p, bool lse_or_f32, hipStream_t stream) {
-  const int force = tuning().prefill_kernel;
-  if (force == 1 || (force != 5 && eight_wavefronts_pay(p))) {
-    launch_window_nw<T, HDP, MODE, 8>(p, prefill_heads_log2(p, 3), stream);
-    return;
-  }
-  const int hl = prefill_heads_log2(p, 2);
-  // (whole where the merge has no form, or a switch asks for a kernel)
-  int parts = lse_or_f32 || force != 0 || (p.d != 64 && p.d != 80 && p.d != 96 && p.d != 112 && p.d != 128) || stream == hipStreamPerThread ? 1 : choose_parts(p);
-  const size_t rows = (size_t)p.total_q * p.Hq, piece_bytes = rows * (p.d + 2) * sizeof(float);
-  if ((size_t)parts * piece_bytes > kWindowScratchBytes) parts = (int)(kWindowScratchBytes / piece_bytes);
-  HeldWorkspace ws;
-  if (parts > 1) ws = try_library_workspace(WS_WINDOW_CHUNKS, kWindowScratchBytes, stream);
-  if (ws.ptr != nullptr) {
-    const int64_t tiles = most_tiles(p, 128 >> hl);
-    p.part_tiles = (int)((tiles + parts - 1) / parts);
-    p.n_parts = (int)((tiles + p.part_tiles - 1) / p.part_tiles);
-    p.part_acc = static_cast<float *>(ws.ptr);
-    p.part_ml = p.part_acc + p.n_parts * rows * p.d;
-  }
-  launch_window_nw<T, HDP, MODE, 4>(p, hl, stream);
-}
-
-template <typename T>
-void dispatch_window(const PrefillWindow::Params &p, bool lse_or_f32, hipStream_t stream) {
-  switch ((p.d + 31) / 32 * 32) {
-    case 32: launch_window<T, 32, W8_PAGED_DMA>(p, lse_or_f32, stream); break;
-#define HA_W8W(H)                                                     \
-  case H:                                                             \
-    if (p.d == H) launch_window<T, H, W8_PAGED_DMA>(p, lse_or_f32, stream);       \
-    else launch_window<T, H, W8_PAGED_DMA_PART>(p, lse_or_f32, stream);           \
-    break
-    HA_W8W(64);
-    HA_W8W(96);
-    HA_W8W(128);
-#undef HA_W8W
-    default: fail("mha_varlen_fwd_paged_window: head size %d not supported by this kernel", p.d);
-  }
-}
 
 void mha_varlen_fwd_paged_window_impl(const hipattn_tensor *q, const hipattn_tensor *key_cache, const hipattn_tensor *value_cache,
                                       const hipattn_tensor *block_tables, const hipattn_tensor *cu_q, const hipattn_tensor *context_lens,
@@ -179,7 +90,7 @@ void mha_varlen_fwd_paged_window_impl(const hipattn_tensor *q, const hipattn_ten
   const char *op = "mha_varlen_fwd_paged_window";
   HA_CHECK(window_left >= 0, "%s: window_size_left must not be negative here, got %d", op, window_left);
   HA_CHECK(sinks >= 0, "%s: sink_tokens must not be negative, got %d", op, sinks);
-  PrefillWindow::Params p;
+  WindowParams p;
   if (!paged_prefill_params(PagedPrefillCall{q, key_cache, value_cache, block_tables, cu_q, context_lens, max_q, max_k, scale, true, op}, out,
                             lse, p))
     return;
@@ -193,14 +104,53 @@ void mha_varlen_fwd_paged_window_impl(const hipattn_tensor *q, const hipattn_ten
   p.part_tiles = 1 << 24;
   p.part_acc = p.part_ml = nullptr;
   hipStream_t stream = resolve_stream(stream_arg);
+  const int force = tuning().prefill_kernel;
+  const bool lse_or_f32 = lse != nullptr || p.out_f32;  // (neither the merges nor the kernel of decode rows have them)
   // Block images go into LDS as they are where they fill most of their place there; else tiles are staged through registers.
-  if (!paged_prefill_copies_images(p) || p.d > 128 || (p.d < 64 && p.d != 32)) {
+  const bool images = p.vc_block % 8 == 0 && p.vc_head % 8 == 0 && tuning().paged_prefill_dma != 0 && p.d <= 128 && (p.d >= 64 || p.d == 32);
+  const bool eight = images && (force == 1 || (force == 0 && eight_wavefronts_pay(p)));
+  // What pieces need lies in a buffer of the stream's of fixed size; without it -- in a capture, for shapes beyond it, on hipStreamPerThread, one
+  // handle for a stream of each thread's own -- nothing is cut that has to be merged.
+  HeldWorkspace ws;
+  const size_t piece_bytes = (size_t)p.total_q * p.Hq * (p.d + 2) * sizeof(float);
+  int most = stream == hipStreamPerThread || lse_or_f32 || force != 0 || eight ? 1 : (int)std::min<size_t>(kWindowScratchBytes / piece_bytes, kMostParts);
+  for (;;) {
+    int parts = 1;
+    double us = images ? 0 : staged_us(p);
+    if (images && !eight) parts = choose_parts(p, p.d == 64 || p.d == 80 || p.d == 96 || p.d == 112 || p.d == 128 ? most : 1, us);
+    RowsPlan rows;
+    const bool as_rows = force == 0 && !eight && !lse_or_f32 && plan_window_rows(p, most, rows) && rows.us < us;
+    if (as_rows) parts = rows.num_parts;
+    if (parts > 1) {
+      ws = try_library_workspace(WS_WINDOW_CHUNKS, kWindowScratchBytes, stream);
+      if (ws.ptr == nullptr) {
+        most = 1;
+        continue;
+      }
+    }
+    if (as_rows) {
+      launch_window_rows(p, rows, q->dtype, ws.ptr, stream);
+      return;
+    }
+    if (parts > 1) {
+      const int64_t tiles = most_tiles(p, 128 >> prefill_heads_log2(p, 2));
+      p.part_tiles = (int)((tiles + parts - 1) / parts);
+      p.n_parts = (int)((tiles + p.part_tiles - 1) / p.part_tiles);
+      p.part_acc = static_cast<float *>(ws.ptr);
+      p.part_ml = p.part_acc + (size_t)p.n_parts * p.total_q * p.Hq * p.d;
+    }
+    break;
+  }
+  if (!images) {
     launch_staged_window(p, q->dtype, stream);
     return;
   }
-  const bool lse_or_f32 = lse != nullptr || p.out_f32;  // (the merge has neither)
-  if (q->dtype == HIPATTN_F16) dispatch_window<half_t>(p, lse_or_f32, stream);
-  else dispatch_window<bf16_t>(p, lse_or_f32, stream);
+  const int waves = eight ? 8 : 4;
+  switch (p.block_log2) {
+    case 3: launch_window_images_8(p, waves, q->dtype, stream); break;
+    case 5: launch_window_images_32(p, waves, q->dtype, stream); break;
+    default: launch_window_images_16(p, waves, q->dtype, stream); break;
+  }
 }
 
 }  // namespace

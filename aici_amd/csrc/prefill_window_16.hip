@@ -1,0 +1,10 @@
+// Windowed prefill over caches of 16-token blocks.
+#include "prefill_window.h"
+
+namespace hipattn {
+
+void launch_window_images_16(const WindowParams &p, int waves, int dtype, hipStream_t stream) {
+  launch_window_images<16>(p, waves, dtype, stream);
+}
+
+}  // namespace hipattn

@@ -37,6 +37,7 @@ struct StepDecode {
     float *part_acc, *part_ml;  // of piece i of row r and head h, at (i * total_q + r) * Hq + h: d sums; maximum and sum
   };
   static constexpr bool value = true, parts = true, window = false;
+  static constexpr int block = kBlockSize;
   static __device__ __forceinline__ void decode(const Params &p, int wg, unsigned char *lds) {
     decode_flat<T, HD, kBlockSize>(p.decode, wg, *reinterpret_cast<FlatLds<HD> *>(lds));
   }
@@ -52,13 +53,9 @@ __global__ __launch_bounds__(128) void step_merge_kernel(typename StepDecode<T, 
     return;
   }
   id -= decode_merges;
-  const int groups = (p.Hq + kMergeHeads - 1) / kMergeHeads, lane = threadIdx.x & 63;
+  const int groups = (p.Hq + kMergeHeads - 1) / kMergeHeads;
   const int r = id / groups, h0 = id % groups * kMergeHeads;
-  int b = -1;
-  for (int s0 = 0; s0 < p.batch && b < 0; s0 += 64) {
-    const unsigned long long past = __ballot(s0 + lane < p.batch && p.cu_q[min(s0 + lane, p.batch - 1) + 1] > r);
-    if (past != 0) b = s0 + __builtin_ctzll(past);
-  }
+  const int b = sequence_of_row(p.cu_q, p.batch, r);
   if (b < 0) return;
   const int q_begin = p.cu_q[b], Lq = p.cu_q[b + 1] - q_begin, Lk = p.context_lens[b], BM = 128 >> p.wg_heads_log2;
   const int last_row = min((r - q_begin) / BM * BM + BM, Lq) - 1;  // of the row's block

@@ -156,18 +156,24 @@ def test_chunks(device, tuning, heads, dtype, bs):
     for n, (window, sinks) in enumerate([(0, 0), (30, 4), (63, 64), (100, 33), (255, 100), (2000, 5)]):
         c = case(200 + n, [a for a, _ in SEQS], [b for _, b in SEQS], heads, dtype, window, sinks, bs)
         expect = want(c)
-        for kernel in ((5, 1) if bs == 16 and 32 <= heads[2] <= 128 else (0,)):
+        # block images in workgroups of four and eight wavefronts, tiles through registers, and what the library picks: for most of these
+        # sizes the kernel of decode rows
+        for kernel, images in ((5, -1), (1, -1), (5, 0), (0, -1)) if heads[2] in (32, 64, 80, 96, 112, 128) else ((5, -1), (0, -1)):
             tuning("prefill_kernel", kernel)
+            tuning("paged_prefill_dma", images)
             check(chunk(c, device), c, expect)
 
 
 @pytest.mark.parametrize("heads", [(8, 2, 64), (4, 2, 96), (8, 2, 128)])
-def test_long_chunks(device, heads):
+def test_long_chunks(device, tuning, heads):
     """Windows of many tiles with sinks of more than one, and the staged route."""
     for window, sinks, lens_q, ctx in ((700, 70, [100, 300], [2100, 1300]), (1023, 4, [40], [1800]), (64, 200, [257], [900])):
-        c = case(31, lens_q, ctx, heads, torch.bfloat16, window, sinks)
-        expect = want(c)
-        check(chunk(c, device), c, expect)
+        for bs in (16, 8, 32):
+            c = case(31, lens_q, ctx, heads, torch.bfloat16, window, sinks, bs)
+            expect = want(c)
+            for kernel in (0, 5, 1):
+                tuning("prefill_kernel", kernel)
+                check(chunk(c, device), c, expect)
 
 
 @pytest.mark.parametrize("heads", [(8, 2, 64), (4, 4, 80), (6, 1, 96), (12, 4, 112), (8, 2, 128)])
@@ -180,6 +186,15 @@ def test_chunks_whose_keys_are_dealt_out(device, heads, dtype):
         expect = want(c)
         check(chunk(c, device), c, expect)
         check(chunk(c, device, out_dtype=torch.float32), c, expect, rounded=False)
+
+
+@pytest.mark.parametrize("heads", [(6, 2, 64), (10, 2, 80), (14, 2, 128), (40, 2, 64), (8, 8, 256)])
+def test_few_rows_of_odd_groups(device, heads):
+    """Columns that no row of heads fills, more heads in a group than columns, batches with empty sequences; in one part and in several."""
+    for n, (window, sinks, lens_q, ctx) in enumerate([(2000, 40, [3, 7], [2600, 900]), (50, 3, [0, 1, 12, 0, 2], [7, 1, 300, 0, 2])]):
+        for bs in (16, 8, 32):
+            c = case(400 + n, lens_q, ctx, heads, torch.float16, window, sinks, bs)
+            check(chunk(c, device), c, want(c))
 
 
 def test_chunk_outputs_in_fp32_lse_and_rows_behind_the_last(device):
