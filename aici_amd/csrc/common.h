@@ -113,6 +113,16 @@ inline bool is_contiguous(const hipattn_tensor *t) {
   return true;
 }
 
+// Whether no byte between the first and the last element of one lies there of the other (strides not negative).
+inline bool apart(const hipattn_tensor *a, const hipattn_tensor *b) {
+  auto end = [](const hipattn_tensor *t) {
+    int64_t last = 0;
+    for (int i = 0; i < t->ndim; i++) last += (t->sizes[i] - 1) * t->strides[i];
+    return static_cast<const char *>(t->data) + (last + 1) * dtype_size(t->dtype);
+  };
+  return numel(a) == 0 || numel(b) == 0 || end(a) <= static_cast<const char *>(b->data) || end(b) <= static_cast<const char *>(a->data);
+}
+
 inline void check_contiguous(const hipattn_tensor *t, const char *name) {
   HA_CHECK(numel(t) == 0 || is_contiguous(t), "%s must be contiguous", name);
 }

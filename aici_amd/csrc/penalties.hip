@@ -267,6 +267,8 @@ void penalize_logits_impl(hipattn_tensor *out, const hipattn_tensor *logits, con
   HA_CHECK(S <= 0x7ffffff0, "penalize_logits: too many sequences");
   check_data(logits, "logits");
   check_data(out, "out");
+  HA_CHECK(apart(out, logits) || (out->data == logits->data && out->dtype == logits->dtype && (S == 1 || out->strides[0] == logits->strides[0])),
+           "penalize_logits: out must be logits or lie apart from them");
   PenaltyParams p;
   memset(&p, 0, sizeof p);
   p.logits = logits->data;

@@ -113,7 +113,7 @@ void mha_varlen_fwd_paged_window_impl(const hipattn_tensor *q, const hipattn_ten
   // handle for a stream of each thread's own -- nothing is cut that has to be merged.
   HeldWorkspace ws;
   const size_t piece_bytes = (size_t)p.total_q * p.Hq * (p.d + 2) * sizeof(float);
-  int most = stream == hipStreamPerThread || lse_or_f32 || force != 0 || eight ? 1 : (int)std::min<size_t>(kWindowScratchBytes / piece_bytes, kMostParts);
+  int most = stream == hipStreamPerThread || lse_or_f32 || force != 0 || eight ? 1 : (int)std::max<size_t>(std::min<size_t>(kWindowScratchBytes / piece_bytes, kMostParts), 1);
   for (;;) {
     int parts = 1;
     double us = images ? 0 : staged_us(p);

@@ -367,6 +367,11 @@ void step_blocks_impl(const hipattn_tensor *new_lens, const hipattn_tensor *stat
   check_i32(totals, "totals", 1, 4);
   check_i32(moves, "workspace", 1, 4 * (R + 1));
   HA_CHECK((reinterpret_cast<uintptr_t>(moves->data) & 15) == 0, "step_blocks: workspace must be 16-byte aligned");
+  HA_CHECK((state->data == state_out->data || apart(state, state_out)) && (ends->data == ends_out->data || apart(ends, ends_out)),
+           "step_blocks: state_out and ring_ends_out must be state and ring_ends or lie apart from them");
+  for (const hipattn_tensor *in : {new_lens, state, (const hipattn_tensor *)tables, (const hipattn_tensor *)ring, ends})
+    for (const hipattn_tensor *o : {served, context_lens, cu, logit_idxs, positions, slots, totals, moves})
+      HA_CHECK(apart(in, o), "step_blocks: an output lies over an input");
   StepParams p;
   p.new_lens = static_cast<const int32_t *>(new_lens->data);
   p.state = static_cast<const int2 *>(state->data);
@@ -398,11 +403,6 @@ void step_blocks_impl(const hipattn_tensor *new_lens, const hipattn_tensor *stat
     check_launch("step_blocks");
     return;
   }
-  auto apart = [](const hipattn_tensor *a, const hipattn_tensor *b) {
-    const char *x = static_cast<const char *>(a->data), *y = static_cast<const char *>(b->data);
-    const int64_t n = numel(a) * dtype_size(a->dtype);
-    return x + n <= y || y + n <= x;
-  };
   if (apart(state, state_out) && apart(ends, ends_out)) {
     const int64_t wgs = (T + 511) / 512;
     const dim3 grid((unsigned)(wgs < 64 ? 64 : (wgs > 256 ? 256 : wgs)));

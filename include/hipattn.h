@@ -116,7 +116,10 @@ char *hipattn_mha_varlen_fwd_paged(const hipattn_tensor *q, const hipattn_tensor
  * and read rows of k / v).  window_size_left >= 0, sink_tokens >= 0; everything else as there, any of its types, head and block sizes.
  * Keys that no new token of a sequence sees may be gone: table columns that hold only such keys may name any block or none (a negative
  * or large number), and their blocks may hold anything.  Values of a key that some of a sequence's new tokens see are taken to be finite,
- * also where others do not see it.  A row that sees nothing (its position is negative) is zero, its LSE +inf. */
+ * also where others do not see it.  A row that sees nothing (its position is negative) is zero, its LSE +inf.
+ * Where few workgroups would leave compute units idle a row's keys are dealt out to several, by way of 64 MiB of scratch memory that are
+ * allocated once per stream; not under capture, on hipStreamPerThread, without that memory, with an f32 out or an LSE, so that last bits
+ * may differ there. */
 char *hipattn_mha_varlen_fwd_paged_window(const hipattn_tensor *q, const hipattn_tensor *key_cache,
                                           const hipattn_tensor *value_cache, const hipattn_tensor *block_tables,
                                           const hipattn_tensor *cu_seqlens_q, const hipattn_tensor *context_lens,
@@ -876,7 +879,8 @@ char *hipattn_block_space_step_generation(
  * Outputs: served int32 [R], the tokens given or the codes above; context_lens int32 [R]: keys of a request that is served, else 0;
  * seqlens_q int32 [R + 1]: sums of the tokens given; logit_idxs int32 [R]: a served request's last row, else 0; positions int64 [T] and
  * slot_mapping int32 [T], of rows without a token 0 and -1; totals int32 [4]: tokens given, requests not served (-1 and -2), blocks
- * free afterwards, blocks taken.  workspace int32 [4 (R + 1)], 16-byte aligned. */
+ * free afterwards, blocks taken.  workspace int32 [4 (R + 1)], 16-byte aligned.  No output but the
+ * two named lies over an input. */
 char *hipattn_step_blocks(const hipattn_tensor *new_lens, const hipattn_tensor *state,
                           hipattn_tensor *block_tables, hipattn_tensor *free_ring,
                           const hipattn_tensor *ring_ends, int block_size, int rows_per_request,

@@ -69,6 +69,14 @@ def test_penalties(device, dtype, S, V, lens):
         check(x, c, expect)
 
 
+def test_a_short_mask_bars_what_lies_behind_it(device):
+    c = make(8, 2, 3000, torch.bfloat16, [40, 300], False, True)
+    a, short = args(c, device), 1000
+    a["mask"] = a["mask"][:, :short // 8].contiguous()
+    c["allowed"][:, short:] = False
+    check(K.penalize_logits(c["logits"].to(device), **a), c, want(c))
+
+
 def test_untouched_logits_keep_their_bits(device):
     """No penalty, nothing said, nothing barred: the logits as they are, infinities and NaN among them."""
     for dtype in (torch.bfloat16, torch.float16, torch.float32):

@@ -5,6 +5,7 @@ window passes go from one request to another.  Every step's logits against a 64-
 Tolerance: 2 layers of 10 tensors that are rounded to fp16 and 3 more, half a step each (2^-11 of their norm), no map between them taken to stretch
 a relative error more than twofold: 23 x 2 x 2^-11 = 0.0225 of the logits' norm."""
 import math
+from dataclasses import replace
 
 import pytest
 import torch
@@ -13,17 +14,19 @@ from aici_amd import llama, paged
 from oracle import steps
 
 pytestmark = pytest.mark.gpu
-CFG = llama.LlamaConfig(512, 768, 1000, 2, 8, 2, 1e-5, 512, 10000.0, torch.float16, sliding_window=41, attention_sinks=5)
+CFG = llama.LlamaConfig(512, 768, 1000, 2, 8, 2, 1e-5, 512, 10000.0, torch.float16)
 TOLERANCE = 23 * 2 * 2.0 ** -11
 
 
-def reference(weights, table, tokens, device):
+def reference(weights, table, tokens, device, window, sinks):
     """Logits of the last token of a sequence, 64 bits."""
     w = {k: v.to(device).double() for k, v in weights.items()}
     n, d, hq, hkv = len(tokens), CFG.head_dim, CFG.num_attention_heads, CFG.num_key_value_heads
     pos = torch.arange(n, device=device)
     cos, sin = (t[:, None, :] for t in table[:n].double().chunk(2, 1))
-    seen = (pos[None, :] <= pos[:, None]) & ((pos[None, :] > pos[:, None] - CFG.sliding_window) | (pos[None, :] < CFG.attention_sinks))
+    seen = pos[None, :] <= pos[:, None]
+    if window is not None:
+        seen &= (pos[None, :] > pos[:, None] - window) | (pos[None, :] < sinks)
 
     def norm(x, scale):
         return x * torch.rsqrt((x * x).mean(1, keepdim=True) + CFG.rms_norm_eps) * scale
@@ -49,13 +52,15 @@ def reference(weights, table, tokens, device):
     return norm(x[-1:], w["model.norm"])[0] @ w["lm_head"].t().contiguous()
 
 
-def test_generation_over_a_window(device):
+@pytest.mark.parametrize("window,sinks,blocks", [(41, 5, 21), (None, 0, 40)])
+def test_generation(device, window, sinks, blocks):
+    """With a window and sinks in a small pool, and over whole contexts."""
     R, L, V = 4, 256, CFG.vocab_size
     weights = llama.random_weights(CFG, 3, std=0.05)
-    model = llama.Llama(CFG, weights, device)
+    model = llama.Llama(replace(CFG, sliding_window=window, attention_sinks=sinks), weights, device)
     # 21 blocks: four windows and their sinks hold five each; without letting go the sequences would need more
-    pool = paged.DeviceBlocks(16, 21, R, L, device, CFG.sliding_window - 1, CFG.attention_sinks)
-    caches = [paged.alloc_gpu_cache_layer(21, CFG.num_key_value_heads, CFG.head_dim, 16, CFG.dtype, device) for _ in range(2)]
+    pool = paged.DeviceBlocks(16, blocks, R, L, device, -1 if window is None else window - 1, sinks)
+    caches = [paged.alloc_gpu_cache_layer(blocks, CFG.num_key_value_heads, CFG.head_dim, 16, CFG.dtype, device) for _ in range(2)]
     for kc, vc in caches:
         kc.fill_(float("nan"))
         vc.fill_(float("nan"))
@@ -79,7 +84,7 @@ def test_generation_over_a_window(device):
 
     def check(logits, before, rows):
         for r in rows:
-            ref = reference(weights, model.rotary.cos_sin, said[r], device)
+            ref = reference(weights, model.rotary.cos_sin, said[r], device, window, sinks)
             err = float((logits[r].double() - ref).norm() / ref.norm())
             assert err <= TOLERANCE, (r, len(said[r]), err)
             knob = [float(knobs[k][0]) for k in ("repetition", "frequency", "presence")]
@@ -143,5 +148,5 @@ def test_generation_over_a_window(device):
             for r in rows:
                 said[r].append(int(tokens[r]))
         new.fill_(1)
-    assert int(pool.ring_ends[0]) > 21  # blocks have been handed out more than once
+    assert window is None or int(pool.ring_ends[0]) > blocks  # blocks have been handed out more than once
     assert [len(s) for s in said] == [37 + 72, 5 + 71, 45 + 41, 20 + 72]

@@ -154,6 +154,8 @@ def _penalty_args(**over):
     (dict(bias=_t(3, 99, dtype=_lib.F32)), "bias rows have 99"), (dict(bias=_t(2, 100, dtype=_lib.F32)), "2 bias or mask rows"),
     (dict(mask=_t(3, 16, dtype=_lib.I32)), "mask must be u8"), (dict(mask=_t(1, 16, dtype=_lib.U8), rows=_t(2, dtype=_lib.I32)), "bias_rows"),
     (dict(mask=_t(0, 16, dtype=_lib.U8), rows=_t(3, dtype=_lib.I32)), "0 bias or mask rows"),
+    (dict(logits=_t(3, 100, data=65536), out=_t(3, 100, data=65536 + 32)), "must be logits or lie apart"),
+    (dict(logits=_t(3, 100, data=65536), out=_t(3, 100, dtype=_lib.F32, data=65536)), "must be logits or lie apart"),
 ])
 def test_penalize_logits_refuses(over, message):
     with pytest.raises(_lib.HipAttnError, match=message):
@@ -165,6 +167,9 @@ def _step_args(**over):
     a = dict(new=_t(5, **i), state=_t(5, 2, **i), tables=_t(5, 8, **i), ring=_t(30, **i), ends=_t(2, **w), bs=16, per=0, window=-1, sinks=0,
              state_out=_t(5, 2, **i), ends_out=_t(2, **w), served=_t(5, **i), ctx=_t(5, **i), cu=_t(6, **i), last=_t(5, **i), pos=_t(9, **w),
              slots=_t(9, **i), totals=_t(4, **i), work=_t(24, **i))
+    for n, t in enumerate(a.values()):  # each in a KB of its own
+        if isinstance(t, _lib.Tensor):
+            t.data = 1024 * (n + 1)
     a.update(over)
     return [*a.values(), None]
 
@@ -176,7 +181,9 @@ def _step_args(**over):
     (dict(ring=_t(0, dtype=_lib.I32)), "there are none"), (dict(ring=_t(1 << 28, dtype=_lib.I32)), "do not fit 32 bits"),
     (dict(ends=_t(2, dtype=_lib.I32)), "must be int64"), (dict(cu=_t(5, dtype=_lib.I32)), "seqlens_q has the wrong shape"),
     (dict(slots=_t(8, dtype=_lib.I32)), "slot_mapping has the wrong shape"), (dict(pos=_t(0, dtype=_lib.I64)), "0 rows"),
-    (dict(work=_t(20, dtype=_lib.I32)), "workspace has the wrong shape"), (dict(state_out=_t(5, 2, dtype=_lib.I32, data=260)), "8-byte aligned"),
+    (dict(work=_t(20, dtype=_lib.I32)), "workspace has the wrong shape"),
+    (dict(state_out=_t(5, 2, dtype=_lib.I32, data=2048 + 16)), "must be state and ring_ends or lie apart"),
+    (dict(served=_t(5, dtype=_lib.I32, data=1024 + 8)), "an output lies over an input"), (dict(state_out=_t(5, 2, dtype=_lib.I32, data=260)), "8-byte aligned"),
 ])
 def test_step_blocks_refuses(over, message):
     with pytest.raises(_lib.HipAttnError, match=message):
