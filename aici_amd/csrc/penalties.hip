@@ -269,6 +269,8 @@ void penalize_logits_impl(hipattn_tensor *out, const hipattn_tensor *logits, con
   check_data(out, "out");
   HA_CHECK(apart(out, logits) || (out->data == logits->data && out->dtype == logits->dtype && (S == 1 || out->strides[0] == logits->strides[0])),
            "penalize_logits: out must be logits or lie apart from them");
+  for (const hipattn_tensor *in : {history, offsets, prompt_lens, repetition, frequency, presence, bias, mask, rows})
+    HA_CHECK(in == nullptr || apart(out, in), "penalize_logits: out lies over an input other than logits");
   PenaltyParams p;
   memset(&p, 0, sizeof p);
   p.logits = logits->data;

@@ -411,35 +411,32 @@ __global__ __launch_bounds__(NW * 64, STEP::value ? 2 : w8_wavefronts(HDP, NW)) 
     }
   };
   auto dma_piece = [&](int tile, int i, int im) {
-    if constexpr (BS != 16) {
-      dma_piece_bs(tile, i, im);
-    } else {
-      const int idx = (tile & 15) * 4 + dma_r;
-      const unsigned lo = __builtin_amdgcn_readlane((int)(uint32_t)tbl_off[im], idx);
-      const unsigned hi = __builtin_amdgcn_readlane((int)(uint32_t)(tbl_off[im] >> 32), idx);
-      // (an "s" operand is not made a scalar for the asm when the compiler holds the value in vector registers)
-      const uint64_t src_v = reinterpret_cast<uint64_t>(dma_base[im]) + (((uint64_t)hi << 32) | lo);
-      const char *src = reinterpret_cast<const char *>(
-          ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(src_v >> 32)) << 32) |
-          (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)src_v));
-      // the instruction's offset field moves both ends of the copy: the address in memory and the one in LDS
-      const unsigned dst = (unsigned)__builtin_amdgcn_readfirstlane(
-          (int)(lds0 + (unsigned)(((tile % NST) * STAGE_ELEMS + dma_v(im) * K_ELEMS + dma_r * BLK_ELEMS) * (int)sizeof(T))));
+    if constexpr (BS != 16) dma_piece_bs(tile, i, im);
+    const int idx = (tile & 15) * 4 + dma_r;
+    const unsigned lo = __builtin_amdgcn_readlane((int)(uint32_t)tbl_off[im], idx);
+    const unsigned hi = __builtin_amdgcn_readlane((int)(uint32_t)(tbl_off[im] >> 32), idx);
+    // (an "s" operand is not made a scalar for the asm when the compiler holds the value in vector registers)
+    const uint64_t src_v = reinterpret_cast<uint64_t>(dma_base[im]) + (((uint64_t)hi << 32) | lo);
+    const char *src = reinterpret_cast<const char *>(
+        ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(src_v >> 32)) << 32) |
+        (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)src_v));
+    // the instruction's offset field moves both ends of the copy: the address in memory and the one in LDS
+    const unsigned dst = (unsigned)__builtin_amdgcn_readfirstlane(
+        (int)(lds0 + (unsigned)(((tile % NST) * STAGE_ELEMS + dma_v(im) * K_ELEMS + dma_r * BLK_ELEMS) * (int)sizeof(T))));
 #define HA_DMA_PIECE(OFF)                                                                          \
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:" #OFF \
                :                                                                                   \
                : "s"(dst), "v"(dma_lane[im]), "s"(src)                                                 \
                : "memory", "m0")
-      if (!DMA_PART || i < NDMA - 1 || dma_last_ok[im]) {
-        switch (i) {
-          case 0: HA_DMA_PIECE(0); break;
-          case 1: HA_DMA_PIECE(1024); break;
-          case 2: HA_DMA_PIECE(2048); break;
-          default: HA_DMA_PIECE(3072); break;
-        }
+    if (BS == 16 && (!DMA_PART || i < NDMA - 1 || dma_last_ok[im])) {
+      switch (i) {
+        case 0: HA_DMA_PIECE(0); break;
+        case 1: HA_DMA_PIECE(1024); break;
+        case 2: HA_DMA_PIECE(2048); break;
+        default: HA_DMA_PIECE(3072); break;
       }
-#undef HA_DMA_PIECE
     }
+#undef HA_DMA_PIECE
     constexpr int LAST = TILES_HELD - 1;  // of the tiles whose ids are held
     if (NST == 2 && i == NDMA - 1) {
       // (K's image is one tile ahead of V's: the ids that are asked for with the one are still there when the other turns to them)

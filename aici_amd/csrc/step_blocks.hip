@@ -369,9 +369,12 @@ void step_blocks_impl(const hipattn_tensor *new_lens, const hipattn_tensor *stat
   HA_CHECK((reinterpret_cast<uintptr_t>(moves->data) & 15) == 0, "step_blocks: workspace must be 16-byte aligned");
   HA_CHECK((state->data == state_out->data || apart(state, state_out)) && (ends->data == ends_out->data || apart(ends, ends_out)),
            "step_blocks: state_out and ring_ends_out must be state and ring_ends or lie apart from them");
-  for (const hipattn_tensor *in : {new_lens, state, (const hipattn_tensor *)tables, (const hipattn_tensor *)ring, ends})
+  for (const hipattn_tensor *in : {new_lens, state, (const hipattn_tensor *)tables, (const hipattn_tensor *)ring, ends}) {
     for (const hipattn_tensor *o : {served, context_lens, cu, logit_idxs, positions, slots, totals, moves})
       HA_CHECK(apart(in, o), "step_blocks: an output lies over an input");
+    HA_CHECK((in == state || apart(in, state_out)) && (in == ends || apart(in, ends_out)),
+             "step_blocks: state_out or ring_ends_out lies over another input");
+  }
   StepParams p;
   p.new_lens = static_cast<const int32_t *>(new_lens->data);
   p.state = static_cast<const int2 *>(state->data);

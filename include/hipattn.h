@@ -114,6 +114,7 @@ char *hipattn_mha_varlen_fwd_paged(const hipattn_tensor *q, const hipattn_tensor
  * iff j <= p and (j >= p - window_size_left or j < sink_tokens) -- window_size_left + 1 tokens with its own, as the window of
  * hipattn_mha_varlen_fwd counts them, and the first sink_tokens of the sequence.  No counterpart in tch-cuda (its windows have no sinks
  * and read rows of k / v).  window_size_left >= 0, sink_tokens >= 0; everything else as there, any of its types, head and block sizes.
+ * max_seqlen_q and max_seqlen_k bound every sequence's new tokens and keys: rows and keys beyond them may be left out.
  * Keys that no new token of a sequence sees may be gone: table columns that hold only such keys may name any block or none (a negative
  * or large number), and their blocks may hold anything.  Values of a key that some of a sequence's new tokens see are taken to be finite,
  * also where others do not see it.  A row that sees nothing (its position is negative) is zero, its LSE +inf.
@@ -479,7 +480,8 @@ char *hipattn_bias_argmax(const hipattn_tensor *logits,
  * history int32 [N]: the tokens of all sequences one after the other, sequence s those from history_offsets[s] (int64 or int32 [S + 1]) on,
  * the first prompt_lens[s] (int32 [S] or NULL: none) of them its prompt; tokens outside the vocabulary count for nothing.  repetition,
  * frequency, presence f32 [S], NULL: 1, 0, 0.  bias f32 rows, mask packed allow-bits and bias_rows as for hipattn_bias_argmax, but any of
- * them, both or none.  out [S, V] in the type of logits or f32, rounded once from fp32; it may be logits itself (same type and strides). */
+ * them, both or none.  out [S, V] in the type of logits or f32, rounded once from fp32; it may be logits itself (same type and strides)
+ * and lies over no other input. */
 char *hipattn_penalize_logits(hipattn_tensor *out, const hipattn_tensor *logits, const hipattn_tensor *history,
                               const hipattn_tensor *history_offsets, const hipattn_tensor *prompt_lens,
                               const hipattn_tensor *repetition, const hipattn_tensor *frequency,

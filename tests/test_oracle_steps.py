@@ -156,6 +156,10 @@ def _penalty_args(**over):
     (dict(mask=_t(0, 16, dtype=_lib.U8), rows=_t(3, dtype=_lib.I32)), "0 bias or mask rows"),
     (dict(logits=_t(3, 100, data=65536), out=_t(3, 100, data=65536 + 32)), "must be logits or lie apart"),
     (dict(logits=_t(3, 100, data=65536), out=_t(3, 100, dtype=_lib.F32, data=65536)), "must be logits or lie apart"),
+    (dict(logits=_t(3, 100, data=65536), out=_t(3, 100, dtype=_lib.F32, data=1 << 20), bias=_t(3, 100, dtype=_lib.F32, data=1 << 20)),
+     "over an input other than logits"),
+    (dict(logits=_t(3, 100, data=65536), out=_t(3, 100, data=1 << 20), history=_t(50, dtype=_lib.I32, data=(1 << 20) + 400)),
+     "over an input other than logits"),
 ])
 def test_penalize_logits_refuses(over, message):
     with pytest.raises(_lib.HipAttnError, match=message):
@@ -183,6 +187,7 @@ def _step_args(**over):
     (dict(slots=_t(8, dtype=_lib.I32)), "slot_mapping has the wrong shape"), (dict(pos=_t(0, dtype=_lib.I64)), "0 rows"),
     (dict(work=_t(20, dtype=_lib.I32)), "workspace has the wrong shape"),
     (dict(state_out=_t(5, 2, dtype=_lib.I32, data=2048 + 16)), "must be state and ring_ends or lie apart"),
+    (dict(state_out=_t(5, 2, dtype=_lib.I32, data=1024)), "over another input"), (dict(ends_out=_t(2, dtype=_lib.I64, data=2048)), "over another input"),
     (dict(served=_t(5, dtype=_lib.I32, data=1024 + 8)), "an output lies over an input"), (dict(state_out=_t(5, 2, dtype=_lib.I32, data=260)), "8-byte aligned"),
 ])
 def test_step_blocks_refuses(over, message):
