@@ -10,6 +10,10 @@
 // window (SeenKeys); columns of the gap are not read, so that their blocks may have gone back to the pool.  A launch is planned as one
 // over contexts of that many tokens (seen_tokens).  The pair at either end of the gap is masked in its scores and its values are cleared:
 // a NaN there meets a probability of zero otherwise.
+//
+// Measured, 128 sequences of up to 16k tokens, 32 / 8 x 128 bf16, a window of 4096: 314 us, 1.99 GB at 6.3 TB/s (a read kernel with the same hint
+// gets 6.5), 6.6 of them the merge.  With few keys it is latency: 48 sequences, 39.7 MB, 11.8 us in one launch (lengths, table, keys one
+// after the other; 8.3 at a copy's rate); one sequence that sees 1028 keys 8.1 us, 5.7 + 3.1 of merge by the trace, whatever the number of partitions.
 #include <algorithm>
 
 #include "paged_decode_parts.h"
