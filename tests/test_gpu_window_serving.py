@@ -108,6 +108,7 @@ def test_generation(device, window, sinks, blocks):
         ids = torch.zeros((150,), dtype=torch.int32, device=device)
         ids[:len(flat)] = torch.tensor(flat, dtype=torch.int32)
         logits = model.forward(pool.batch_info(step, ids, max_new=max(lens)), caches, fused=True)
+        assert torch.equal(logits, model.forward(pool.batch_info(step, ids, max_new=max(lens)), caches))
         assert step.served.tolist() == [max(n, 0) for n in lens]
         finish(logits, step.context_lens)
         check(logits, None, [r for r, n in enumerate(lens) if n > 0])
