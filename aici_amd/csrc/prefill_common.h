@@ -47,6 +47,7 @@ struct PrefillParams {
   // query rows of each (wavefront w: head w % heads, row group w / heads).
   int wg_heads_log2;
   int sinks;  // windows with sinks: the first keys of a sequence that stay visible (kernels with STEP::window or SINKS)
+  int row_blocks;  // the same kernels: 0, or the row blocks of the grid, one sequence's behind the other's (row_block_of)
 };
 
 template <typename T>
@@ -63,6 +64,45 @@ struct Mfma32<bf16_t> {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
 };
+
+// A row block of a launch over sequences of very different lengths.
+struct RowBlock {
+  int seq, block, begin, rows;  // of the sequence: its first row and how many it has; block < 0: none
+};
+
+// The id-th block of `size` rows, at most `most` of a sequence, where sequences' blocks lie one behind the other, a sequence's last one first; by
+// whole wavefronts.  A grid of as many blocks as the longest sequence has for each of them is mostly workgroups that end at once: with a
+// window of 1000 and sinks, 63 sequences of 20 new tokens beside one of 4096, 32 / 8 x 128 291 us that way, 150 so, 16 / 2 x 64 147 and 49; 100 of one
+// token beside one of 1000, 8 / 2 x 256 261 and 107; 8 of 65 to 1001, 16 / 2 x 64 48 to 49 and 41 to 49, whichever comes first.
+__device__ __forceinline__ RowBlock row_block_of(const int32_t *cu_q, int batch, int size, int most, int id) {
+  const int lane = threadIdx.x & 63;
+  for (int s0 = 0; s0 < batch; s0 += 64) {
+    const int s = s0 + lane;
+    int begin = 0, rows = 0;
+    if (s < batch) {
+      begin = cu_q[s];
+      rows = max(cu_q[s + 1] - begin, 0);
+    }
+    int upto = min((rows + size - 1) / size, most);
+    for (int o = 1; o < 64 && o < batch; o <<= 1) {
+      const int t = __shfl_up(upto, o, 64);
+      if (lane >= o) upto += t;
+    }
+    const unsigned long long past = __ballot(upto > id);
+    if (past != 0) {
+      const int at = __builtin_ctzll(past);
+      return RowBlock{s0 + at, (int)__builtin_amdgcn_readlane(upto, at) - 1 - id, (int)__builtin_amdgcn_readlane(begin, at),
+                      (int)__builtin_amdgcn_readlane(rows, at)};
+    }
+    id -= __builtin_amdgcn_readlane(upto, 63);
+  }
+  return RowBlock{0, -1, 0, 0};
+}
+// Blocks of `size` rows that sequences of `rows` rows together, each of at most `most` blocks, can have; 0: as many as a grid of `most` for each.
+inline int64_t row_blocks_of(int64_t rows, int batch, int size, int64_t most) {
+  const int64_t n = rows / size + batch;
+  return n < batch * most ? n : 0;
+}
 
 // A pointer that is the same in every lane, as the scalar it is: an "s" operand of inline asm is not made one
 // when the compiler holds the value in vector registers.

@@ -94,13 +94,20 @@ __global__ __launch_bounds__(256) void prefill_varlen_kernel(PrefillParams p) {
   int id = blockIdx.x;
   const int slot = id % p.Hq;
   id /= p.Hq;
-  const int b = id % p.batch;
-  const int qb = p.n_qblocks - 1 - id / p.batch;
+  RowBlock blk = {0, 0, 0, 0};
+  const bool listed = SINKS && p.row_blocks > 0;
+  if constexpr (SINKS)
+    if (listed) {
+      blk = row_block_of(p.cu_q, p.batch, BM, p.n_qblocks, id);
+      if (blk.block < 0) return;
+    }
+  const int b = listed ? blk.seq : id % p.batch;
+  const int qb = listed ? blk.block : p.n_qblocks - 1 - id / p.batch;
   const int h = (slot % p.Hkv) * p.G + slot / p.Hkv;
   const int kvh = h / p.G;
 
-  const int q_begin = p.cu_q[b];
-  const int Lq = p.cu_q[b + 1] - q_begin;
+  const int q_begin = listed ? blk.begin : p.cu_q[b];
+  const int Lq = listed ? blk.rows : p.cu_q[b + 1] - q_begin;
   const int k_begin = PAGED ? 0 : p.cu_k[b];
   int Lk = PAGED ? p.context_lens[b] : p.cu_k[b + 1] - k_begin;
   if (!PAGED && p.seqused_k) Lk = min(Lk, p.seqused_k[b]);
@@ -536,8 +543,10 @@ void launch_prefill(PrefillParams p, hipStream_t stream) {
     attr_set = true;
   }
   p.n_qblocks = (p.max_q + BM - 1) / BM;
-  const int64_t n_wg = (int64_t)p.n_qblocks * p.batch * p.Hq;
+  const int64_t listed = SINKS ? row_blocks_of(p.total_q, p.batch, BM, p.n_qblocks) : 0;
+  const int64_t n_wg = (listed > 0 ? listed : (int64_t)p.n_qblocks * p.batch) * p.Hq;
   HA_CHECK(n_wg <= 0x7fffffff, "mha_varlen_fwd: too many workgroups");
+  p.row_blocks = (int)listed;
   kernel<<<dim3((unsigned)n_wg), 256, Tile<HDP>::LDS_BYTES, stream>>>(p);
   check_launch("mha_varlen_fwd");
 }

@@ -131,14 +131,21 @@ __global__ __launch_bounds__(NW * 64, STEP::value ? 2 : w8_wavefronts(HDP, NW)) 
     part = id % p.n_parts;
     id /= p.n_parts;
   }
-  const int b = id / p.n_qblocks;
-  const int qb = p.n_qblocks - 1 - id % p.n_qblocks;
+  RowBlock blk = {0, 0, 0, 0};
+  const bool listed = STEP::window && p.row_blocks > 0;
+  if constexpr (STEP::window)
+    if (listed) {
+      blk = row_block_of(p.cu_q, p.batch, BM, p.n_qblocks, id);
+      if (blk.block < 0) return;
+    }
+  const int b = listed ? blk.seq : id / p.n_qblocks;
+  const int qb = listed ? blk.block : p.n_qblocks - 1 - id % p.n_qblocks;
   const int head0 = ((slot % p.Hkv) * (p.G >> hl) + slot / p.Hkv) << hl;  // first query head of the workgroup
   const int h = head0 + (wave & ((1 << hl) - 1));
   const int kvh = head0 / p.G;
 
-  const int q_begin = p.cu_q[b];
-  const int Lq = p.cu_q[b + 1] - q_begin;
+  const int q_begin = listed ? blk.begin : p.cu_q[b];
+  const int Lq = listed ? blk.rows : p.cu_q[b + 1] - q_begin;
   const int k_begin = PAGED ? 0 : p.cu_k[b];
   int Lk = PAGED ? p.context_lens[b] : p.cu_k[b + 1] - k_begin;
   if (!PAGED && p.seqused_k) Lk = min(Lk, p.seqused_k[b]);

@@ -44,8 +44,10 @@ void launch_window_nw(WindowParams p, int hl, hipStream_t stream) {
   p.wg_heads_log2 = hl;
   const int bm = p.block_rows = (NW * 32) >> hl;
   p.n_qblocks = (p.max_q + bm - 1) / bm;
-  const int64_t n_wg = (int64_t)p.n_qblocks * p.batch * (p.Hq >> hl) * p.n_parts;
+  const int64_t listed = row_blocks_of(p.total_q, p.batch, bm, p.n_qblocks);
+  const int64_t n_wg = (listed > 0 ? listed : (int64_t)p.n_qblocks * p.batch) * (p.Hq >> hl) * p.n_parts;
   HA_CHECK(n_wg <= 0x7fffffff, "mha_varlen_fwd_paged_window: too many workgroups");
+  p.row_blocks = (int)listed;
   kernel<<<dim3((unsigned)n_wg), NW * 64, lds_bytes, stream>>>(p);
   check_launch("mha_varlen_fwd_paged_window");
   if (p.n_parts > 1) {

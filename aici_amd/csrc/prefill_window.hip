@@ -9,8 +9,8 @@
 // key some row of the workgroup sees (prefill_w8.h, STEP::window).  What bounds them is the matrix pipe and the vector unit on
 // (window + rows of a block) keys a row, and with few workgroups the chain of a row block's tiles.  Measured: 2 x 4096 new tokens, 32 / 8 x 128 bf16,
 // a window of 4096 542 us, 0.95 PFLOP/s of what is seen (causal prefill of 8 x 4096 without a window 1.0 to 1.1); 8 chunks of
-// 65 to 1001 tokens, 16 / 2 x 64 fp16, a window of 1001 47 us, 0.33 PFLOP/s: the softmax of narrow heads, and 533 workgroups of unequal chains on
-// 256 compute units.
+// 65 to 1001 tokens, 16 / 2 x 64 fp16, a window of 1001 43 to 46 us by the order of the chunks, 0.35 PFLOP/s: the softmax of narrow heads, and 552 workgroups, two or three to a
+// compute unit (8 x 512 tokens, 512 workgroups, 39).
 #include <algorithm>
 
 #include "paged_decode.h"

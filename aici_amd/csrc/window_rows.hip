@@ -25,7 +25,8 @@ struct RowsParams {
   const int32_t *cu_q;
   int batch, Hq, Hkv, G;
   int rows_per_group, head_groups;  // columns: that many rows with all G heads, or one row with 16 of them
-  int groups;                       // column groups of a sequence, at most
+  int row_groups;                   // groups of rows of a sequence, at most
+  int listed;                       // 0, or the groups of rows of the grid, one sequence's behind the other's (row_block_of)
   int part_pairs, num_parts, waves;
   float *part_acc, *part_ml;  // of part i of row r and head h, at (i * total_q + r) * Hq + h: d sums; maximum and sum
 };
@@ -45,12 +46,22 @@ __global__ __launch_bounds__(WAVES * 64) void window_rows_kernel(RowsParams p) {
   int id = blockIdx.x;
   const int kvh = id % p.Hkv;
   id /= p.Hkv;
-  const int cg = id % p.groups;
-  id /= p.groups;
-  const int seq = id % p.batch, part = id / p.batch;
-  const int q_begin = p.cu_q[seq], Lq = p.cu_q[seq + 1] - q_begin;
-  const int i0 = cg / p.head_groups * p.rows_per_group;  // the group's first row
-  if (i0 >= Lq) return;
+  const int hg = id % p.head_groups;
+  id /= p.head_groups;
+  const int all_groups = p.listed > 0 ? p.listed : p.row_groups * p.batch, part = id / all_groups;
+  id %= all_groups;
+  RowBlock blk;
+  if (p.listed > 0) {
+    blk = row_block_of(p.cu_q, p.batch, p.rows_per_group, p.row_groups, id);
+  } else {
+    blk.seq = id / p.row_groups;
+    blk.block = id % p.row_groups;
+    blk.begin = p.cu_q[blk.seq];
+    blk.rows = p.cu_q[blk.seq + 1] - blk.begin;
+  }
+  const int seq = blk.seq, q_begin = blk.begin, Lq = blk.rows;
+  const int i0 = blk.block * p.rows_per_group;  // the group's first row
+  if (i0 < 0 || i0 >= Lq) return;
   const int i1 = min(i0 + p.rows_per_group, Lq) - 1;
   const int Lk = p.cache.context_lens[seq];
   const SeenKeys seen = rows_see(p, Lq, Lk, i0, i1);
@@ -63,7 +74,7 @@ __global__ __launch_bounds__(WAVES * 64) void window_rows_kernel(RowsParams p) {
   if (lane < tn && seen.column(t0 + lane, BS) < p.cache.table_cols) tbl = table[seen.column(t0 + lane, BS)];
   if (BS == 8 && 64 + lane < tn && seen.column(t0 + 64 + lane, BS) < p.cache.table_cols) tbl_hi = table[seen.column(t0 + 64 + lane, BS)];
 
-  const int row = i0 + (p.head_groups > 1 ? 0 : col / p.G), g = p.head_groups > 1 ? cg % p.head_groups * 16 + col : col % p.G;
+  const int row = i0 + (p.head_groups > 1 ? 0 : col / p.G), g = p.head_groups > 1 ? hg * 16 + col : col % p.G;
   const bool col_ok = row <= i1 && g < p.G && (p.head_groups > 1 || col < p.rows_per_group * p.G);
   const int qh = kvh * p.G + g;
   const KeyRange mine = rows_see(p, Lq, Lk, row, row);
@@ -168,7 +179,7 @@ __global__ __launch_bounds__(128) void window_rows_merge_kernel(RowsParams p) {
 
 template <typename T, int HD>
 void launch_rows(const RowsParams &p, int block_size, hipStream_t stream) {
-  const int64_t n_wg = (int64_t)p.num_parts * p.batch * p.groups * p.Hkv;
+  const int64_t n_wg = (int64_t)p.num_parts * (p.listed > 0 ? p.listed : (int64_t)p.batch * p.row_groups) * p.head_groups * p.Hkv;
   HA_CHECK(n_wg <= 0x7fffffff, "mha_varlen_fwd_paged_window: too many workgroups");
   const dim3 grid((unsigned)n_wg);
 #define HA_ROWS(BS)                                                                       \
@@ -259,7 +270,8 @@ void launch_window_rows(const PrefillParams &pp, const RowsPlan &plan, int dtype
   p.G = pp.G;
   p.rows_per_group = pp.G <= 16 ? 16 / pp.G : 1;
   p.head_groups = (pp.G + 15) / 16;
-  p.groups = (pp.max_q + p.rows_per_group - 1) / p.rows_per_group * p.head_groups;
+  p.row_groups = (pp.max_q + p.rows_per_group - 1) / p.rows_per_group;
+  p.listed = (int)row_blocks_of(pp.total_q, pp.batch, p.rows_per_group, p.row_groups);
   p.part_pairs = plan.part_pairs;
   p.num_parts = plan.num_parts;
   p.waves = plan.waves;

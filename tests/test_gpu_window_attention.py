@@ -349,3 +349,27 @@ def test_two_streams_at_once(device):
     for (chunk, out), c, r in zip(alone, cases, rows):
         check(chunk, c, want(c))
         check(out, r, want(r))
+
+
+@pytest.mark.parametrize("heads", [(8, 2, 64), (4, 2, 160), (4, 2, 128), (40, 2, 64)])
+def test_one_long_chunk_among_many_short_ones(device, tuning, heads):
+    """More sequences than lanes, of none to a few new tokens, and one of many: row blocks lie one sequence behind the other in the launch."""
+    for n, (long, window, sinks) in enumerate([(200, 60, 10), (9, 40, 3)]):
+        lens_q = [3, 0, 1] * 22 + [0] * 64 + [long] + [2, 1, 0] * 3
+        ctx = [a + (7 * k) % 90 for k, a in enumerate(lens_q)]
+        c = case(500 + n, lens_q, ctx, heads, torch.bfloat16, window, sinks)
+        expect = want(c)
+        for kernel, images in ((0, -1), (5, -1), (1, -1), (5, 0)):
+            tuning("prefill_kernel", kernel)
+            tuning("paged_prefill_dma", images)
+            check(chunk(c, device), c, expect)
+        tuning("prefill_kernel", 0)
+        tuning("paged_prefill_dma", -1)
+        bare = [c[k].to(device) for k in ("q", "kc", "vc", "tables")]
+        tail = torch.cat([bare[0], torch.full((150, *bare[0].shape[1:]), NAN, dtype=torch.bfloat16, device=device)])
+        out = torch.full_like(tail, 5.0)
+        # rows behind the last sequence, and a bound that no sequence reaches
+        _native.mha_varlen_fwd_paged_window(tail, *bare[1:], W.offsets(lens_q).to(device), torch.tensor(ctx, dtype=torch.int32, device=device),
+                                            long + 300, bare[3].size(1) * 16, c["scale"], window, sinks, out, None)
+        check(out[:-150], c, expect)
+        assert bool((out[-150:] == 5).all())
