@@ -77,7 +77,8 @@ _ERR_FUNCS = {
     "hipattn_mha_varlen_fwd": [TP, TP, TP, TP, TP, TP, c_int, c_int, c_float, c_float, c_bool, c_bool, c_int, c_int,
                                TP, TP, c_void_p],
     "hipattn_mha_varlen_fwd_paged": [TP, TP, TP, TP, TP, TP, c_int, c_int, c_float, c_bool, TP, TP, c_void_p],
-    "hipattn_mha_varlen_fwd_paged_window": [TP, TP, TP, TP, TP, TP, c_int, c_int, c_float, c_int, c_int, TP, TP, c_void_p],
+    "hipattn_mha_varlen_fwd_paged_window": [TP, TP, TP, TP, TP, TP, c_int, c_int, c_float, c_int, c_int, TP, TP, TP, c_void_p],
+    "hipattn_mha_varlen_fwd_paged_window_workspace_size": [c_int64, c_int, c_int, POINTER(c_int64)],
     "hipattn_paged_attention_window": [TP, TP, TP, TP, c_int, c_float, TP, TP, c_int, c_int, c_int, c_int, TP, TP, c_void_p],
     "hipattn_paged_attention_window_workspace_size": [c_int64, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int32,
                                                       POINTER(c_int64)],

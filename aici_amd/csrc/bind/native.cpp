@@ -336,7 +336,7 @@ PyMethodDef g_methods[] = {
     BIND(mha_varlen_fwd_paged, "q,key_cache,value_cache,block_tables,cu_seqlens_q,context_lens,max_seqlen_q,max_seqlen_k,"
                                "softmax_scale,causal,out,lse"),
     BIND(mha_varlen_fwd_paged_window, "q,key_cache,value_cache,block_tables,cu_seqlens_q,context_lens,max_seqlen_q,max_seqlen_k,"
-                                      "softmax_scale,window_size_left,sink_tokens,out,lse"),
+                                      "softmax_scale,window_size_left,sink_tokens,out,lse,workspace"),
     BIND(paged_attention_window, "out,query,key_cache,value_cache,num_kv_heads,scale,block_tables,context_lens,block_size,"
                                  "max_context_len,window_size_left,sink_tokens,alibi,workspace"),
     BIND(paged_attention_v1, "out,query,key_cache,value_cache,num_kv_heads,scale,block_tables,context_lens,block_size,"

@@ -134,7 +134,7 @@ extern "C" char *hipattn_varlen_attn_paged_window(const hipattn_tensor *q, const
       hipattn_tensor qm = rows(q, 0, q_multi);
       hipattn_tensor ym = rows(y, 0, q_multi);
       raise(hipattn_mha_varlen_fwd_paged_window(&qm, key_cache, value_cache, multi_block_tables, seqlens_q, multi_context_lens, max_seqlen_q,
-                                                max_seqlen_k, softmax_scale, window_size_left, sink_tokens, &ym, nullptr, stream));
+                                                max_seqlen_k, softmax_scale, window_size_left, sink_tokens, &ym, nullptr, nullptr, stream));
     }
     if (q_multi < T) {
       hipattn_tensor qs = rows(q, q_multi, T);

@@ -83,16 +83,25 @@ double staged_us(const PrefillParams &p) {
   return 10 + (double)most_tiles(p, 128) * 3.5 * std::max(p.d, 128) / 256 * std::max(1.0, 0.6 * (double)wgs / compute_units());
 }
 
-// A stream's buffer, allocated once.
+// A stream's buffer, allocated once; and what a call may need of it or of a caller's.
 constexpr size_t kWindowScratchBytes = (size_t)64 << 20;
+size_t piece_bytes(int64_t total_q, int heads, int d) { return (size_t)total_q * heads * (d + 2) * sizeof(float); }
+size_t scratch_bytes(int64_t total_q, int heads, int d) {
+  return kMostParts * std::min(piece_bytes(total_q, heads, d), kWindowScratchBytes / kMostParts);
+}
 
 void mha_varlen_fwd_paged_window_impl(const hipattn_tensor *q, const hipattn_tensor *key_cache, const hipattn_tensor *value_cache,
                                       const hipattn_tensor *block_tables, const hipattn_tensor *cu_q, const hipattn_tensor *context_lens,
                                       int max_q, int max_k, float scale, int window_left, int sinks, hipattn_tensor *out,
-                                      hipattn_tensor *lse, void *stream_arg) {
+                                      hipattn_tensor *lse, const hipattn_tensor *workspace, void *stream_arg) {
   const char *op = "mha_varlen_fwd_paged_window";
   HA_CHECK(window_left >= 0, "%s: window_size_left must not be negative here, got %d", op, window_left);
   HA_CHECK(sinks >= 0, "%s: sink_tokens must not be negative, got %d", op, sinks);
+  if (workspace) {
+    check_tensor(workspace, "workspace", 1);
+    HA_CHECK(workspace->dtype == HIPATTN_U8, "%s: workspace must be u8", op);
+    check_contiguous(workspace, "workspace");
+  }
   WindowParams p;
   if (!paged_prefill_params(PagedPrefillCall{q, key_cache, value_cache, block_tables, cu_q, context_lens, max_q, max_k, scale, true, op}, out,
                             lse, p))
@@ -112,11 +121,23 @@ void mha_varlen_fwd_paged_window_impl(const hipattn_tensor *q, const hipattn_ten
   // Block images go into LDS as they are where they fill most of their place there; else tiles are staged through registers.
   const bool images = p.vc_block % 8 == 0 && p.vc_head % 8 == 0 && tuning().paged_prefill_dma != 0 && p.d <= 128 && (p.d >= 64 || p.d == 32);
   const bool eight = images && (force == 1 || (force == 0 && eight_wavefronts_pay(p)));
-  // What pieces need lies in a buffer of the stream's of fixed size; without it -- in a capture, for shapes beyond it, on hipStreamPerThread, one
-  // handle for a stream of each thread's own -- nothing is cut that has to be merged.
+  // What pieces need lies in the caller's workspace or a buffer of the stream's, of one size, so that either gives the same bits; without it -- in a
+  // capture, for shapes beyond it, on hipStreamPerThread, one handle for a stream of each thread's own -- nothing is cut that has to be merged.
+  char *given = nullptr;
+  if (workspace) {
+    const size_t need = scratch_bytes(p.total_q, p.Hq, p.d);
+    HA_CHECK(workspace->data != nullptr && (reinterpret_cast<uintptr_t>(workspace->data) & 255) == 0,
+             "%s: workspace must be 256-byte aligned", op);
+    HA_CHECK((size_t)workspace->sizes[0] >= need,
+             "%s: workspace of %lld bytes is too small, %zu are needed (hipattn_mha_varlen_fwd_paged_window_workspace_size)", op,
+             (long long)workspace->sizes[0], need);
+    given = static_cast<char *>(workspace->data);
+  }
   HeldWorkspace ws;
-  const size_t piece_bytes = (size_t)p.total_q * p.Hq * (p.d + 2) * sizeof(float);
-  int most = stream == hipStreamPerThread || lse_or_f32 || force != 0 || eight ? 1 : (int)std::max<size_t>(std::min<size_t>(kWindowScratchBytes / piece_bytes, kMostParts), 1);
+  void *scratch = given;
+  int most = (stream == hipStreamPerThread && !given) || lse_or_f32 || force != 0 || eight
+                 ? 1
+                 : (int)std::max<size_t>(std::min<size_t>(kWindowScratchBytes / piece_bytes(p.total_q, p.Hq, p.d), kMostParts), 1);
   for (;;) {
     int parts = 1;
     double us = images ? 0 : staged_us(p);
@@ -124,22 +145,23 @@ void mha_varlen_fwd_paged_window_impl(const hipattn_tensor *q, const hipattn_ten
     RowsPlan rows;
     const bool as_rows = force == 0 && !eight && !lse_or_f32 && plan_window_rows(p, most, rows) && rows.us < us;
     if (as_rows) parts = rows.num_parts;
-    if (parts > 1) {
+    if (parts > 1 && !given) {
       ws = try_library_workspace(WS_WINDOW_CHUNKS, kWindowScratchBytes, stream);
-      if (ws.ptr == nullptr) {
+      scratch = ws.ptr;
+      if (scratch == nullptr) {
         most = 1;
         continue;
       }
     }
     if (as_rows) {
-      launch_window_rows(p, rows, q->dtype, ws.ptr, stream);
+      launch_window_rows(p, rows, q->dtype, scratch, stream);
       return;
     }
     if (parts > 1) {
       const int64_t tiles = most_tiles(p, 128 >> prefill_heads_log2(p, 2));
       p.part_tiles = (int)((tiles + parts - 1) / parts);
       p.n_parts = (int)((tiles + p.part_tiles - 1) / p.part_tiles);
-      p.part_acc = static_cast<float *>(ws.ptr);
+      p.part_acc = static_cast<float *>(scratch);
       p.part_ml = p.part_acc + (size_t)p.n_parts * p.total_q * p.Hq * p.d;
     }
     break;
@@ -165,7 +187,19 @@ extern "C" char *hipattn_mha_varlen_fwd_paged_window(const hipattn_tensor *q, co
                                                      const hipattn_tensor *value_cache, const hipattn_tensor *block_tables,
                                                      const hipattn_tensor *cu_seqlens_q, const hipattn_tensor *context_lens,
                                                      int max_seqlen_q, int max_seqlen_k, float softmax_scale, int window_size_left,
-                                                     int sink_tokens, hipattn_tensor *out, hipattn_tensor *softmax_lse, void *stream) {
+                                                     int sink_tokens, hipattn_tensor *out, hipattn_tensor *softmax_lse,
+                                                     const hipattn_tensor *workspace, void *stream) {
   HA_PROTECT(mha_varlen_fwd_paged_window_impl(q, key_cache, value_cache, block_tables, cu_seqlens_q, context_lens, max_seqlen_q,
-                                              max_seqlen_k, softmax_scale, window_size_left, sink_tokens, out, softmax_lse, stream));
+                                              max_seqlen_k, softmax_scale, window_size_left, sink_tokens, out, softmax_lse, workspace,
+                                              stream));
+}
+
+extern "C" char *hipattn_mha_varlen_fwd_paged_window_workspace_size(int64_t total_q, int num_heads, int head_size, int64_t *bytes) {
+  HA_PROTECT({
+    const char *op = "mha_varlen_fwd_paged_window_workspace_size";
+    HA_CHECK(bytes != nullptr, "%s: bytes is NULL", op);
+    HA_CHECK(total_q >= 0 && total_q <= 0x7fffffff && num_heads >= 0 && num_heads <= 1 << 20, "%s: a size is negative or too large", op);
+    HA_CHECK(head_size >= 0 && head_size <= 256, "%s: head size %d not supported (at most 256)", op, head_size);
+    *bytes = (int64_t)scratch_bytes(total_q, num_heads, head_size);
+  });
 }

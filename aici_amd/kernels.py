@@ -98,16 +98,25 @@ def flash_attn_varlen_paged(q: torch.Tensor, key_cache: torch.Tensor, value_cach
 def flash_attn_varlen_paged_window(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, block_tables: torch.Tensor,
                                    seqlens_q: torch.Tensor, context_lens: torch.Tensor, max_seqlen_q: int, max_seqlen_k: int,
                                    softmax_scale: float, window_size_left: int, sink_tokens: int = 0, return_lse: bool = False,
-                                   out_dtype: Optional[torch.dtype] = None):
+                                   out_dtype: Optional[torch.dtype] = None, workspace: Optional[torch.Tensor] = None):
     """`flash_attn_varlen_paged`, causal, with a sliding window and sinks: the query at position p of its sequence sees key j iff j <= p
-    and (j >= p - window_size_left or j < sink_tokens).  Blocks of keys that none of a sequence's new tokens sees may be gone."""
+    and (j >= p - window_size_left or j < sink_tokens).  Blocks of keys that none of a sequence's new tokens sees may be gone.
+    workspace: uint8, `flash_attn_varlen_paged_window_workspace_size` bytes, for calls that are captured and for those that must not
+    allocate; None: a buffer that the library keeps per stream, and under capture none, which takes longer for few rows over long windows."""
     out = torch.empty_like(q, dtype=out_dtype or q.dtype)
     lse = None
     if return_lse:
         lse = torch.empty((context_lens.numel(), q.size(1), max(int(max_seqlen_q), 1)), dtype=torch.float32, device=q.device)
     _native.mha_varlen_fwd_paged_window(q, key_cache, value_cache, block_tables, seqlens_q, context_lens, max_seqlen_q, max_seqlen_k,
-                                        softmax_scale, window_size_left, sink_tokens, out, lse)
+                                        softmax_scale, window_size_left, sink_tokens, out, lse, workspace)
     return (out, lse) if return_lse else out
+
+
+def flash_attn_varlen_paged_window_workspace_size(total_q: int, num_heads: int, head_size: int) -> int:
+    """Bytes of scratch memory flash_attn_varlen_paged_window can make use of for total_q rows."""
+    n = ctypes.c_int64(0)
+    call("hipattn_mha_varlen_fwd_paged_window_workspace_size", int(total_q), int(num_heads), int(head_size), ctypes.byref(n))
+    return int(n.value)
 
 
 def paged_attention_window(out: torch.Tensor, query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,

@@ -118,15 +118,17 @@ char *hipattn_mha_varlen_fwd_paged(const hipattn_tensor *q, const hipattn_tensor
  * Keys that no new token of a sequence sees may be gone: table columns that hold only such keys may name any block or none (a negative
  * or large number), and their blocks may hold anything.  Values of a key that some of a sequence's new tokens see are taken to be finite,
  * also where others do not see it.  A row that sees nothing (its position is negative) is zero, its LSE +inf.
- * Where few workgroups would leave compute units idle a row's keys are dealt out to several, by way of 64 MiB of scratch memory that are
- * allocated once per stream; not under capture, on hipStreamPerThread, without that memory, with an f32 out or an LSE, so that last bits
- * may differ there. */
+ * Where few workgroups would leave compute units idle a row's keys are dealt out to several (not with an f32 out or an LSE), by way of
+ * workspace: u8, 256-byte aligned, hipattn_mha_varlen_fwd_paged_window_workspace_size bytes (at most 64 MiB), not shared by calls that overlap,
+ * replays of captured ones included.  NULL: a buffer of 64 MiB that the library allocates once per stream; under capture, on
+ * hipStreamPerThread and without that memory keys are then not dealt out, so that last bits, and the time of few long rows, may differ. */
 char *hipattn_mha_varlen_fwd_paged_window(const hipattn_tensor *q, const hipattn_tensor *key_cache,
                                           const hipattn_tensor *value_cache, const hipattn_tensor *block_tables,
                                           const hipattn_tensor *cu_seqlens_q, const hipattn_tensor *context_lens,
                                           int max_seqlen_q, int max_seqlen_k, float softmax_scale,
                                           int window_size_left, int sink_tokens, hipattn_tensor *out,
-                                          hipattn_tensor *softmax_lse, void *stream);
+                                          hipattn_tensor *softmax_lse, const hipattn_tensor *workspace, void *stream);
+char *hipattn_mha_varlen_fwd_paged_window_workspace_size(int64_t total_q, int num_heads, int head_size, int64_t *bytes);
 
 /* Replaces paged_attention_v1_C (lib.rs:107-120; attention_kernels.cu:679-700).
  * out/query [S, Hq, d]; key_cache [nb, Hkv, d/x, BS, x]; value_cache

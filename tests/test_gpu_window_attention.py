@@ -215,7 +215,7 @@ def test_chunk_outputs_in_fp32_lse_and_rows_behind_the_last(device):
     frame = torch.full((T + 5, 12, 128), 7.0, dtype=torch.bfloat16, device=device)
     _native.mha_varlen_fwd_paged_window(wide[:, 1:9], c["kc"].to(device), c["vc"].to(device), c["tables"].to(device),
                                         W.offsets(c["lens_q"]).to(device), torch.tensor(c["ctx"], dtype=torch.int32, device=device), 70, 300,
-                                        c["scale"], 90, 10, frame[:, 2:10], None)
+                                        c["scale"], 90, 10, frame[:, 2:10], None, None)
     check(frame[:T, 2:10], c, expect)
     assert bool((frame[T:] == 7).all()) and bool((frame[:, :2] == 7).all()) and bool((frame[:, 10:] == 7).all())
 
@@ -370,6 +370,36 @@ def test_one_long_chunk_among_many_short_ones(device, tuning, heads):
         out = torch.full_like(tail, 5.0)
         # rows behind the last sequence, and a bound that no sequence reaches
         _native.mha_varlen_fwd_paged_window(tail, *bare[1:], W.offsets(lens_q).to(device), torch.tensor(ctx, dtype=torch.int32, device=device),
-                                            long + 300, bare[3].size(1) * 16, c["scale"], window, sinks, out, None)
+                                            long + 300, bare[3].size(1) * 16, c["scale"], window, sinks, out, None, None)
         check(out[:-150], c, expect)
         assert bool((out[-150:] == 5).all())
+
+
+@pytest.mark.parametrize("heads,lens_q,ctx", [((8, 2, 64), [16], [4000]), ((8, 2, 128), [40, 300], [2600, 2900]), ((8, 2, 256), [3, 9], [2600, 2000])])
+def test_chunks_with_a_workspace_of_the_callers(device, heads, lens_q, ctx):
+    """The same bits as with the library's buffer, eager, captured without a call before, and replayed."""
+    c, other = (case(600 + k, lens_q, ctx, heads, torch.bfloat16, 2500, 30) for k in range(2))
+    need = K.flash_attn_varlen_paged_window_workspace_size(sum(lens_q), heads[0], heads[2])
+    assert need == min(16 * sum(lens_q) * heads[0] * (heads[2] + 2) * 4, 64 << 20)
+    store = torch.full((need + 512,), 255, dtype=torch.uint8, device=device)  # (NaN, read as fp32)
+    with pytest.raises(HipAttnError, match="too small"):
+        chunk(c, device, workspace=store[:need - 1])
+    alone = [chunk(x, device) for x in (c, other)]
+    check(alone[0], c, want(c))
+    q, kc, vc, tables = (c[k].to(device) for k in ("q", "kc", "vc", "tables"))
+    cu, lk = W.offsets(lens_q).to(device), torch.tensor(ctx, dtype=torch.int32, device=device)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        out = K.flash_attn_varlen_paged_window(q, kc, vc, tables, cu, lk, max(lens_q), max(ctx), c["scale"], 2500, 30, workspace=store[:need])
+    for k in range(4):
+        x = (other, c)[k % 2]
+        for t, n in ((q, "q"), (kc, "kc"), (vc, "vc"), (tables, "tables")):
+            t.copy_(x[n])
+        out.fill_(NAN)
+        store.fill_(255)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, alone[(k + 1) % 2])
+        assert torch.equal(chunk(x, device, workspace=store[:need]), out)
+        assert bool((store[need:] == 255).all())

@@ -121,7 +121,7 @@ def test_paged_attention_window_refuses(over, message):
 
 def _chunk_args(**over):
     a = dict(q=_t(20, 8, 128), kc=_t(9, 2, 16, 16, 8), vc=_t(9, 2, 128, 16), tables=_t(2, 4, dtype=_lib.I32), cu=_t(3, dtype=_lib.I32),
-             ctx=_t(2, dtype=_lib.I32), max_q=12, max_k=64, scale=1.0, window=31, sinks=4, out=_t(20, 8, 128), lse=None)
+             ctx=_t(2, dtype=_lib.I32), max_q=12, max_k=64, scale=1.0, window=31, sinks=4, out=_t(20, 8, 128), lse=None, ws=None)
     a.update(over)
     return [*a.values(), None]
 
@@ -131,7 +131,8 @@ def _chunk_args(**over):
     (dict(q=_t(20, 8, 128, dtype=_lib.F32)), "only fp16 and bf16"), (dict(q=_t(20, 7, 128), out=_t(20, 7, 128)), "not divisible"),
     (dict(max_k=65), "mha_varlen_fwd_paged_window: max_seqlen_k 65 needs more"), (dict(scale=0.0), "softmax_scale must be positive"),
     (dict(ctx=_t(3, dtype=_lib.I32)), "need 2 rows"), (dict(out=_t(19, 8, 128)), "out shape differs"),
-    (dict(lse=_t(2, 8, 11, dtype=_lib.F32)), "softmax_lse"),
+    (dict(lse=_t(2, 8, 11, dtype=_lib.F32)), "softmax_lse"), (dict(ws=_t(1 << 20, dtype=_lib.F32)), "workspace must be u8"),
+    (dict(ws=_t(16 * 20 * 8 * 130 * 4 - 1, dtype=_lib.U8)), "too small"), (dict(ws=_t(1 << 24, dtype=_lib.U8, data=128)), "256-byte aligned"),
 ])
 def test_flash_attn_varlen_paged_window_refuses(over, message):
     with pytest.raises(_lib.HipAttnError, match=message):
