@@ -1,5 +1,5 @@
-// The launches of paged decode, partitioned and as one flat split, each with the merge behind it, for all of a context's keys (paged_decode.hip) and for a window with
-// sinks (window_decode.hip).  Device code; included by those two.
+// The launches of paged decode, partitioned and as one flat split, each with the merge behind it, for all of a context's keys
+// (paged_decode.hip) and for a window with sinks (window_decode.hip).  Device code; included by those two.
 #pragma once
 
 #include "paged_decode.h"

@@ -9,8 +9,8 @@
 // key some row of the workgroup sees (prefill_w8.h, STEP::window).  What bounds them is the matrix pipe and the vector unit on
 // (window + rows of a block) keys a row, and with few workgroups the chain of a row block's tiles.  Measured: 2 x 4096 new tokens, 32 / 8 x 128 bf16,
 // a window of 4096 542 us, 0.95 PFLOP/s of what is seen (causal prefill of 8 x 4096 without a window 1.0 to 1.1); 8 chunks of
-// 65 to 1001 tokens, 16 / 2 x 64 fp16, a window of 1001 43 to 46 us by the order of the chunks, 0.35 PFLOP/s: the softmax of narrow heads, and 552 workgroups, two or three to a
-// compute unit (8 x 512 tokens, 512 workgroups, 39).
+// 65 to 1001 tokens, 16 / 2 x 64 fp16, a window of 1001 43 to 46 us by the order of the chunks, 0.35 PFLOP/s: the softmax of narrow heads, and
+// 552 workgroups, two or three to a compute unit (8 x 512 tokens, 512 workgroups, 39).
 #include <algorithm>
 
 #include "paged_decode.h"
@@ -26,7 +26,8 @@ constexpr int kTileKeys = 64;
 
 // Tiles of the longest chain: what a row block of `rows` rows sees at most.
 int64_t most_tiles(const PrefillParams &p, int rows) {
-  return std::min<int64_t>(((int64_t)p.max_k + kTileKeys - 1) / kTileKeys, ((int64_t)p.sinks + kTileKeys - 1) / kTileKeys + ((int64_t)p.win_left + rows + kTileKeys - 1) / kTileKeys + 1);
+  auto tiles = [](int64_t keys) { return (keys + kTileKeys - 1) / kTileKeys; };
+  return std::min<int64_t>(tiles(p.max_k), tiles(p.sinks) + tiles((int64_t)p.win_left + rows) + 1);
 }
 
 // Workgroups of `waves` wavefronts with work to do, about.
@@ -49,7 +50,8 @@ bool eight_wavefronts_pay(const PrefillParams &p) {
 // instructions, some 1.4 us a tile with a wavefront per SIMD (five tiles in LDS instead of two change nothing), so where compute units are idle
 // more of them take a part each.  All in us: a tile, which takes longer from one workgroup per compute unit on, but less than in proportion,
 // as two or three of them fill each other's gaps; the merge's launch, and what writing and reading the pieces costs.  In 56 measured shapes (16
-// x 4 new tokens to 2 x 4096, windows of 100 to 4096) the choice among 1, 2, 3, 4, 6, 10 and 16, which asks for a tenth before it cuts, is 0.7 % off the best on average.  us, whole / best:
+// x 4 new tokens to 2 x 4096, windows of 100 to 4096) the choice among 1, 2, 3, 4, 6, 10 and 16, which asks for a tenth before it cuts, is
+// 0.7 % off the best on average.  us, whole / best:
 // 32 / 8 x 128, 1 x 16 over 4096 keys 102 / 25 (16 pieces), 1 x 300 106 / 47 (6), 4 x 64 over 2048 62 / 33 (4), 16 x 20 over 4096 104 / 63 (4);
 // 16 / 2 x 64, 1 x 45 over 256 17.5 / 11.1 (7); 32 / 8 x 128, 4 x 8 over 100 10.5 / 10.5 (1; in 2 13.7).
 // At most `most`; us: about what the launch takes then.

@@ -34,6 +34,11 @@ void check_window(const char *op, int window_left, int sinks) {
   HA_CHECK(sinks >= 0, "%s: sink_tokens must not be negative, got %d", op, sinks);
 }
 
+void check_head_size(const char *op, int hd) {
+  HA_CHECK(hd == 64 || hd == 80 || hd == 96 || hd == 112 || hd == 128 || hd == 256,
+           "%s: unsupported head size %d (supported: 64, 80, 96, 112, 128, 256)", op, hd);
+}
+
 template <typename T, int HD>
 void launch_head(const DecodeParams &p, const DecodePlan &pl, int block_size, char *ws, hipStream_t stream) {
   if (pl.flat) {
@@ -70,8 +75,7 @@ void paged_attention_window_impl(hipattn_tensor *out, const hipattn_tensor *quer
   HA_CHECK(query->dtype == HIPATTN_F16 || query->dtype == HIPATTN_BF16, "%s: unsupported data type %s (supported: f16, bf16)", op,
            dtype_name(query->dtype));
   const int hd = (int)query->sizes[2];
-  HA_CHECK(hd == 64 || hd == 80 || hd == 96 || hd == 112 || hd == 128 || hd == 256,
-           "%s: unsupported head size %d (supported: 64, 80, 96, 112, 128, 256)", op, hd);
+  check_head_size(op, hd);
   if (workspace) {
     check_tensor(workspace, "workspace", 1);
     HA_CHECK(workspace->dtype == HIPATTN_U8, "%s: workspace must be u8", op);
@@ -137,6 +141,7 @@ extern "C" char *hipattn_paged_attention_window_workspace_size(int64_t num_seqs,
     HA_CHECK(block_size == 8 || block_size == 16 || block_size == 32, "%s: unsupported block size %d (supported: 8, 16, 32)", op, block_size);
     HA_CHECK(num_kv_heads > 0 && num_heads % num_kv_heads == 0, "%s: %d query heads not divisible by %d kv heads", op, num_heads, num_kv_heads);
     check_window(op, window_size_left, sink_tokens);
+    check_head_size(op, head_size);
     *bytes = (int64_t)plan_decode(num_seqs, num_heads, num_kv_heads, head_size, block_size, dtype,
                                   (int)seen_tokens(max_context_len, window_size_left, sink_tokens))
                  .bytes;

@@ -141,3 +141,19 @@ def test_replays(device):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, K.penalize_logits(x, **a)) and (k > 0 or torch.equal(out, eager))
+
+
+def test_rows_beyond_32_bits(device):
+    """Rows of logits and of the output that lie more than 2^31 elements apart."""
+    V, apart = 1003, (1 << 31) + 24
+    store, out_store = (torch.empty((apart + V,), dtype=torch.bfloat16, device=device) for _ in range(2))
+    logits, out = (s.as_strided((2, V), (apart, 1)) for s in (store, out_store))
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn((2, V), generator=g).to(torch.bfloat16)
+    logits.copy_(x)
+    said = torch.randint(0, V, (90,), generator=g, dtype=torch.int32)
+    offsets = torch.tensor([0, 40, 90], device=device)
+    knobs = dict(repetition=torch.tensor([1.3, 0.8], device=device), presence=torch.tensor([0.5, -0.25], device=device))
+    K.penalize_logits(logits, said.to(device), offsets, out=out, **knobs)
+    small = K.penalize_logits(x.to(device), said.to(device), offsets, **knobs)
+    assert torch.equal(out, small) and not torch.equal(small, x.to(device))

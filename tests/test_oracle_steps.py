@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 import torch
 
-from aici_amd import _lib, attn, paged
+from aici_amd import _lib, attn, kernels, paged
 from oracle import steps
 
 
@@ -200,3 +200,22 @@ def test_varlen_attn_refuses_sinks_without_a_window():
     x = torch.zeros((1, 1, 8))
     with pytest.raises(ValueError, match="needs a window"):
         attn.varlen_attn(x, x, x, None, x, x, sink_tokens=4)
+
+
+@pytest.mark.parametrize("args,message", [
+    ((4, 8, 2, 72, 16, 100, 31, 4), "unsupported head size 72"), ((4, 8, 3, 64, 16, 100, 31, 4), "not divisible"),
+    ((4, 8, 2, 64, 12, 100, 31, 4), "unsupported block size 12"), ((4, 8, 2, 64, 16, 100, -1, 4), "must not be negative"),
+    ((-1, 8, 2, 64, 16, 100, 31, 4), "negative size"),
+])
+def test_paged_attention_window_workspace_size_refuses(args, message):
+    with pytest.raises(_lib.HipAttnError, match=message):
+        _lib.call("hipattn_paged_attention_window_workspace_size", *args, _lib.BF16, ctypes.byref(ctypes.c_int64(0)))
+
+
+def test_chunk_workspace_sizes():
+    size = kernels.flash_attn_varlen_paged_window_workspace_size
+    assert size(0, 8, 128) == 0 and size(1, 1, 64) == 16 * 66 * 4 and size(2 ** 31 - 1, 2 ** 20, 256) == 64 << 20
+    with pytest.raises(_lib.HipAttnError, match="negative or too large"):
+        size(-1, 8, 128)
+    with pytest.raises(_lib.HipAttnError, match="head size 257"):
+        size(4, 8, 257)
