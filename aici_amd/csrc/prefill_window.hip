@@ -30,51 +30,44 @@ int64_t most_tiles(const PrefillParams &p, int rows) {
   return std::min<int64_t>(tiles(p.max_k), tiles(p.sinks) + tiles((int64_t)p.win_left + rows) + 1);
 }
 
-// Workgroups of `waves` wavefronts with work to do, about.
-int64_t busy_workgroups(const PrefillParams &p, int waves, int hl) {
-  return std::max<int64_t>(p.total_q / ((waves * 32) >> hl) + (p.batch + 1) / 2, 1) * (p.Hq >> hl);
-}
-
-// Workgroups of eight wavefronts instead of four: where windows are long enough for what their alternation between the pipes gains a tile, and
-// there is one of them for nearly every compute unit, or several, of more than one head.  us, eight / four: 32 / 8 x 128, 2 x 4096 new tokens
-// with a window of 4096 549 / 574, 16 x 512 of 2048 327 / 333, 1 x 2000 of 4096 (250 workgroups) 145 / 154, 4 x 2048 of 1024 182 / 174; 32 / 32 x 80,
-// 1 x 2000 of 4096 133 / 152, 2 x 4096 502 / 493; 16 / 2 x 64, 2 x 4096 215 / 228, 1 x 2000 of 4096 (125) 108 / 88; 12 / 4 x 112, 16 x 512 of 2048 173 /
-// 151, 2 x 4096 277 / 275.
+// Workgroups of eight wavefronts instead of four: what their alternation between the pipes gains a tile is lost again where a block of twice as many
+// rows is filled less or the last round of workgroups is, so only for chunks of like lengths over long windows whose workgroups fill the compute
+// units once, or many times with heads of 128.  us, eight / four: 32 / 8 x 128, 1 x 2000 new tokens (256 workgroups) with a window of 4096 157 / 163, of
+// 2000 85 / 89, of 1000 52.2 / 52.2; 2 x 4096 of 4096 614 / 625, of 2000 330 / 332, of 1000 199 / 189; 8 x 533 of 4096 399 / 386; 63 x 20 beside 1 x 4096 of
+// 4096 530 / 512; 32 / 32 x 80, 1 x 2000 of 4096 136 / 151, 2 x 4096 535 / 510; 12 / 4 x 112, 16 x 512 296 / 262; 16 / 2 x 64, 2 x 4096 225 / 216, 8 x 533 199 / 144.
 bool eight_wavefronts_pay(const PrefillParams &p) {
-  const int hl = prefill_heads_log2(p, 3);
-  const int64_t wgs = busy_workgroups(p, 8, hl);
-  return most_tiles(p, 256 >> hl) >= 32 && wgs >= 200 && (wgs <= 256 || hl > 0);
+  const int hl = prefill_heads_log2(p, 3), rows = 256 >> hl;
+  const int64_t wgs = (int64_t)p.batch * ((p.max_q + rows - 1) / rows) * (p.Hq >> hl), tiles = most_tiles(p, rows);
+  const bool alike = p.total_q * 10 >= (int64_t)p.batch * p.max_q * 9, once = wgs <= compute_units() && wgs * 8 > compute_units() * 7;
+  return alike && ((once && p.d > 64 && tiles >= 32) || (wgs >= 1000 && hl > 0 && p.d > 112 && tiles >= 48));
 }
 
 // Pieces that a row block's keys are dealt out in (workgroups of four wavefronts).  A workgroup's chain of tiles is bound by its own
-// instructions, some 1.4 us a tile with a wavefront per SIMD (five tiles in LDS instead of two change nothing), so where compute units are idle
-// more of them take a part each.  All in us: a tile, which takes longer from one workgroup per compute unit on, but less than in proportion,
-// as two or three of them fill each other's gaps; the merge's launch, and what writing and reading the pieces costs.  In 56 measured shapes (16
-// x 4 new tokens to 2 x 4096, windows of 100 to 4096) the choice among 1, 2, 3, 4, 6, 10 and 16, which asks for a tenth before it cuts, is
-// 0.7 % off the best on average.  us, whole / best:
-// 32 / 8 x 128, 1 x 16 over 4096 keys 102 / 25 (16 pieces), 1 x 300 106 / 47 (6), 4 x 64 over 2048 62 / 33 (4), 16 x 20 over 4096 104 / 63 (4);
-// 16 / 2 x 64, 1 x 45 over 256 17.5 / 11.1 (7); 32 / 8 x 128, 4 x 8 over 100 10.5 / 10.5 (1; in 2 13.7).
+// instructions, some 2 us a tile with a wavefront per SIMD (five tiles in LDS instead of two change nothing), so where compute units are idle
+// more of them take a part each.  All in us: the launch, a tile, which takes longer from two workgroups per compute unit on, as two or three of them
+// fill each other's gaps; the merge, and what writing and reading the pieces costs.  In 400 measured shapes (1 x 5 new tokens to 2 x 4096, alike and
+// 63 x 20 beside one of 4096, windows of 100 to 4096, four kinds of heads) the choice among these and the kernel of decode rows is 1.8 % off the best on
+// average and 20 % at most; whole blocks alone are 39 %.  us, whole / best: 32 / 8 x 128, 1 x 5 over 4096 keys 99 / 16 (rows), 1 x 300 106 / 48 (6
+// pieces), 4 x 64 over 2000 61 / 29 (4); 32 / 32 x 80, 12 of 1 to 64 over 2000 83 / 65 (2); 16 / 2 x 64, 100 x 4 over 2000 66 / 39 (rows).
 // At most `most`; us: about what the launch takes then.
 int choose_parts(const PrefillParams &p, int most, double &us) {
-  const int hl = prefill_heads_log2(p, 2);
-  const int64_t tiles = most_tiles(p, 128 >> hl), wgs = busy_workgroups(p, 4, hl);
-  const double tile = p.d > 96 ? 1.45 : (p.d > 64 ? 1.55 : 1.25), share = (p.d > 96 ? 0.6 : 0.4) / compute_units();
+  const int hl = prefill_heads_log2(p, 2), rows = 128 >> hl;
+  const int64_t tiles = most_tiles(p, rows);
+  const double wgs = ((double)(p.total_q / rows) + 0.7 * (p.batch + 1)) * (p.Hq >> hl);
+  const double launch = p.d > 96 ? 8 : (p.d > 64 ? 16 : 9), tile = p.d > 64 ? 2.1 : 1.7;
+  const double share = (p.d > 96 ? 0.62 : (p.d > 64 ? 0.45 : 0.5)) / compute_units();
   const double piece = (double)p.total_q * p.Hq * (p.d + 2) * 2e-6;
-  double best = 0, whole = 0;
   int parts = 1;
-  for (int n = 1; n <= most && n <= tiles; n++) {
+  us = 0;
+  for (int n : {1, 2, 3, 4, 6, 10, 16}) {
     const int64_t part_tiles = (tiles + n - 1) / n;
-    if ((tiles + part_tiles - 1) / part_tiles != n) continue;
-    const double t = (double)part_tiles * tile * std::max(1.0, share * (double)(wgs * n)) + (n > 1 ? 3.0 + n * piece : 0.0);
-    if (n == 1 || t < 0.9 * whole) {
-      if (n == 1) whole = t;
-      if (n == 1 || t < best) {
-        best = t;
-        parts = n;
-      }
+    if (n > 1 && (n > most || n > tiles || (tiles + part_tiles - 1) / part_tiles != n)) continue;
+    const double t = launch + (double)part_tiles * tile * std::max(1.0, share * wgs * n) + (n > 1 ? 5.0 + n * piece : 0.0);
+    if (n == 1 || t < (parts == 1 ? 0.87 : 1.0) * us) {
+      us = t;
+      parts = n;
     }
   }
-  us = 1.4 * best + (p.d > 96 ? 7.7 : (p.d > 64 ? 8.5 : 4.5));
   return parts;
 }
 

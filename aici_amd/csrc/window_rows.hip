@@ -215,25 +215,24 @@ void dispatch_rows(const RowsParams &p, int head_size, int block_size, hipStream
 
 }  // namespace
 
-// All in us, for each form: a launch, the chain of a wavefront's pairs, each longer where more workgroups run than some per compute unit (1.74 of
-// four wavefronts, 0.82 of eight), and the merge.  In 92 measured shapes (16 x 2 new tokens to 16 x 512, windows of 63 to 4095) the form and the choice
-// between this kernel and those of prefill are 3 % off the best on average.  us, prefill / here: 32 / 8 x 128, 1 x 2 over 64 keys 10.7 / 6.3, 16 x 5
-// over 500 21.6 / 10.0, 1 x 45 over 256 18.3 / 8.3, 2 x 2 over 2048 22.0 / 14.9, 8 x 16 over 512 23.8 / 10.0, 1 x 300 over 4096 47 / 86; 12 / 4 x 112, 64
-// x 4 over 1024 75 / 27, 4 x 64 over 2048 29 / 24; 16 / 2 x 64, 1 x 16 over 4096 16.0 / 10.2.
+// All in us, for each form: a launch, the chain of a wavefront's pairs, each longer where more workgroups run than some per compute unit (1.4 of
+// four wavefronts, 0.68 of eight), and the merge (prefill_window.hip's choose_parts says how far off the choice is).  us, prefill / here: 32 / 8 x 128, 1 x 2
+// over 64 keys 10.7 / 6.3, 16 x 5 over 500 21.6 / 10.0, 1 x 45 over 256 18.3 / 8.3, 2 x 2 over 2048 22.0 / 14.9, 8 x 16 over 512 23.8 / 10.0, 1 x 300 over
+// 4096 47 / 86; 12 / 4 x 112, 64 x 4 over 1024 75 / 27, 4 x 64 over 2048 29 / 24; 16 / 2 x 64, 1 x 16 over 4096 16.0 / 10.2.
 bool plan_window_rows(const PrefillParams &p, int most_parts, RowsPlan &plan) {
   if (p.d != 64 && p.d != 80 && p.d != 96 && p.d != 112 && p.d != 128 && p.d != 256) return false;
   const int per = p.G <= 16 ? 16 / p.G : 1;
   const int64_t pairs = std::max<int64_t>(
       std::min<int64_t>(((int64_t)p.max_k + 31) / 32, ((int64_t)p.win_left + per + 30) / 32 + 1 + ((int64_t)p.sinks + 31) / 32), 1);
-  const double wgs = (double)((p.G + 15) / 16) * (double)((p.total_q + per - 1) / per + p.batch / 2) * p.Hkv;
-  const double pair = 1.3 * (0.4 + 0.6 * p.d / 128), piece = (double)p.total_q * p.Hq * (p.d + 2) * 1.6e-6;
+  const double wgs = (double)((p.G + 15) / 16) * ((double)((p.total_q + per - 1) / per) + 1.1 * p.batch) * p.Hkv;
+  const double pair = 1.5 * (0.2 + 0.8 * p.d / 128), piece = (double)p.total_q * p.Hq * (p.d + 2) * 1.9e-6;
   plan.us = 0;
   for (int waves : {4, 8})
-    for (int64_t part = 4; part <= 32; part += 4) {  // (the columns of 32 pairs' blocks lie in the lanes)
+    for (int64_t part : {4, 8, 12, 16, 24, 32}) {  // (the columns of 32 pairs' blocks lie in the lanes)
       const int64_t parts = (pairs + part - 1) / part;
       if (parts > most_parts) continue;
-      const double load = std::max(1.0, wgs * (double)parts / compute_units() / (waves == 4 ? 1.74 : 0.82));
-      const double us = 5.3 + (double)((std::min(part, pairs) + waves - 1) / waves) * pair * load + (parts > 1 ? 6.1 + (double)parts * piece : 0.0);
+      const double load = std::max(1.0, wgs * (double)parts / compute_units() / (waves == 4 ? 1.4 : 0.68));
+      const double us = 6.6 + (double)((std::min(part, pairs) + waves - 1) / waves) * pair * load + (parts > 1 ? 3.7 + (double)parts * piece : 0.0);
       if (plan.us == 0 || us < plan.us) plan = RowsPlan{waves, (int)part, (int)parts, us};
     }
   return plan.us > 0;
