@@ -110,14 +110,6 @@ void mha_varlen_fwd_paged_window_impl(const hipattn_tensor *q, const hipattn_ten
   p.n_parts = 1;
   p.part_tiles = 1 << 24;
   p.part_acc = p.part_ml = nullptr;
-  hipStream_t stream = resolve_stream(stream_arg);
-  const int force = tuning().prefill_kernel;
-  const bool lse_or_f32 = lse != nullptr || p.out_f32;  // (neither the merges nor the kernel of decode rows have them)
-  // Block images go into LDS as they are where they fill most of their place there; else tiles are staged through registers.
-  const bool images = p.vc_block % 8 == 0 && p.vc_head % 8 == 0 && tuning().paged_prefill_dma != 0 && p.d <= 128 && (p.d >= 64 || p.d == 32);
-  const bool eight = images && (force == 1 || (force == 0 && eight_wavefronts_pay(p)));
-  // What pieces need lies in the caller's workspace or a buffer of the stream's, of one size, so that either gives the same bits; without it -- in a
-  // capture, for shapes beyond it, on hipStreamPerThread, one handle for a stream of each thread's own -- nothing is cut that has to be merged.
   char *given = nullptr;
   if (workspace) {
     const size_t need = scratch_bytes(p.total_q, p.Hq, p.d);
@@ -128,6 +120,14 @@ void mha_varlen_fwd_paged_window_impl(const hipattn_tensor *q, const hipattn_ten
              (long long)workspace->sizes[0], need);
     given = static_cast<char *>(workspace->data);
   }
+  hipStream_t stream = resolve_stream(stream_arg);
+  const int force = tuning().prefill_kernel;
+  const bool lse_or_f32 = lse != nullptr || p.out_f32;  // (neither the merges nor the kernel of decode rows have them)
+  // Block images go into LDS as they are where they fill most of their place there; else tiles are staged through registers.
+  const bool images = p.vc_block % 8 == 0 && p.vc_head % 8 == 0 && tuning().paged_prefill_dma != 0 && p.d <= 128 && (p.d >= 64 || p.d == 32);
+  const bool eight = images && (force == 1 || (force == 0 && eight_wavefronts_pay(p)));
+  // What pieces need lies in the caller's workspace or a buffer of the stream's, of one size, so that either gives the same bits; without it -- in a
+  // capture, for shapes beyond it, on hipStreamPerThread, one handle for a stream of each thread's own -- nothing is cut that has to be merged.
   HeldWorkspace ws;
   void *scratch = given;
   int most = (stream == hipStreamPerThread && !given) || lse_or_f32 || force != 0 || eight
