@@ -73,29 +73,34 @@ struct RowBlock {
 // The id-th block of `size` rows, at most `most` of a sequence, where sequences' blocks lie one behind the other, a sequence's last one first; by
 // whole wavefronts.  A grid of as many blocks as the longest sequence has for each of them is mostly workgroups that end at once: with a
 // window of 1000 and sinks, 63 sequences of 20 new tokens beside one of 4096, 32 / 8 x 128 291 us that way, 150 so, 16 / 2 x 64 147 and 49; 100 of one
-// token beside one of 1000, 8 / 2 x 256 261 and 107; 8 of 65 to 1001, 16 / 2 x 64 48 to 49 and 41 to 49, whichever comes first.
-__device__ __forceinline__ RowBlock row_block_of(const int32_t *cu_q, int batch, int size, int most, int id) {
+// token beside one of 1000, 8 / 2 x 256 261 and 107; 8 of 65 to 1001, 16 / 2 x 64 48 to 49 and 40 to 48, whichever comes first.
+// Sequences of more than `keys` keys come first, as the launch otherwise ends with their long chains: a window of 2000, 30 of 1 to 300 of which half
+// have 3000 keys more, 16 / 2 x 64 80 us in order and 65 so, 32 / 8 x 128 144 and 135.  Half a window there: with all of it 20 of 50 to 297 behind 0 to
+// 1900, a window of 1500, 16 / 2 x 64 49 and 45 but 32 / 8 x 128, two workgroups to a compute unit, 99 and 110; so all of it for small heads alone.
+__device__ __forceinline__ RowBlock row_block_of(const int32_t *cu_q, const int32_t *context_lens, int keys, int batch, int size, int most,
+                                                 int id) {
   const int lane = threadIdx.x & 63;
-  for (int s0 = 0; s0 < batch; s0 += 64) {
-    const int s = s0 + lane;
-    int begin = 0, rows = 0;
-    if (s < batch) {
-      begin = cu_q[s];
-      rows = max(cu_q[s + 1] - begin, 0);
+  for (int turn = 0; turn < 2; turn++)
+    for (int s0 = 0; s0 < batch; s0 += 64) {
+      const int s = s0 + lane;
+      int begin = 0, rows = 0, upto = 0;
+      if (s < batch) {
+        begin = cu_q[s];
+        rows = max(cu_q[s + 1] - begin, 0);
+        if ((context_lens[s] > keys) == (turn == 0)) upto = min((rows + size - 1) / size, most);
+      }
+      for (int o = 1; o < 64 && o < batch; o <<= 1) {
+        const int t = __shfl_up(upto, o, 64);
+        if (lane >= o) upto += t;
+      }
+      const unsigned long long past = __ballot(upto > id);
+      if (past != 0) {
+        const int at = __builtin_ctzll(past);
+        return RowBlock{s0 + at, (int)__builtin_amdgcn_readlane(upto, at) - 1 - id, (int)__builtin_amdgcn_readlane(begin, at),
+                        (int)__builtin_amdgcn_readlane(rows, at)};
+      }
+      id -= __builtin_amdgcn_readlane(upto, min(batch - s0, 64) - 1);
     }
-    int upto = min((rows + size - 1) / size, most);
-    for (int o = 1; o < 64 && o < batch; o <<= 1) {
-      const int t = __shfl_up(upto, o, 64);
-      if (lane >= o) upto += t;
-    }
-    const unsigned long long past = __ballot(upto > id);
-    if (past != 0) {
-      const int at = __builtin_ctzll(past);
-      return RowBlock{s0 + at, (int)__builtin_amdgcn_readlane(upto, at) - 1 - id, (int)__builtin_amdgcn_readlane(begin, at),
-                      (int)__builtin_amdgcn_readlane(rows, at)};
-    }
-    id -= __builtin_amdgcn_readlane(upto, 63);
-  }
   return RowBlock{0, -1, 0, 0};
 }
 // Blocks of `size` rows that sequences of `rows` rows together, each of at most `most` blocks, can have; 0: as many as a grid of `most` for each.

@@ -98,7 +98,7 @@ __global__ __launch_bounds__(256) void prefill_varlen_kernel(PrefillParams p) {
   const bool listed = SINKS && p.row_blocks > 0;
   if constexpr (SINKS)
     if (listed) {
-      blk = row_block_of(p.cu_q, p.batch, BM, p.n_qblocks, id);
+      blk = row_block_of(p.cu_q, p.context_lens, p.win_left / 2, p.batch, BM, p.n_qblocks, id);
       if (blk.block < 0) return;
     }
   const int b = listed ? blk.seq : id % p.batch;

@@ -52,7 +52,7 @@ __global__ __launch_bounds__(WAVES * 64) void window_rows_kernel(RowsParams p) {
   id %= all_groups;
   RowBlock blk;
   if (p.listed > 0) {
-    blk = row_block_of(p.cu_q, p.batch, p.rows_per_group, p.row_groups, id);
+    blk = row_block_of(p.cu_q, p.cache.context_lens, p.cache.window_left / 2, p.batch, p.rows_per_group, p.row_groups, id);
   } else {
     blk.seq = id / p.row_groups;
     blk.block = id % p.row_groups;
@@ -216,8 +216,8 @@ void dispatch_rows(const RowsParams &p, int head_size, int block_size, hipStream
 }  // namespace
 
 // All in us, for each form: a launch, the chain of a wavefront's pairs, each longer where more workgroups run than some per compute unit (1.4 of
-// four wavefronts, 0.68 of eight), and the merge (prefill_window.hip's choose_parts says how far off the choice is).  us, prefill / here: 32 / 8 x 128, 1 x 2
-// over 64 keys 10.7 / 6.3, 16 x 5 over 500 21.6 / 10.0, 1 x 45 over 256 18.3 / 8.3, 2 x 2 over 2048 22.0 / 14.9, 8 x 16 over 512 23.8 / 10.0, 1 x 300 over
+// four wavefronts, 0.68 of eight), and the merge (prefill_window.hip's choose_parts says how far off the choice is).  us, prefill / here:
+// 32 / 8 x 128, 1 x 2 over 64 keys 10.7 / 6.3, 16 x 5 over 500 21.6 / 10.0, 1 x 45 over 256 18.3 / 8.3, 2 x 2 over 2048 22.0 / 14.9, 8 x 16 over 512 23.8 / 10.0, 1 x 300 over
 // 4096 47 / 86; 12 / 4 x 112, 64 x 4 over 1024 75 / 27, 4 x 64 over 2048 29 / 24; 16 / 2 x 64, 1 x 16 over 4096 16.0 / 10.2.
 bool plan_window_rows(const PrefillParams &p, int most_parts, RowsPlan &plan) {
   if (p.d != 64 && p.d != 80 && p.d != 96 && p.d != 112 && p.d != 128 && p.d != 256) return false;
