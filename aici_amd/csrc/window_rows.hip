@@ -35,7 +35,11 @@ struct RowsParams {
 __device__ __forceinline__ SeenKeys rows_see(const RowsParams &p, int Lq, int Lk, int i0, int i1) {
   return SeenKeys(p.cache, Lk - Lq + i1 + 1, i1 - i0 + 1);
 }
-__device__ __forceinline__ int seen_runs(const SeenKeys &s) { return s.ctx > 0 ? (s.ctx + kBlockSize - 1) / kBlockSize - 2 * s.skip : 0; }
+// Runs of 16 tokens that hold them.  The parts hold what max_seqlen_k allows: of a context beyond that the last ones are left out, as there is
+// neither a part nor scratch memory for them.
+__device__ __forceinline__ int seen_runs(const RowsParams &p, const SeenKeys &s) {
+  return s.ctx > 0 ? min((s.ctx + kBlockSize - 1) / kBlockSize - 2 * s.skip, 2 * p.part_pairs * p.num_parts) : 0;
+}
 
 template <typename T, int HD, int BS, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void window_rows_kernel(RowsParams p) {
@@ -65,7 +69,7 @@ __global__ __launch_bounds__(WAVES * 64) void window_rows_kernel(RowsParams p) {
   const int i1 = min(i0 + p.rows_per_group, Lq) - 1;
   const int Lk = p.cache.context_lens[seq];
   const SeenKeys seen = rows_see(p, Lq, Lk, i0, i1);
-  const int nblk = seen_runs(seen), b0 = part * p.part_pairs * 2;
+  const int nblk = seen_runs(p, seen), b0 = part * p.part_pairs * 2;
   if (b0 >= nblk && part > 0) return;
   const int nb = min(b0 + p.part_pairs * 2, nblk) - b0;  // runs of this part
   const int t0 = b0 * kBlockSize / BS, tn = p.part_pairs * 2 * kBlockSize / BS;
@@ -172,9 +176,9 @@ __global__ __launch_bounds__(128) void window_rows_merge_kernel(RowsParams p) {
   const int b = sequence_of_row(p.cu_q, p.batch, r);
   if (b < 0) return;
   const int q_begin = p.cu_q[b], Lq = p.cu_q[b + 1] - q_begin, i0 = (r - q_begin) / p.rows_per_group * p.rows_per_group;
-  const int nblk = seen_runs(rows_see(p, Lq, p.cache.context_lens[b], i0, min(i0 + p.rows_per_group, Lq) - 1));
+  const int nblk = seen_runs(p, rows_see(p, Lq, p.cache.context_lens[b], i0, min(i0 + p.rows_per_group, Lq) - 1));
   if (nblk <= p.part_pairs * 2) return;  // written
-  merge_parts<T, HD>(p, r, h0, min((nblk + p.part_pairs * 2 - 1) / (p.part_pairs * 2), p.num_parts));
+  merge_parts<T, HD>(p, r, h0, (nblk + p.part_pairs * 2 - 1) / (p.part_pairs * 2));
 }
 
 template <typename T, int HD>

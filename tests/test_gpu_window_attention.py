@@ -403,3 +403,23 @@ def test_chunks_with_a_workspace_of_the_callers(device, heads, lens_q, ctx):
         assert torch.equal(out, alone[(k + 1) % 2])
         assert torch.equal(chunk(x, device, workspace=store[:need]), out)
         assert bool((store[need:] == 255).all())
+
+
+@pytest.mark.parametrize("heads", [(8, 2, 64), (8, 2, 128), (4, 2, 256)])
+@pytest.mark.parametrize("kernel", [0, 5])
+def test_contexts_beyond_the_bound(device, tuning, heads, kernel):
+    """A sequence with more keys than max_seqlen_k: some of them may be left out, and nothing else changes -- not the other sequences, not
+    the caller's workspace behind what the call needs.  With a bound that one part holds, and with one that several do."""
+    tuning("prefill_kernel", kernel)
+    for bound_k, lens_q, ctx in ((64, [3, 5], [2000, 40]), (1500, [2, 7, 1], [2900, 1400, 1500])):
+        c = case(700 + bound_k, lens_q, ctx, heads, torch.bfloat16, 3000, 5)
+        bare = [c[k].to(device) for k in ("q", "kc", "vc", "tables")]
+        need = K.flash_attn_varlen_paged_window_workspace_size(sum(lens_q), heads[0], heads[2])
+        for store in (None, torch.full((need + 4096,), 255, dtype=torch.uint8, device=device)):
+            out = K.flash_attn_varlen_paged_window(*bare, W.offsets(lens_q).to(device), torch.tensor(ctx, dtype=torch.int32, device=device),
+                                                   max(lens_q), bound_k, c["scale"], 3000, 5, workspace=None if store is None else store[:need])
+            first = lens_q[0]
+            assert bool((out[:first].abs() <= 1.01 * bare[2].nan_to_num(0).abs().max()).all())  # (no NaN: an average of some values)
+            expect, mass, _ = want(c)
+            check(out[first:], c, (expect[first:], mass[first:], None))
+            assert store is None or bool((store[need:] == 255).all())
