@@ -24,6 +24,7 @@ __global__ __launch_bounds__(128) void window_merge_kernel(WindowParams p) {
   const int b = sequence_of_row(p.cu_q, p.batch, r);
   if (b < 0) return;
   const int q_begin = p.cu_q[b], Lq = p.cu_q[b + 1] - q_begin, Lk = p.context_lens[b];
+  if ((r - q_begin) / p.block_rows >= p.n_qblocks) return;  // beyond max_seqlen_q: left out
   const int first_row = (r - q_begin) / p.block_rows * p.block_rows, last_row = min(first_row + p.block_rows, Lq) - 1;  // of the row's block
   int tiles = (max(min(Lk, last_row + Lk - Lq + 1), 0) + BN - 1) / BN;
   const int seen_from = max(first_row + Lk - Lq - p.win_left, 0);  // (the kernel's arithmetic)

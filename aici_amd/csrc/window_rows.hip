@@ -175,7 +175,8 @@ __global__ __launch_bounds__(128) void window_rows_merge_kernel(RowsParams p) {
   const int r = blockIdx.x / head_blocks, h0 = blockIdx.x % head_blocks * kMergeHeads;
   const int b = sequence_of_row(p.cu_q, p.batch, r);
   if (b < 0) return;
-  const int q_begin = p.cu_q[b], Lq = p.cu_q[b + 1] - q_begin, i0 = (r - q_begin) / p.rows_per_group * p.rows_per_group;
+  const int q_begin = p.cu_q[b], Lq = p.cu_q[b + 1] - q_begin, group = (r - q_begin) / p.rows_per_group, i0 = group * p.rows_per_group;
+  if (group >= p.row_groups) return;  // beyond max_seqlen_q: left out
   const int nblk = seen_runs(p, rows_see(p, Lq, p.cache.context_lens[b], i0, min(i0 + p.rows_per_group, Lq) - 1));
   if (nblk <= p.part_pairs * 2) return;  // written
   merge_parts<T, HD>(p, r, h0, (nblk + p.part_pairs * 2 - 1) / (p.part_pairs * 2));

@@ -423,3 +423,20 @@ def test_contexts_beyond_the_bound(device, tuning, heads, kernel):
             expect, mass, _ = want(c)
             check(out[first:], c, (expect[first:], mass[first:], None))
             assert store is None or bool((store[need:] == 255).all())
+
+
+@pytest.mark.parametrize("heads", [(8, 2, 64), (8, 2, 128), (8, 8, 256)])
+def test_rows_beyond_the_bound(device, heads):
+    """A sequence with more new tokens than max_seqlen_q: a row beyond is left as it was or right, never made of scratch memory."""
+    lens_q, ctx, bound_q = [40, 3, 8], [2600, 900, 2000], 8
+    c = case(750, lens_q, ctx, heads, torch.bfloat16, 2500, 30)
+    bare = [c[k].to(device) for k in ("q", "kc", "vc", "tables")]
+    expect, mass, _ = want(c)
+    need = K.flash_attn_varlen_paged_window_workspace_size(sum(lens_q), heads[0], heads[2])
+    for store in (None, torch.full((need,), 255, dtype=torch.uint8, device=device)):  # (NaN, read as fp32)
+        out = torch.full_like(bare[0], 7.0)
+        _native.mha_varlen_fwd_paged_window(*bare, W.offsets(lens_q).to(device), torch.tensor(ctx, dtype=torch.int32, device=device), bound_q,
+                                            max(ctx), c["scale"], 2500, 30, out, None, store)
+        left = (out == 7).flatten(1).all(1).cpu()
+        assert not bool(left[:bound_q].any()) and not bool(left[40:].any())
+        check(out[~left], c, (expect[~left], mass[~left], None))
