@@ -447,7 +447,7 @@ __global__ __launch_bounds__(768) void prefill_varlen_r3_kernel(PrefillParams p)
           }
         }
     }
-    if (p.lse != nullptr && g_e == 0) {
+    if (p.lse != nullptr && g_e == 0 && row < p.lse_pitch) {
       // Natural-log sum-exp of the scaled scores; +inf for a row without keys (flash_fwd_kernel.h:629-668).
       const float lse = l_tot > 0.f ? (m_run + __builtin_amdgcn_logf(l_tot)) * kLn2 : INFINITY;
       p.lse[((int64_t)b * p.Hq + h) * p.lse_pitch + row] = lse;

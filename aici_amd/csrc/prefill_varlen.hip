@@ -454,7 +454,7 @@ __global__ __launch_bounds__(256) void prefill_varlen_kernel(PrefillParams p) {
           *reinterpret_cast<u32x2_t *>(op + (int64_t)row * p.o_row + dcol) = *reinterpret_cast<u32x2_t *>(r);
         }
       }
-    if (p.lse != nullptr && g == 0) {
+    if (p.lse != nullptr && g == 0 && row < p.lse_pitch) {
       // Natural-log sum-exp of the scaled scores; +inf for a row without keys
       // (flash_fwd_kernel.h:629-668).
       const float lse = l_tot > 0.f ? (m_run[qt] + __builtin_amdgcn_logf(l_tot)) * kLn2 : INFINITY;

@@ -1151,7 +1151,7 @@ __global__ __launch_bounds__(NW * 64, STEP::value ? 2 : w8_wavefronts(HDP, NW)) 
           }
         }
     }
-    if (p.lse != nullptr && g_e == 0 && row < Lq) {
+    if (p.lse != nullptr && g_e == 0 && row < min(Lq, p.lse_pitch)) {
       const float lse = l_tot > 0.f ? (m_run + __builtin_amdgcn_logf(l_tot)) * kLn2 : INFINITY;
       p.lse[((int64_t)b * p.Hq + h_e) * p.lse_pitch + row] = lse;
     }
@@ -1177,7 +1177,7 @@ __global__ __launch_bounds__(NW * 64, STEP::value ? 2 : w8_wavefronts(HDP, NW)) 
       __builtin_nontemporal_store(*reinterpret_cast<const u32x4_t *>(ost + r * OSTR + ch * 8),
                                   reinterpret_cast<u32x4_t *>(op + (int64_t)row * p.o_row + ch * 8));
   }
-  if (p.lse != nullptr && g_e == 0 && wave_row0_e + c_e < Lq) {
+  if (p.lse != nullptr && g_e == 0 && wave_row0_e + c_e < min(Lq, p.lse_pitch)) {
     const float lse = l_tot > 0.f ? (m_run + __builtin_amdgcn_logf(l_tot)) * kLn2 : INFINITY;
     p.lse[((int64_t)b * p.Hq + h_e) * p.lse_pitch + wave_row0_e + c_e] = lse;
   }

@@ -440,3 +440,27 @@ def test_rows_beyond_the_bound(device, heads):
         left = (out == 7).flatten(1).all(1).cpu()
         assert not bool(left[:bound_q].any()) and not bool(left[40:].any())
         check(out[~left], c, (expect[~left], mass[~left], None))
+
+
+@pytest.mark.parametrize("kernel,images,heads", [(5, -1, (8, 2, 64)), (1, -1, (8, 2, 128)), (5, 0, (8, 2, 128)), (0, -1, (4, 2, 160))])
+def test_lse_of_rows_beyond_the_bound(device, tuning, kernel, images, heads):
+    """An LSE holds max_seqlen_q rows a head: a sequence with more new tokens writes nothing into the next head's, or behind the last."""
+    tuning("prefill_kernel", kernel)
+    tuning("paged_prefill_dma", images)
+    lens_q, ctx, bound_q = [8, 3, 50], [60, 90, 200], 8
+    c = case(760, lens_q, ctx, heads, torch.bfloat16, 100, 3)
+    bare = [c[k].to(device) for k in ("q", "kc", "vc", "tables")]
+    expect = want(c)
+    for dtype in (torch.bfloat16, torch.float32):
+        frame = torch.full((3 * heads[0] * bound_q + 256,), 7.0, dtype=torch.float32, device=device)
+        lse = frame[:3 * heads[0] * bound_q].view(3, heads[0], bound_q)
+        out = torch.full_like(bare[0], 7.0, dtype=dtype)
+        _native.mha_varlen_fwd_paged_window(*bare, W.offsets(lens_q).to(device), torch.tensor(ctx, dtype=torch.int32, device=device), bound_q,
+                                            max(ctx), c["scale"], 100, 3, out, lse, None)
+        assert bool((frame[lse.numel():] == 7).all())
+        row = 0
+        for b, n in enumerate(lens_q):
+            n = min(n, bound_q)
+            assert float((lse[b, :, :n].cpu().double() - expect[2][row:row + n].T).abs().max()) < 2e-3
+            assert bool((lse[b, :, n:] == 7).all())
+            row += lens_q[b]
