@@ -727,8 +727,8 @@ void bias_argmax_impl(const hipattn_tensor *logits, const hipattn_tensor *bias, 
     chunks = (V + per_slice - 1) / per_slice;
     // The row states are cleared on the stream in front of every launch: a call never depends on what the
     // one before it (or a replay of a captured graph overlapping it on another stream) left behind.
-    ArgmaxRowState *st =
-        static_cast<ArgmaxRowState *>(library_workspace(WS_BIAS_ARGMAX, (size_t)S * sizeof(ArgmaxRowState), stream));
+    const HeldWorkspace ws = library_workspace(WS_BIAS_ARGMAX, (size_t)S * sizeof(ArgmaxRowState), stream);
+    ArgmaxRowState *st = static_cast<ArgmaxRowState *>(ws.ptr);
     argmax_state_clear_kernel<<<dim3((unsigned)((S + 255) / 256)), 256, 0, stream>>>(st, (int)S);
     int32_t *ot = static_cast<int32_t *>(out_tokens->data);
     const dim3 grid((unsigned)chunks, (unsigned)S);

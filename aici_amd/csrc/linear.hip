@@ -1182,6 +1182,7 @@ void linear_impl(hipattn_tensor *out, const hipattn_tensor *x, const hipattn_ten
   p.total_stages = (int)(K / kLinStageK);
   p.half = gated ? (int)(N / 2) : 0;
   hipStream_t stream = resolve_stream(stream_arg);
+  HeldWorkspace held;  // over all launches
   if (pl.partial_bytes > 0 && !pl.stream) {  // (the few-rows kernel leaves finished rows: a launch of rms_norm normalises them)
     if (workspace != nullptr) {
       check_tensor(workspace, "workspace", 1);
@@ -1192,7 +1193,8 @@ void linear_impl(hipattn_tensor *out, const hipattn_tensor *x, const hipattn_ten
       check_data(workspace, "workspace");
       p.partial = static_cast<float *>(workspace->data);
     } else {
-      p.partial = static_cast<float *>(library_workspace(WS_LINEAR, pl.partial_bytes, stream));
+      held = library_workspace(WS_LINEAR, pl.partial_bytes, stream);
+      p.partial = static_cast<float *>(held.ptr);
     }
   }
   if (qkv != nullptr) {
@@ -1204,6 +1206,7 @@ void linear_impl(hipattn_tensor *out, const hipattn_tensor *x, const hipattn_ten
       // A row and the one that it is rotated with would have to share an order of k, and here they may have different ones (heads of 80, 96,
       // 256, ...): the calls themselves, with their bits.  us, an order without turns in one launch / the calls: 9216 x 2048 16 rows 12.5 /
       // 16.4, 12288 x 4096 16 and 64 rows 25.0 / 27.3, 29.6 / 31.2, 15360 x 8192 64 rows 64.7 / 57.0, 21504 x 8192 16 rows 80.5 / 63.4.
+      held = HeldWorkspace{};  // (the call below takes it for itself)
       linear_impl(out, x, weight, nullptr, nullptr, nullptr, stream_arg, nullptr, nullptr, norm_weight, eps, false, false, norm_in);
       const int hd = p.qkv.g.head_size, Hkv = p.qkv.g.num_heads;
       auto columns = [&](int64_t first, int64_t heads) {

@@ -237,9 +237,10 @@ char *static_scratch() {
   return ptr;
 }
 
-// The scratch memory of one call (pl.bytes of it; nothing in it outlives the call).
-char *scratch_memory(const Scratch &from, const DecodePlan &pl, hipStream_t stream, const char *op) {
-  if (pl.bytes == 0) return nullptr;
+// The scratch memory of one call (pl.bytes of it; nothing in it outlives the call), the library's held for it.
+HeldWorkspace scratch_memory(const Scratch &from, const DecodePlan &pl, hipStream_t stream, const char *op) {
+  HeldWorkspace ws;
+  if (pl.bytes == 0) return ws;
   switch (from.kind) {
     case Scratch::CALLER:
       HA_CHECK(from.ptr != nullptr, "%s: workspace is NULL but %zu bytes are needed", op, pl.bytes);
@@ -247,15 +248,17 @@ char *scratch_memory(const Scratch &from, const DecodePlan &pl, hipStream_t stre
       HA_CHECK(from.bytes >= 0 && (size_t)from.bytes >= pl.bytes,
                "%s: workspace of %lld bytes is too small, %zu are needed (hipattn_paged_attention_workspace_size)", op,
                (long long)from.bytes, pl.bytes);
-      return static_cast<char *>(from.ptr);
+      ws.ptr = from.ptr;
+      return ws;
     case Scratch::STATIC:
       HA_CHECK(pl.bytes <= kStaticScratchBytes,
                "%s: this call needs %zu bytes of scratch memory, more than the %zu bytes of the built-in array; use "
                "hipattn_paged_attention_v1 or hipattn_paged_attention_v1_ws for it",
                op, pl.bytes, kStaticScratchBytes);
-      return static_scratch();
+      ws.ptr = static_scratch();
+      return ws;
     default:
-      return static_cast<char *>(library_workspace(WS_PAGED_ATTENTION, pl.bytes, stream));
+      return library_workspace(WS_PAGED_ATTENTION, pl.bytes, stream);
   }
 }
 
@@ -485,6 +488,7 @@ void paged_attention_impl(hipattn_tensor *out, hipattn_tensor *exp_sums, hipattn
   // The MFMA kernels take the 2-byte types at the reference's head sizes; fp32 caches go to the fp32-FMA kernel.
   const bool generic = takes_generic_kernel(query->dtype, block_size, hd);
   hipStream_t stream = resolve_stream(stream_arg);
+  HeldWorkspace held;  // over all launches
   if (v2) {
     check_tensor(exp_sums, "exp_sums", 3);
     check_tensor(max_logits, "max_logits", 3);
@@ -527,7 +531,8 @@ void paged_attention_impl(hipattn_tensor *out, hipattn_tensor *exp_sums, hipattn
     p.tmp_out = tmp_out->data;
   } else {
     const DecodePlan pl = plan_decode(S, Hq, num_kv_heads, hd, block_size, query->dtype, max_context_len);
-    char *ws = scratch_memory(scratch_from, pl, stream, op);
+    held = scratch_memory(scratch_from, pl, stream, op);
+    char *ws = static_cast<char *>(held.ptr);
     if (pl.generic) {
       paged_decode_generic(generic_params(p, hd, block_size, scale), query->dtype, false, max_context_len, pl.num_parts,
                            reinterpret_cast<float *>(ws), stream);

@@ -37,12 +37,19 @@ constexpr int kMaxDevices = 64;
 struct ScratchKey {
   int user, device;
   hipStream_t stream;
+  uint64_t thread;  // 0 but on hipStreamPerThread, one handle for a stream of each thread's own
   bool operator<(const ScratchKey &o) const {
     if (user != o.user) return user < o.user;
     if (device != o.device) return device < o.device;
-    return stream < o.stream;
+    if (stream != o.stream) return stream < o.stream;
+    return thread < o.thread;
   }
 };
+uint64_t stream_thread(hipStream_t stream) {
+  static std::atomic<uint64_t> threads{0};
+  thread_local const uint64_t mine = ++threads;
+  return stream == hipStreamPerThread ? mine : 0;
+}
 struct ScratchBuffer {
   void *ptr = nullptr;
   size_t bytes = 0;
@@ -101,14 +108,19 @@ hipStream_t resolve_stream(void *stream) {
   return tl_current_stream;
 }
 
-// The buffer of (user, current device, stream), at least `bytes` large; where it has to be allocated, `spare` more.
-static ScratchBuffer &scratch_buffer(WorkspaceUser user, size_t bytes, size_t spare, hipStream_t stream) {
+// The buffer of (user, current device, stream), at least `bytes` large; where it has to be allocated, `spare` more.  Its address as it is now
+// (a larger one may replace it, which leaves this one alive), and what is to be locked while launches share it.
+struct FoundScratch {
+  void *ptr;
+  std::mutex *holder;
+};
+static FoundScratch scratch_buffer(WorkspaceUser user, size_t bytes, size_t spare, hipStream_t stream) {
   int dev = 0;
   HA_HIP(hipGetDevice(&dev));
   HA_CHECK(dev >= 0 && dev < kMaxDevices, "device index %d out of range", dev);
   std::lock_guard<std::mutex> lock(g_mutex);
-  ScratchBuffer &ws = g_scratch[ScratchKey{(int)user, dev, stream}];
-  if (ws.bytes >= bytes && ws.ptr != nullptr) return ws;
+  ScratchBuffer &ws = g_scratch[ScratchKey{(int)user, dev, stream, stream_thread(stream)}];
+  if (ws.bytes >= bytes && ws.ptr != nullptr) return FoundScratch{ws.ptr, &ws.holder};
   // Allocating is not something a capture can record, and the graph would keep the old pointer.
   hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
   const hipError_t asked = hipStreamIsCapturing(stream, &capturing);
@@ -135,44 +147,46 @@ static ScratchBuffer &scratch_buffer(WorkspaceUser user, size_t bytes, size_t sp
   g_lib_allocated[dev] += (int64_t)want;
   ws.ptr = fresh;
   ws.bytes = want;
+  return FoundScratch{ws.ptr, &ws.holder};
+}
+
+static HeldWorkspace hold(const FoundScratch &found) {
+  HeldWorkspace ws;
+  ws.ptr = found.ptr;
+  if (found.holder != nullptr) ws.held = std::unique_lock<std::mutex>(*found.holder);
   return ws;
 }
 
-void *library_workspace(WorkspaceUser user, size_t bytes, hipStream_t stream) {
-  return scratch_buffer(user, bytes, bytes / 2, stream).ptr;
+HeldWorkspace library_workspace(WorkspaceUser user, size_t bytes, hipStream_t stream) {
+  return hold(scratch_buffer(user, bytes, bytes / 2, stream));
 }
 
-// scratch_buffer, or null where it throws and while the stream is being captured.
-static ScratchBuffer *try_scratch_buffer(WorkspaceUser user, size_t bytes, size_t spare, hipStream_t stream) {
+// scratch_buffer, or nulls where it throws and while the stream is being captured.
+static FoundScratch try_scratch_buffer(WorkspaceUser user, size_t bytes, size_t spare, hipStream_t stream) {
+  FoundScratch found = {nullptr, nullptr};
   hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
   if (hipStreamIsCapturing(stream, &capturing) != hipSuccess) {
     (void)hipGetLastError();
-    return nullptr;
+    return found;
   }
-  if (capturing != hipStreamCaptureStatusNone) return nullptr;
+  if (capturing != hipStreamCaptureStatusNone) return found;
   // A capture on some other stream forbids allocations, in every thread unless the thread says otherwise.
   hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
   if (hipThreadExchangeStreamCaptureMode(&mode) != hipSuccess) {
     (void)hipGetLastError();
-    return nullptr;
+    return found;
   }
-  ScratchBuffer *buffer = nullptr;
   try {
-    buffer = &scratch_buffer(user, bytes, spare, stream);
+    found = scratch_buffer(user, bytes, spare, stream);
   } catch (const Error &) {
     (void)hipGetLastError();
   }
   (void)hipThreadExchangeStreamCaptureMode(&mode);
-  return buffer;
+  return found;
 }
 
 HeldWorkspace try_library_workspace(WorkspaceUser user, size_t bytes, hipStream_t stream) {
-  HeldWorkspace ws;
-  if (ScratchBuffer *buffer = try_scratch_buffer(user, bytes, 0, stream)) {
-    ws.ptr = buffer->ptr;
-    ws.held = std::unique_lock<std::mutex>(buffer->holder);
-  }
-  return ws;
+  return hold(try_scratch_buffer(user, bytes, 0, stream));
 }
 
 void reserve_library_workspace(WorkspaceUser user, size_t bytes, hipStream_t stream) {

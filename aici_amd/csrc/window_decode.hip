@@ -92,6 +92,7 @@ void paged_attention_window_impl(hipattn_tensor *out, const hipattn_tensor *quer
   const DecodePlan pl = plan_decode(p.num_seqs, p.Hq, num_kv_heads, hd, block_size, query->dtype,
                                     (int)seen_tokens(p.max_ctx, window_left, sinks));
   char *ws = nullptr;
+  HeldWorkspace held;  // over both launches
   if (pl.bytes > 0 && workspace) {
     HA_CHECK(workspace->data != nullptr && (reinterpret_cast<uintptr_t>(workspace->data) & 255) == 0,
              "%s: workspace must be 256-byte aligned", op);
@@ -100,7 +101,8 @@ void paged_attention_window_impl(hipattn_tensor *out, const hipattn_tensor *quer
              (long long)workspace->sizes[0], pl.bytes);
     ws = static_cast<char *>(workspace->data);
   } else if (pl.bytes > 0) {
-    ws = static_cast<char *>(library_workspace(WS_WINDOW_ATTENTION, pl.bytes, stream));
+    held = library_workspace(WS_WINDOW_ATTENTION, pl.bytes, stream);
+    ws = static_cast<char *>(held.ptr);
   }
   if (!pl.flat) {
     p.part_blocks = pl.part_blocks;

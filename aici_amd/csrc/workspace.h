@@ -12,23 +12,25 @@ namespace hipattn {
 enum WorkspaceUser { WS_PAGED_ATTENTION = 0, WS_BIAS_ARGMAX = 1, WS_LINEAR = 2, WS_SAMPLE = 3, WS_STEP_ATTENTION = 4,
                      WS_WINDOW_ATTENTION = 5, WS_WINDOW_CHUNKS = 6 };
 
+// A stream's scratch memory, and the right to it: until `held` goes, no call of another thread on that stream gets it.  A call keeps it over
+// all its launches: the work of two calls is then in order on the stream, where the launches of one could else come between those of the other.
+struct HeldWorkspace {
+  void *ptr = nullptr;
+  std::unique_lock<std::mutex> held;
+};
+
 // Returns at least `bytes` of device memory on the current device for `user`,
-// private to `stream`: calls on different streams never share a buffer, so
+// private to `stream` (on hipStreamPerThread, to the calling thread): calls on different streams never share a buffer, so
 // they may overlap.  A buffer is zero-filled when it is allocated.  Growing allocates a new buffer and
 // keeps the old one alive until hipattn_shutdown (work already enqueued, or a
 // captured graph, may still point at it); nothing is synchronised.  A stream
 // that is being captured cannot grow its buffer: the call fails with a
 // message that says so.
-void *library_workspace(WorkspaceUser user, size_t bytes, hipStream_t stream);
+HeldWorkspace library_workspace(WorkspaceUser user, size_t bytes, hipStream_t stream);
 
-// A buffer that several launches of a call share, for an op that has another way without: null while the stream is being captured
+// The same for an op that has another way without: null while the stream is being captured
 // (also where the buffer is there: a graph may be replayed on any stream, beside calls that use it) and where there is no memory to be
-// had.  `bytes` is the op's constant -- the buffer has that size and never grows -- and no other call, of another thread on this stream,
-// gets the buffer while `held` lives.
-struct HeldWorkspace {
-  void *ptr = nullptr;
-  std::unique_lock<std::mutex> held;
-};
+// had.  `bytes` is the op's constant: the buffer has that size and never grows.
 HeldWorkspace try_library_workspace(WorkspaceUser user, size_t bytes, hipStream_t stream);
 
 // library_workspace ahead of need: what a later call of the same shapes asks for while the stream is being captured.  Does nothing where

@@ -135,7 +135,10 @@ char *hipattn_mha_varlen_fwd_paged_window_workspace_size(int64_t total_q, int nu
  * [nb, Hkv, d, BS]; block_tables int32 [S, max_blocks]; context_lens int32 [S].
  * alibi_slopes f32 [Hq] or NULL.  A context length above max_context_len is
  * cut there.  Runs the split-K kernels on scratch memory the library owns: one
- * buffer per (device, stream), so calls on different streams may overlap; it
+ * buffer per (device, stream), so calls on different streams may overlap, and
+ * threads may share a stream (a call has the buffer to itself until its
+ * launches are enqueued; hipStreamPerThread counts as one stream per thread, each
+ * with a buffer until hipattn_shutdown); it
  * grows with hipMalloc when a call needs more than it has (the old buffer stays
  * alive until hipattn_shutdown, nothing is synchronised); a stream that is being
  * captured into a graph cannot grow it -- run the call once with the largest
@@ -218,8 +221,8 @@ char *hipattn_paged_attention_workspace_size(int64_t num_seqs, int num_heads,
  * sinks and the window may name any block or none, and their blocks hold anything.  f16 and bf16 caches, head sizes 64, 80, 96, 112, 128
  * and 256, block sizes 8, 16 and 32; window_size_left >= 0, sink_tokens >= 0; arguments else as for hipattn_paged_attention_v1.
  * workspace: u8, 256-byte aligned, hipattn_paged_attention_window_workspace_size bytes -- a function of the shapes, max_context_len, the
- * window and the sinks -- or NULL for a buffer that the library keeps per stream, with what hipattn_paged_attention_v1 says about captures
- * and overlapping calls. */
+ * window and the sinks -- or NULL for a buffer that the library keeps per stream, with what hipattn_paged_attention_v1 says about captures,
+ * threads and overlapping calls. */
 char *hipattn_paged_attention_window(hipattn_tensor *out, const hipattn_tensor *query,
                                      const hipattn_tensor *key_cache, const hipattn_tensor *value_cache,
                                      int num_kv_heads, float scale, const hipattn_tensor *block_tables,
