@@ -101,6 +101,7 @@ void mha_varlen_fwd_paged_window_impl(const hipattn_tensor *q, const hipattn_ten
   if (!paged_prefill_params(PagedPrefillCall{q, key_cache, value_cache, block_tables, cu_q, context_lens, max_q, max_k, scale, true, op}, out,
                             lse, p))
     return;
+  p.max_q = (int)std::min<int64_t>(p.max_q, p.total_q);  // (no sequence has more; what is rounded up to row blocks stays within 32 bits)
   // (no context is longer than its table: what lies beyond that sees everything, and row + Lk - Lq - window_left stays within 32 bits)
   const int64_t longest = (int64_t)p.table_cols << p.block_log2;
   p.win_left = (int)std::min<int64_t>(window_left, std::min<int64_t>(longest, 1 << 30));

@@ -464,3 +464,18 @@ def test_lse_of_rows_beyond_the_bound(device, tuning, kernel, images, heads):
             assert float((lse[b, :, :n].cpu().double() - expect[2][row:row + n].T).abs().max()) < 2e-3
             assert bool((lse[b, :, n:] == 7).all())
             row += lens_q[b]
+
+
+@pytest.mark.parametrize("heads", [(8, 2, 64), (16, 1, 128), (4, 2, 160)])
+def test_bounds_of_31_bits(device, tuning, heads):
+    """max_seqlen_q far beyond the rows there are, as the header allows: the launch is one over those there are."""
+    lens_q, ctx = [3, 70, 1], [30, 400, 90]
+    c = case(770, lens_q, ctx, heads, torch.bfloat16, 150, 3)
+    bare = [c[k].to(device) for k in ("q", "kc", "vc", "tables")]
+    expect = want(c)
+    for kernel in (0, 5, 1):
+        tuning("prefill_kernel", kernel)
+        for bound in (2 ** 31 - 1, 2 ** 31 - 64):
+            out = K.flash_attn_varlen_paged_window(*bare, W.offsets(lens_q).to(device), torch.tensor(ctx, dtype=torch.int32, device=device),
+                                                   bound, max(ctx), c["scale"], 150, 3)
+            check(out, c, expect)
