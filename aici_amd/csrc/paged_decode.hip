@@ -366,7 +366,7 @@ bool decode_params(const DecodeCall &c, hipattn_tensor *out, DecodeParams &p) {
   check_contiguous(context_lens, "context_lens");
   HA_CHECK(block_tables->sizes[1] <= 1 || block_tables->strides[1] == 1, "%s: block_tables rows must be contiguous", op);
   HA_CHECK(max_context_len >= 0, "%s: negative max_context_len", op);
-  HA_CHECK((int64_t)(max_context_len + block_size - 1) / block_size <= block_tables->sizes[1],
+  HA_CHECK(((int64_t)max_context_len + block_size - 1) / block_size <= block_tables->sizes[1],
            "%s: max_context_len %d needs more than the %lld block-table columns", op, max_context_len,
            (long long)block_tables->sizes[1]);
   if (alibi) {

@@ -219,3 +219,13 @@ def test_chunk_workspace_sizes():
         size(-1, 8, 128)
     with pytest.raises(_lib.HipAttnError, match="head size 257"):
         size(4, 8, 257)
+
+
+@pytest.mark.parametrize("max_ctx", [2 ** 31 - 1, 2 ** 31 - 15])
+def test_paged_attention_refuses_context_bounds_of_31_bits(max_ctx):
+    """(rounded up to blocks they leave 32 bits)"""
+    with pytest.raises(_lib.HipAttnError, match="block-table columns"):
+        _call("hipattn_paged_attention_window", *_decode_args(max_ctx=max_ctx))
+    a = _decode_args(max_ctx=max_ctx)
+    with pytest.raises(_lib.HipAttnError, match="block-table columns"):
+        _call("hipattn_paged_attention_v1", *a[:10], None, None)
