@@ -84,6 +84,10 @@ size_t piece_bytes(int64_t total_q, int heads, int d) { return (size_t)total_q *
 size_t scratch_bytes(int64_t total_q, int heads, int d) {
   return kMostParts * std::min(piece_bytes(total_q, heads, d), kWindowScratchBytes / kMostParts);
 }
+// Pieces that it holds, at most.
+int held_parts(int64_t total_q, int heads, int d) {
+  return (int)std::max<size_t>(std::min<size_t>(kWindowScratchBytes / piece_bytes(total_q, heads, d), kMostParts), 1);
+}
 
 void mha_varlen_fwd_paged_window_impl(const hipattn_tensor *q, const hipattn_tensor *key_cache, const hipattn_tensor *value_cache,
                                       const hipattn_tensor *block_tables, const hipattn_tensor *cu_q, const hipattn_tensor *context_lens,
@@ -111,9 +115,13 @@ void mha_varlen_fwd_paged_window_impl(const hipattn_tensor *q, const hipattn_ten
   p.n_parts = 1;
   p.part_tiles = 1 << 24;
   p.part_acc = p.part_ml = nullptr;
+  const int force = tuning().prefill_kernel;
+  const bool lse_or_f32 = lse != nullptr || p.out_f32;  // (neither the merges nor the kernel of decode rows have them)
+  const bool merged_head = p.d == 64 || p.d == 80 || p.d == 96 || p.d == 112 || p.d == 128;  // (there is a merge for it; 256: decode rows alone)
+  const int possible = lse_or_f32 || force != 0 || !(merged_head || p.d == 256) ? 1 : held_parts(p.total_q, p.Hq, p.d);
   char *given = nullptr;
-  if (workspace) {
-    const size_t need = scratch_bytes(p.total_q, p.Hq, p.d);
+  if (workspace && possible > 1) {  // (else there is nothing to put there)
+    const size_t need = possible * piece_bytes(p.total_q, p.Hq, p.d);
     HA_CHECK(workspace->data != nullptr && (reinterpret_cast<uintptr_t>(workspace->data) & 255) == 0,
              "%s: workspace must be 256-byte aligned", op);
     HA_CHECK((size_t)workspace->sizes[0] >= need,
@@ -122,8 +130,6 @@ void mha_varlen_fwd_paged_window_impl(const hipattn_tensor *q, const hipattn_ten
     given = static_cast<char *>(workspace->data);
   }
   hipStream_t stream = resolve_stream(stream_arg);
-  const int force = tuning().prefill_kernel;
-  const bool lse_or_f32 = lse != nullptr || p.out_f32;  // (neither the merges nor the kernel of decode rows have them)
   // Block images go into LDS as they are where they fill most of their place there; else tiles are staged through registers.
   const bool images = p.vc_block % 8 == 0 && p.vc_head % 8 == 0 && tuning().paged_prefill_dma != 0 && p.d <= 128 && (p.d >= 64 || p.d == 32);
   const bool eight = images && (force == 1 || (force == 0 && eight_wavefronts_pay(p)));
@@ -131,13 +137,11 @@ void mha_varlen_fwd_paged_window_impl(const hipattn_tensor *q, const hipattn_ten
   // capture, for shapes beyond it, on hipStreamPerThread, one handle for a stream of each thread's own -- nothing is cut that has to be merged.
   HeldWorkspace ws;
   void *scratch = given;
-  int most = (stream == hipStreamPerThread && !given) || lse_or_f32 || force != 0 || eight
-                 ? 1
-                 : (int)std::max<size_t>(std::min<size_t>(kWindowScratchBytes / piece_bytes(p.total_q, p.Hq, p.d), kMostParts), 1);
+  int most = (stream == hipStreamPerThread && !given) || eight ? 1 : possible;
   for (;;) {
     int parts = 1;
     double us = images ? 0 : staged_us(p);
-    if (images && !eight) parts = choose_parts(p, p.d == 64 || p.d == 80 || p.d == 96 || p.d == 112 || p.d == 128 ? most : 1, us);
+    if (images && !eight) parts = choose_parts(p, merged_head ? most : 1, us);
     RowsPlan rows;
     const bool as_rows = force == 0 && !eight && !lse_or_f32 && plan_window_rows(p, most, rows) && rows.us < us;
     if (as_rows) parts = rows.num_parts;

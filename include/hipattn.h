@@ -120,7 +120,8 @@ char *hipattn_mha_varlen_fwd_paged(const hipattn_tensor *q, const hipattn_tensor
  * also where others do not see it.  A row that sees nothing (its position is negative) is zero, its LSE +inf.
  * Where few workgroups would leave compute units idle a row's keys are dealt out to several (not with an f32 out or an LSE), by way of
  * workspace: u8, 256-byte aligned, hipattn_mha_varlen_fwd_paged_window_workspace_size bytes (at most 64 MiB), not shared by calls that overlap,
- * replays of captured ones included.  NULL: a buffer of 64 MiB that the library allocates once per stream; under capture, on
+ * replays of captured ones included; where no keys can be dealt out (as well: head sizes other than 64, 80, 96, 112, 128 and 256, and rows of
+ * which two pieces exceed 64 MiB) nothing is asked of it.  NULL: a buffer of 64 MiB that the library allocates once per stream; under capture, on
  * hipStreamPerThread and without that memory keys are then not dealt out, so that last bits, and the time of few long rows, may differ. */
 char *hipattn_mha_varlen_fwd_paged_window(const hipattn_tensor *q, const hipattn_tensor *key_cache,
                                           const hipattn_tensor *value_cache, const hipattn_tensor *block_tables,

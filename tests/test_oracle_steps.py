@@ -221,6 +221,19 @@ def test_chunk_workspace_sizes():
         size(4, 8, 257)
 
 
+@pytest.mark.parametrize("over", [
+    dict(q=_t(80000, 8, 128), out=_t(80000, 8, 128)),  # two pieces of 320 MiB
+    dict(lse=_t(2, 8, 12, dtype=_lib.F32)), dict(out=_t(20, 8, 128, dtype=_lib.F32)),
+    dict(q=_t(20, 8, 160), out=_t(20, 8, 160), kc=_t(9, 2, 20, 16, 8), vc=_t(9, 2, 160, 16)),
+])
+def test_chunks_ask_for_no_workspace_that_they_cannot_use(over):
+    """Without a device the call gets as far as the device."""
+    for ws in (_t(0, dtype=_lib.U8, data=0), _t(1000, dtype=_lib.U8)):
+        with pytest.raises(_lib.HipAttnError) as e:
+            _call("hipattn_mha_varlen_fwd_paged_window", *_chunk_args(ws=ws, **over))
+        assert "workspace" not in str(e.value)
+
+
 @pytest.mark.parametrize("max_ctx", [2 ** 31 - 1, 2 ** 31 - 15])
 def test_paged_attention_refuses_context_bounds_of_31_bits(max_ctx):
     """(rounded up to blocks they leave 32 bits)"""
