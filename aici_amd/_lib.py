@@ -173,6 +173,8 @@ _ERR_FUNCS = {
                                   c_float, TP, c_void_p],
     "hipattn_varlen_attn_paged_window": [TP, TP, TP, TP, TP, TP, TP, TP, TP, c_int64, c_int, c_int, TP, TP, c_int, c_int,
                                          c_float, c_int, c_int, TP, c_void_p],
+    "hipattn_varlen_attn_paged_window_ws": [TP, TP, TP, TP, TP, TP, TP, TP, TP, c_int64, c_int, c_int, TP, TP, c_int, c_int,
+                                            c_float, c_int, c_int, TP, TP, c_void_p],
 }
 
 # name -> (restype, argtypes) for the few calls that do not return an error string.

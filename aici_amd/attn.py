@@ -77,10 +77,21 @@ def _reads_through_tables(q: torch.Tensor, k: torch.Tensor, batch_info: BatchInf
             and key_cache.data_ptr() % 16 == 0 and value_cache.data_ptr() % 16 == 0)
 
 
+def window_workspace_size(batch_info: BatchInfo, num_heads: int, num_kv_heads: int, head_size: int, dtype: torch.dtype,
+                          window_size_left: int, sink_tokens: int = 0) -> int:
+    """Bytes of scratch memory `varlen_attn` with a window can make use of for batches of these shapes."""
+    single = batch_info.tokens.numel() - batch_info.q_multi
+    need = kernels.flash_attn_varlen_paged_window_workspace_size(batch_info.q_multi, num_heads, head_size)
+    if single > 0:
+        need = max(need, kernels.paged_attention_window_workspace_size(single, num_heads, num_kv_heads, head_size, batch_info.paged_block_size,
+                                                                       batch_info.paged_max_context_len, window_size_left, sink_tokens, dtype))
+    return need
+
+
 def varlen_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch_info: BatchInfo, key_cache: torch.Tensor,
                 value_cache: torch.Tensor, softmax_scale: Optional[float] = None,
                 paged_prefill: bool = False, cached: bool = False, window_size_left: Optional[int] = None,
-                sink_tokens: int = 0) -> torch.Tensor:
+                sink_tokens: int = 0, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """mod.rs:318-354: q [T,Hq,d], k/v [T,Hkv,d] -> [T, Hq*d].  `cached`: the new K/V are in the cache
     already (kernels.rotary_embedding_and_cache) and the scatter is skipped.
 
@@ -91,7 +102,9 @@ def varlen_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch_info: B
     always through the tables (needs the builder's multi_block_tables).
 
     window_size_left: a token sees that many tokens before it, itself and the first sink_tokens of its sequence
-    (None: all of them); multi-token rows then always read through the tables."""
+    (None: all of them); multi-token rows then always read through the tables.  workspace (with a window): uint8,
+    `window_workspace_size` bytes, so that a captured step gives the eager step's bits and shares no scratch memory with other graphs; None: what
+    the library keeps per stream, and under capture chunks whose keys are not dealt out."""
     T, Hq, d = q.shape
     Hkv = k.size(1)
     if softmax_scale is None:
@@ -101,15 +114,15 @@ def varlen_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch_info: B
         has_m, has_p = batch_info.q_multi > 0, batch_info.q_multi < T
         if has_m and batch_info.multi_block_tables is None:
             raise ValueError("a window needs batch_info.multi_block_tables (slots must follow the blocks in order)")
-        _native.varlen_attn_paged_window(q, k, v, key_cache, value_cache, None if cached else batch_info.slot_mapping,
-                                         batch_info.multi_block_tables if has_m else None, batch_info.seqlens_q if has_m else None,
-                                         batch_info.multi_context_lens if has_m else None, batch_info.q_multi, batch_info.max_seqlen_q,
-                                         batch_info.max_seqlen_k, batch_info.paged_block_tables if has_p else None,
-                                         batch_info.paged_context_lens if has_p else None, batch_info.paged_block_size,
-                                         batch_info.paged_max_context_len, softmax_scale, window_size_left, sink_tokens, y)
+        _native.varlen_attn_paged_window_ws(q, k, v, key_cache, value_cache, None if cached else batch_info.slot_mapping,
+                                            batch_info.multi_block_tables if has_m else None, batch_info.seqlens_q if has_m else None,
+                                            batch_info.multi_context_lens if has_m else None, batch_info.q_multi, batch_info.max_seqlen_q,
+                                            batch_info.max_seqlen_k, batch_info.paged_block_tables if has_p else None,
+                                            batch_info.paged_context_lens if has_p else None, batch_info.paged_block_size,
+                                            batch_info.paged_max_context_len, softmax_scale, window_size_left, sink_tokens, y, workspace)
         return y.reshape(T, Hq * d)
-    if sink_tokens != 0:
-        raise ValueError("sink_tokens needs a window")
+    if sink_tokens != 0 or workspace is not None:
+        raise ValueError(f"{'sink_tokens' if sink_tokens != 0 else 'workspace'} needs a window")
     if paged_prefill or _reads_through_tables(q, k, batch_info, key_cache, value_cache):
         if batch_info.multi_block_tables is None:
             raise ValueError("paged_prefill needs batch_info.multi_block_tables (slots must follow the blocks in order)")

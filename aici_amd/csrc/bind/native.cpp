@@ -376,6 +376,9 @@ PyMethodDef g_methods[] = {
     BIND(varlen_attn_paged_window, "q,k,v,key_cache,value_cache,slot_mapping,multi_block_tables,seqlens_q,multi_context_lens,"
                                    "q_multi,max_seqlen_q,max_seqlen_k,paged_block_tables,paged_context_lens,paged_block_size,"
                                    "paged_max_context_len,softmax_scale,window_size_left,sink_tokens,y"),
+    BIND(varlen_attn_paged_window_ws, "q,k,v,key_cache,value_cache,slot_mapping,multi_block_tables,seqlens_q,multi_context_lens,"
+                                      "q_multi,max_seqlen_q,max_seqlen_k,paged_block_tables,paged_context_lens,paged_block_size,"
+                                      "paged_max_context_len,softmax_scale,window_size_left,sink_tokens,y,workspace"),
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_native", "Bindings of libhipattn.so's hot entry points.", -1, g_methods,

@@ -109,14 +109,15 @@ extern "C" char *hipattn_varlen_attn_paged(const hipattn_tensor *q, const hipatt
   });
 }
 
-extern "C" char *hipattn_varlen_attn_paged_window(const hipattn_tensor *q, const hipattn_tensor *k, const hipattn_tensor *v,
-                                                  hipattn_tensor *key_cache, hipattn_tensor *value_cache,
-                                                  const hipattn_tensor *slot_mapping, const hipattn_tensor *multi_block_tables,
-                                                  const hipattn_tensor *seqlens_q, const hipattn_tensor *multi_context_lens,
-                                                  int64_t q_multi, int max_seqlen_q, int max_seqlen_k,
-                                                  const hipattn_tensor *paged_block_tables, const hipattn_tensor *paged_context_lens,
-                                                  int paged_block_size, int paged_max_context_len, float softmax_scale,
-                                                  int window_size_left, int sink_tokens, hipattn_tensor *y, void *stream) {
+extern "C" char *hipattn_varlen_attn_paged_window_ws(const hipattn_tensor *q, const hipattn_tensor *k, const hipattn_tensor *v,
+                                                     hipattn_tensor *key_cache, hipattn_tensor *value_cache,
+                                                     const hipattn_tensor *slot_mapping, const hipattn_tensor *multi_block_tables,
+                                                     const hipattn_tensor *seqlens_q, const hipattn_tensor *multi_context_lens,
+                                                     int64_t q_multi, int max_seqlen_q, int max_seqlen_k,
+                                                     const hipattn_tensor *paged_block_tables, const hipattn_tensor *paged_context_lens,
+                                                     int paged_block_size, int paged_max_context_len, float softmax_scale,
+                                                     int window_size_left, int sink_tokens, hipattn_tensor *y,
+                                                     const hipattn_tensor *workspace, void *stream) {
   HA_PROTECT({
     check_tensor(q, "q", 3);
     check_tensor(k, "k", 3);
@@ -134,14 +135,27 @@ extern "C" char *hipattn_varlen_attn_paged_window(const hipattn_tensor *q, const
       hipattn_tensor qm = rows(q, 0, q_multi);
       hipattn_tensor ym = rows(y, 0, q_multi);
       raise(hipattn_mha_varlen_fwd_paged_window(&qm, key_cache, value_cache, multi_block_tables, seqlens_q, multi_context_lens, max_seqlen_q,
-                                                max_seqlen_k, softmax_scale, window_size_left, sink_tokens, &ym, nullptr, nullptr, stream));
+                                                max_seqlen_k, softmax_scale, window_size_left, sink_tokens, &ym, nullptr, workspace, stream));
     }
     if (q_multi < T) {
       hipattn_tensor qs = rows(q, q_multi, T);
       hipattn_tensor ys = rows(y, q_multi, T);
       raise(hipattn_paged_attention_window(&ys, &qs, key_cache, value_cache, (int)k->sizes[1], softmax_scale, paged_block_tables,
                                            paged_context_lens, paged_block_size, paged_max_context_len, window_size_left, sink_tokens,
-                                           nullptr, nullptr, stream));
+                                           nullptr, workspace, stream));
     }
   });
+}
+
+extern "C" char *hipattn_varlen_attn_paged_window(const hipattn_tensor *q, const hipattn_tensor *k, const hipattn_tensor *v,
+                                                  hipattn_tensor *key_cache, hipattn_tensor *value_cache,
+                                                  const hipattn_tensor *slot_mapping, const hipattn_tensor *multi_block_tables,
+                                                  const hipattn_tensor *seqlens_q, const hipattn_tensor *multi_context_lens,
+                                                  int64_t q_multi, int max_seqlen_q, int max_seqlen_k,
+                                                  const hipattn_tensor *paged_block_tables, const hipattn_tensor *paged_context_lens,
+                                                  int paged_block_size, int paged_max_context_len, float softmax_scale,
+                                                  int window_size_left, int sink_tokens, hipattn_tensor *y, void *stream) {
+  return hipattn_varlen_attn_paged_window_ws(q, k, v, key_cache, value_cache, slot_mapping, multi_block_tables, seqlens_q, multi_context_lens,
+                                             q_multi, max_seqlen_q, max_seqlen_k, paged_block_tables, paged_context_lens, paged_block_size,
+                                             paged_max_context_len, softmax_scale, window_size_left, sink_tokens, y, nullptr, stream);
 }

@@ -23,7 +23,7 @@ from typing import Dict, List, Optional, Tuple
 import torch
 
 from . import kernels
-from .attn import RotaryEmbedding, varlen_attn
+from .attn import RotaryEmbedding, varlen_attn, window_workspace_size
 from .paged import BatchInfo
 
 
@@ -171,16 +171,27 @@ class Llama:
         x = y + x
         return x, self._rms(x, norm_weight)
 
+    def workspace_size(self, batch_info: BatchInfo) -> int:
+        """Bytes of a workspace for `forward` of batches of these shapes: what attention with a window can make use of; 0 without one."""
+        cfg = self.cfg
+        if cfg.sliding_window is None:
+            return 0
+        return window_workspace_size(batch_info, cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim, cfg.dtype,
+                                     cfg.sliding_window - 1, cfg.attention_sinks)
+
     def forward(self, batch_info: BatchInfo, caches: List[Tuple[torch.Tensor, torch.Tensor]],
-                paged_prefill: bool = False, fused: bool = False) -> torch.Tensor:
+                paged_prefill: bool = False, fused: bool = False, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
         """batch_info on the device; caches[layer] = (key_cache, value_cache), updated in place.
         paged_prefill: multi-token rows read their context through block tables (no gather copy).
         fused: q, k, v stay views of the fused projection's output (the kernels honour the row stride) and
         rotary + cache scatter are one launch, or part of the projection's -- four or five launches fewer per layer, the same
-        bits."""
+        bits.
+        workspace: uint8, `workspace_size` bytes, of a model with a window: a captured step's attention is then the eager one and lies in no memory of the
+        library's."""
         cfg = self.cfg
         Hq, Hkv, d = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
-        window = {} if cfg.sliding_window is None else {"window_size_left": cfg.sliding_window - 1, "sink_tokens": cfg.attention_sinks}
+        window = {} if cfg.sliding_window is None else {"window_size_left": cfg.sliding_window - 1, "sink_tokens": cfg.attention_sinks,
+                                                           "workspace": workspace}
         x = _rows(self.wte, batch_info.tokens)                                   # llama.rs:203
         T = x.size(0)
         # h: the normalised rows, None where the projection that takes them does it

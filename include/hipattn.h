@@ -958,7 +958,8 @@ char *hipattn_varlen_attn_paged(
     void *stream);
 
 /* The same for a model with a sliding window and sinks: hipattn_reshape_and_cache (slot_mapping not NULL),
- * hipattn_mha_varlen_fwd_paged_window for the first q_multi rows, hipattn_paged_attention_window for the rest. */
+ * hipattn_mha_varlen_fwd_paged_window for the first q_multi rows, hipattn_paged_attention_window for the rest.  _ws: with a workspace for both, which
+ * run one after the other -- the larger of their two sizes, or NULL -- so that a captured step is the eager one and shares no scratch memory. */
 char *hipattn_varlen_attn_paged_window(
     const hipattn_tensor *q, const hipattn_tensor *k, const hipattn_tensor *v,
     hipattn_tensor *key_cache, hipattn_tensor *value_cache,
@@ -969,6 +970,17 @@ char *hipattn_varlen_attn_paged_window(
     const hipattn_tensor *paged_context_lens, int paged_block_size,
     int paged_max_context_len, float softmax_scale, int window_size_left,
     int sink_tokens, hipattn_tensor *y, void *stream);
+char *hipattn_varlen_attn_paged_window_ws(
+    const hipattn_tensor *q, const hipattn_tensor *k, const hipattn_tensor *v,
+    hipattn_tensor *key_cache, hipattn_tensor *value_cache,
+    const hipattn_tensor *slot_mapping, const hipattn_tensor *multi_block_tables,
+    const hipattn_tensor *seqlens_q, const hipattn_tensor *multi_context_lens,
+    int64_t q_multi, int max_seqlen_q, int max_seqlen_k,
+    const hipattn_tensor *paged_block_tables,
+    const hipattn_tensor *paged_context_lens, int paged_block_size,
+    int paged_max_context_len, float softmax_scale, int window_size_left,
+    int sink_tokens, hipattn_tensor *y, const hipattn_tensor *workspace,
+    void *stream);
 
 #ifdef __cplusplus
 }

@@ -479,3 +479,66 @@ def test_bounds_of_31_bits(device, tuning, heads):
             out = K.flash_attn_varlen_paged_window(*bare, W.offsets(lens_q).to(device), torch.tensor(ctx, dtype=torch.int32, device=device),
                                                    bound, max(ctx), c["scale"], 150, 3)
             check(out, c, expect)
+
+
+class Mixed:
+    """A batch of chunks and decode rows for attn.varlen_attn, on the device."""
+
+    def __init__(self, seed, heads, chunks, rows, window, sinks, device):
+        (self.lens_q, self.ctx), (hq, hkv, d) = zip(*chunks, *[(1, n) for n in rows]), heads
+        self.c = case(seed, list(self.lens_q), list(self.ctx), heads, torch.bfloat16, window, sinks)
+        m, T = len(chunks), sum(self.lens_q)
+        lens = torch.tensor(self.ctx, dtype=torch.int32, device=device)
+        self.tokens, self.q_multi = torch.zeros((T,), dtype=torch.int32), T - len(rows)
+        self.max_seqlen_q, self.max_seqlen_k = max(self.lens_q), max(self.ctx[:m])
+        self.seqlens_q, self.multi_context_lens, self.paged_context_lens = W.offsets(list(self.lens_q[:m])).to(device), lens[:m], lens[m:]
+        self.paged_block_size, self.paged_max_context_len = 16, max(rows)
+        self.q, self.kc, self.vc, tables = (self.c[k].to(device) for k in ("q", "kc", "vc", "tables"))
+        self.multi_block_tables, self.paged_block_tables = tables[:m], tables[m:]
+        self.kv = torch.zeros((T, hkv, d), dtype=torch.bfloat16, device=device)
+        self.how = dict(window_size_left=window, sink_tokens=sinks)
+
+    def attend(self, workspace=None):
+        return attn.varlen_attn(self.q, self.kv, self.kv, self, self.kc, self.vc, cached=True, workspace=workspace, **self.how)
+
+    def workspace(self, device):
+        hq, hkv, d = self.c["heads"]
+        need = attn.window_workspace_size(self, hq, hkv, d, torch.bfloat16, *self.how.values())
+        return torch.full((need,), 255, dtype=torch.uint8, device=device)  # (NaN, read as fp32)
+
+    def check(self, y):
+        check(y.view(self.c["q"].shape), self.c, want(self.c))
+
+
+def test_captured_composition_with_a_workspace(device):
+    """Chunks whose keys are dealt out and decode rows in partitions: captured with a workspace the composed call gives the eager call's bits, and
+    two graphs captured on one stream, each with its own, run at the same time."""
+    made = [Mixed(800 + k, (8, 2, 128), [(16, 3000), (5, 900 + k)], [2000, 1500 - k, 40], 2500, 20, device) for k in range(2)]
+    alone = [b.attend() for b in made]
+    stores = [b.workspace(device) for b in made]
+    assert stores[0].numel() > 0
+    for b, y, store in zip(made, alone, stores):
+        b.check(y)
+        assert torch.equal(b.attend(store), y) and not bool((store == 255).all())  # (made use of)
+        store.fill_(255)
+    with pytest.raises(HipAttnError, match="too small"):
+        made[0].attend(stores[0][:4096])
+    side, graphs, outs = torch.cuda.Stream(), [], []
+    torch.cuda.synchronize()
+    for b, store in zip(made, stores):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=side):
+            outs.append(b.attend(store))
+    streams = [torch.cuda.Stream() for _ in made]
+    for _ in range(4):
+        for out, store in zip(outs, stores):
+            out.fill_(NAN)
+            store.fill_(255)
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                for _ in range(5):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for b, out, y in zip(made, outs, alone):
+            assert torch.equal(out, y) and torch.equal(b.attend(), y)

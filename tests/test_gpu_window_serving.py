@@ -151,3 +151,39 @@ def test_generation(device, window, sinks, blocks):
         new.fill_(1)
     assert window is None or int(pool.ring_ends[0]) > blocks  # blocks have been handed out more than once
     assert [len(s) for s in said] == [37 + 72, 5 + 71, 45 + 41, 20 + 72]
+
+
+def test_captured_chunks_with_a_workspace(device):
+    """A captured prompt step of the model, its attention in a workspace of the caller's, has the eager step's bits."""
+    R, T = 2, 20
+    model = llama.Llama(replace(CFG, sliding_window=300, attention_sinks=4), llama.random_weights(CFG, 5, "cpu"), device)
+    pool = paged.DeviceBlocks(16, 80, R, 512, device, 299, 4)
+    caches = [paged.alloc_gpu_cache_layer(80, CFG.num_key_value_heads, CFG.head_dim, 16, CFG.dtype, device) for _ in range(2)]
+    for kc, vc in caches:
+        kc.zero_()
+        vc.zero_()
+    g = torch.Generator().manual_seed(3)
+    ids = torch.randint(0, CFG.vocab_size, (420,), generator=g).to(torch.int32).to(device)
+    for n in (400, T):
+        step = pool.step(torch.tensor([n, 0], dtype=torch.int32, device=device), n)
+        batch = pool.batch_info(step, ids[:n], max_new=n)
+        eager = model.forward(batch, caches, fused=True)
+    need = model.workspace_size(batch)
+    assert need == 16 * T * CFG.num_attention_heads * (CFG.head_dim + 2) * 4
+    assert llama.Llama.workspace_size(llama.Llama(CFG, llama.random_weights(CFG, 5, "cpu"), device), batch) == 0
+    store = torch.full((need,), 255, dtype=torch.uint8, device=device)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        assert torch.equal(model.forward(batch, caches, fused=True, workspace=store), eager)
+    torch.cuda.synchronize()
+    assert not bool((store == 255).all())  # (made use of)
+    with torch.cuda.graph(graph, stream=side):
+        logits = model.forward(batch, caches, fused=True, workspace=store)
+    for _ in range(3):
+        logits.fill_(float("nan"))
+        store.fill_(255)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(logits, eager)
+        assert torch.equal(model.forward(batch, caches, fused=True), eager)

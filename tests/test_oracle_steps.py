@@ -202,6 +202,12 @@ def test_varlen_attn_refuses_sinks_without_a_window():
         attn.varlen_attn(x, x, x, None, x, x, sink_tokens=4)
 
 
+def test_varlen_attn_refuses_a_workspace_without_a_window():
+    x = torch.zeros((1, 1, 8))
+    with pytest.raises(ValueError, match="workspace needs a window"):
+        attn.varlen_attn(x, x, x, None, x, x, workspace=x)
+
+
 @pytest.mark.parametrize("args,message", [
     ((4, 8, 2, 72, 16, 100, 31, 4), "unsupported head size 72"), ((4, 8, 3, 64, 16, 100, 31, 4), "not divisible"),
     ((4, 8, 2, 64, 12, 100, 31, 4), "unsupported block size 12"), ((4, 8, 2, 64, 16, 100, -1, 4), "must not be negative"),
