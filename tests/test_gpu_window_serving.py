@@ -156,21 +156,22 @@ def test_generation(device, window, sinks, blocks):
 def test_captured_chunks_with_a_workspace(device):
     """A captured prompt step of the model, its attention in a workspace of the caller's, has the eager step's bits."""
     R, T = 2, 20
-    model = llama.Llama(replace(CFG, sliding_window=300, attention_sinks=4), llama.random_weights(CFG, 5, "cpu"), device)
-    pool = paged.DeviceBlocks(16, 80, R, 512, device, 299, 4)
-    caches = [paged.alloc_gpu_cache_layer(80, CFG.num_key_value_heads, CFG.head_dim, 16, CFG.dtype, device) for _ in range(2)]
+    cfg = replace(CFG, max_position_embeddings=3200)
+    model = llama.Llama(replace(cfg, sliding_window=2500, attention_sinks=4), llama.random_weights(cfg, 5, "cpu"), device)
+    pool = paged.DeviceBlocks(16, 200, R, 3200, device, 2499, 4)
+    caches = [paged.alloc_gpu_cache_layer(200, CFG.num_key_value_heads, CFG.head_dim, 16, CFG.dtype, device) for _ in range(2)]
     for kc, vc in caches:
         kc.zero_()
         vc.zero_()
     g = torch.Generator().manual_seed(3)
-    ids = torch.randint(0, CFG.vocab_size, (420,), generator=g).to(torch.int32).to(device)
-    for n in (400, T):
+    ids = torch.randint(0, CFG.vocab_size, (3000,), generator=g).to(torch.int32).to(device)
+    for n in (3000, T):
         step = pool.step(torch.tensor([n, 0], dtype=torch.int32, device=device), n)
         batch = pool.batch_info(step, ids[:n], max_new=n)
         eager = model.forward(batch, caches, fused=True)
     need = model.workspace_size(batch)
     assert need == 16 * T * CFG.num_attention_heads * (CFG.head_dim + 2) * 4
-    assert llama.Llama.workspace_size(llama.Llama(CFG, llama.random_weights(CFG, 5, "cpu"), device), batch) == 0
+    assert llama.Llama(cfg, llama.random_weights(cfg, 5, "cpu"), device).workspace_size(batch) == 0
     store = torch.full((need,), 255, dtype=torch.uint8, device=device)
     side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
     torch.cuda.synchronize()
