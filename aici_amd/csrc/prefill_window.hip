@@ -31,15 +31,17 @@ int64_t most_tiles(const PrefillParams &p, int rows) {
 }
 
 // Workgroups of eight wavefronts instead of four: what their alternation between the pipes gains a tile is lost again where a block of twice as many
-// rows is filled less or the last round of workgroups is, so only for chunks of like lengths over long windows whose workgroups fill the compute
-// units once, or many times with heads of 128.  us, eight / four: 32 / 8 x 128, 1 x 2000 new tokens (256 workgroups) with a window of 4096 157 / 163, of
-// 2000 85 / 89, of 1000 52.2 / 52.2; 2 x 4096 of 4096 614 / 625, of 2000 330 / 332, of 1000 199 / 189; 8 x 533 of 4096 399 / 386; 63 x 20 beside 1 x 4096 of
-// 4096 530 / 512; 32 / 32 x 80, 1 x 2000 of 4096 136 / 151, 2 x 4096 535 / 510; 12 / 4 x 112, 16 x 512 296 / 262; 16 / 2 x 64, 2 x 4096 225 / 216, 8 x 533 199 / 144.
+// rows is filled less, or where one of them ends before the others and leaves its compute unit idle.  So only where they fill the compute units
+// once and nearly all, with chains alike and long: chunks of like lengths, all of whose rows see a whole window.  us, eight / four: 1 x 2000 new tokens
+// behind 4096 (256 workgroups, 224 to 256 take the same) with a window of 4096, 32 / 8 x 128 149 / 155, 32 / 8 x 112 147 / 156, 32 / 32 x 80 127 / 147;
+// 1 x 4000, 16 / 2 x 96 128 / 138; behind nothing 64 / 57, 64 / 59, 59 / 60, 111 / 105, as the first rows have few keys.  264 workgroups, 24 / 8 x 96 218 / 146.
+// Heads of 128, two to ten rounds of workgroups, 96 shapes: four are 2.7 % faster on average and 14 % at most, eight 2.9 % at most.  16 / 2 x 64, 2 x
+// 4096 225 / 216.
 bool eight_wavefronts_pay(const PrefillParams &p) {
   const int hl = prefill_heads_log2(p, 3), rows = 256 >> hl;
   const int64_t wgs = (int64_t)p.batch * ((p.max_q + rows - 1) / rows) * (p.Hq >> hl), tiles = most_tiles(p, rows);
-  const bool alike = p.total_q * 10 >= (int64_t)p.batch * p.max_q * 9, once = wgs <= compute_units() && wgs * 8 > compute_units() * 7;
-  return alike && ((once && p.d > 64 && tiles >= 32) || (wgs >= 1000 && hl > 0 && p.d > 112 && tiles >= 48));
+  const bool alike = p.total_q * 10 >= (int64_t)p.batch * p.max_q * 9 && p.max_k - p.max_q >= p.win_left;
+  return alike && wgs <= compute_units() && wgs * 8 > compute_units() * 7 && p.d > 64 && tiles >= 32;
 }
 
 // Pieces that a row block's keys are dealt out in (workgroups of four wavefronts).  A workgroup's chain of tiles is bound by its own

@@ -6,6 +6,7 @@ Tolerance, per element: the output's own rounding, half a step of |out|; the pro
 the second product, half a step of sum p |v|; and 1e-4 of sum p |v| for scores and sums in fp32 (128 products of up to 6 x 6 x scale, 2^-24 each,
 in the exponent; some thousand terms in the sums)."""
 import math
+import re
 
 import numpy as np
 import pytest
@@ -542,3 +543,35 @@ def test_captured_composition_with_a_workspace(device):
         torch.cuda.synchronize()
         for b, out, y in zip(made, outs, alone):
             assert torch.equal(out, y) and torch.equal(b.attend(), y)
+
+
+def launched(call):
+    """Names of the kernels that a call launches."""
+    call()
+    torch.cuda.synchronize()
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as prof:
+        call()
+        torch.cuda.synchronize()
+    return [e.key for e in prof.key_averages() if "kernel" in e.key]
+
+
+@pytest.mark.filterwarnings("ignore:Profiler clears events")
+@pytest.mark.parametrize("heads,lens_q,past,window,form", [
+    ((32, 8, 128), [2000], 4096, 4096, 8), ((32, 32, 80), [1000, 1000], 3000, 2500, 8), ((16, 2, 96), [4000], 4096, 4096, 8),
+    ((32, 8, 128), [2000], 0, 4096, 4),         # the first rows of a prompt have short chains
+    ((32, 8, 128), [4096, 4096], 4096, 4096, 4), ((64, 8, 128), [4096], 4096, 4096, 4),  # several rounds of workgroups
+    ((24, 8, 96), [2600], 4096, 4096, 4), ((16, 2, 64), [4000], 4096, 4096, 4),
+    ((32, 8, 128), [2100], 4096, 4096, 4),      # a few more than one to a compute unit
+])
+def test_the_form_of_the_workgroups(device, heads, lens_q, past, window, form):
+    hq, hkv, d = heads
+    cols = -(-(max(lens_q) + past) // 16)
+    q = torch.zeros((sum(lens_q), hq, d), dtype=torch.bfloat16, device=device)
+    kc = torch.zeros((len(lens_q) * cols, hkv, d // 8, 16, 8), dtype=torch.bfloat16, device=device)
+    vc = torch.zeros((len(lens_q) * cols, hkv, d, 16), dtype=torch.bfloat16, device=device)
+    tables = torch.arange(len(lens_q) * cols, dtype=torch.int32, device=device).view(-1, cols)
+    ctx = [n + past for n in lens_q]
+    args = (q, kc, vc, tables, W.offsets(lens_q).to(device), torch.tensor(ctx, dtype=torch.int32, device=device), max(lens_q), max(ctx), 0.1)
+    names = launched(lambda: K.flash_attn_varlen_paged_window(*args, window, 4))
+    assert len(names) == 1 and "prefill_varlen_w8_kernel" in names[0], names
+    assert int((re.search(r", (\d+)>\(", names[0]) or re.search(r"Li(\d+)EEEv", names[0])).group(1)) == form
