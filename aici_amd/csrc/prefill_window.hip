@@ -134,7 +134,8 @@ void mha_varlen_fwd_paged_window_impl(const hipattn_tensor *q, const hipattn_ten
   hipStream_t stream = resolve_stream(stream_arg);
   // Block images go into LDS as they are where they fill most of their place there; else tiles are staged through registers.
   const bool images = p.vc_block % 8 == 0 && p.vc_head % 8 == 0 && tuning().paged_prefill_dma != 0 && p.d <= 128 && (p.d >= 64 || p.d == 32);
-  const bool eight = images && (force == 1 || (force == 0 && eight_wavefronts_pay(p)));
+  const int pieces = images && merged_head ? tuning().window_parts : 0;
+  const bool eight = images && (force == 1 || (force == 0 && pieces == 0 && eight_wavefronts_pay(p)));
   // What pieces need lies in the caller's workspace or a buffer of the stream's, of one size, so that either gives the same bits; without it -- in a
   // capture, for shapes beyond it, on hipStreamPerThread, one handle for a stream of each thread's own -- nothing is cut that has to be merged.
   HeldWorkspace ws;
@@ -143,9 +144,10 @@ void mha_varlen_fwd_paged_window_impl(const hipattn_tensor *q, const hipattn_ten
   for (;;) {
     int parts = 1;
     double us = images ? 0 : staged_us(p);
-    if (images && !eight) parts = choose_parts(p, merged_head ? most : 1, us);
+    if (pieces > 0) parts = std::min(pieces, most);
+    else if (images && !eight) parts = choose_parts(p, merged_head ? most : 1, us);
     RowsPlan rows;
-    const bool as_rows = force == 0 && !eight && !lse_or_f32 && plan_window_rows(p, most, rows) && rows.us < us;
+    const bool as_rows = force == 0 && pieces == 0 && !eight && !lse_or_f32 && plan_window_rows(p, most, rows) && rows.us < us;
     if (as_rows) parts = rows.num_parts;
     if (parts > 1 && !given) {
       ws = try_library_workspace(WS_WINDOW_CHUNKS, kWindowScratchBytes, stream);

@@ -575,3 +575,74 @@ def test_the_form_of_the_workgroups(device, heads, lens_q, past, window, form):
     names = launched(lambda: K.flash_attn_varlen_paged_window(*args, window, 4))
     assert len(names) == 1 and "prefill_varlen_w8_kernel" in names[0], names
     assert int((re.search(r", (\d+)>\(", names[0]) or re.search(r"Li(\d+)EEEv", names[0])).group(1)) == form
+
+
+PIECES = [(64, 2), (80, 4), (96, 1), (112, 4), (128, 2)]  # head size, kv heads
+
+
+@pytest.mark.parametrize("d,hkv", PIECES)
+@pytest.mark.parametrize("parts,bs", [(2, 16), (3, 8), (5, 32), (16, 16)])
+def test_pieces_of_a_row_blocks_keys(device, tuning, d, hkv, bs, parts):
+    """Keys of a row block dealt out to as many workgroups as asked for: pieces that begin in the sinks, in the gap and in the window, blocks with fewer
+    tiles than pieces, rows that see nothing of a piece or nothing at all, passed blocks that name no block; whatever the scratch memory held."""
+    tuning("window_parts", parts)
+    dtype = torch.float16 if parts == 3 else torch.bfloat16
+    heads = ((6 if d == 96 else 2 * hkv) if d != 80 else hkv, hkv, d)
+    sets = [(SEQS, 255, 100), (SEQS, 63, 64), ([(100, 2100), (300, 1300), (9, 5), (0, 40), (1, 1)], 700, 70), ([(257, 900)], 64, 200),
+            ([(3, 1100), (0, 0)] * 40 + [(200, 1500)], 1000, 0)]  # the last: listed row blocks, more sequences than lanes
+    for n, (seqs, window, sinks) in enumerate(sets):
+        lens_q, ctx = [a for a, _ in seqs], [b for _, b in seqs]
+        c = case(900 + n, lens_q, ctx, heads, dtype, window, sinks, bs)
+        need = K.flash_attn_varlen_paged_window_workspace_size(sum(lens_q), heads[0], d)
+        store = torch.full((need + 4096,), 255, dtype=torch.uint8, device=device)  # (NaN, read as fp32)
+        out = chunk(c, device, workspace=store[:need])
+        check(out, c, want(c))
+        assert bool((store[need:] == 255).all()) and not bool((store[:need] == 255).all())
+        assert torch.equal(chunk(c, device), out)
+
+
+@pytest.mark.filterwarnings("ignore:Profiler clears events")
+@pytest.mark.parametrize("heads,rows,bs", [((16, 2, 64), 300, 16), ((32, 32, 80), 300, 8), ((6, 1, 96), 600, 16), ((12, 4, 112), 300, 32),
+                                           ((8, 2, 128), 300, 16), ((8, 2, 128), 300, 8)])
+def test_pieces_that_the_library_chooses(device, heads, rows, bs):
+    """Chunks of some hundred rows over long windows, which the library itself deals out this way."""
+    for lens_q, ctx in (([rows], [4000 + rows]), ([rows, 150], [4000 + rows, 4000])):
+        c = case(950, lens_q, ctx, heads, torch.bfloat16, 4000, 33, bs)
+        to = {n: c[n].to(device) for n in ("q", "kc", "vc", "tables")}
+        cu, lk = W.offsets(lens_q).to(device), torch.tensor(ctx, dtype=torch.int32, device=device)
+        call = lambda: K.flash_attn_varlen_paged_window(*to.values(), cu, lk, max(lens_q), max(ctx), c["scale"], 4000, 33)
+        out = call()
+        check(out, c, want(c))
+        if len(lens_q) == 1:
+            names = launched(call)
+            assert len(names) == 2 and any("window_merge_kernel" in n for n in names), names
+
+
+@pytest.mark.parametrize("heads", [(16, 2, 64), (8, 2, 128)])
+def test_pieces_of_bounds_that_do_not_hold(device, tuning, heads):
+    """More new tokens than max_seqlen_q, more keys than max_seqlen_k, and two graphs with a workspace each: as without pieces."""
+    tuning("window_parts", 4)
+    lens_q, ctx = [400, 3, 8], [2600, 900, 2000]
+    c = case(960, lens_q, ctx, heads, torch.bfloat16, 2500, 30)
+    bare = [c[k].to(device) for k in ("q", "kc", "vc", "tables")]
+    expect, mass, _ = want(c)
+    cu, lk = W.offsets(lens_q).to(device), torch.tensor(ctx, dtype=torch.int32, device=device)
+    store = torch.full((K.flash_attn_varlen_paged_window_workspace_size(sum(lens_q), heads[0], heads[2]),), 255, dtype=torch.uint8, device=device)
+    for bound_q, bound_k in ((100, 2600), (400, 700)):
+        store.fill_(255)
+        out = torch.full_like(bare[0], 7.0)
+        _native.mha_varlen_fwd_paged_window(*bare, cu, lk, bound_q, bound_k, c["scale"], 2500, 30, out, None, store)
+        left = (out == 7).flatten(1).all(1).cpu()
+        assert not bool(left[:bound_q].any()) and not bool(left[400:].any()) and bool(left[:400].any()) == (bound_q < 400)
+        check(out[~left], c, (expect[~left], mass[~left], None))  # (this kernel's last piece takes the keys beyond the bound)
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        out = K.flash_attn_varlen_paged_window(*bare, cu, lk, 400, 2600, c["scale"], 2500, 30, workspace=store)
+    first = chunk(c, device)
+    for _ in range(3):
+        store.fill_(255)
+        out.fill_(NAN)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, first) and torch.equal(chunk(c, device), first)
