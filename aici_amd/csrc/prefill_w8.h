@@ -135,7 +135,7 @@ __global__ __launch_bounds__(NW * 64, STEP::value ? 2 : w8_wavefronts(HDP, NW)) 
   const bool listed = STEP::window && p.row_blocks > 0;
   if constexpr (STEP::window)
     if (listed) {
-      blk = row_block_of(p.cu_q, p.context_lens, HDP <= 64 ? p.win_left : p.win_left / 2, p.batch, BM, p.n_qblocks, id);
+      blk = row_block_of(p.cu_q, p.context_lens, p.win_left / 2, p.batch, BM, p.n_qblocks, id);
       if (blk.block < 0) return;
     }
   const int b = listed ? blk.seq : id / p.n_qblocks;
