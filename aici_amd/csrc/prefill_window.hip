@@ -46,7 +46,7 @@ bool eight_wavefronts_pay(const PrefillParams &p) {
 
 // Pieces that a row block's keys are dealt out in (workgroups of four wavefronts).  A workgroup's chain of tiles is bound by its own
 // instructions, some 2 us a tile with a wavefront per SIMD (five tiles in LDS instead of two change nothing), so where compute units are idle
-// more of them take a part each.  All in us: the launch, a tile, which takes longer from two workgroups per compute unit on, as two or three of them
+// more of them take a part each.  All in us, and fitted: what does not grow with the tiles, a tile, which takes longer from two workgroups per compute unit on, as two or three of them
 // fill each other's gaps; the merge, and what writing and reading the pieces costs.  In 400 measured shapes (1 x 5 new tokens to 2 x 4096, alike and
 // 63 x 20 beside one of 4096, windows of 100 to 4096, four kinds of heads) the choice among these and the kernel of decode rows is 1.8 % off the best on
 // average and 20 % at most; whole blocks alone are 39 %.  us, whole / best: 32 / 8 x 128, 1 x 5 over 4096 keys 99 / 16 (rows), 1 x 300 106 / 48 (6
@@ -56,7 +56,7 @@ int choose_parts(const PrefillParams &p, int most, double &us) {
   const int hl = prefill_heads_log2(p, 2), rows = 128 >> hl;
   const int64_t tiles = most_tiles(p, rows);
   const double wgs = ((double)(p.total_q / rows) + 0.7 * (p.batch + 1)) * (p.Hq >> hl);
-  const double launch = p.d > 96 ? 8 : (p.d > 64 ? 16 : 9), tile = p.d > 64 ? 2.1 : 1.7;
+  const double fixed = p.d > 96 ? 8 : (p.d > 64 ? 16 : 9), tile = p.d > 64 ? 2.1 : 1.7;
   const double share = (p.d > 96 ? 0.62 : (p.d > 64 ? 0.45 : 0.5)) / compute_units();
   const double piece = (double)p.total_q * p.Hq * (p.d + 2) * 2e-6;
   int parts = 1;
@@ -64,7 +64,7 @@ int choose_parts(const PrefillParams &p, int most, double &us) {
   for (int n : {1, 2, 3, 4, 6, 10, 16}) {
     const int64_t part_tiles = (tiles + n - 1) / n;
     if (n > 1 && (n > most || n > tiles || (tiles + part_tiles - 1) / part_tiles != n)) continue;
-    const double t = launch + (double)part_tiles * tile * std::max(1.0, share * wgs * n) + (n > 1 ? 5.0 + n * piece : 0.0);
+    const double t = fixed + (double)part_tiles * tile * std::max(1.0, share * wgs * n) + (n > 1 ? 5.0 + n * piece : 0.0);
     if (n == 1 || t < (parts == 1 ? 0.87 : 1.0) * us) {
       us = t;
       parts = n;
@@ -107,6 +107,7 @@ void mha_varlen_fwd_paged_window_impl(const hipattn_tensor *q, const hipattn_ten
   if (!paged_prefill_params(PagedPrefillCall{q, key_cache, value_cache, block_tables, cu_q, context_lens, max_q, max_k, scale, true, op}, out,
                             lse, p))
     return;
+  HA_CHECK(p.table_cols > 0, "%s: block_tables has no columns", op);  // (a context says on the device whether there is one to be read)
   p.max_q = (int)std::min<int64_t>(p.max_q, p.total_q);  // (no sequence has more; what is rounded up to row blocks stays within 32 bits)
   // (no context is longer than its table: what lies beyond that sees everything, and row + Lk - Lq - window_left stays within 32 bits)
   const int64_t longest = (int64_t)p.table_cols << p.block_log2;

@@ -240,6 +240,12 @@ def test_chunks_ask_for_no_workspace_that_they_cannot_use(over):
         assert "workspace" not in str(e.value)
 
 
+def test_chunks_refuse_tables_without_columns():
+    """A context on the device that says otherwise would have its blocks read from there."""
+    with pytest.raises(_lib.HipAttnError, match="no columns"):
+        _call("hipattn_mha_varlen_fwd_paged_window", *_chunk_args(tables=_t(2, 0, dtype=_lib.I32, data=0), max_k=0))
+
+
 @pytest.mark.parametrize("max_ctx", [2 ** 31 - 1, 2 ** 31 - 15])
 def test_paged_attention_refuses_context_bounds_of_31_bits(max_ctx):
     """(rounded up to blocks they leave 32 bits)"""
