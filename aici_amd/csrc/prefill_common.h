@@ -73,7 +73,7 @@ struct RowBlock {
 // The id-th block of `size` rows, at most `most` of a sequence, where sequences' blocks lie one behind the other, a sequence's last one first; by
 // whole wavefronts.  A grid of as many blocks as the longest sequence has for each of them is mostly workgroups that end at once: with a
 // window of 1000 and sinks, 63 sequences of 20 new tokens beside one of 4096, 32 / 8 x 128 291 us that way, 150 so, 16 / 2 x 64 147 and 49; 100 of one
-// token beside one of 1000, 8 / 2 x 256 261 and 107; 8 of 65 to 1001, 16 / 2 x 64 48 to 49 and 40 to 48, whichever comes first.
+// token beside one of 1000, 8 / 2 x 256 261 and 107; 8 of 65 to 1001, 16 / 2 x 64 48 to 49 and 40 to 50, whichever comes first.
 // Sequences of more than `keys` keys come first, as the launch otherwise ends with their long chains; `keys` is half a window.  Over 360 shapes (24
 // ragged batches of 12 to 60 sequences, windows of 500, 1500 and 4000, five layouts of heads of 64 to 128) the order as it comes is 8.7 % slower on
 // average and 55 % at most; limits of a quarter and a whole window 2.7 % and 2.5 % (a whole one is up to 19 % faster where it parts the batch better,

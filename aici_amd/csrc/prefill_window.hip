@@ -8,9 +8,11 @@
 // between the matrix pipe and the vector ALU, or workgroups of four wavefronts several to a compute unit -- over the 64-key tiles that hold a
 // key some row of the workgroup sees (prefill_w8.h, STEP::window).  What bounds them is the matrix pipe and the vector unit on
 // (window + rows of a block) keys a row, and with few workgroups the chain of a row block's tiles.  Measured: 2 x 4096 new tokens, 32 / 8 x 128 bf16,
-// a window of 4096 542 us, 0.95 PFLOP/s of what is seen (causal prefill of 8 x 4096 without a window 1.0 to 1.1); 8 chunks of
-// 65 to 1001 tokens, 16 / 2 x 64 fp16, a window of 1001 43 to 46 us by the order of the chunks, 0.35 PFLOP/s: the softmax of narrow heads, and
-// 552 workgroups, two or three to a compute unit (8 x 512 tokens, 512 workgroups, 39).
+// a window of 4096 535 us, 0.96 PFLOP/s of what is seen (causal prefill of 8 x 4096 without a window 1.0 to 1.1); 8 chunks of
+// 65 to 1001 tokens, 16 / 2 x 64 fp16, a window of 1001 40 to 50 us by the order of the chunks, 0.31 to 0.39 PFLOP/s: the softmax of narrow heads, and
+// 552 workgroups, two or three to a compute unit (8 x 512 tokens, 512 workgroups, 39).  Head sizes above 128 and those below 64 but 32 take tiles
+// staged through registers (prefill_varlen.hip), a row block's keys by one workgroup: 8 / 2 x 256, 1 x 2000 behind 4096 279 us, 0.24 PFLOP/s.
+// Probabilities are rounded to the cache's type as operands of the second product, as in all attention here; scores, sums and pieces are fp32.
 #include <algorithm>
 
 #include "paged_decode.h"

@@ -9,7 +9,8 @@
 // split or partitions, a merge -- over the 32-token pairs that hold a seen key, numbered without the gap between the sinks and the
 // window (SeenKeys); columns of the gap are not read, so that their blocks may have gone back to the pool.  A launch is planned as one
 // over contexts of that many tokens (seen_tokens).  The pair at either end of the gap is masked in its scores and its values are cleared:
-// a NaN there meets a probability of zero otherwise.
+// a NaN there meets a probability of zero otherwise.  Probabilities are rounded to the cache's type as operands of the second product, as in all paged
+// decode; scores, sums, partitions and the merge are fp32.
 //
 // Measured, 128 sequences of up to 16k tokens, 32 / 8 x 128 bf16, a window of 4096: 314 us, 1.99 GB at 6.3 TB/s (a read kernel with the same hint
 // gets 6.5), 6.6 of them the merge.  With few keys it is latency: 48 sequences, 39.7 MB, 11.8 us in one launch (lengths, table, keys one

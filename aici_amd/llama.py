@@ -40,8 +40,10 @@ class LlamaConfig:
     max_position_embeddings: int = 8192
     rope_theta: float = 10000.0
     dtype: torch.dtype = torch.bfloat16
-    sliding_window: Optional[int] = None  # tokens a token sees, with itself (None: all); no field of the reference's
-    attention_sinks: int = 0              # the first tokens of a sequence, which stay visible beside the window
+    sliding_window: Optional[int] = None  # tokens a token sees, with itself (None: all), in every layer; no field of the reference's
+    # The first tokens of a sequence, whose keys stay visible beside the window at the rotary positions they have in the sequence: neither counted
+    # anew inside the cache nor a learned term of the softmax, which other models mean by sinks.
+    attention_sinks: int = 0
 
     @property
     def head_dim(self) -> int:

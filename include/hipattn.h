@@ -113,7 +113,8 @@ char *hipattn_mha_varlen_fwd_paged(const hipattn_tensor *q, const hipattn_tensor
 /* hipattn_mha_varlen_fwd_paged with a sliding window and sinks: always causal, and the query at position p of its sequence sees key j
  * iff j <= p and (j >= p - window_size_left or j < sink_tokens) -- window_size_left + 1 tokens with its own, as the window of
  * hipattn_mha_varlen_fwd counts them, and the first sink_tokens of the sequence.  No counterpart in tch-cuda (its windows have no sinks
- * and read rows of k / v).  window_size_left >= 0, sink_tokens >= 0; everything else as there, any of its types, head and block sizes.
+ * and read rows of k / v).  Sinks are keys like others, as the cache holds them: nothing is rotated anew, and no term is added to the softmax.
+ * window_size_left >= 0, sink_tokens >= 0; everything else as there, any of its types, head and block sizes.
  * max_seqlen_q and max_seqlen_k bound every sequence's new tokens and keys: rows and keys beyond them may be left out.
  * Keys that no new token of a sequence sees may be gone: table columns that hold only such keys may name any block or none (a negative
  * or large number), and their blocks may hold anything.  Values of a key that some of a sequence's new tokens see are taken to be finite,
