@@ -21,7 +21,7 @@ struct PrefillParams {
   int max_q;      // caller's bound on Lq; sizes the grid
   int max_k;      // ... and on Lk
   int64_t total_q;  // query rows of all sequences
-  int lse_pitch;  // elements between (batch, head) rows of lse; a sequence's rows beyond that many (and beyond the caller's bound) have none
+  int lse_pitch;  // elements between (batch, head) rows of lse; a sequence's rows beyond that many have none
   int n_qblocks;
   float scale_log2;
   int causal;  // win_left < 0 && win_right == 0

@@ -48,11 +48,13 @@ bool eight_wavefronts_pay(const PrefillParams &p) {
 
 // Pieces that a row block's keys are dealt out in (workgroups of four wavefronts).  A workgroup's chain of tiles is bound by its own
 // instructions, some 2 us a tile with a wavefront per SIMD (five tiles in LDS instead of two change nothing), so where compute units are idle
-// more of them take a part each.  All in us, and fitted: what does not grow with the tiles, a tile, which takes longer from two workgroups per compute unit on, as two or three of them
-// fill each other's gaps; the merge, and what writing and reading the pieces costs.  In 400 measured shapes (1 x 5 new tokens to 2 x 4096, alike and
-// 63 x 20 beside one of 4096, windows of 100 to 4096, four kinds of heads) the choice among these and the kernel of decode rows is 1.8 % off the best on
-// average and 20 % at most; whole blocks alone are 39 %.  us, whole / best: 32 / 8 x 128, 1 x 5 over 4096 keys 99 / 16 (rows), 1 x 300 106 / 48 (6
-// pieces), 4 x 64 over 2000 61 / 29 (4); 32 / 32 x 80, 12 of 1 to 64 over 2000 83 / 65 (2); 16 / 2 x 64, 100 x 4 over 2000 66 / 39 (rows).
+// more of them take a part each.  All in us, and fitted: what does not grow with the tiles; a tile, which takes longer from two workgroups per
+// compute unit on, as two or three of them fill each other's gaps; the merge, and what writing and reading the pieces costs.  In 400 measured shapes
+// (1 x 5 new tokens to 2 x 4096, alike and 63 x 20 beside one of 4096, windows of 100 to 4096, four kinds of heads) the choice among these and the
+// kernel of decode rows is 1.8 % off the best on average and 20 % at most; whole blocks alone are 39 %.  In 90 whose sequences have contexts of very
+// different lengths 3.2 %, at most 2.2 times: the host knows the longest context alone.  us, whole / best: 32 / 8 x 128, 1 x 5 over 4096 keys 99 / 16
+// (rows), 1 x 300 106 / 48 (6 pieces), 4 x 64 over 2000 61 / 29 (4); 32 / 32 x 80, 12 of 1 to 64 over 2000 83 / 65 (2); 16 / 2 x 64, 100 x 4 over
+// 2000 66 / 39 (rows).
 // At most `most`; us: about what the launch takes then.
 int choose_parts(const PrefillParams &p, int most, double &us) {
   const int hl = prefill_heads_log2(p, 2), rows = 128 >> hl;

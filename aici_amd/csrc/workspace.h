@@ -50,7 +50,7 @@ struct Tuning {
   int cache_move_lds;      // -1: the library chooses; 0: never the LDS-transposing kernels
   int prefill_wg_heads;      // prefill_kernel 1 and (up to four) 5: query heads of one kv group per workgroup, at most (0: the library chooses -- up to four; 1: one)
   int prefill_rescale_log2;  // prefill: a row's reference maximum moves when outgrown by more than 2^this (0..16, default 8)
-  int window_parts;          // prefill over a window: 0: the library chooses; else workgroups of four wavefronts, a row block's keys dealt out to so many (where there is a merge for the head size, and scratch memory)
+  int window_parts;          // prefill over a window: pieces a row block's keys are dealt out in, by workgroups of four wavefronts, where there is a merge for the head size (0: the library chooses; else 1..16)
   int linear_tiles;          // linear: 64-row tiles of the weight per workgroup (0: the library chooses; 1 or 2)
   int linear_waves;          // linear: wavefronts per workgroup, 16 rows of the weight each (0: the library chooses; 4 or 8)
   int linear_splits;         // linear: ranges of the inner dimension (0: the library chooses; else 1..32)

@@ -370,7 +370,8 @@ class DeviceBlocks:
     """The blocks of a paged cache on the device (`kernels.step_blocks`), for up to max_requests requests that share none: every step's block
     tables, slots and positions come from how many tokens each request brings, without the host knowing a length, so that a step can be
     captured into a graph.  With a window (window_size_left >= 0, as in `attn.varlen_attn`) blocks that it has passed, sinks aside,
-    go back to the pool: the window of every layer, as the layers share the tables.  A request is a row of the tables; the row is free again when its request has ended."""
+    go back to the pool: the window of every layer, as the layers share the tables.  A request is a row of the tables; the row is free again
+    when its request has ended."""
 
     def __init__(self, block_size: int, num_blocks: int, max_requests: int, max_model_len: int, device, window_size_left: int = -1,
                  sink_tokens: int = 0):

@@ -615,8 +615,8 @@ char *hipattn_shutdown(void);
  * more than 2^value; 0 follows the row maximum exactly, as the reference
  * does), window_parts (prefill over a window: 0 library's choice, else the
  * number of workgroups, at most 16, that a row block's keys are dealt out to
- * where there is a merge for the head size), linear_tiles (0 library's choice, 1 / 2: workgroups of 64 /
- * 128 rows of the weight in hipattn_linear), linear_splits (0 library's choice, else
+ * where there is a merge for the head size), linear_tiles (0 library's choice,
+ * 1 / 2: workgroups of 64 / 128 rows of the weight in hipattn_linear), linear_splits (0 library's choice, else
  * the number of ranges the inner dimension is cut into, at most 32).  Every
  * setting computes the same results -- prefill_kernel 2 to 4 (over a window any
  * but 0), prefill_rescale_log2, window_parts and linear_splits up to rounding.  Not
