@@ -337,6 +337,10 @@ PyMethodDef g_methods[] = {
                                "softmax_scale,causal,out,lse"),
     BIND(mha_varlen_fwd_paged_window, "q,key_cache,value_cache,block_tables,cu_seqlens_q,context_lens,max_seqlen_q,max_seqlen_k,"
                                       "softmax_scale,window_size_left,sink_tokens,out,lse,workspace"),
+    BIND(paged_attention_tree, "q,key_cache,value_cache,block_tables,cu_seqlens_q,context_lens,max_seqlen_q,max_seqlen_k,softmax_scale,"
+                               "tree_mask,out,workspace"),
+    BIND(tree_rows, "parents,seqlens_q,context_lens,max_seqlen_q,positions,mask"),
+    BIND(tree_accept, "tokens,parents,chosen,seqlens_q,max_seqlen_q,slot_mapping,key_cache_ptrs,value_cache_ptrs,key0,value0,lens,path,next"),
     BIND(paged_attention_window, "out,query,key_cache,value_cache,num_kv_heads,scale,block_tables,context_lens,block_size,"
                                  "max_context_len,window_size_left,sink_tokens,alibi,workspace"),
     BIND(paged_attention_v1, "out,query,key_cache,value_cache,num_kv_heads,scale,block_tables,context_lens,block_size,"

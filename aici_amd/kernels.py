@@ -119,6 +119,28 @@ def flash_attn_varlen_paged_window_workspace_size(total_q: int, num_heads: int, 
     return int(n.value)
 
 
+def paged_attention_tree(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, block_tables: torch.Tensor,
+                         seqlens_q: torch.Tensor, context_lens: torch.Tensor, max_seqlen_q: int, max_seqlen_k: int, softmax_scale: float,
+                         tree_mask: torch.Tensor, out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of trees of drafted tokens over the paged cache.  q [Tq,Hq,d], block_tables, seqlens_q and context_lens as for
+    `flash_attn_varlen_paged` (the rows' own keys are the last of the context); a row sees every key in front of its tree and, of the tree's
+    keys, those that tree_mask int64 [Tq, words] names: bit j % 64 of word j / 64 for the sequence's j-th row (`tree_rows`).  A row that sees
+    nothing is zero.  workspace: uint8, `paged_attention_tree_workspace_size` bytes, for calls that are captured and for those that must not
+    allocate; None: a buffer that the library keeps per stream, and under capture none, which takes longer for few long contexts."""
+    if out is None:
+        out = torch.empty_like(q)
+    _native.paged_attention_tree(q, key_cache, value_cache, block_tables, seqlens_q, context_lens, max_seqlen_q, max_seqlen_k, softmax_scale,
+                                 tree_mask, out, workspace)
+    return out
+
+
+def paged_attention_tree_workspace_size(total_q: int, num_heads: int, head_size: int) -> int:
+    """Bytes of scratch memory paged_attention_tree can make use of for total_q rows."""
+    n = ctypes.c_int64(0)
+    call("hipattn_paged_attention_tree_workspace_size", int(total_q), int(num_heads), int(head_size), ctypes.byref(n))
+    return int(n.value)
+
+
 def paged_attention_window(out: torch.Tensor, query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
                            num_kv_heads: int, scale: float, block_tables: torch.Tensor, context_lens: torch.Tensor, block_size: int,
                            max_context_len: int, window_size_left: int, sink_tokens: int = 0,
@@ -490,6 +512,68 @@ def step_blocks(new_lens: torch.Tensor, state: torch.Tensor, block_tables: torch
     _native.step_blocks(new_lens, state, block_tables, free_ring, ring_ends, block_size, rows_per_request, window_size_left, sink_tokens,
                         state_out, ring_ends_out, served, context_lens, seqlens_q, logit_idxs, positions, slots, totals, work)
     return StepBlocks(state_out, ring_ends_out, served, context_lens, seqlens_q, logit_idxs, positions, slots, totals)
+
+
+# --------------------------------------------------------------------------- trees of drafted tokens
+
+class TreeRows(NamedTuple):
+    """What `tree_rows` says of a step's trees."""
+    positions: torch.Tensor  # int64 [T]
+    mask: torch.Tensor       # int64 [T, (max_seqlen_q + 63) / 64]: bits of the rows of its tree that a row sees
+
+
+def tree_rows(parents: torch.Tensor, seqlens_q: torch.Tensor, context_lens: torch.Tensor, max_seqlen_q: int) -> TreeRows:
+    """Positions and masks of trees of drafted tokens (hipattn_tree_rows in hipattn.h): parents int32 [T], the row of its own tree that a
+    row continues, negative: none; a row sees itself and its ancestors and lies behind as many of them.  At most 1024 rows a tree."""
+    T = parents.size(0)
+    rows = TreeRows(torch.empty((T,), dtype=torch.int64, device=parents.device),
+                    torch.empty((T, (int(max_seqlen_q) + 63) // 64), dtype=torch.int64, device=parents.device))
+    _native.tree_rows(parents, seqlens_q, context_lens, max_seqlen_q, rows.positions, rows.mask)
+    return rows
+
+
+class CacheList:
+    """Every layer's key and value cache as `tree_accept` takes them: made once, when the caches are, and kept with them."""
+
+    def __init__(self, key_caches: Sequence[torch.Tensor], value_caches: Sequence[torch.Tensor]):
+        self.key_caches, self.value_caches = list(key_caches), list(value_caches)
+        if not self.key_caches or len(self.key_caches) != len(self.value_caches):
+            raise HipAttnError(f"CacheList: {len(self.key_caches)} key caches and {len(self.value_caches)} value caches")
+        for caches in (self.key_caches, self.value_caches):
+            first = caches[0]
+            for t in caches:
+                if not t.is_cuda or t.device != self.key_caches[0].device:
+                    raise HipAttnError(f"CacheList: expected GPU tensors of one device, got one on {t.device}")
+                if t.dtype != self.key_caches[0].dtype or t.size() != first.size() or t.stride() != first.stride() or t.data_ptr() % 16 != 0:
+                    raise HipAttnError("CacheList: the layers' caches must have one type, one shape and the same strides, and start on 16-byte boundaries")
+        device = self.key_caches[0].device
+        self.key_ptrs = torch.tensor([t.data_ptr() for t in self.key_caches], dtype=torch.int64).to(device)
+        self.value_ptrs = torch.tensor([t.data_ptr() for t in self.value_caches], dtype=torch.int64).to(device)
+
+
+class TreeAccept(NamedTuple):
+    """What `tree_accept` keeps of a step's trees."""
+    lens: torch.Tensor         # int32 [R]: rows kept, the root among them; 0 without rows
+    path: torch.Tensor         # int32 [R, max_seqlen_q]: which, counted in the tree; -1 behind the last
+    next_tokens: torch.Tensor  # int32 [R]: the token that follows the last of them; -1 without rows
+
+
+def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, chosen: torch.Tensor, seqlens_q: torch.Tensor, max_seqlen_q: int,
+                slot_mapping: Optional[torch.Tensor] = None, caches: Optional[CacheList] = None) -> TreeAccept:
+    """The drafted tokens that the model's choices confirm (hipattn_tree_accept in hipattn.h): tokens, parents, chosen int32 [T], `chosen`
+    what `bias_argmax` or `bias_sample` gives for every row.  With slot_mapping [T] and caches the kept rows' keys and values move to the slots of
+    the tree's first rows, in every layer."""
+    R, device = seqlens_q.size(0) - 1, tokens.device
+    kept = TreeAccept(torch.empty((max(R, 0),), dtype=torch.int32, device=device),
+                      torch.empty((max(R, 0), int(max_seqlen_q)), dtype=torch.int32, device=device),
+                      torch.empty((max(R, 0),), dtype=torch.int32, device=device))
+    if caches is None:
+        _native.tree_accept(tokens, parents, chosen, seqlens_q, max_seqlen_q, slot_mapping, None, None, None, None, kept.lens, kept.path,
+                            kept.next_tokens)
+    else:
+        _native.tree_accept(tokens, parents, chosen, seqlens_q, max_seqlen_q, slot_mapping, caches.key_ptrs, caches.value_ptrs,
+                            caches.key_caches[0], caches.value_caches[0], kept.lens, kept.path, kept.next_tokens)
+    return kept
 
 
 # --------------------------------------------------------------------------- runtime plumbing

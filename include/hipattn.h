@@ -132,6 +132,48 @@ char *hipattn_mha_varlen_fwd_paged_window(const hipattn_tensor *q, const hipattn
                                           hipattn_tensor *softmax_lse, const hipattn_tensor *workspace, void *stream);
 char *hipattn_mha_varlen_fwd_paged_window_workspace_size(int64_t total_q, int num_heads, int head_size, int64_t *bytes);
 
+/* Attention of trees of drafted tokens over the paged cache (speculative decoding); no counterpart in tch-cuda, which generates a token at a
+ * time.  Sequence s has the rows cu_seqlens_q[s] .. cu_seqlens_q[s + 1] of q, n of them, whose keys are the last n of its context_lens[s] keys,
+ * row i's at context_lens[s] - n + i (hipattn_reshape_and_cache or hipattn_rotary_embedding_and_cache have put them there; their rotary
+ * positions are hipattn_tree_rows').  Every row sees the keys in front of the tree, and of the tree's keys those that its mask names:
+ * tree_mask int64 [total_q, words], words * 64 >= max_seqlen_q, rows may lie apart: bit j % 64 of word j / 64 for the key of the sequence's j-th
+ * row; bits from n on are not looked at.  Any mask will do, a tree's or not; a causal one gives hipattn_mha_varlen_fwd_paged's result.
+ * A row that sees nothing is zero.  What a row does not see of its tree has no say in its result, NaN and infinities among them.
+ * q/out [total_q, Hq, d] f16 or bf16, d 64, 80, 96, 112, 128 or 256; caches, block_tables and the other arguments as for
+ * hipattn_mha_varlen_fwd_paged; rows and keys beyond max_seqlen_q and max_seqlen_k may be left out, rows of no sequence are left as they are.
+ * Contexts are dealt out to several workgroups where few would leave compute units idle, by way of workspace: u8, 256-byte aligned,
+ * hipattn_paged_attention_tree_workspace_size bytes (at most 64 MiB), not shared by calls that overlap, replays of captured ones included.
+ * NULL: a buffer of 64 MiB that the library allocates once per stream; under capture, on hipStreamPerThread and without that memory contexts
+ * are not dealt out, so that last bits, and the time of few long contexts, may differ. */
+char *hipattn_paged_attention_tree(const hipattn_tensor *q, const hipattn_tensor *key_cache, const hipattn_tensor *value_cache,
+                                   const hipattn_tensor *block_tables, const hipattn_tensor *cu_seqlens_q,
+                                   const hipattn_tensor *context_lens, int max_seqlen_q, int max_seqlen_k, float softmax_scale,
+                                   const hipattn_tensor *tree_mask, hipattn_tensor *out, const hipattn_tensor *workspace, void *stream);
+char *hipattn_paged_attention_tree_workspace_size(int64_t total_q, int num_heads, int head_size, int64_t *bytes);
+
+/* Positions and masks of trees of drafted tokens from the parents of their rows.  parents int32 [T]: the row, counted in its own tree, that a
+ * row continues; negative, or not in front of the row: none.  seqlens_q int32 [R + 1], context_lens int32 [R] as for
+ * hipattn_paged_attention_tree; max_seqlen_q at most 1024.  positions int64 [T]: context_lens - n + the number of a row's ancestors;
+ * mask int64 [T, (max_seqlen_q + 63) / 64]: the bits of the row and its ancestors.  Rows of no sequence and those beyond max_seqlen_q get position
+ * 0 and an empty mask. */
+char *hipattn_tree_rows(const hipattn_tensor *parents, const hipattn_tensor *seqlens_q, const hipattn_tensor *context_lens,
+                        int max_seqlen_q, hipattn_tensor *positions, hipattn_tensor *mask, void *stream);
+
+/* What a step has confirmed of trees of drafted tokens.  tokens, parents, chosen int32 [T]: a row's token, its parent as above, and what the
+ * model has chosen to follow it (hipattn_bias_argmax, or hipattn_bias_sample: drafts are kept where the model's own choice is the draft, so
+ * that what is generated has the model's own distribution, whatever drafted).  From a sequence's row 0, which is no draft, the way goes to
+ * the lowest row behind the one in hand whose parent that is and whose token was chosen there.  lens int32 [R]: rows of the way, 0 without rows;
+ * path int32 [R, max_seqlen_q]: the rows, counted in the tree, -1 behind the last; next int32 [R]: what was chosen at the last of them, -1 without
+ * rows.  max_seqlen_q at most 1024; rows beyond it are left out.
+ * With slot_mapping [T] (int32 or int64, -1: none), key_cache_ptrs and value_cache_ptrs (int64 [layers] on the device: the caches of every
+ * layer, each like key0 and value0 in type, sizes and strides) the keys and values of the way's k-th row are moved to the slot of the tree's
+ * k-th row, so that the sequence's first context_lens - n + lens keys are those of its tokens.  Rows may not share slots.  All five NULL: nothing
+ * is moved.  At most 65535 sequences and layers. */
+char *hipattn_tree_accept(const hipattn_tensor *tokens, const hipattn_tensor *parents, const hipattn_tensor *chosen,
+                          const hipattn_tensor *seqlens_q, int max_seqlen_q, const hipattn_tensor *slot_mapping,
+                          const hipattn_tensor *key_cache_ptrs, const hipattn_tensor *value_cache_ptrs, hipattn_tensor *key0,
+                          hipattn_tensor *value0, hipattn_tensor *lens, hipattn_tensor *path, hipattn_tensor *next, void *stream);
+
 /* Replaces paged_attention_v1_C (lib.rs:107-120; attention_kernels.cu:679-700).
  * out/query [S, Hq, d]; key_cache [nb, Hkv, d/x, BS, x]; value_cache
  * [nb, Hkv, d, BS]; block_tables int32 [S, max_blocks]; context_lens int32 [S].
