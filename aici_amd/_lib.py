@@ -13,7 +13,7 @@ from pathlib import Path
 LIB_PATH = Path(__file__).resolve().parent / "libhipattn.so"
 
 MAX_DIMS = 5
-F32, F16, BF16, I32, I64, U8 = range(6)
+F32, F16, BF16, I32, I64, U8, E4M3 = range(7)
 
 
 class Tensor(ctypes.Structure):
@@ -105,6 +105,8 @@ _ERR_FUNCS = {
     "hipattn_fused_add_rms_norm": [TP, TP, TP, c_float, c_void_p],
     "hipattn_add_rms_norm": [TP, TP, TP, TP, c_float, c_void_p],
     "hipattn_linear": [TP, TP, TP, TP, TP, TP, c_void_p],
+    "hipattn_linear_fp8": [TP, TP, TP, TP, TP, TP, TP, c_void_p],
+    "hipattn_linear_fp8_workspace_size": [TP, TP, POINTER(c_int64)],
     "hipattn_linear_silu_and_mul": [TP, TP, TP, TP, c_void_p],
     "hipattn_rms_norm_linear": [TP, TP, TP, c_float, TP, c_bool, c_void_p],
     "hipattn_qkv_linear": [TP, TP, TP, c_float, TP, TP, TP, TP, TP, TP, c_void_p],

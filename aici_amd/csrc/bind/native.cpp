@@ -49,6 +49,7 @@ bool dtype_of(const DLDataType &t, int32_t *out) {
     case kDLFloat: if (t.bits == 32) *out = HIPATTN_F32; else if (t.bits == 16) *out = HIPATTN_F16; else return false; return true;
     case kDLBfloat: if (t.bits != 16) return false; *out = HIPATTN_BF16; return true;
     case kDLInt: if (t.bits == 32) *out = HIPATTN_I32; else if (t.bits == 64) *out = HIPATTN_I64; else return false; return true;
+    case kDLFloat8_e4m3fn: if (t.bits != 8) return false; *out = HIPATTN_E4M3; return true;
     case kDLUInt: if (t.bits != 8) return false; *out = HIPATTN_U8; return true;
     default: return false;
   }
@@ -359,6 +360,7 @@ PyMethodDef g_methods[] = {
     BIND(fused_add_rms_norm, "input,residual,weight,epsilon"),
     BIND(add_rms_norm, "out,input,residual,weight,epsilon"),
     BIND(linear, "out,x,weight,bias,residual,workspace"),
+    BIND(linear_fp8, "out,x,weight,weight_scale,bias,residual,workspace"),
     BIND(linear_silu_and_mul, "out,x,weight,workspace"),
     BIND(linear_rms_norm, "out,norm_out,x,weight,bias,residual,norm_weight,epsilon,workspace"),
     BIND(rms_norm_linear, "out,x,norm_weight,epsilon,weight,silu_and_mul"),

@@ -69,6 +69,7 @@ inline int dtype_size(int dtype) {
     case HIPATTN_I32: return 4;
     case HIPATTN_I64: return 8;
     case HIPATTN_U8: return 1;
+    case HIPATTN_E4M3: return 1;
   }
   fail("unknown dtype %d", dtype);
 }
@@ -81,6 +82,7 @@ inline const char *dtype_name(int dtype) {
     case HIPATTN_I32: return "i32";
     case HIPATTN_I64: return "i64";
     case HIPATTN_U8: return "u8";
+    case HIPATTN_E4M3: return "e4m3";
   }
   return "?";
 }

@@ -1,0 +1,469 @@
+// Linear layer on a weight of 8-bit floating point (e4m3) with a scale for each 128 x 128 of it: y = x . Wᵀ (+ bias) (+ residual), any number
+// of rows of x.  No counterpart in the reference, whose weights are those of hipattn_linear.
+//
+//   e[m, b] = the least integer with max |x[m, block b]| <= 448 2^e (at least -126);  q[m, k] = x[m, k] 2^-e rounded to e4m3, ties to even
+//   y[m, n] = T( sum over blocks b of 2^e[m, b] ws[n / 128, b] (sum over k in b of q[m, k] w[n, k])  + bias[n] ) (+ residual[m, n], rounded again)
+//
+// The scales of x are powers of two, so that scaling is exact and what is rounded is x itself; the largest of a block lands in (224, 448], and e4m3
+// has the same relative steps there as below.  Sums of a block are the matrix pipe's, the sum over blocks is one fp32 FMA per block.
+//
+// The matrix pipe adds the products of 8-bit numbers eight at a time, each cut at 2^-13 of the largest one's power of two (measured; seen also
+// across lanes: fp32 from there on).  Against a row of 4096 random products that is some 2^-13 of the sum, a tenth of the rounding to bf16 and about
+// that to fp16; products of 16-bit operands would keep all of it, at half the rate and with every byte of W unpacked first.
+//
+// A launch rounds the rows of x to 8 bits, with the blocks' scales beside them; the product's launch copies rows of W and x global -> LDS
+// (128 bytes of a row at a time: a block of 128) into a ring, and takes v_mfma_f32_16x16x128 over them.  W is operand A, so that a lane's sums
+// belong to one row of x and one scale serves all of them; which rows of W make a tile is chosen so that a lane's outputs lie end to end.
+#include "common.h"
+#include "device_types.h"
+#include "workspace.h"
+
+#include <algorithm>
+
+// The copies set M0, and say so; the compiler reports that it is a reserved register.
+#pragma clang diagnostic ignored "-Winline-asm"
+
+namespace hipattn {
+namespace {
+
+constexpr int kBlock = 128;  // columns (and rows of W) that share a scale; bytes of a row per stage
+
+struct Fp8Params {
+  const void *x, *bias, *residual;
+  const uint8_t *w, *xq;  // xq [M, KB * 128]
+  const float *ws;
+  float *xs;  // [KB, Mp]
+  void *out;
+  float *partial;  // [splits, M, N]
+  int M, N, K, KB, Mp;
+  int64_t ldx, ldw, ldws, ldr, ldo;
+  int splits, stages_per_split;
+  int tiles_m, tiles_n;
+  int wide_out;  // rows of out (and residual, and bias) on 16-byte boundaries
+};
+
+// ------------------------------------------------------------------ rows of x to 8 bits
+
+// A thread takes eight elements, 16 threads a block.
+template <typename T>
+__global__ __launch_bounds__(256) void quantize_rows_kernel(const Fp8Params p) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int b = (int)(i / 16 % p.KB), m = (int)(i / 16 / p.KB), k = b * kBlock + (int)(i % 16) * 8;
+  if (m >= p.M) return;
+  uint4 raw = make_uint4(0, 0, 0, 0);
+  if (k < p.K) raw = *reinterpret_cast<const uint4 *>(static_cast<const T *>(p.x) + (int64_t)m * p.ldx + k);
+  const T *e = reinterpret_cast<const T *>(&raw);
+  float v[8];
+  unsigned most = 0;  // bits of the largest magnitude; infinities and NaN are larger than any number
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    v[j] = to_float(e[j]);
+    most = max(most, bit_cast<unsigned>(v[j]) & 0x7fffffffu);
+  }
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) most = max(most, (unsigned)__shfl_xor((int)most, o, 16));
+  // the least power of two s with most <= 448 s = 1.75 * 2^8 s
+  const int up = max((int)((most + 0x1fffffu) >> 23) - 8, 1);  // its exponent's bits
+  const float down = bit_cast<float>((unsigned)(254 - up) << 23);
+  int lo = 0, hi = 0;
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * down, v[1] * down, lo, false);
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * down, v[3] * down, lo, true);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[4] * down, v[5] * down, hi, false);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[6] * down, v[7] * down, hi, true);
+  *reinterpret_cast<uint2 *>(const_cast<uint8_t *>(p.xq) + ((int64_t)m * p.KB + b) * kBlock + (i % 16) * 8) = make_uint2((unsigned)lo, (unsigned)hi);
+  if (i % 16 == 0) p.xs[(int64_t)b * p.Mp + m] = most >= 0x7f800000u ? bit_cast<float>(0x7fc00000u) : bit_cast<float>((unsigned)up << 23);
+}
+
+// ------------------------------------------------------------------ the product
+
+template <int N>
+__device__ __forceinline__ void wait_copies() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ uint32_t lds_address(const void *p) {
+  return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char *)p);
+}
+
+__device__ __forceinline__ const char *uniform_base(const char *ptr) {
+  const uint64_t v = reinterpret_cast<uint64_t>(ptr);
+  return reinterpret_cast<const char *>(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32)) << 32) |
+                                        (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v));
+}
+
+// 64 lanes x 16 bytes, global -> LDS: lane l's bytes go to lds + 16 l.
+__device__ __forceinline__ void copy_1k(uint32_t lds, const char *base, uint32_t off) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
+}
+// 64 lanes x 4 bytes.
+__device__ __forceinline__ void copy_256(uint32_t lds, const char *base, uint32_t off) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
+}
+
+typedef int i32x8_t __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ f32x4_t mfma_fp8(i32x8_t a, i32x8_t b) {
+  const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, zero, 0, 0, 0, 0, 0, 0);
+}
+
+// The runs of 16 bytes of a row lie in LDS in the order q ^ turn, so that the rows of a tile do not meet in the same banks.
+__device__ __forceinline__ i32x8_t operand(const char *rows, int r, int turn, int kg) {
+  const uint4 a = *reinterpret_cast<const uint4 *>(rows + r * kBlock + ((kg ^ turn) * 16));
+  const uint4 b = *reinterpret_cast<const uint4 *>(rows + r * kBlock + (((4 + kg) ^ turn) * 16));
+  return i32x8_t{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w};
+}
+
+// v: the sums of y[m][n .. n + 3].
+template <typename T>
+__device__ __forceinline__ void finish4(const Fp8Params &p, const f32x4_t v, int m, int n, T *o) {
+  typedef T vec4 __attribute__((ext_vector_type(4)));
+  const T *bias = static_cast<const T *>(p.bias), *res = static_cast<const T *>(p.residual);
+  vec4 b4 = vec4{(T)0.f, (T)0.f, (T)0.f, (T)0.f}, r4 = b4;
+  if (bias != nullptr) b4 = *reinterpret_cast<const vec4 *>(bias + n);
+  if (res != nullptr) r4 = *reinterpret_cast<const vec4 *>(res + (int64_t)m * p.ldr + n);
+#pragma unroll
+  for (int r = 0; r < 4; r++) {
+    float f = v[r];
+    if (bias != nullptr) f += to_float<T>(b4[r]);
+    o[r] = from_float<T>(f);
+    if (res != nullptr) o[r] = add_t<T>(o[r], r4[r]);
+  }
+}
+
+// GN x GM wavefronts, each with WN x WM tiles of 16 rows of W x 16 rows of x; S stages in the ring.
+template <typename T, int WN, int WM, int GN, int GM, int S>
+__global__ __launch_bounds__(GN *GM * 64) void fp8_tile_kernel(const Fp8Params p) {
+  constexpr int WAVES = GN * GM, BN = GN * WN * 16, BM = GM * WM * 16;
+  constexpr int kCopiesW = BN / 8 / WAVES, kAllX = BM / 8, kCopiesX = (kAllX + WAVES - 1) / WAVES;
+  static_assert(BN % (8 * WAVES) == 0, "copies of W divide evenly");
+  constexpr int kScales = (BM + 63) / 64;  // pieces of 64 scales
+  constexpr int kCopies = kCopiesW + kCopiesX + 1;
+  constexpr int kStageBytes = (BN + BM) * kBlock + kScales * 256;
+  __shared__ __align__(1024) char ring[S * kStageBytes];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, kg = lane >> 4;
+  const int wn = wave % GN, wm = wave / GN;
+  // Tiles in groups of four of W by all of x, and of that list a contiguous part to each XCD, which shares an L2.
+  const int tiles = p.tiles_m * p.tiles_n, per_xcd = (tiles + 7) / 8;
+  const int at = (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
+  if (at >= tiles) return;
+  const int group = at / (4 * p.tiles_m), in_group = at - group * 4 * p.tiles_m, width = min(4, p.tiles_n - group * 4);
+  const int n0 = (group * 4 + in_group % width) * BN, m0 = in_group / width * BM;
+  const int stage0 = blockIdx.y * p.stages_per_split, nst = max(0, min(p.stages_per_split, p.KB - stage0));
+
+  // What a lane copies of eight rows: run q of row r to this lane's place.  Rows past the last repeat it; columns past the last of W, where x is zero,
+  // repeat the row's last run.
+  const char *wbase[kCopiesW], *xbase[kCopiesX];
+  uint32_t woff[kCopiesW], xoff[kCopiesX];
+  int wrun[kCopiesW];
+  const int row8 = lane >> 3;
+#pragma unroll
+  for (int i = 0; i < kCopiesW; i++) {
+    const int r = (wave * kCopiesW + i) * 8, in_tile = r + row8;  // row of the workgroup's
+    const int in_wave = in_tile % (WN * 16), turn = (in_wave & 3) + 4 * (in_wave / (4 * WN) & 1);
+    const int first = min(n0 + r, p.N - 1), rows_on = min(n0 + in_tile, p.N - 1) - first;
+    wrun[i] = ((lane & 7) ^ turn) * 16;
+    wbase[i] = uniform_base(reinterpret_cast<const char *>(p.w) + (int64_t)first * p.ldw);
+    woff[i] = (uint32_t)rows_on * (uint32_t)p.ldw;
+  }
+#pragma unroll
+  for (int i = 0; i < kCopiesX; i++) {
+    const int r = (wave + i * WAVES) % kAllX * 8, in_tile = r + row8;
+    const int first = min(m0 + r, p.M - 1), rows_on = min(m0 + in_tile, p.M - 1) - first;
+    xbase[i] = uniform_base(reinterpret_cast<const char *>(p.xq) + (int64_t)first * p.KB * kBlock);
+    xoff[i] = (uint32_t)rows_on * (uint32_t)(p.KB * kBlock) + ((lane & 7) ^ (row8 & 7)) * 16;
+  }
+  const uint32_t ring_lds = lds_address(ring);
+  const char *sbase = uniform_base(reinterpret_cast<const char *>(p.xs + m0 + wave % kScales * 64));
+  auto ask = [&](int slot, int st) {
+    const int b = stage0 + st;
+    const uint32_t to = ring_lds + slot * kStageBytes;
+#pragma unroll
+    for (int i = 0; i < kCopiesX; i++) copy_1k(to + (BN + (wave + i * WAVES) % kAllX * 8) * kBlock, xbase[i] + (int64_t)b * kBlock, xoff[i]);
+#pragma unroll
+    for (int i = 0; i < kCopiesW; i++)
+      copy_1k(to + (wave * kCopiesW + i) * 1024, wbase[i], woff[i] + (uint32_t)min(b * kBlock + wrun[i], p.K - 16));
+    copy_256(to + (BN + BM) * kBlock + wave % kScales * 256, sbase + (int64_t)b * p.Mp * 4, lane * 4);
+  };
+
+  f32x4_t acc[WN][WM];
+#pragma unroll
+  for (int nt = 0; nt < WN; nt++)
+#pragma unroll
+    for (int mt = 0; mt < WM; mt++) acc[nt][mt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  const float *ws = p.ws + (int64_t)(min(n0 + wn * WN * 16, p.N - 1) / kBlock) * p.ldws + stage0;
+  const int turn_w = (col & 3) + 4 * (col >> 2 & 1);  // of this lane's row of every tile of W
+#pragma unroll
+  for (int j = 0; j < S - 1; j++)
+    if (j < nst) ask(j, j);
+  for (int base = 0; base < nst; base += S) {
+#pragma unroll
+    for (int j = 0; j < S; j++) {
+      const int st = base + j;
+      if (st < nst) {
+        // This wavefront's copies of the stage have landed, and behind the barrier everybody's; the barrier also says that the stage before has
+        // been read, so its place takes the copies of the stage S - 1 further on.
+        if (st + S - 2 < nst) wait_copies<(S - 2) * kCopies>();
+        else wait_copies<0>();
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (st + S - 1 < nst) ask((j + S - 1) % S, st + S - 1);
+        const char *stage = ring + j * kStageBytes;
+        const char *wrows = stage + wn * WN * 16 * kBlock, *xrows = stage + BN * kBlock;
+        const float *scales = reinterpret_cast<const float *>(stage + (BN + BM) * kBlock);
+        const float sw = ws[st];
+        i32x8_t xf[WM];
+        float s[WM];
+#pragma unroll
+        for (int mt = 0; mt < WM; mt++) {
+          const int r = (wm * WM + mt) * 16 + col;
+          xf[mt] = operand(xrows, r, col & 7, kg);
+          s[mt] = scales[r] * sw;
+        }
+        // A tile's products go into the sums while the matrix pipe has the next tile's; the rows of W of the tile behind that are on their way.
+        auto rows_of = [&](int nt) { return operand(wrows, (col >> 2) * (4 * WN) + nt * 4 + (col & 3), turn_w, kg); };
+        i32x8_t wf = rows_of(0);
+        f32x4_t part[WM];
+#pragma unroll
+        for (int nt = 0; nt <= WN; nt++) {
+          const i32x8_t now = wf;
+          if (nt + 1 < WN) wf = rows_of(nt + 1);
+#pragma unroll
+          for (int mt = 0; mt < WM; mt++) {
+            f32x4_t next;
+            if (nt < WN) next = mfma_fp8(now, xf[mt]);
+            if (nt > 0) {
+#pragma unroll
+              for (int i = 0; i < 4; i++) acc[nt - 1][mt][i] = __builtin_fmaf(part[mt][i], s[mt], acc[nt - 1][mt][i]);
+            }
+            part[mt] = next;
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    }
+  }
+
+  // A lane has 4 WN outputs of a row, end to end.
+  const int n = n0 + wn * WN * 16 + kg * 4 * WN;
+#pragma unroll
+  for (int mt = 0; mt < WM; mt++) {
+    const int m = m0 + (wm * WM + mt) * 16 + col;
+    if (m >= p.M) continue;
+    if (p.splits > 1) {
+      float *to = p.partial + ((int64_t)blockIdx.y * p.M + m) * p.N + n;
+#pragma unroll
+      for (int nt = 0; nt < WN; nt++)
+        if (n + nt * 4 < p.N) *reinterpret_cast<f32x4_t *>(to + nt * 4) = acc[nt][mt];
+      continue;
+    }
+    T *to = static_cast<T *>(p.out) + (int64_t)m * p.ldo + n;
+    if constexpr (WN % 2 == 0) {
+      if (p.wide_out) {
+#pragma unroll
+        for (int nt = 0; nt < WN; nt += 2) {
+          if (n + nt * 4 >= p.N) continue;  // (N is a multiple of 16, so of the eight that lie here)
+          __align__(16) T o[8];
+          finish4<T>(p, acc[nt][mt], m, n + nt * 4, o);
+          finish4<T>(p, acc[nt + 1][mt], m, n + nt * 4 + 4, o + 4);
+          *reinterpret_cast<uint4 *>(to + nt * 4) = *reinterpret_cast<uint4 *>(o);
+        }
+        continue;
+      }
+    }
+#pragma unroll
+    for (int nt = 0; nt < WN; nt++) {
+      if (n + nt * 4 >= p.N) continue;
+      __align__(8) T o[4];
+      finish4<T>(p, acc[nt][mt], m, n + nt * 4, o);
+      *reinterpret_cast<uint2 *>(to + nt * 4) = *reinterpret_cast<uint2 *>(o);
+    }
+  }
+}
+
+// Adds up the ranges' sums, the first range first: a thread for four outputs.
+template <typename T>
+__global__ __launch_bounds__(256) void fp8_reduce_kernel(const Fp8Params p) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int quads = p.N / 4, n = (int)(i % quads) * 4;
+  const int64_t m = i / quads;
+  if (m >= p.M) return;
+  const float *from = p.partial + m * p.N + n;
+  f32x4_t sum = *reinterpret_cast<const f32x4_t *>(from);
+  for (int s = 1; s < p.splits; s++) {
+    const f32x4_t v = *reinterpret_cast<const f32x4_t *>(from + (int64_t)s * p.M * p.N);
+#pragma unroll
+    for (int r = 0; r < 4; r++) sum[r] += v[r];
+  }
+  __align__(8) T o[4];
+  finish4<T>(p, sum, (int)m, n, o);
+  *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + m * p.ldo + n) = *reinterpret_cast<uint2 *>(o);
+}
+
+// ------------------------------------------------------------------ choices
+
+enum Fp8Form { FP8_16, FP8_32, FP8_64, FP8_128, FP8_256 };
+struct Fp8Plan {
+  Fp8Form form;
+  int bn, bm, splits, stages_per_split;
+  size_t xq_bytes, xs_bytes, bytes;  // rounded rows of x, their scales, everything
+  int Mp;
+};
+
+Fp8Plan plan_fp8(int64_t M, int N, int K) {
+  Fp8Plan pl;
+  const int KB = (K + kBlock - 1) / kBlock;
+  pl.form = M <= 16 ? FP8_16 : (M <= 32 ? FP8_32 : (M <= 64 ? FP8_64 : FP8_128));
+  const int64_t large = ((M + 255) / 256) * ((N + 255) / 256);
+  if (M > 128 && large >= 200) pl.form = FP8_256;
+  pl.bn = pl.form == FP8_256 ? 256 : 128;
+  pl.bm = pl.form == FP8_16 ? 16 : (pl.form == FP8_32 ? 32 : (pl.form == FP8_64 ? 64 : (pl.form == FP8_128 ? 128 : 256)));
+  const int64_t tiles = ((M + pl.bm - 1) / pl.bm) * ((N + pl.bn - 1) / pl.bn);
+  int splits = 1;
+  while (splits < 8 && tiles * splits < 256 && KB / (2 * splits) >= 4) splits *= 2;
+  pl.stages_per_split = (KB + splits - 1) / splits;
+  pl.splits = (KB + pl.stages_per_split - 1) / pl.stages_per_split;
+  auto up = [](size_t b) { return (b + 255) / 256 * 256; };
+  pl.Mp = (int)((M + 255) / 256 * 256);
+  pl.xq_bytes = up((size_t)M * KB * kBlock);
+  pl.xs_bytes = up((size_t)KB * pl.Mp * 4);
+  pl.bytes = pl.xq_bytes + pl.xs_bytes + (pl.splits > 1 ? up((size_t)pl.splits * M * N * 4) : 0);
+  return pl;
+}
+
+template <typename T>
+void launch_fp8(const Fp8Params &p, const Fp8Plan &pl, hipStream_t stream) {
+  const int64_t threads = (int64_t)p.M * p.KB * 16;
+  quantize_rows_kernel<T><<<dim3((unsigned)((threads + 255) / 256)), 256, 0, stream>>>(p);
+  check_launch("linear_fp8 (rows)");
+  const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
+  const dim3 grid((unsigned)((tiles + 7) / 8 * 8), (unsigned)p.splits);
+  switch (pl.form) {
+    case FP8_16: fp8_tile_kernel<T, 2, 1, 4, 1, 4><<<grid, 256, 0, stream>>>(p); break;
+    case FP8_32: fp8_tile_kernel<T, 2, 2, 4, 1, 3><<<grid, 256, 0, stream>>>(p); break;
+    case FP8_64: fp8_tile_kernel<T, 2, 4, 4, 1, 3><<<grid, 256, 0, stream>>>(p); break;
+    case FP8_128: fp8_tile_kernel<T, 4, 4, 2, 2, 2><<<grid, 256, 0, stream>>>(p); break;
+    case FP8_256: fp8_tile_kernel<T, 8, 4, 2, 4, 2><<<grid, 512, 0, stream>>>(p); break;
+  }
+  check_launch("linear_fp8");
+  if (p.splits > 1) {
+    const int64_t quads = (int64_t)p.M * (p.N / 4);
+    fp8_reduce_kernel<T><<<dim3((unsigned)((quads + 255) / 256)), 256, 0, stream>>>(p);
+    check_launch("linear_fp8 (sum of the ranges)");
+  }
+}
+
+bool at_multiple(const void *p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+void linear_fp8_impl(hipattn_tensor *out, const hipattn_tensor *x, const hipattn_tensor *weight, const hipattn_tensor *scale,
+                     const hipattn_tensor *bias, const hipattn_tensor *residual, const hipattn_tensor *workspace, void *stream_arg,
+                     int64_t *ws_query) {
+  const char *op = "linear_fp8";
+  check_tensor(x, "x", 2);
+  check_tensor(weight, "weight", 2);
+  const int dt = x->dtype;
+  HA_CHECK(dt == HIPATTN_F16 || dt == HIPATTN_BF16, "%s: x must be f16 or bf16, got %s", op, dtype_name(dt));
+  HA_CHECK(weight->dtype == HIPATTN_E4M3, "%s: weight must be e4m3, got %s", op, dtype_name(weight->dtype));
+  const int64_t M = x->sizes[0], K = x->sizes[1], N = weight->sizes[0];
+  HA_CHECK(weight->sizes[1] == K, "%s: weight has %lld columns, x has %lld", op, (long long)weight->sizes[1], (long long)K);
+  HA_CHECK(K > 0 && K % 16 == 0 && N % 16 == 0, "%s: the inner size %lld must be a positive multiple of 16, the rows of weight %lld one of 16", op,
+           (long long)K, (long long)N);
+  HA_CHECK(N < (1 << 24) && K < (1 << 24) && M < (1 << 24), "%s: sizes out of range", op);
+  const Fp8Plan pl = plan_fp8(M, (int)N, (int)K);
+  if (ws_query != nullptr) {
+    *ws_query = M == 0 || N == 0 ? 0 : (int64_t)pl.bytes;
+    return;
+  }
+  check_tensor(scale, "weight_scale", 2);
+  check_tensor(out, "out", 2);
+  HA_CHECK(out->dtype == dt, "%s: out is %s, x is %s", op, dtype_name(out->dtype), dtype_name(dt));
+  HA_CHECK(out->sizes[0] == M && out->sizes[1] == N, "%s: out is [%lld, %lld], expected [%lld, %lld]", op, (long long)out->sizes[0],
+           (long long)out->sizes[1], (long long)M, (long long)N);
+  const int64_t NB = (N + kBlock - 1) / kBlock, KB = (K + kBlock - 1) / kBlock;
+  HA_CHECK(scale->dtype == HIPATTN_F32 && scale->sizes[0] == NB && scale->sizes[1] == KB,
+           "%s: weight_scale must be f32 [%lld, %lld], one for each 128 x 128 of weight", op, (long long)NB, (long long)KB);
+  HA_CHECK(KB == 1 || scale->strides[1] == 1, "%s: rows of weight_scale must be contiguous", op);
+  if (M == 0 || N == 0) return;
+  check_data(x, "x");
+  check_data(weight, "weight");
+  check_data(scale, "weight_scale");
+  check_data(out, "out");
+  HA_CHECK(x->strides[1] == 1 && weight->strides[1] == 1 && out->strides[1] == 1,
+           "%s: the last dimension of x, weight and out must be contiguous", op);
+  HA_CHECK((M == 1 || x->strides[0] % 8 == 0) && weight->strides[0] % 16 == 0 && at_multiple(x->data, 16) && at_multiple(weight->data, 16),
+           "%s: rows of x and weight must start on 16-byte boundaries", op);
+  HA_CHECK((M == 1 || out->strides[0] % 4 == 0) && at_multiple(out->data, 8), "%s: rows of out must start on 8-byte boundaries", op);
+  HA_CHECK(weight->strides[0] >= 0 && weight->strides[0] < (1 << 28), "%s: rows of weight lie too far apart", op);
+  Fp8Params p{};
+  if (bias != nullptr) {
+    check_tensor(bias, "bias", 1);
+    HA_CHECK(bias->dtype == dt && bias->sizes[0] == N && bias->strides[0] == 1 && at_multiple(bias->data, 8),
+             "%s: bias must be %lld contiguous %s on an 8-byte boundary", op, (long long)N, dtype_name(dt));
+    check_data(bias, "bias");
+    p.bias = bias->data;
+  }
+  if (residual != nullptr) {
+    check_tensor(residual, "residual", 2);
+    HA_CHECK(residual->dtype == dt && residual->sizes[0] == M && residual->sizes[1] == N && residual->strides[1] == 1,
+             "%s: residual must be [%lld, %lld] %s with a contiguous last dimension", op, (long long)M, (long long)N, dtype_name(dt));
+    HA_CHECK((M == 1 || residual->strides[0] % 4 == 0) && at_multiple(residual->data, 8), "%s: rows of residual must start on 8-byte boundaries",
+             op);
+    check_data(residual, "residual");
+    p.residual = residual->data;
+    p.ldr = residual->strides[0];
+  }
+  p.x = x->data;
+  p.w = static_cast<const uint8_t *>(weight->data);
+  p.ws = static_cast<const float *>(scale->data);
+  p.out = out->data;
+  p.M = (int)M;
+  p.N = (int)N;
+  p.K = (int)K;
+  p.KB = (int)KB;
+  p.Mp = pl.Mp;
+  p.ldx = M == 1 ? 0 : x->strides[0];
+  p.ldw = weight->strides[0];
+  p.ldws = scale->strides[0];
+  p.ldo = M == 1 ? 0 : out->strides[0];
+  if (M == 1) p.ldr = 0;
+  p.splits = pl.splits;
+  p.stages_per_split = pl.stages_per_split;
+  p.tiles_m = (int)((M + pl.bm - 1) / pl.bm);
+  p.tiles_n = (int)((N + pl.bn - 1) / pl.bn);
+  p.wide_out = p.ldo % 8 == 0 && at_multiple(out->data, 16);
+  HA_CHECK((int64_t)p.tiles_m * p.tiles_n < 0x7fffff00 / 8 && M * KB < (int64_t)0x7fffffff * 16, "%s: sizes out of range", op);
+  hipStream_t stream = resolve_stream(stream_arg);
+  HeldWorkspace held;  // over all launches
+  char *store;
+  if (workspace != nullptr) {
+    check_tensor(workspace, "workspace", 1);
+    HA_CHECK(workspace->dtype == HIPATTN_U8 && workspace->strides[0] == 1, "%s: workspace must be contiguous u8", op);
+    HA_CHECK((size_t)workspace->sizes[0] >= pl.bytes, "%s: workspace has %lld bytes, %zu are needed", op, (long long)workspace->sizes[0], pl.bytes);
+    HA_CHECK(workspace->data != nullptr && at_multiple(workspace->data, 256), "%s: workspace must be 256-byte aligned", op);
+    store = static_cast<char *>(workspace->data);
+  } else {
+    held = library_workspace(WS_LINEAR_FP8, pl.bytes, stream);
+    store = static_cast<char *>(held.ptr);
+  }
+  p.xq = reinterpret_cast<const uint8_t *>(store);
+  p.xs = reinterpret_cast<float *>(store + pl.xq_bytes);
+  p.partial = reinterpret_cast<float *>(store + pl.xq_bytes + pl.xs_bytes);
+  if (dt == HIPATTN_BF16) launch_fp8<bf16_t>(p, pl, stream);
+  else launch_fp8<half_t>(p, pl, stream);
+}
+
+}  // namespace
+}  // namespace hipattn
+
+using namespace hipattn;
+
+extern "C" char *hipattn_linear_fp8(hipattn_tensor *out, const hipattn_tensor *x, const hipattn_tensor *weight, const hipattn_tensor *weight_scale,
+                                    const hipattn_tensor *bias, const hipattn_tensor *residual, const hipattn_tensor *workspace, void *stream) {
+  HA_PROTECT(linear_fp8_impl(out, x, weight, weight_scale, bias, residual, workspace, stream, nullptr));
+}
+
+extern "C" char *hipattn_linear_fp8_workspace_size(const hipattn_tensor *x, const hipattn_tensor *weight, int64_t *bytes) {
+  HA_PROTECT({
+    HA_CHECK(bytes != nullptr, "linear_fp8_workspace_size: bytes is NULL");
+    linear_fp8_impl(nullptr, x, weight, nullptr, nullptr, nullptr, nullptr, nullptr, bytes);
+  });
+}

@@ -10,7 +10,7 @@ namespace hipattn {
 
 // Which op a library-owned scratch buffer belongs to: ops never share one.
 enum WorkspaceUser { WS_PAGED_ATTENTION = 0, WS_BIAS_ARGMAX = 1, WS_LINEAR = 2, WS_SAMPLE = 3, WS_STEP_ATTENTION = 4,
-                     WS_WINDOW_ATTENTION = 5, WS_WINDOW_CHUNKS = 6, WS_TREE_ATTENTION = 7 };
+                     WS_WINDOW_ATTENTION = 5, WS_WINDOW_CHUNKS = 6, WS_TREE_ATTENTION = 7, WS_LINEAR_FP8 = 8 };
 
 // A stream's scratch memory, and the right to it: until `held` goes, no call of another thread on that stream gets it.  A call keeps it over
 // all its launches: the work of two calls is then in order on the stream, where the launches of one could else come between those of the other.

@@ -29,6 +29,7 @@ _DTYPES = {
     torch.int32: _lib.I32,
     torch.int64: _lib.I64,
     torch.uint8: _lib.U8,
+    torch.float8_e4m3fn: _lib.E4M3,
 }
 
 
@@ -342,6 +343,43 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
         out = torch.empty((x.size(0), weight.size(0)), dtype=x.dtype, device=x.device)
     _native.linear(out, x, weight, bias, residual, workspace)
     return out
+
+
+def linear_fp8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
+               residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+               workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """out = x @ (weight * its scales).T (+ bias) (+ residual) for any number of rows of x [M, K], f16 or bf16: weight [N, K] float8_e4m3fn,
+    weight_scale f32 [ceil(N / 128), ceil(K / 128)], one for each 128 x 128 of weight (`quantize_weight_fp8`).  The rows of x are rounded to
+    e4m3 in blocks of 128 columns, scaled by powers of two.  workspace: uint8, `linear_fp8_workspace_size` bytes; None: a buffer that the
+    library keeps per stream."""
+    if out is None:
+        out = torch.empty((x.size(0), weight.size(0)), dtype=x.dtype, device=x.device)
+    _native.linear_fp8(out, x, weight, weight_scale, bias, residual, workspace)
+    return out
+
+
+def linear_fp8_workspace_size(x: torch.Tensor, weight: torch.Tensor) -> int:
+    n = ctypes.c_int64(0)
+    call("hipattn_linear_fp8_workspace_size", _desc(x, "x"), _desc(weight, "weight"), ctypes.byref(n))
+    return int(n.value)
+
+
+def quantize_weight_fp8(weight: torch.Tensor):
+    """(weight in float8_e4m3fn, f32 scales [ceil(N / 128), ceil(K / 128)]) of a weight [N, K] for `linear_fp8`: in each 128 x 128 of it the
+    largest magnitude becomes 448.  For loading, a strip of 128 rows at a time: nothing of the weight's size is held in 32 bits."""
+    n, k = weight.shape
+    nb, kb = (n + 127) // 128, (k + 127) // 128
+    data = torch.empty((n, k), dtype=torch.float8_e4m3fn, device=weight.device)
+    scale = torch.empty((nb, kb), dtype=torch.float32, device=weight.device)
+    for b in range(nb):
+        rows = weight[128 * b:128 * b + 128]
+        strip = torch.zeros((rows.size(0), kb * 128), dtype=torch.float32, device=weight.device)
+        strip[:, :k] = rows
+        strip = strip.view(-1, kb, 128)
+        most = strip.abs().amax((0, 2)) / 448.0
+        scale[b] = torch.where(most > 0, most, torch.ones_like(most))
+        data[128 * b:128 * b + 128] = (strip / scale[b][None, :, None]).clamp(-448.0, 448.0).view(rows.size(0), -1)[:, :k].to(torch.float8_e4m3fn)
+    return data, scale
 
 
 def linear_silu_and_mul(x: torch.Tensor, weight: torch.Tensor, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
