@@ -101,6 +101,7 @@ __device__ __forceinline__ void copy_256(uint32_t lds, const char *base, uint32_
 }
 
 typedef int i32x8_t __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(4))) float uniform_float;
 
 __device__ __forceinline__ f32x4_t mfma_fp8(i32x8_t a, i32x8_t b) {
   const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
@@ -191,56 +192,66 @@ __global__ __launch_bounds__(GN *GM * 64) void fp8_tile_kernel(const Fp8Params p
   for (int nt = 0; nt < WN; nt++)
 #pragma unroll
     for (int mt = 0; mt < WM; mt++) acc[nt][mt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  const float *ws = p.ws + (int64_t)(min(n0 + wn * WN * 16, p.N - 1) / kBlock) * p.ldws + stage0;
+  // (through the scalar cache: a vector load would wait for the copies in front of it)
+  const uniform_float *ws = (const uniform_float *)uniform_base(
+      reinterpret_cast<const char *>(p.ws + (int64_t)(min(n0 + wn * WN * 16, p.N - 1) / kBlock) * p.ldws + stage0));
+  float sw = nst > 0 ? ws[0] : 0.f;
   const int turn_w = (col & 3) + 4 * (col >> 2 & 1);  // of this lane's row of every tile of W
 #pragma unroll
   for (int j = 0; j < S - 1; j++)
     if (j < nst) ask(j, j);
-  for (int base = 0; base < nst; base += S) {
+  int slot = 0;
+  for (int st = 0; st < nst; st++) {
+    // This wavefront's copies of the stage have landed, and behind the barrier everybody's; the barrier also says that the stage before has
+    // been read, so its place takes the copies of the stage S - 1 further on.
+    if (st + S - 2 < nst) wait_copies<(S - 2) * kCopies>();
+    else wait_copies<0>();
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (st + S - 1 < nst) ask(slot == 0 ? S - 1 : slot - 1, st + S - 1);
+    const char *stage = ring + slot * kStageBytes;
+    slot = slot == S - 1 ? 0 : slot + 1;
+    const char *wrows = stage + wn * WN * 16 * kBlock, *xrows = stage + BN * kBlock;
+    const float *scales = reinterpret_cast<const float *>(stage + (BN + BM) * kBlock);
+    i32x8_t xf[WM];
+    float s[WM];
 #pragma unroll
-    for (int j = 0; j < S; j++) {
-      const int st = base + j;
-      if (st < nst) {
-        // This wavefront's copies of the stage have landed, and behind the barrier everybody's; the barrier also says that the stage before has
-        // been read, so its place takes the copies of the stage S - 1 further on.
-        if (st + S - 2 < nst) wait_copies<(S - 2) * kCopies>();
-        else wait_copies<0>();
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (st + S - 1 < nst) ask((j + S - 1) % S, st + S - 1);
-        const char *stage = ring + j * kStageBytes;
-        const char *wrows = stage + wn * WN * 16 * kBlock, *xrows = stage + BN * kBlock;
-        const float *scales = reinterpret_cast<const float *>(stage + (BN + BM) * kBlock);
-        const float sw = ws[st];
-        i32x8_t xf[WM];
-        float s[WM];
-#pragma unroll
-        for (int mt = 0; mt < WM; mt++) {
-          const int r = (wm * WM + mt) * 16 + col;
-          xf[mt] = operand(xrows, r, col & 7, kg);
-          s[mt] = scales[r] * sw;
-        }
-        // A tile's products go into the sums while the matrix pipe has the next tile's; the rows of W of the tile behind that are on their way.
-        auto rows_of = [&](int nt) { return operand(wrows, (col >> 2) * (4 * WN) + nt * 4 + (col & 3), turn_w, kg); };
-        i32x8_t wf = rows_of(0);
-        f32x4_t part[WM];
-#pragma unroll
-        for (int nt = 0; nt <= WN; nt++) {
-          const i32x8_t now = wf;
-          if (nt + 1 < WN) wf = rows_of(nt + 1);
-#pragma unroll
-          for (int mt = 0; mt < WM; mt++) {
-            f32x4_t next;
-            if (nt < WN) next = mfma_fp8(now, xf[mt]);
-            if (nt > 0) {
-#pragma unroll
-              for (int i = 0; i < 4; i++) acc[nt - 1][mt][i] = __builtin_fmaf(part[mt][i], s[mt], acc[nt - 1][mt][i]);
-            }
-            part[mt] = next;
-          }
-          __builtin_amdgcn_sched_barrier(0);
-        }
-      }
+    for (int mt = 0; mt < WM; mt++) {
+      const int r = (wm * WM + mt) * 16 + col;
+      xf[mt] = operand(xrows, r, col & 7, kg);
+      s[mt] = scales[r];
     }
+    // A tile's products go into the sums while the matrix pipe has the next tile's; the rows of W of the tile behind that are on their way.
+    auto rows_of = [&](int nt) { return operand(wrows, (col >> 2) * (4 * WN) + nt * 4 + (col & 3), turn_w, kg); };
+    i32x8_t wf = rows_of(0);
+    f32x4_t part[WM];
+#pragma unroll
+    for (int nt = 0; nt <= WN; nt++) {
+      const i32x8_t now = wf;
+      if (nt + 1 < WN) wf = rows_of(nt + 1);
+      if (nt == 1) {
+#pragma unroll
+        for (int mt = 0; mt < WM; mt++) s[mt] *= sw;
+      }
+#pragma unroll
+      for (int mt = 0; mt < WM; mt++) {
+        f32x4_t next = {0.f, 0.f, 0.f, 0.f};
+        if (nt < WN) next = mfma_fp8(now, xf[mt]);
+        if (nt > 0) {
+#pragma unroll
+          for (int i = 0; i < 4; i++) acc[nt - 1][mt][i] = __builtin_fmaf(part[mt][i], s[mt], acc[nt - 1][mt][i]);
+        }
+        part[mt] = next;
+      }
+      // (in this order: left to itself the compiler puts the additions in front, where they wait)
+      if (nt + 1 < WN) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+#pragma unroll
+      for (int mt = 0; mt < WM; mt++) {
+        if (nt < WN) __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        if (nt > 0) __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    sw = ws[min(st + 1, nst - 1)];
   }
 
   // A lane has 4 WN outputs of a row, end to end.
