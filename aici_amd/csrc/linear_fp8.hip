@@ -19,6 +19,7 @@
 #include "workspace.h"
 
 #include <algorithm>
+#include <type_traits>
 
 // The copies set M0, and say so; the compiler reports that it is a reserved register.
 #pragma clang diagnostic ignored "-Winline-asm"
@@ -26,6 +27,7 @@
 namespace hipattn {
 namespace {
 
+constexpr int kMostSplits = 8;  // ranges of k
 constexpr int kBlock = 128;  // columns (and rows of W) that share a scale; bytes of a row per stage
 
 struct Fp8Params {
@@ -44,14 +46,9 @@ struct Fp8Params {
 
 // ------------------------------------------------------------------ rows of x to 8 bits
 
-// A thread takes eight elements, 16 threads a block.
+// Eight elements of a block of which 16 lanes in a row hold the others: in 8 bits, and the block's scale (NaN for a block with a NaN or an infinity).
 template <typename T>
-__global__ __launch_bounds__(256) void quantize_rows_kernel(const Fp8Params p) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int b = (int)(i / 16 % p.KB), m = (int)(i / 16 / p.KB), k = b * kBlock + (int)(i % 16) * 8;
-  if (m >= p.M) return;
-  uint4 raw = make_uint4(0, 0, 0, 0);
-  if (k < p.K) raw = *reinterpret_cast<const uint4 *>(static_cast<const T *>(p.x) + (int64_t)m * p.ldx + k);
+__device__ __forceinline__ uint2 round_run(const uint4 raw, float &scale) {
   const T *e = reinterpret_cast<const T *>(&raw);
   float v[8];
   unsigned most = 0;  // bits of the largest magnitude; infinities and NaN are larger than any number
@@ -70,8 +67,22 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const Fp8Params p) {
   lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * down, v[3] * down, lo, true);
   hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[4] * down, v[5] * down, hi, false);
   hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[6] * down, v[7] * down, hi, true);
-  *reinterpret_cast<uint2 *>(const_cast<uint8_t *>(p.xq) + ((int64_t)m * p.KB + b) * kBlock + (i % 16) * 8) = make_uint2((unsigned)lo, (unsigned)hi);
-  if (i % 16 == 0) p.xs[(int64_t)b * p.Mp + m] = most >= 0x7f800000u ? bit_cast<float>(0x7fc00000u) : bit_cast<float>((unsigned)up << 23);
+  scale = most >= 0x7f800000u ? bit_cast<float>(0x7fc00000u) : bit_cast<float>((unsigned)up << 23);
+  return make_uint2((unsigned)lo, (unsigned)hi);
+}
+
+// A thread takes eight elements, 16 threads a block.
+template <typename T>
+__global__ __launch_bounds__(256) void quantize_rows_kernel(const Fp8Params p) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int b = (int)(i / 16 % p.KB), m = (int)(i / 16 / p.KB), k = b * kBlock + (int)(i % 16) * 8;
+  if (m >= p.M) return;
+  uint4 raw = make_uint4(0, 0, 0, 0);
+  if (k < p.K) raw = *reinterpret_cast<const uint4 *>(static_cast<const T *>(p.x) + (int64_t)m * p.ldx + k);
+  float scale;
+  const uint2 q = round_run<T>(raw, scale);
+  *reinterpret_cast<uint2 *>(const_cast<uint8_t *>(p.xq) + ((int64_t)m * p.KB + b) * kBlock + (i % 16) * 8) = q;
+  if (i % 16 == 0) p.xs[(int64_t)b * p.Mp + m] = scale;
 }
 
 // ------------------------------------------------------------------ the product
@@ -91,9 +102,13 @@ __device__ __forceinline__ const char *uniform_base(const char *ptr) {
                                         (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v));
 }
 
-// 64 lanes x 16 bytes, global -> LDS: lane l's bytes go to lds + 16 l.
+// 64 lanes x 16 bytes, global -> LDS: lane l's bytes go to lds + 16 l.  ONCE: with the hint that they are read once.
+template <bool ONCE = false>
 __device__ __forceinline__ void copy_1k(uint32_t lds, const char *base, uint32_t off) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
+  if constexpr (ONCE)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
 }
 // 64 lanes x 4 bytes.
 __device__ __forceinline__ void copy_256(uint32_t lds, const char *base, uint32_t off) {
@@ -132,35 +147,186 @@ __device__ __forceinline__ void finish4(const Fp8Params &p, const f32x4_t v, int
   }
 }
 
-// GN x GM wavefronts, each with WN x WM tiles of 16 rows of W x 16 rows of x; S stages in the ring.
-template <typename T, int WN, int WM, int GN, int GM, int S>
-__global__ __launch_bounds__(GN *GM * 64) void fp8_tile_kernel(const Fp8Params p) {
-  constexpr int WAVES = GN * GM, BN = GN * WN * 16, BM = GM * WM * 16;
-  constexpr int kCopiesW = BN / 8 / WAVES, kAllX = BM / 8, kCopiesX = (kAllX + WAVES - 1) / WAVES;
-  static_assert(BN % (8 * WAVES) == 0, "copies of W divide evenly");
-  constexpr int kScales = (BM + 63) / 64;  // pieces of 64 scales
-  constexpr int kCopies = kCopiesW + kCopiesX + 1;
-  constexpr int kStageBytes = (BN + BM) * kBlock + kScales * 256;
-  __shared__ __align__(1024) char ring[S * kStageBytes];
+// The order in which the stages of a range of k are taken: from one on that follows from the rows of W, and round.  Workgroups that all walk their
+// rows front to back ask for the same bytes of every row at a time, and where rows lie a power of two apart those are a few of the memory's
+// channels.
+__device__ __forceinline__ int turned(int st, int n, int stages) {
+  const int t = st + (int)((unsigned)(n / kBlock * 21) % (unsigned)stages);
+  return t < stages ? t : t - stages;
+}
+
+// Up to 16 rows of x.  A wavefront owns 16 rows of W over one range of k, with a ring of its own that only its own copies fill, so that it waits for
+// nothing else; `per_tile` wavefronts of a workgroup share the rows and meet in LDS at the end.
+// HELD: the few rows of x are copied into LDS whole, behind the first stages of W in the queue but in front of them in time, and rounded there: no
+// launch for that.  Else the rounded rows go through the ring as well.
+// LDS: ring | sums | rows of x | their scales.
+constexpr int kHeldBytes = 32 * 1024;
+__host__ __device__ constexpr int held_pitch(int K) { return (K * 2 + 1023) / 1024 * 1024; }
+template <bool HELD>
+constexpr int few_stage_bytes() { return HELD ? 2048 : 4096 + 256; }
+
+template <typename T, int S, int WAVES, bool HELD>
+__global__ __launch_bounds__(WAVES * 64) void fp8_few_kernel(const Fp8Params p) {
+  constexpr int kStage = few_stage_bytes<HELD>(), kCopies = HELD ? 2 : 5;
+  extern __shared__ __align__(1024) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, kg = lane >> 4;
-  const int wn = wave % GN, wm = wave / GN;
-  // Tiles in groups of four of W by all of x, and of that list a contiguous part to each XCD, which shares an L2.
+  const int tile = wave / p.splits, range = wave % p.splits, tiles = WAVES / p.splits;
+  const int n0 = (blockIdx.x * tiles + tile) * 16;
+  const int stage0 = range * p.stages_per_split, nst = max(0, min(p.stages_per_split, p.KB - stage0));
+  char *ring = lds + wave * S * kStage;
+  f32x4_t *sums = reinterpret_cast<f32x4_t *>(lds + WAVES * S * kStage);
+  char *rows = reinterpret_cast<char *>(sums + WAVES * 64);
+  const int pitch = held_pitch(p.K), xr = min(col, p.M - 1);
+  float *scales = reinterpret_cast<float *>(rows + p.M * pitch);  // [KB][M]
+
+  if constexpr (HELD) {
+    const int per_row = pitch / 1024, last = p.K / 8 - 1;
+    const uint32_t to = lds_address(rows);
+    for (int i = wave; i < p.M * per_row; i += WAVES) {
+      const int r = i / per_row, run = i % per_row * 64 + lane;
+      copy_1k(to + i * 1024, uniform_base(reinterpret_cast<const char *>(static_cast<const T *>(p.x) + r * p.ldx)), (uint32_t)min(run, last) * 16);
+    }
+  }
+  const int row8 = lane >> 3, run = ((lane & 7) ^ row8) * 16;  // run q of row r lies at place q ^ (r & 7)
+  const char *wbase[2], *xbase[2];
+  uint32_t woff[2], xoff[2];
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const int first = min(n0 + i * 8, p.N - 1);
+    wbase[i] = uniform_base(reinterpret_cast<const char *>(p.w) + (int64_t)first * p.ldw);
+    woff[i] = (uint32_t)(min(n0 + i * 8 + row8, p.N - 1) - first) * (uint32_t)p.ldw;
+    const int xfirst = min(i * 8, p.M - 1);
+    xbase[i] = uniform_base(reinterpret_cast<const char *>(p.xq) + (int64_t)xfirst * p.KB * kBlock);
+    xoff[i] = (uint32_t)(min(i * 8 + row8, p.M - 1) - xfirst) * (uint32_t)(p.KB * kBlock) + run;
+  }
+  const uint32_t ring_lds = lds_address(ring);
+  auto ask = [&](int slot, int st) {
+    const int b = stage0 + turned(st, n0, nst);
+    const uint32_t to = ring_lds + slot * kStage;
+    if constexpr (!HELD) {
+#pragma unroll
+      for (int i = 0; i < 2; i++) copy_1k(to + 2048 + i * 1024, xbase[i] + (int64_t)b * kBlock, xoff[i]);
+      copy_256(to + 4096, uniform_base(reinterpret_cast<const char *>(p.xs + (int64_t)b * p.Mp)), lane * 4);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; i++) copy_1k<true>(to + i * 1024, wbase[i], woff[i] + (uint32_t)min(b * kBlock + run, p.K - 16));
+  };
+#pragma unroll
+  for (int j = 0; j < S; j++)
+    if (j < nst) ask(j, j);
+  if constexpr (HELD) {
+    if (nst >= S) wait_copies<S * kCopies>();
+    else wait_copies<0>();
+    asm volatile("s_barrier" ::: "memory");
+    const int runs = p.KB * 16;  // of a row, up to the end of its last block
+    for (int i = threadIdx.x; i < p.M * runs; i += WAVES * 64) {
+      const int r = i / runs, q = i - r * runs;
+      uint4 *at = reinterpret_cast<uint4 *>(rows + r * pitch + q * 16);
+      const uint4 raw = q * 8 < p.K ? *at : make_uint4(0, 0, 0, 0);
+      float scale;
+      *reinterpret_cast<uint2 *>(at) = round_run<T>(raw, scale);  // eight bytes in the place of sixteen
+      if (q % 16 == 0) scales[q / 16 * p.M + r] = scale;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  }
+  const uniform_float *ws = (const uniform_float *)uniform_base(
+      reinterpret_cast<const char *>(p.ws + (int64_t)(min(n0, p.N - 1) / kBlock) * p.ldws + stage0));
+  const char *xrow = rows + xr * pitch + kg * 32;
+  f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+  static_assert(S % 2 == 0, "stages are taken two at a time");
+  for (int base = 0; base < nst; base += S) {
+#pragma unroll
+    for (int j = 0; j < S; j += 2) {
+      const int st = base + j;
+      if (st >= nst) break;
+      // S stages are on their way, these two first; near the end fewer, and the wait is for all of them
+      if (st + S - 1 < nst) wait_copies<(S - 2) * kCopies>();
+      else wait_copies<0>();
+      // (of two, as a stage by itself is a chain of waits; what lies in the place behind the last one is not added)
+      i32x8_t wf[2], xf[2];
+      float sx[2], sw[2];
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        const char *stage = ring + (j + u) * kStage;
+        const int at = turned(min(st + u, nst - 1), n0, nst), b = stage0 + at;
+        sw[u] = ws[at];
+        wf[u] = operand(stage, col, col & 7, kg);
+        if constexpr (HELD) {
+          const uint2 *x = reinterpret_cast<const uint2 *>(xrow + b * 256);
+          const uint2 x0 = x[0], x1 = x[2], x2 = x[16], x3 = x[18];
+          xf[u] = i32x8_t{(int)x0.x, (int)x0.y, (int)x1.x, (int)x1.y, (int)x2.x, (int)x2.y, (int)x3.x, (int)x3.y};
+          sx[u] = scales[b * p.M + xr];
+        } else {
+          xf[u] = operand(stage + 2048, col, col & 7, kg);
+          sx[u] = reinterpret_cast<const float *>(stage + 4096)[col];
+        }
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stages are in registers: their places can be filled again
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+        if (st + u + S < nst) ask(j + u, st + u + S);
+      f32x4_t part[2];
+#pragma unroll
+      for (int u = 0; u < 2; u++) part[u] = mfma_fp8(wf[u], xf[u]);
+      const float s0 = sx[0] * sw[0], s1 = sx[1] * sw[1];
+#pragma unroll
+      for (int i = 0; i < 4; i++) acc[i] = __builtin_fmaf(part[0][i], s0, acc[i]);
+      if (st + 1 < nst) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[i] = __builtin_fmaf(part[1][i], s1, acc[i]);
+      }
+    }
+  }
+  if (p.splits > 1) {
+    sums[wave * 64 + lane] = acc;
+    __syncthreads();
+    if (range > 0) return;
+    for (int i = 1; i < p.splits; i++) {
+      const f32x4_t v = sums[(wave + i) * 64 + lane];
+#pragma unroll
+      for (int r = 0; r < 4; r++) acc[r] += v[r];
+    }
+  }
+  const int n = n0 + kg * 4;
+  if (col >= p.M || n >= p.N) return;
+  __align__(8) T o[4];
+  finish4<T>(p, acc, col, n, o);
+  *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + (int64_t)col * p.ldo + n) = *reinterpret_cast<uint2 *>(o);
+}
+
+// KG groups of GN x GM wavefronts, each with WN x WM tiles of 16 rows of W x 16 rows of x; a group takes every KG-th stage of k, and their sums meet in
+// LDS at the end.  S rounds of KG stages in the ring.  ONCE: no other workgroup reads the rows of W.
+template <typename T, int WN, int WM, int GN, int GM, int KG, int S, bool ONCE>
+__global__ __launch_bounds__(GN *GM *KG * 64) void fp8_tile_kernel(const Fp8Params p) {
+  constexpr int WAVES = GN * GM * KG, BN = GN * WN * 16, BM = GM * WM * 16;
+  constexpr int kAllW = KG * BN / 8, kCopiesW = (kAllW + WAVES - 1) / WAVES, kAllX = KG * BM / 8, kCopiesX = (kAllX + WAVES - 1) / WAVES;
+  constexpr int kPieces = (BM + 63) / 64, kAllS = KG * kPieces, kCopiesS = (kAllS + WAVES - 1) / WAVES;  // of 64 scales
+  constexpr int kCopies = kCopiesW + kCopiesX + kCopiesS;
+  constexpr int kStageBytes = (BN + BM) * kBlock + kPieces * 256, kRoundBytes = KG * kStageBytes;
+  constexpr int kMeetBytes = (KG - 1) * GN * GM * WN * WM * 1024;
+  constexpr int kLds = S * kRoundBytes > kMeetBytes ? S * kRoundBytes : kMeetBytes;
+  __shared__ __align__(1024) char ring[kLds];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, kg = lane >> 4;
+  const int wn = wave % GN, wm = wave / GN % GM, group = wave / (GN * GM);
+  // Tiles in strips of four of W by all of x, and of that list a contiguous part to each XCD, which shares an L2.
   const int tiles = p.tiles_m * p.tiles_n, per_xcd = (tiles + 7) / 8;
   const int at = (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
-  if (at >= tiles) return;
-  const int group = at / (4 * p.tiles_m), in_group = at - group * 4 * p.tiles_m, width = min(4, p.tiles_n - group * 4);
-  const int n0 = (group * 4 + in_group % width) * BN, m0 = in_group / width * BM;
+  if ((int)(blockIdx.x >> 3) >= per_xcd || at >= tiles) return;
+  const int strip = at / (4 * p.tiles_m), in_strip = at - strip * 4 * p.tiles_m, width = min(4, p.tiles_n - strip * 4);
+  const int n0 = (strip * 4 + in_strip % width) * BN, m0 = in_strip / width * BM;
   const int stage0 = blockIdx.y * p.stages_per_split, nst = max(0, min(p.stages_per_split, p.KB - stage0));
+  const int rounds = (nst + KG - 1) / KG;
 
   // What a lane copies of eight rows: run q of row r to this lane's place.  Rows past the last repeat it; columns past the last of W, where x is zero,
-  // repeat the row's last run.
+  // repeat the row's last run; stages past the last repeat that.  Copies that do not divide evenly are made twice (the same bytes to the same place):
+  // every wavefront counts the same number of them.
   const char *wbase[kCopiesW], *xbase[kCopiesX];
   uint32_t woff[kCopiesW], xoff[kCopiesX];
   int wrun[kCopiesW];
   const int row8 = lane >> 3;
 #pragma unroll
   for (int i = 0; i < kCopiesW; i++) {
-    const int r = (wave * kCopiesW + i) * 8, in_tile = r + row8;  // row of the workgroup's
+    const int r = (wave + i * WAVES) % kAllW % (BN / 8) * 8, in_tile = r + row8;  // row of the workgroup's
     const int in_wave = in_tile % (WN * 16), turn = (in_wave & 3) + 4 * (in_wave / (4 * WN) & 1);
     const int first = min(n0 + r, p.N - 1), rows_on = min(n0 + in_tile, p.N - 1) - first;
     wrun[i] = ((lane & 7) ^ turn) * 16;
@@ -169,22 +335,34 @@ __global__ __launch_bounds__(GN *GM * 64) void fp8_tile_kernel(const Fp8Params p
   }
 #pragma unroll
   for (int i = 0; i < kCopiesX; i++) {
-    const int r = (wave + i * WAVES) % kAllX * 8, in_tile = r + row8;
+    const int r = (wave + i * WAVES) % kAllX % (BM / 8) * 8, in_tile = r + row8;
     const int first = min(m0 + r, p.M - 1), rows_on = min(m0 + in_tile, p.M - 1) - first;
     xbase[i] = uniform_base(reinterpret_cast<const char *>(p.xq) + (int64_t)first * p.KB * kBlock);
     xoff[i] = (uint32_t)rows_on * (uint32_t)(p.KB * kBlock) + ((lane & 7) ^ (row8 & 7)) * 16;
   }
   const uint32_t ring_lds = lds_address(ring);
-  const char *sbase = uniform_base(reinterpret_cast<const char *>(p.xs + m0 + wave % kScales * 64));
-  auto ask = [&](int slot, int st) {
-    const int b = stage0 + st;
-    const uint32_t to = ring_lds + slot * kStageBytes;
-#pragma unroll
-    for (int i = 0; i < kCopiesX; i++) copy_1k(to + (BN + (wave + i * WAVES) % kAllX * 8) * kBlock, xbase[i] + (int64_t)b * kBlock, xoff[i]);
-#pragma unroll
-    for (int i = 0; i < kCopiesW; i++)
-      copy_1k(to + (wave * kCopiesW + i) * 1024, wbase[i], woff[i] + (uint32_t)min(b * kBlock + wrun[i], p.K - 16));
-    copy_256(to + (BN + BM) * kBlock + wave % kScales * 256, sbase + (int64_t)b * p.Mp * 4, lane * 4);
+  const char *sbase = uniform_base(reinterpret_cast<const char *>(p.xs + m0));
+  // The block of the u-th stage of a round (see `turned`; without its division here).
+  const int turn = nst > 0 ? turned(0, n0, nst) : 0;
+  auto block_of = [&](int round, int u) {
+    const int t = min(round * KG + u, nst - 1) + turn;
+    return stage0 + (t < nst ? t : t - nst);
+  };
+  // The c-th of a wavefront's copies of a round.
+  auto ask = [&](int slot, int round, int c) {
+    const uint32_t to = ring_lds + slot * kRoundBytes;
+    if (c < kCopiesX) {
+      const int i = (wave + c * WAVES) % kAllX, u = i / (BM / 8);
+      copy_1k(to + u * kStageBytes + (BN + i % (BM / 8) * 8) * kBlock, xbase[c] + (int64_t)block_of(round, u) * kBlock, xoff[c]);
+    } else if (c < kCopiesX + kCopiesW) {
+      c -= kCopiesX;
+      const int i = (wave + c * WAVES) % kAllW, u = i / (BN / 8);
+      copy_1k<ONCE>(to + u * kStageBytes + i % (BN / 8) * 1024, wbase[c], woff[c] + (uint32_t)min(block_of(round, u) * kBlock + wrun[c], p.K - 16));
+    } else {
+      c -= kCopiesX + kCopiesW;
+      const int i = (wave + c * WAVES) % kAllS, u = i / kPieces, piece = i % kPieces;
+      copy_256(to + u * kStageBytes + (BN + BM) * kBlock + piece * 256, sbase + ((int64_t)block_of(round, u) * p.Mp + piece * 64) * 4, lane * 4);
+    }
   };
 
   f32x4_t acc[WN][WM];
@@ -193,23 +371,29 @@ __global__ __launch_bounds__(GN *GM * 64) void fp8_tile_kernel(const Fp8Params p
 #pragma unroll
     for (int mt = 0; mt < WM; mt++) acc[nt][mt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   // (through the scalar cache: a vector load would wait for the copies in front of it)
-  const uniform_float *ws = (const uniform_float *)uniform_base(
-      reinterpret_cast<const char *>(p.ws + (int64_t)(min(n0 + wn * WN * 16, p.N - 1) / kBlock) * p.ldws + stage0));
-  float sw = nst > 0 ? ws[0] : 0.f;
+  const uniform_float *ws =
+      (const uniform_float *)uniform_base(reinterpret_cast<const char *>(p.ws + (int64_t)(min(n0 + wn * WN * 16, p.N - 1) / kBlock) * p.ldws));
+  float sw = nst > 0 ? ws[block_of(0, group)] : 0.f;
   const int turn_w = (col & 3) + 4 * (col >> 2 & 1);  // of this lane's row of every tile of W
 #pragma unroll
-  for (int j = 0; j < S - 1; j++)
-    if (j < nst) ask(j, j);
+  for (int j = 0; j < S - 1; j++) {
+    if (j >= rounds) continue;
+#pragma unroll
+    for (int c = 0; c < kCopies; c++) ask(j, j, c);
+  }
   int slot = 0;
-  for (int st = 0; st < nst; st++) {
-    // This wavefront's copies of the stage have landed, and behind the barrier everybody's; the barrier also says that the stage before has
-    // been read, so its place takes the copies of the stage S - 1 further on.
-    if (st + S - 2 < nst) wait_copies<(S - 2) * kCopies>();
+  // (MORE: there is a round S - 1 further on to ask for; a loop of its own, as a condition around every copy keeps the products apart)
+  auto take = [&](int st, auto more) {
+    constexpr bool MORE = decltype(more)::value;
+    // This wavefront's copies of the round have landed, and behind the barrier everybody's; the barrier also says that the round before has
+    // been read, so its place takes the copies of the round S - 1 further on.
+    if (MORE || st + S - 2 < rounds) wait_copies<(S - 2) * kCopies>();
     else wait_copies<0>();
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (st + S - 1 < nst) ask(slot == 0 ? S - 1 : slot - 1, st + S - 1);
-    const char *stage = ring + slot * kStageBytes;
+    const char *stage = ring + slot * kRoundBytes + group * kStageBytes;
+    const int fill = slot == 0 ? S - 1 : slot - 1;
     slot = slot == S - 1 ? 0 : slot + 1;
+    if (!MORE && KG > 1 && st * KG + group >= nst) return;  // (the last round)
     const char *wrows = stage + wn * WN * 16 * kBlock, *xrows = stage + BN * kBlock;
     const float *scales = reinterpret_cast<const float *>(stage + (BN + BM) * kBlock);
     i32x8_t xf[WM];
@@ -242,6 +426,13 @@ __global__ __launch_bounds__(GN *GM * 64) void fp8_tile_kernel(const Fp8Params p
         }
         part[mt] = next;
       }
+      // The copies go out between the products, as the matrix pipe would wait for them if they were in front; behind the first of them where the
+      // ring is short and they are needed in the next round.
+      if constexpr (MORE) {
+#pragma unroll
+        for (int c = S > 2 ? kCopies * nt / (WN + 1) : 0; c < (S > 2 ? kCopies * (nt + 1) / (WN + 1) : (nt == 0 ? kCopies : 0)); c++)
+          ask(fill, st + S - 1, c);
+      }
       // (in this order: left to itself the compiler puts the additions in front, where they wait)
       if (nt + 1 < WN) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
 #pragma unroll
@@ -251,7 +442,33 @@ __global__ __launch_bounds__(GN *GM * 64) void fp8_tile_kernel(const Fp8Params p
       }
       __builtin_amdgcn_sched_barrier(0);
     }
-    sw = ws[min(st + 1, nst - 1)];
+    sw = ws[block_of(st + 1, group)];
+  };
+  int st = 0;
+  for (; st + S - 1 < rounds; st++) take(st, std::true_type{});
+  for (; st < rounds; st++) take(st, std::false_type{});
+  if constexpr (KG > 1) {
+    __syncthreads();
+    f32x4_t *meet = reinterpret_cast<f32x4_t *>(ring) + (wave % (GN * GM)) * WN * WM * 64 + lane;
+    constexpr int kGroup = GN * GM * WN * WM * 64;
+    if (group > 0) {
+#pragma unroll
+      for (int nt = 0; nt < WN; nt++)
+#pragma unroll
+        for (int mt = 0; mt < WM; mt++) meet[(group - 1) * kGroup + (nt * WM + mt) * 64] = acc[nt][mt];
+    }
+    __syncthreads();
+    if (group > 0) return;
+#pragma unroll
+    for (int g = 0; g < KG - 1; g++)
+#pragma unroll
+      for (int nt = 0; nt < WN; nt++)
+#pragma unroll
+        for (int mt = 0; mt < WM; mt++) {
+          const f32x4_t v = meet[g * kGroup + (nt * WM + mt) * 64];
+#pragma unroll
+          for (int i = 0; i < 4; i++) acc[nt][mt][i] += v[i];
+        }
   }
 
   // A lane has 4 WN outputs of a row, end to end.
@@ -299,12 +516,17 @@ __global__ __launch_bounds__(256) void fp8_reduce_kernel(const Fp8Params p) {
   const int64_t m = i / quads;
   if (m >= p.M) return;
   const float *from = p.partial + m * p.N + n;
-  f32x4_t sum = *reinterpret_cast<const f32x4_t *>(from);
-  for (int s = 1; s < p.splits; s++) {
-    const f32x4_t v = *reinterpret_cast<const f32x4_t *>(from + (int64_t)s * p.M * p.N);
+  f32x4_t v[kMostSplits];  // (all asked for at once)
 #pragma unroll
-    for (int r = 0; r < 4; r++) sum[r] += v[r];
-  }
+  for (int s = 0; s < kMostSplits; s++)
+    if (s < p.splits) v[s] = *reinterpret_cast<const f32x4_t *>(from + (int64_t)s * p.M * p.N);
+  f32x4_t sum = v[0];
+#pragma unroll
+  for (int s = 1; s < kMostSplits; s++)
+    if (s < p.splits) {
+#pragma unroll
+      for (int r = 0; r < 4; r++) sum[r] += v[s][r];
+    }
   __align__(8) T o[4];
   finish4<T>(p, sum, (int)m, n, o);
   *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + m * p.ldo + n) = *reinterpret_cast<uint2 *>(o);
@@ -312,28 +534,94 @@ __global__ __launch_bounds__(256) void fp8_reduce_kernel(const Fp8Params p) {
 
 // ------------------------------------------------------------------ choices
 
-enum Fp8Form { FP8_16, FP8_32, FP8_64, FP8_128, FP8_256 };
+// The forms of the product: of few rows, and of tiles with the sizes of fp8_tile_kernel.
+enum Fp8Form { FP8_HELD, FP8_FEW, FP8_TILES };
+#define FP8_TILE_FORMS(X)          \
+  X(0, 1, 2, 1, 1, 4, 4, true)     \
+  X(1, 1, 2, 2, 1, 2, 4, true)     \
+  X(2, 2, 2, 4, 1, 1, 4, true)     \
+  X(3, 1, 4, 1, 1, 4, 3, true)     \
+  X(4, 1, 4, 2, 1, 4, 3, true)     \
+  X(5, 1, 4, 4, 1, 1, 4, true)     \
+  X(6, 1, 4, 8, 1, 1, 4, true)     \
+  X(7, 1, 4, 4, 2, 1, 4, true)     \
+  X(8, 2, 4, 4, 2, 1, 3, true)     \
+  X(9, 4, 4, 2, 2, 1, 2, false)    \
+  X(10, 8, 4, 2, 4, 1, 2, false)
+struct TileForm {
+  int bn, bm;
+};
+constexpr TileForm kTileForms[] = {
+#define X(i, WN, WM, GN, GM, KG, S, ONCE) {GN * WN * 16, GM * WM * 16},
+    FP8_TILE_FORMS(X)
+#undef X
+};
+
 struct Fp8Plan {
   Fp8Form form;
+  int tile;  // of kTileForms
   int bn, bm, splits, stages_per_split;
   size_t xq_bytes, xs_bytes, bytes;  // rounded rows of x, their scales, everything
   int Mp;
 };
 
+// What bounds the tiles is what a compute unit gets from L2, some 30 to 40 bytes a nanosecond with 64 to 96 KB on their way, whoever else asks:
+// narrow tiles of W give every unit work, wide ones copy x less often.  us with the rows' launch, in rows of W per workgroup:
+//   up to 32 rows   4096 x 4096 16: 10.2, 32: 11.2, 128: 17.9; 6144 x 4096 14.8, 12.1, 18.4; 4096 x 14336 20.5, 24.7, 49.7; 28672 x 4096 42.9, 29.4, 24.6
+//   up to 64        4096 x 4096 16: 11.8, 32: 12.8, 64: 17.3, 128: 22.0; 6144 x 4096 18.9, 13.9, 17.8, 22.2; 28672 x 4096 50.7, 38.1, 27.6, 25.5
+//   up to 128       6144 x 4096 64: 22.3, 128: 29.8; 28672 x 4096 46.2, 36.8
+// Beyond 128 rows workgroups of 256 x 256, 2.25 us a stage, or of 128 x 128, two to a compute unit, 1.2 a stage and 1.37 where there are two; ranges of k
+// of workgroups of their own cost a launch and their sums' way through memory (4096 x 14336, 301 rows: one range 134, two 81, four 52).
 Fp8Plan plan_fp8(int64_t M, int N, int K) {
   Fp8Plan pl;
   const int KB = (K + kBlock - 1) / kBlock;
-  pl.form = M <= 16 ? FP8_16 : (M <= 32 ? FP8_32 : (M <= 64 ? FP8_64 : FP8_128));
-  const int64_t large = ((M + 255) / 256) * ((N + 255) / 256);
-  if (M > 128 && large >= 200) pl.form = FP8_256;
-  pl.bn = pl.form == FP8_256 ? 256 : 128;
-  pl.bm = pl.form == FP8_16 ? 16 : (pl.form == FP8_32 ? 32 : (pl.form == FP8_64 ? 64 : (pl.form == FP8_128 ? 128 : 256)));
-  const int64_t tiles = ((M + pl.bm - 1) / pl.bm) * ((N + pl.bn - 1) / pl.bn);
+  auto up = [](size_t b) { return (b + 255) / 256 * 256; };
+  if (M <= 16) {
+    // Rows held in LDS cost the compute unit its second workgroup from three of 4096 on (us, 6144 x 4096, 4 rows: held 11.3, through the ring 9.2).
+    const bool held = M <= 2 && M * held_pitch(K) <= kHeldBytes;
+    pl.form = held ? FP8_HELD : FP8_FEW;
+    // Wavefronts to a tile of 16 rows of W: until every compute unit has three, or four where a wavefront's chain of stages is long.  us, one row, 1 / 2
+    // / 4 / 8: 4096 x 4096 10.3, 7.8, 6.7, 7.5; 6144 x 4096 10.5, 8.4, 8.6, 12.3; 4096 x 14336 26.4, 17.4, 14.9, 13.4; 28672 x 4096 20.6, 22.8, 25.2, 39.9.
+    int per = 1;
+    const int64_t tiles = (N + 15) / 16;
+    while (per < 8 && KB / (2 * per) >= 2 && (tiles * per < 768 || (KB > 16 * per && tiles * per <= 1024))) per *= 2;
+    pl.splits = per;
+    pl.stages_per_split = (KB + per - 1) / per;
+    pl.bn = pl.bm = 16;
+    pl.tile = 0;
+    pl.Mp = 64;
+    pl.xq_bytes = held ? 0 : up((size_t)M * KB * kBlock);
+    pl.xs_bytes = held ? 0 : up((size_t)KB * pl.Mp * 4);
+    pl.bytes = pl.xq_bytes + pl.xs_bytes;
+    return pl;
+  }
+  pl.form = FP8_TILES;
   int splits = 1;
-  while (splits < 8 && tiles * splits < 256 && KB / (2 * splits) >= 4) splits *= 2;
+  if (M <= 32) {
+    pl.tile = N < 4800 ? 0 : (N < 16384 ? 1 : 2);
+  } else if (M <= 64) {
+    pl.tile = N < 4800 ? 3 : (N <= 8192 ? 4 : (N < 16384 ? 5 : 6));
+  } else if (M <= 128) {
+    pl.tile = N < 16384 ? 7 : 8;
+    while (splits < kMostSplits && 2 * splits * ((N + 63) / 64) <= 256 && KB / (2 * splits) >= 8) splits *= 2;
+  } else {
+    const int64_t large = ((M + 255) / 256) * ((N + 255) / 256), small = ((M + 127) / 128) * ((N + 127) / 128);
+    double us = (double)((large + 255) / 256) * 2.25 * KB;
+    pl.tile = 10;
+    for (int s = 1; s <= kMostSplits && (s == 1 || KB / s >= 4); s++) {
+      const double t = (double)((small * s + 511) / 512) * ((KB + s - 1) / s) * (small * s <= 256 ? 1.2 : 1.37) +
+                       (s > 1 ? 4 + (double)M * N * s * (8 / 3.5e6) : 0);
+      if (t < us) {
+        us = t;
+        pl.tile = 9;
+        splits = s;
+      }
+    }
+  }
+  pl.bn = kTileForms[pl.tile].bn;
+  pl.bm = kTileForms[pl.tile].bm;
   pl.stages_per_split = (KB + splits - 1) / splits;
   pl.splits = (KB + pl.stages_per_split - 1) / pl.stages_per_split;
-  auto up = [](size_t b) { return (b + 255) / 256 * 256; };
   pl.Mp = (int)((M + 255) / 256 * 256);
   pl.xq_bytes = up((size_t)M * KB * kBlock);
   pl.xs_bytes = up((size_t)KB * pl.Mp * 4);
@@ -341,19 +629,43 @@ Fp8Plan plan_fp8(int64_t M, int N, int K) {
   return pl;
 }
 
+template <typename T, int S, int WAVES, bool HELD>
+void launch_few(const Fp8Params &p, hipStream_t stream) {
+  auto kernel = fp8_few_kernel<T, S, WAVES, HELD>;
+  constexpr size_t fixed = (size_t)WAVES * (S * few_stage_bytes<HELD>() + 1024);
+  static bool attr_set = false;  // benign race: setting twice is harmless
+  if (!attr_set) {
+    HA_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+    attr_set = true;
+  }
+  const int rows = 16 * (WAVES / p.splits);
+  const size_t bytes = fixed + (HELD ? (size_t)p.M * (held_pitch(p.K) + p.KB * 4) : 0);
+  kernel<<<dim3((unsigned)((p.N + rows - 1) / rows)), WAVES * 64, bytes, stream>>>(p);
+  check_launch("linear_fp8 (few rows)");
+}
+
 template <typename T>
 void launch_fp8(const Fp8Params &p, const Fp8Plan &pl, hipStream_t stream) {
+  if (pl.form == FP8_HELD) {
+    if (p.splits > 4) launch_few<T, 6, 8, true>(p, stream);
+    else launch_few<T, 8, 4, true>(p, stream);
+    return;
+  }
   const int64_t threads = (int64_t)p.M * p.KB * 16;
   quantize_rows_kernel<T><<<dim3((unsigned)((threads + 255) / 256)), 256, 0, stream>>>(p);
   check_launch("linear_fp8 (rows)");
+  if (pl.form == FP8_FEW) {
+    if (p.splits > 4) launch_few<T, 4, 8, false>(p, stream);
+    else launch_few<T, 4, 4, false>(p, stream);
+    return;
+  }
   const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
   const dim3 grid((unsigned)((tiles + 7) / 8 * 8), (unsigned)p.splits);
-  switch (pl.form) {
-    case FP8_16: fp8_tile_kernel<T, 2, 1, 4, 1, 4><<<grid, 256, 0, stream>>>(p); break;
-    case FP8_32: fp8_tile_kernel<T, 2, 2, 4, 1, 3><<<grid, 256, 0, stream>>>(p); break;
-    case FP8_64: fp8_tile_kernel<T, 2, 4, 4, 1, 3><<<grid, 256, 0, stream>>>(p); break;
-    case FP8_128: fp8_tile_kernel<T, 4, 4, 2, 2, 2><<<grid, 256, 0, stream>>>(p); break;
-    case FP8_256: fp8_tile_kernel<T, 8, 4, 2, 4, 2><<<grid, 512, 0, stream>>>(p); break;
+  switch (pl.tile) {
+#define X(i, WN, WM, GN, GM, KG, S, ONCE) \
+  case i: fp8_tile_kernel<T, WN, WM, GN, GM, KG, S, ONCE><<<grid, GN * GM * KG * 64, 0, stream>>>(p); break;
+    FP8_TILE_FORMS(X)
+#undef X
   }
   check_launch("linear_fp8");
   if (p.splits > 1) {
@@ -444,8 +756,9 @@ void linear_fp8_impl(hipattn_tensor *out, const hipattn_tensor *x, const hipattn
   HA_CHECK((int64_t)p.tiles_m * p.tiles_n < 0x7fffff00 / 8 && M * KB < (int64_t)0x7fffffff * 16, "%s: sizes out of range", op);
   hipStream_t stream = resolve_stream(stream_arg);
   HeldWorkspace held;  // over all launches
-  char *store;
-  if (workspace != nullptr) {
+  char *store = nullptr;
+  if (pl.bytes == 0) {
+  } else if (workspace != nullptr) {
     check_tensor(workspace, "workspace", 1);
     HA_CHECK(workspace->dtype == HIPATTN_U8 && workspace->strides[0] == 1, "%s: workspace must be contiguous u8", op);
     HA_CHECK((size_t)workspace->sizes[0] >= pl.bytes, "%s: workspace has %lld bytes, %zu are needed", op, (long long)workspace->sizes[0], pl.bytes);

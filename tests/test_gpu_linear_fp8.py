@@ -171,7 +171,7 @@ def test_refusals(device):
     refuse("rows of weight_scale must be contiguous", x, w, scale.t().contiguous().t())
     refuse("16-byte boundaries", x[:, 4:500], w[:, :496], scale)
     refuse("16-byte boundaries", x, torch.zeros((256, 520), dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)[:, :512], scale)
-    refuse("workspace has 16 bytes", x, w, scale, workspace=torch.empty((16,), dtype=torch.uint8, device=device))
+    refuse("workspace has 16 bytes", x.repeat(4, 1), w, scale, workspace=torch.empty((16,), dtype=torch.uint8, device=device))
     refuse("bias must be", x, w, scale, bias=torch.zeros((255,), dtype=torch.bfloat16, device=device))
     refuse("residual must be", x, w, scale, residual=torch.zeros((7, 256), dtype=torch.bfloat16, device=device))
     refuse("out is", x, w, scale, out=torch.zeros((8, 256), dtype=torch.float16, device=device))
