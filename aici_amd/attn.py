@@ -101,6 +101,9 @@ def varlen_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch_info: B
     caches are not what that takes, from a gathered copy; with `paged_prefill`
     always through the tables (needs the builder's multi_block_tables).
 
+    A batch of trees of drafted tokens (`BatchInfo.with_trees`): its multi-token rows see the context in front of their tree and the tree's rows
+    that their mask names (kernels.paged_attention_tree, which takes the workspace, `paged_attention_tree_workspace_size` bytes).
+
     window_size_left: a token sees that many tokens before it, itself and the first sink_tokens of its sequence
     (None: all of them); multi-token rows then always read through the tables.  workspace (with a window): uint8,
     `window_workspace_size` bytes, so that a captured step gives the eager step's bits and shares no scratch memory with other graphs; None: what
@@ -110,6 +113,19 @@ def varlen_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch_info: B
     if softmax_scale is None:
         softmax_scale = 1.0 / math.sqrt(d)
     y = torch.empty((T, Hq, d), dtype=q.dtype, device=q.device)
+    if getattr(batch_info, "tree_mask", None) is not None:
+        if window_size_left is not None or sink_tokens != 0:
+            raise ValueError("trees of drafted tokens have no window")
+        if not cached:
+            kernels.reshape_and_cache(k, v, key_cache, value_cache, batch_info.slot_mapping)
+        multi = batch_info.q_multi
+        kernels.paged_attention_tree(q[:multi], key_cache, value_cache, batch_info.multi_block_tables, batch_info.seqlens_q,
+                                     batch_info.multi_context_lens, batch_info.max_seqlen_q, batch_info.max_seqlen_k, softmax_scale,
+                                     batch_info.tree_mask, out=y[:multi], workspace=workspace)
+        if multi < T:
+            kernels.paged_attention_v1(y[multi:], q[multi:], key_cache, value_cache, Hkv, softmax_scale, batch_info.paged_block_tables,
+                                       batch_info.paged_context_lens, batch_info.paged_block_size, batch_info.paged_max_context_len)
+        return y.reshape(T, Hq * d)
     if window_size_left is not None:
         has_m, has_p = batch_info.q_multi > 0, batch_info.q_multi < T
         if has_m and batch_info.multi_block_tables is None:

@@ -94,7 +94,11 @@ struct TreeAcceptParams {
   int32_t *lens, *path, *next;
 };
 
-// One workgroup per (sequence, layer): each finds the way for itself, the first of a sequence's says it.
+// One workgroup per (sequence, layer): each finds the way for itself, the first of a sequence's says it.  A token's values lie in a cache line of
+// their own with those of its neighbours for every element of d, so that what is moved of a few tokens is most of their blocks' bytes: up to kBatch
+// tokens are in flight at once, and a line that several of them lie in is asked for once (64 trees of 16 to 61 rows, 8 heads of 128, 32 layers: one token
+// after the other 175 us, so 157).
+constexpr int kBatch = 8;
 template <typename E>
 __global__ __launch_bounds__(256) void tree_accept_kernel(TreeAcceptParams p) {
   constexpr int X = 16 / sizeof(E);
@@ -132,28 +136,62 @@ __global__ __launch_bounds__(256) void tree_accept_kernel(TreeAcceptParams p) {
     }
   }
   if (p.slots == nullptr) return;
-  auto slot_of = [&](int row) -> int64_t {
-    return p.slot64 ? static_cast<const int64_t *>(p.slots)[begin + row] : (int64_t)static_cast<const int32_t *>(p.slots)[begin + row];
-  };
+  // The rows that move, as the elements of the first head's cache where a row of K begins and where the first of V's lies.
+  __shared__ int s_moves;
+  __shared__ int64_t s_key[2][kBatch], s_value[2][kBatch];
   const int layer = blockIdx.y;
   E *kc = reinterpret_cast<E *>(p.key_ptrs[layer]), *vc = reinterpret_cast<E *>(p.value_ptrs[layer]);
   const int runs = p.g.head_size / X, key_items = p.g.num_heads * runs, items = key_items + p.g.num_heads * p.g.head_size;
-  for (int i = tid; i < items; i += 256) {
-    const bool key = i < key_items;
-    const int e = key ? i : i - key_items, per = key ? runs : p.g.head_size, head = e / per, at = e - head * per;
-    for (int k = 1; k < len; k++) {
-      const int row = s_path[k];
-      if (row == k) continue;
-      int from_off, to_off;
-      const int64_t from = slot_block(slot_of(row), p.g, from_off), to = slot_block(slot_of(k), p.g, to_off);
-      if (from < 0 || to < 0) continue;
-      if (key) {
-        E *base = kc + head * p.g.k_head_stride + (int64_t)at * p.g.block_size * X;
-        *reinterpret_cast<uint4 *>(base + to * p.g.k_block_stride + to_off * X) =
-            *reinterpret_cast<const uint4 *>(base + from * p.g.k_block_stride + from_off * X);
+  for (int k0 = 1; k0 < len; k0 += kBatch) {
+    __syncthreads();
+    if (tid < 64) {
+      bool moves = false;
+      int64_t from = -1, to = -1;
+      int from_off = 0, to_off = 0;
+      if (tid < kBatch && k0 + tid < len && s_path[k0 + tid] != k0 + tid) {
+        const int rows[2] = {s_path[k0 + tid], k0 + tid};
+        int64_t slot[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+          slot[i] = p.slot64 ? static_cast<const int64_t *>(p.slots)[begin + rows[i]] : (int64_t)static_cast<const int32_t *>(p.slots)[begin + rows[i]];
+        from = slot_block(slot[0], p.g, from_off);
+        to = slot_block(slot[1], p.g, to_off);
+        moves = from >= 0 && to >= 0;
+      }
+      const unsigned long long all = __ballot(moves);
+      const int at = __popcll(all & ((1ull << tid) - 1));
+      if (moves) {
+        s_key[0][at] = from * p.g.k_block_stride + from_off * X;
+        s_key[1][at] = to * p.g.k_block_stride + to_off * X;
+        s_value[0][at] = from * p.g.v_block_stride + from_off;
+        s_value[1][at] = to * p.g.v_block_stride + to_off;
+      }
+      if (tid == 0) s_moves = __popcll(all);
+    }
+    __syncthreads();
+    const int moves = s_moves;
+    // All that a batch reads is asked for before anything is written: a row of the way comes from one that no earlier row of it goes to.
+    for (int i = tid; i < items; i += 256) {
+      if (i < key_items) {
+        const int head = i / runs;
+        E *base = kc + head * p.g.k_head_stride + (int64_t)(i - head * runs) * p.g.block_size * X;
+        uint4 v[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; k++)
+          if (k < moves) v[k] = *reinterpret_cast<const uint4 *>(base + s_key[0][k]);
+#pragma unroll
+        for (int k = 0; k < kBatch; k++)
+          if (k < moves) *reinterpret_cast<uint4 *>(base + s_key[1][k]) = v[k];
       } else {
-        E *base = vc + head * p.g.v_head_stride + (int64_t)at * p.g.block_size;
-        base[to * p.g.v_block_stride + to_off] = base[from * p.g.v_block_stride + from_off];
+        const int e = i - key_items, head = e / p.g.head_size;
+        E *base = vc + head * p.g.v_head_stride + (int64_t)(e - head * p.g.head_size) * p.g.block_size;
+        E v[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; k++)
+          if (k < moves) v[k] = base[s_value[0][k]];
+#pragma unroll
+        for (int k = 0; k < kBatch; k++)
+          if (k < moves) base[s_value[1][k]] = v[k];
       }
     }
   }

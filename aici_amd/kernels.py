@@ -371,12 +371,13 @@ def quantize_weight_fp8(weight: torch.Tensor):
     nb, kb = (n + 127) // 128, (k + 127) // 128
     data = torch.empty((n, k), dtype=torch.float8_e4m3fn, device=weight.device)
     scale = torch.empty((nb, kb), dtype=torch.float32, device=weight.device)
+    largest = torch.full((1,), 448.0, device=weight.device)  # (a tensor: by a number a GPU multiplies with the reciprocal, and a CPU divides)
     for b in range(nb):
         rows = weight[128 * b:128 * b + 128]
         strip = torch.zeros((rows.size(0), kb * 128), dtype=torch.float32, device=weight.device)
         strip[:, :k] = rows
         strip = strip.view(-1, kb, 128)
-        most = strip.abs().amax((0, 2)) / 448.0
+        most = strip.abs().amax((0, 2)) / largest
         scale[b] = torch.where(most > 0, most, torch.ones_like(most))
         data[128 * b:128 * b + 128] = (strip / scale[b][None, :, None]).clamp(-448.0, 448.0).view(rows.size(0), -1)[:, :k].to(torch.float8_e4m3fn)
     return data, scale

@@ -10,6 +10,8 @@ gate and up products are finished, and so do the residual addition and, from 17 
 RMS norm that follow o_proj and down_proj; up to 4 rows are normalised by the projections
 behind the norm.  Projections of more rows are library GEMMs
 (torch on ROCm).
+Projections with weights of 8 bits (`Fp8Weight`) go through the C ABI's linear_fp8, whatever
+the rows.
 Everything else -- rms_norm, rotary, the paged-KV attention composition,
 silu_and_mul, bias + argmax -- goes through the C ABI as well.  Weights are random
 (there are no checkpoints here): the harness measures and checks the step's
@@ -18,7 +20,7 @@ data path, not a language model.
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Dict, List, Optional, Tuple
+from typing import Dict, List, NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -89,20 +91,36 @@ def random_weights(cfg: LlamaConfig, seed: int, device=None, std: float = 0.02) 
     return ws
 
 
+class Fp8Weight(NamedTuple):
+    """A weight [N, K] in float8_e4m3fn with its f32 scales [ceil(N / 128), ceil(K / 128)], as `kernels.linear_fp8` takes it."""
+    data: torch.Tensor
+    scale: torch.Tensor
+
+
+def _cat_rows(weights: Sequence[Union[torch.Tensor, Fp8Weight]]) -> Union[torch.Tensor, Fp8Weight]:
+    """One weight of the rows of several."""
+    if not any(isinstance(w, Fp8Weight) for w in weights):
+        return torch.cat(list(weights))
+    if not all(isinstance(w, Fp8Weight) for w in weights) or any(w.data.size(0) % 128 for w in weights[:-1]):
+        raise ValueError("weights of 8 bits are joined with one another, and behind rows that are multiples of 128")
+    return Fp8Weight(torch.cat([w.data for w in weights]), torch.cat([w.scale for w in weights]))
+
+
 def _rows(t: torch.Tensor, idx: torch.Tensor) -> torch.Tensor:
     """t[idx]: index_select takes 32- and 64-bit indices as they are, others are converted."""
     return t.index_select(0, idx if idx.dtype in (torch.int32, torch.int64) else idx.long())
 
 
 class Llama:
-    """llama.rs:194-213.  `forward` returns the logits of every sequence's last token."""
+    """llama.rs:194-213.  `forward` returns the logits of every sequence's last token, of a batch of trees (`BatchInfo.with_trees`) those of every row.
+    The projections' weights may be `Fp8Weight`s; with fp8 those that are not become such.  Embedding, norms and lm_head stay as they are."""
 
-    def __init__(self, cfg: LlamaConfig, weights: Dict[str, torch.Tensor], device):
+    def __init__(self, cfg: LlamaConfig, weights: Dict[str, Union[torch.Tensor, Fp8Weight]], device, fp8: bool = False):
         self.cfg = cfg
         self.device = device
         self.skinny_linear = True  # False: every projection is a library GEMM
         self.fused_norm = True     # False: the norm behind those projections is a launch of its own
-        w = {k: v.to(device) for k, v in weights.items()}
+        w = {k: Fp8Weight(v.data.to(device), v.scale.to(device)) if isinstance(v, Fp8Weight) else v.to(device) for k, v in weights.items()}
         self.wte = w["model.embed_tokens"]
         self.ln_f = w["model.norm"]
         self.lm_head = w["lm_head"]
@@ -112,12 +130,17 @@ class Llama:
             self.layers.append({
                 "rms_1": w[p + "input_layernorm"],
                 # one GEMM for q, k, v and one for gate, up: rows concatenated
-                "qkv": torch.cat([w[p + "self_attn.q_proj"], w[p + "self_attn.k_proj"], w[p + "self_attn.v_proj"]]),
+                "qkv": _cat_rows([w[p + "self_attn.q_proj"], w[p + "self_attn.k_proj"], w[p + "self_attn.v_proj"]]),
                 "o": w[p + "self_attn.o_proj"],
                 "rms_2": w[p + "post_attention_layernorm"],
-                "gate_up": torch.cat([w[p + "mlp.gate_proj"], w[p + "mlp.up_proj"]]),
+                "gate_up": _cat_rows([w[p + "mlp.gate_proj"], w[p + "mlp.up_proj"]]),
                 "down": w[p + "mlp.down_proj"],
             })
+            if fp8:
+                layer = self.layers[-1]
+                for name in ("qkv", "o", "gate_up", "down"):
+                    if not isinstance(layer[name], Fp8Weight):
+                        layer[name] = Fp8Weight(*kernels.quantize_weight_fp8(layer[name]))
         self.rotary = RotaryEmbedding(cfg.head_dim, cfg.rope_theta, cfg.max_position_embeddings,
                                       cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim, cfg.dtype, device)
 
@@ -126,40 +149,50 @@ class Llama:
         kernels.rms_norm(out, x, weight, self.cfg.rms_norm_eps)
         return out
 
-    def _norm_in_proj(self, x: torch.Tensor, norm_weight: torch.Tensor, weight: torch.Tensor) -> bool:
+    def _norm_in_proj(self, x: torch.Tensor, norm_weight: torch.Tensor, weight: Union[torch.Tensor, Fp8Weight]) -> bool:
         """Whether the projection normalises its rows itself, the same bits (us, 4096 columns, norm and projection / one launch: 6144
         rows 13.3 / 11.3 with one row of x, 13.5 / 13.3 with four; 28672 gated rows 38.6 / 37.7 with one, 38.4 / 39.4 with four, which in a
         step of eight layers comes out even: 915 / 915)."""
-        return (x.size(0) <= kernels.RMS_NORM_LINEAR_MAX_ROWS and self.skinny_linear and self.fused_norm
+        return (not isinstance(weight, Fp8Weight) and x.size(0) <= kernels.RMS_NORM_LINEAR_MAX_ROWS and self.skinny_linear and self.fused_norm
                 and kernels.rms_norm_linear_takes(x, norm_weight, weight))
 
-    def _proj(self, x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
+    def _proj(self, x: torch.Tensor, weight: Union[torch.Tensor, Fp8Weight]) -> torch.Tensor:
         """x @ weight.T (llama.rs:81-83, 210).  A vocabulary's rows with more than 64 sequences stay with the library where the kernel reads
         them front to back (columns no multiple of 2048, rows none of 256), and with long rows from 97 sequences on.  us, library / C ABI:
         128256 x 4096 32 rows 197 / 161, 64 rows 209 / 176, 128 rows 233 / 219; 64 / 96 / 128 rows 65536 x 5120 118 / 115, 122 / 140, 126 / 150,
         65536 x 3072 77 / 70, 81 / 85, 84 / 91, 151936 x 4096 260 / 253, 268 / 287, 278 / 296, 131072 x 8192 0.91, 0.95, 1.05 of the library's.
         49 to 64 rows: 0.65 to 1.06 of it, 0.87 on average."""
+        if isinstance(weight, Fp8Weight):
+            return kernels.linear_fp8(x, weight.data, weight.scale)
         rows, (n, k) = x.size(0), weight.shape
         if self.skinny_linear and kernels.linear_takes(x, weight) and (
                 rows <= 64 or n < 65536 or (n % 256 == 0 and k % 2048 == 0 and (k <= 4096 or (k <= 8192 and rows <= 96)))):
             return kernels.linear(x, weight)
         return x @ weight.t()
 
-    def _gate_up_silu(self, h: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
+    def _gate_up_silu(self, h: torch.Tensor, weight: Union[torch.Tensor, Fp8Weight]) -> torch.Tensor:
         """silu(h @ gate.T) * (h @ up.T) (llama.rs:135-142), weight = the gate rows and then the up rows."""
-        if self.skinny_linear and kernels.linear_takes(h, weight) and weight.size(0) % 32 == 0:
+        if isinstance(weight, Fp8Weight):
+            gu = kernels.linear_fp8(h, weight.data, weight.scale)
+        elif self.skinny_linear and kernels.linear_takes(h, weight) and weight.size(0) % 32 == 0:
             return kernels.linear_silu_and_mul(h, weight)
-        gu = h @ weight.t()
-        act = torch.empty((h.size(0), weight.size(0) // 2), dtype=h.dtype, device=h.device)
+        else:
+            gu = h @ weight.t()
+        act = torch.empty((h.size(0), gu.size(1) // 2), dtype=h.dtype, device=h.device)
         kernels.silu_and_mul(act, gu)
         return act
 
-    def _proj_add_norm(self, y: torch.Tensor, weight: torch.Tensor, x: torch.Tensor, norm_weight: torch.Tensor, behind=None):
+    def _proj_add_norm(self, y: torch.Tensor, weight: Union[torch.Tensor, Fp8Weight], x: torch.Tensor, norm_weight: torch.Tensor, behind=None):
         """x' = y @ weight.T + x (llama.rs:96 + 166, 143 + 173) and the RMS norm of x' that follows it (:169, :165 of the
         next block, :207), or None where the projection `behind` normalises its rows itself.  Few rows: the C ABI's kernel,
         which splits the inner dimension over the device and finishes the rows -- residual and norm -- in the launch that adds
         the parts up; else a library GEMM and one launch for the addition and the norm (742 x 4096: 6.3 us, two launches 5.4
         and 6.2).  The same bits either way as far as the norm goes."""
+        if isinstance(weight, Fp8Weight):
+            x = kernels.linear_fp8(y, weight.data, weight.scale, residual=x)
+            if behind is not None and self._norm_in_proj(x, norm_weight, behind):
+                return x, None
+            return x, self._rms(x, norm_weight)
         if self.skinny_linear and weight.size(0) <= 8192 and kernels.linear_takes(y, weight):
             if behind is not None and self._norm_in_proj(x, norm_weight, behind):
                 return kernels.linear(y, weight, residual=x), None
@@ -174,8 +207,10 @@ class Llama:
         return x, self._rms(x, norm_weight)
 
     def workspace_size(self, batch_info: BatchInfo) -> int:
-        """Bytes of a workspace for `forward` of batches of these shapes: what attention with a window can make use of; 0 without one."""
+        """Bytes of a workspace for `forward` of batches of these shapes: what attention with a window, or of trees, can make use of; 0 without either."""
         cfg = self.cfg
+        if batch_info.tree_mask is not None:
+            return kernels.paged_attention_tree_workspace_size(batch_info.q_multi, cfg.num_attention_heads, cfg.head_dim)
         if cfg.sliding_window is None:
             return 0
         return window_workspace_size(batch_info, cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim, cfg.dtype,
@@ -188,12 +223,13 @@ class Llama:
         fused: q, k, v stay views of the fused projection's output (the kernels honour the row stride) and
         rotary + cache scatter are one launch, or part of the projection's -- four or five launches fewer per layer, the same
         bits.
-        workspace: uint8, `workspace_size` bytes, of a model with a window: a captured step's attention is then the eager one and lies in no memory of the
+        workspace: uint8, `workspace_size` bytes, of a model with a window or a batch of trees: a captured step's attention is then the eager one and lies in no memory of the
         library's."""
         cfg = self.cfg
         Hq, Hkv, d = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
-        window = {} if cfg.sliding_window is None else {"window_size_left": cfg.sliding_window - 1, "sink_tokens": cfg.attention_sinks,
-                                                           "workspace": workspace}
+        window = {} if cfg.sliding_window is None else {"window_size_left": cfg.sliding_window - 1, "sink_tokens": cfg.attention_sinks}
+        if cfg.sliding_window is not None or batch_info.tree_mask is not None:
+            window["workspace"] = workspace
         x = _rows(self.wte, batch_info.tokens)                                   # llama.rs:203
         T = x.size(0)
         # h: the normalised rows, None where the projection that takes them does it
@@ -201,7 +237,7 @@ class Llama:
         h = None if self._norm_in_proj(x, first["rms_1"], first["qkv"]) else self._rms(x, first["rms_1"])  # :165
         for li, (layer, (kc, vc)) in enumerate(zip(self.layers, caches)):
             # few rows: rotary and the cache writes happen in the projection's launch too (:85 + mod.rs:147-164)
-            rotated = (fused and self.skinny_linear and kc.dim() == 5 and kc.size(1) == Hkv
+            rotated = (fused and self.skinny_linear and not isinstance(layer["qkv"], Fp8Weight) and kc.dim() == 5 and kc.size(1) == Hkv
                        and kernels.qkv_linear_takes(x if h is None else h, layer["qkv"], self.rotary.cos_sin, kc, vc))
             if rotated:
                 qkv = kernels.qkv_linear(*((x, layer["rms_1"]) if h is None else (h, None)), cfg.rms_norm_eps, layer["qkv"],

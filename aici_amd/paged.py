@@ -7,7 +7,7 @@ GPU.
 from __future__ import annotations
 
 import ctypes
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 from typing import List, Optional, Sequence, Tuple
 
 import numpy as np
@@ -253,6 +253,23 @@ class BatchInfo:
     # walk its blocks in order, in which case only the gather route applies)
     multi_block_tables: Optional[torch.Tensor] = None
     multi_context_lens: Optional[torch.Tensor] = None
+    # extension: the multi-token entries are trees of drafted tokens (`with_trees`)
+    tree_mask: Optional[torch.Tensor] = None
+
+    def with_trees(self, parents: torch.Tensor) -> "BatchInfo":
+        """The batch, on the device, with its multi-token entries as trees of drafted tokens: parents int32 [q_multi], the row of its own entry that a
+        row continues, the first row of each (its sequence's newest token, no draft) -1.  Rows see the context in front of their entry, themselves
+        and their ancestors, and are rotated to the positions that follow; every row has logits.  What a step does not keep
+        (`kernels.tree_accept`) goes back with `BlockAllocator.trim`; `DeviceBlocks` cannot give tokens back."""
+        from . import kernels
+
+        if self.multi_block_tables is None or self.q_multi == 0:
+            raise ValueError("trees are multi-token entries whose slots follow their blocks in order: the batch has none")
+        rows = kernels.tree_rows(parents, self.seqlens_q, self.multi_context_lens, self.max_seqlen_q)
+        positions = self.positions.clone()
+        positions[:self.q_multi] = rows.positions
+        return replace(self, positions=positions, logit_idxs=torch.arange(positions.numel(), dtype=torch.int32, device=positions.device),
+                       tree_mask=rows.mask)
 
     def to(self, device) -> "BatchInfo":
         """The batch with its arrays on `device`, there when the call returns: they may be used on any stream.  On the way
