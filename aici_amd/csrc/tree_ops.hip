@@ -95,9 +95,10 @@ struct TreeAcceptParams {
 };
 
 // One workgroup per (sequence, layer): each finds the way for itself, the first of a sequence's says it.  A token's values lie in a cache line of
-// their own with those of its neighbours for every element of d, so that what is moved of a few tokens is most of their blocks' bytes: up to kBatch
-// tokens are in flight at once, and a line that several of them lie in is asked for once (64 trees of 16 to 61 rows, 8 heads of 128, 32 layers: one token
-// after the other 175 us, so 157).
+// their own with those of its neighbours for every element of d, and its keys 256 bytes apart, so that what is touched of a few tokens is every line of
+// their blocks, some 64 KB for each block that a way leaves or enters: 64 trees of 16 to 61 rows, 8 heads of 128, 32 layers move 33 MB and touch
+// some 500, in 106 us (among other work 157; one token after the other, not eight at a time, 175).  Half rows of V read at a time and neighbours written
+// together changed nothing: it is the lines.
 constexpr int kBatch = 8;
 template <typename E>
 __global__ __launch_bounds__(256) void tree_accept_kernel(TreeAcceptParams p) {
