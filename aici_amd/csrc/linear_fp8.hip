@@ -570,7 +570,8 @@ struct Fp8Plan {
 //   up to 32 rows   4096 x 4096 16: 10.2, 32: 11.2, 128: 17.9; 6144 x 4096 14.8, 12.1, 18.4; 4096 x 14336 20.5, 24.7, 49.7; 28672 x 4096 42.9, 29.4, 24.6
 //   up to 64        4096 x 4096 16: 11.8, 32: 12.8, 64: 17.3, 128: 22.0; 6144 x 4096 18.9, 13.9, 17.8, 22.2; 28672 x 4096 50.7, 38.1, 27.6, 25.5
 //   up to 128       6144 x 4096 64: 22.3, 128: 29.8; 28672 x 4096 46.2, 36.8
-// Beyond 128 rows workgroups of 256 x 256, 2.25 us a stage, or of 128 x 128, two to a compute unit, 1.2 a stage and 1.37 where there are two; ranges of k
+// Beyond 128 rows workgroups of 256 x 256, 2.25 us a stage (of whose 4100 cycles the matrix pipe is busy 2048; LDS 18 %, no bank conflicts.  Refilling each
+// part of a stage's place as soon as it has been read, with two more barriers, 4096 x 28672 x 4096: 502 -> 661 us), or of 128 x 128, two to a compute unit, 1.2 a stage and 1.37 where there are two; ranges of k
 // of workgroups of their own cost a launch and their sums' way through memory (4096 x 14336, 301 rows: one range 134, two 81, four 52).
 Fp8Plan plan_fp8(int64_t M, int N, int K) {
   Fp8Plan pl;

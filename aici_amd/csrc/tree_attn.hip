@@ -488,10 +488,15 @@ __global__ __launch_bounds__(512) void tree_many_kernel(TreeParams p) {
         const int64_t column = BS == 8 ? 2 * run + h : (BS == 32 ? run / 2 : run);
         int id = column < p.cache.table_cols ? sq.table[column] : 0;
         ids[i][h] = id < 0 ? 0 : (id < p.cache.num_blocks ? id : (int)p.cache.num_blocks - 1);
-        // (used here, so that what uses it later does not wait for the copies in front of it every time)
-        asm volatile("" : "+v"(ids[i][h]));
       }
     }
+  };
+  // (used as soon as they are there, so that what uses them later does not wait for the copies in front of it every time)
+  auto use_ids = [&]() {
+#pragma unroll
+    for (int i = 0; i < IMAGES; i++)
+#pragma unroll
+      for (int h = 0; h < (BS == 8 ? 2 : 1); h++) asm volatile("" : "+v"(ids[i][h]));
   };
   // A lane's place in a piece of an image, in bytes from the block's start; from piece to piece it moves on by as much.  Beyond the image, where it
   // does not fill its last piece: the image's last 16 bytes.
@@ -512,7 +517,10 @@ __global__ __launch_bounds__(512) void tree_many_kernel(TreeParams p) {
   const char *base = reinterpret_cast<const char *>(is_v ? vbase : kbase);
   const int64_t stride = (is_v ? p.cache.v_block_stride : p.cache.k_block_stride) * (int64_t)sizeof(T);
   auto ask = [&](int slot, int round) {
-    if ((round & 63) == 0) fetch_ids(round);
+    if (round > 0 && (round & 63) == 0) {
+      fetch_ids(round);
+      use_ids();
+    }
 #pragma unroll
     for (int i = 0; i < IMAGES; i++) {
       const uint32_t to = ring_lds + ((slot * P + (wave >> 2) + 2 * i) * 4 + (wave & 3)) * IMG;
@@ -531,7 +539,9 @@ __global__ __launch_bounds__(512) void tree_many_kernel(TreeParams p) {
     }
   };
   TreeColumns<T, HD, NT> c;
+  fetch_ids(0);
   c.begin(p, c0, at.kvh, sq.q_begin, sq.n);
+  use_ids();
 #pragma unroll
   for (int t = 0; t < NT; t++)
 #pragma unroll
