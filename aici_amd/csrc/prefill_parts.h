@@ -1,5 +1,5 @@
 // Row blocks whose keys several workgroups of prefill_varlen_w8_kernel share (STEP::parts): the merge of what they leave, for a step's
-// attention (step_attn.hip) and that of windows (prefill_window.hip).  Device code; included by those two.
+// attention (step_attn.hip) and that of windows (prefill_window.hip); the search for a row's sequence is also that of trees (tree_attn.hip).  Device code.
 #pragma once
 
 #include "prefill_common.h"

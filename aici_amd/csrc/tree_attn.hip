@@ -4,9 +4,9 @@
 //   out[i] = sum_t p[t] v[t] / sum_t p[t],  p[t] = 2^(log2(e) scale q[i].k[t] - m) where t < ctx - n or bit t - (ctx - n) of mask[i] is set, else 0
 //
 // The rows of a tree with the query heads of a kv group are columns of the decode kernel's products (paged_decode.h), 16 to a tile and two tiles to a
-// wavefront (one with heads of 256): 32 tokens' keys and values in registers go through both.  Up to that many columns a workgroup's eight wavefronts
-// take pairs of runs of their own, straight from the cache (tree_few_kernel); with more of them wavefronts with different columns read the same
-// pairs from LDS, so that a context is read once for 128 columns (tree_many_kernel).  The parts of a long context go to several workgroups, whose
+// wavefront (one with heads of 256): 32 tokens' keys and values in registers go through both.  Up to that many columns, and where there is little work, a
+// workgroup's eight wavefronts take pairs of runs of their own, straight from the cache (tree_few_kernel); else wavefronts with different columns read
+// the same pairs from LDS, so that a context is read once for 128 columns (tree_many_kernel).  The parts of a long context go to several workgroups, whose
 // results a second launch adds up.
 //
 // A tree is memory-bound in theory up to some 300 columns (its products per byte of the cache).  Only pairs that reach into the tree look at the mask.
@@ -17,6 +17,7 @@
 
 #include "paged_decode.h"
 #include "prefill_common.h"
+#include "prefill_parts.h"
 
 // The copies set M0, and say so; the compiler reports that it is a reserved register.
 #pragma clang diagnostic ignored "-Winline-asm"
@@ -49,17 +50,16 @@ __device__ __forceinline__ int tree_pairs(const TreeParams &p, int ctx) {
   return ctx > 0 ? min((int)(((int64_t)ctx + 31) / 32), p.max_pairs) : 0;
 }
 
-// Bits j .. j + 3 of a row's mask; bits in front of the tree are set, those behind it are not.
-__device__ __forceinline__ unsigned tree_bits(const unsigned long long *row, int words, int n, int j) {
-  unsigned bits = 0;
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const int b = j + i;
-    bool seen = b < 0;
-    if (b >= 0 && b < n && (b >> 6) < words) seen = (row[b >> 6] >> (b & 63)) & 1;
-    bits |= (unsigned)seen << i;
-  }
-  return bits;
+// Bits j .. j + 63 of a row's mask; bits in front of the tree are set, those behind its n rows are not.  Two words are read whatever they are needed
+// for: a condition in front of each makes every one of them a wait (us, 1 tree of 24 rows over 1500 keys, 32 / 8 x 128: 21.5 -> 19.2 with the merge below).
+__device__ __forceinline__ unsigned long long tree_bits(const unsigned long long *row, int words, int n, int j) {
+  const int w = j >> 6, s = j & 63, last = words - 1;
+  unsigned long long lo = row[min(max(w, 0), last)], hi = row[min(max(w + 1, 0), last)];
+  lo = w < 0 ? ~0ull : (w > last ? 0ull : lo);
+  hi = w + 1 < 0 ? ~0ull : (w + 1 > last ? 0ull : hi);
+  const unsigned long long bits = s == 0 ? lo : lo >> s | hi << (64 - s);
+  const int left = n - j;  // up to the tree's last row
+  return left <= 0 ? 0ull : (left < 64 ? bits & ((1ull << left) - 1) : bits);
 }
 
 template <typename T>
@@ -172,10 +172,18 @@ __device__ __forceinline__ void tree_pair(const TreeParams &p, const TreeSeq &sq
       }
     }
     seen = 0;
+    unsigned of_tile[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) {
       const unsigned long long *words = p.mask + (int64_t)(sq.q_begin + min(c.row(p, t), sq.n - 1)) * p.mask_row;
-      const unsigned bits = tree_bits(words, p.words, sq.n, tok_a - sq.front) | tree_bits(words, p.words, sq.n, tok_b - sq.front) << 4;
+      if constexpr (EIGHTS)
+        of_tile[t] = (unsigned)tree_bits(words, p.words, sq.n, tok_a - sq.front) & 0xff;
+      else
+        of_tile[t] = ((unsigned)tree_bits(words, p.words, sq.n, tok_a - sq.front) & 15) | ((unsigned)tree_bits(words, p.words, sq.n, tok_b - sq.front) & 15) << 4;
+    }
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+      const unsigned bits = of_tile[t];
       seen |= (unsigned long long)bits << (8 * t);
 #pragma unroll
       for (int i = 0; i < 8; i++)
@@ -591,38 +599,43 @@ __global__ __launch_bounds__(512) void tree_many_kernel(TreeParams p) {
   tree_finish<T, HD, NT, CW, KG>(p, sq, at.part, at.parts == 1, c, ring);
 }
 
-// The merge: a thread for four elements of a (row, head).
+// The merge: a thread for four elements of a (row, head), workgroups of 256 of a row; parts eight at a time, all of which are asked for at once.
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeParams p) {
-  constexpr int QUADS = HD / 4;
-  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x, rh = idx / QUADS;
-  const int r = (int)(rh / p.Hq), h = (int)(rh % p.Hq), e = (int)(idx % QUADS) * 4;
-  if (r >= p.total_q) return;
-  // the sequence that holds row r: the first that ends behind it
-  int lo = 0, hi = p.batch;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (p.cu_q[mid + 1] > r) hi = mid;
-    else lo = mid + 1;
-  }
-  if (lo == p.batch || r < p.cu_q[lo]) return;
-  const int parts = TreeParts(p, tree_pairs(p, p.cache.context_lens[lo])).count;
-  if (parts == 1 || r - p.cu_q[lo] >= p.max_rows) return;  // written, or left out
-  const int64_t step = p.total_q * p.Hq;
-  float top = -INFINITY;
-  for (int k = 0; k < parts; k++) top = fmaxf(top, p.part_ml[2 * (k * step + rh)]);
-  const float base = top == -INFINITY ? 0.f : top;
-  float sum = 0.f;
+  constexpr int QUADS = HD / 4, kAtOnce = 8;
+  const int of_row = (p.Hq * QUADS + 255) / 256, r = blockIdx.x / of_row, i = blockIdx.x % of_row * 256 + threadIdx.x;
+  const int h = i / QUADS, e = i % QUADS * 4;
+  const int seq = sequence_of_row(p.cu_q, p.batch, r);
+  if (seq < 0 || h >= p.Hq) return;
+  const int parts = TreeParts(p, tree_pairs(p, p.cache.context_lens[seq])).count;
+  if (parts == 1 || r - p.cu_q[seq] >= p.max_rows) return;  // written, or left out
+  const int64_t step = p.total_q * p.Hq, rh = (int64_t)r * p.Hq + h;
+  float top = -INFINITY, sum = 0.f;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int k = 0; k < parts; k++) {
-    const int64_t at = k * step + rh;
-    const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + 2 * at);
-    const f32x4_t a = *reinterpret_cast<const f32x4_t *>(p.part_acc + at * HD + e);
-    const float w = fast_exp2(ml.x - base);
-    sum += w * ml.y;
+  for (int k0 = 0; k0 < parts; k0 += kAtOnce) {
+    float2 ml[kAtOnce];
+    f32x4_t a[kAtOnce];
 #pragma unroll
-    for (int j = 0; j < 4; j++) o[j] += w * a[j];
+    for (int k = 0; k < kAtOnce; k++) {
+      const int64_t at = min(k0 + k, parts - 1) * step + rh;
+      ml[k] = *reinterpret_cast<const float2 *>(p.part_ml + 2 * at);
+      a[k] = *reinterpret_cast<const f32x4_t *>(p.part_acc + at * HD + e);
+    }
+    float most = top;
+#pragma unroll
+    for (int k = 0; k < kAtOnce; k++) most = fmaxf(most, ml[k].x);
+    const float base = most == -INFINITY ? 0.f : most, before = fast_exp2(top - base);
+    top = most;
+    sum *= before;
+    o *= before;
+#pragma unroll
+    for (int k = 0; k < kAtOnce; k++) {
+      if (k0 + k >= parts) continue;
+      const float w = fast_exp2(ml[k].x - base);
+      sum += w * ml[k].y;
+#pragma unroll
+      for (int j = 0; j < 4; j++) o[j] += w * a[k][j];
+    }
   }
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
   T out[4];
@@ -634,7 +647,7 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeParams p) {
 // How columns and keys are dealt out.
 struct TreePlan {
   int tiles;  // of 16 columns to a wavefront
-  int cw;     // wavefronts beside one another that share pairs in LDS, 4; 0: few columns, every wavefront pairs of its own
+  int cw;     // wavefronts beside one another that share pairs in LDS, 4; 0: every wavefront pairs of its own
   int part_pairs, num_parts, max_pairs;
   int64_t groups;  // (sequence, column group, kv head), at most
 };
@@ -642,19 +655,35 @@ struct TreePlan {
 TreePlan plan_tree(const PrefillParams &p, int most_parts) {
   TreePlan pl;
   const int64_t cols = (int64_t)std::min<int64_t>(p.max_q, p.total_q) * p.G;
-  pl.cw = cols <= (p.d > 128 ? 16 : 32) ? 0 : 4;
-  pl.tiles = p.d > 128 || cols <= 16 || (cols > 32 && cols <= 64) ? 1 : 2;
-  const int wide = 16 * pl.tiles * std::max(pl.cw, 1);
   const int64_t pairs = std::max<int64_t>(((int64_t)p.max_k + 31) / 32, 1);
   // (column groups that trees of these rows together can have)
-  const int64_t groups = std::min<int64_t>((cols + wide - 1) / wide * p.batch, (p.total_q * p.G) / wide + p.batch) * p.Hkv;
-  // Parts for two workgroups to a compute unit: what a workgroup takes before its first keys are there is some 8 us.  us, for one / two / four / eight: 12
+  const auto groups_of = [&](int wide) {
+    return std::min<int64_t>((cols + wide - 1) / wide * p.batch, (p.total_q * p.G) / wide + p.batch) * p.Hkv;
+  };
+  pl.max_pairs = (int)pairs;
+  // Little work, that a workgroup to a compute unit does in twelve rounds of its wavefronts: columns in groups of 16, each with the keys to itself, start
+  // some 5 us sooner than those that share them.  us, so / with groups of 128: 1 tree of 24 rows over 1500 keys, 32 / 8 x 128 13.2 / 19.2, 8 of 12 over up
+  // to 3000 25.9 / 34.3, 4 of 24 over up to 6000, 12 / 4 x 112 23.0 / 35.6; at sixteen rounds 12 of 1 to 45 over up to 4000, 12 / 4 x 112 28.3 / 26.0.
+  const int64_t alone = compute_units() / groups_of(16);
+  if (alone > 0 && pairs <= alone * 96) {
+    pl.cw = 0;
+    pl.tiles = 1;
+    pl.groups = groups_of(16);
+    const int64_t parts = std::min<int64_t>(std::min<int64_t>(alone, most_parts), (pairs + 7) / 8);
+    pl.part_pairs = (int)((pairs + parts - 1) / parts);
+    pl.num_parts = (int)((pairs + pl.part_pairs - 1) / pl.part_pairs);
+    return pl;
+  }
+  pl.cw = cols <= (p.d > 128 ? 16 : 32) ? 0 : 4;
+  pl.tiles = p.d > 128 || cols <= 16 || (cols > 32 && cols <= 64) ? 1 : 2;
+  const int64_t groups = groups_of(16 * pl.tiles * std::max(pl.cw, 1));
+  // Parts for two workgroups to a compute unit, or one where there are few sequences, whose lengths differ less: what a workgroup takes before its first
+  // keys are there is some 8 us.  us, for one / two / four / eight: 2 trees of 40 rows over up to 8000 keys, 32 / 8 x 128 38 / 49 / - / -; 12
   // trees of 1 to 45 rows over up to 4000 keys, 12 / 4 x 112 38 / 29 / 40 / 39; 8 of 64 over up to 8000, 32 / 32 x 80 87 / 88 / 93 / 108; 64 of 16 to 32
   // over up to 15000, 32 / 8 x 128 386 / 386 / 446 / 482.  No part of less than 8 pairs (1 of 24 over 1500, 32 / 8 x 128, of 2 / 4 / 8 / 16 pairs at least
   // 26.6 / 21.6 / 21.2 / 24.0).
-  int64_t parts = std::max<int64_t>((int64_t)2 * compute_units() / std::max<int64_t>(groups, 1), 1);
+  int64_t parts = std::max<int64_t>((int64_t)(p.batch <= 4 ? 1 : 2) * compute_units() / std::max<int64_t>(groups, 1), 1);
   parts = std::min<int64_t>(std::min<int64_t>(parts, most_parts), (pairs + 7) / 8);
-  pl.max_pairs = (int)pairs;
   pl.part_pairs = (int)((pairs + parts - 1) / parts);
   pl.num_parts = (int)((pairs + pl.part_pairs - 1) / pl.part_pairs);
   pl.groups = groups;
@@ -673,7 +702,7 @@ void launch_tree_bs(const TreeParams &p, const TreePlan &pl, dim3 grid, hipStrea
 
 template <typename T, int HD>
 void launch_tree(const TreeParams &p, const TreePlan &pl, int block_size, hipStream_t stream) {
-  const int64_t wgs = pl.groups * p.num_parts, merges = (p.total_q * p.Hq * (HD / 4) + 255) / 256;
+  const int64_t wgs = pl.groups * p.num_parts, merges = p.total_q * ((p.Hq * (HD / 4) + 255) / 256);
   HA_CHECK(wgs <= 0x7fffffff && merges <= 0x7fffffff, "paged_attention_tree: too many workgroups");
   const dim3 grid((unsigned)wgs);
   switch (block_size) {
