@@ -573,13 +573,15 @@ struct Fp8Plan {
 // Beyond 128 rows workgroups of 256 x 256, 2.25 us a stage (of whose 4100 cycles the matrix pipe is busy 2048; LDS 18 %, no bank conflicts.  Refilling each
 // part of a stage's place as soon as it has been read, with two more barriers, 4096 x 28672 x 4096: 502 -> 661 us), or of 128 x 128, two to a compute unit, 1.2 a stage and 1.37 where there are two; ranges of k
 // of workgroups of their own cost a launch and their sums' way through memory (4096 x 14336, 301 rows: one range 134, two 81, four 52).
-Fp8Plan plan_fp8(int64_t M, int N, int K) {
+// apart: out does not lie over x.
+Fp8Plan plan_fp8(int64_t M, int N, int K, bool apart) {
   Fp8Plan pl;
   const int KB = (K + kBlock - 1) / kBlock;
   auto up = [](size_t b) { return (b + 255) / 256 * 256; };
   if (M <= 16) {
     // Rows held in LDS cost the compute unit its second workgroup from three of 4096 on (us, 6144 x 4096, 4 rows: held 11.3, through the ring 9.2).
-    const bool held = M <= 2 && M * held_pitch(K) <= kHeldBytes;
+    // Every workgroup reads them while others write out, which is then no place over x.
+    const bool held = apart && M <= 2 && M * held_pitch(K) <= kHeldBytes;
     pl.form = held ? FP8_HELD : FP8_FEW;
     // Wavefronts to a tile of 16 rows of W: until every compute unit has three, or four where a wavefront's chain of stages is long.  us, one row, 1 / 2
     // / 4 / 8: 4096 x 4096 10.3, 7.8, 6.7, 7.5; 6144 x 4096 10.5, 8.4, 8.6, 12.3; 4096 x 14336 26.4, 17.4, 14.9, 13.4; 28672 x 4096 20.6, 22.8, 25.2, 39.9.
@@ -676,6 +678,19 @@ void launch_fp8(const Fp8Params &p, const Fp8Plan &pl, hipStream_t stream) {
   }
 }
 
+// Whether two matrices of 16-bit elements with contiguous rows have bytes in common (what lies between rows counts as theirs).
+bool meet(const hipattn_tensor *a, const hipattn_tensor *b) {
+  auto ends = [](const hipattn_tensor *t, const char *&lo, const char *&hi) {
+    const int64_t last = (t->sizes[0] - 1) * t->strides[0];
+    lo = static_cast<const char *>(t->data) + 2 * std::min<int64_t>(last, 0);
+    hi = static_cast<const char *>(t->data) + 2 * (std::max<int64_t>(last, 0) + t->sizes[1]);
+  };
+  const char *a0, *a1, *b0, *b1;
+  ends(a, a0, a1);
+  ends(b, b0, b1);
+  return a0 < b1 && b0 < a1;
+}
+
 bool at_multiple(const void *p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
 void linear_fp8_impl(hipattn_tensor *out, const hipattn_tensor *x, const hipattn_tensor *weight, const hipattn_tensor *scale,
@@ -692,9 +707,8 @@ void linear_fp8_impl(hipattn_tensor *out, const hipattn_tensor *x, const hipattn
   HA_CHECK(K > 0 && K % 16 == 0 && N % 16 == 0, "%s: the inner size %lld must be a positive multiple of 16, the rows of weight %lld one of 16", op,
            (long long)K, (long long)N);
   HA_CHECK(N < (1 << 24) && K < (1 << 24) && M < (1 << 24), "%s: sizes out of range", op);
-  const Fp8Plan pl = plan_fp8(M, (int)N, (int)K);
-  if (ws_query != nullptr) {
-    *ws_query = M == 0 || N == 0 ? 0 : (int64_t)pl.bytes;
+  if (ws_query != nullptr) {  // (of either place of out)
+    *ws_query = M == 0 || N == 0 ? 0 : (int64_t)plan_fp8(M, (int)N, (int)K, false).bytes;
     return;
   }
   check_tensor(scale, "weight_scale", 2);
@@ -717,6 +731,7 @@ void linear_fp8_impl(hipattn_tensor *out, const hipattn_tensor *x, const hipattn
            "%s: rows of x and weight must start on 16-byte boundaries", op);
   HA_CHECK((M == 1 || out->strides[0] % 4 == 0) && at_multiple(out->data, 8), "%s: rows of out must start on 8-byte boundaries", op);
   HA_CHECK(weight->strides[0] >= 0 && weight->strides[0] < (1 << 28), "%s: rows of weight lie too far apart", op);
+  const Fp8Plan pl = plan_fp8(M, (int)N, (int)K, !meet(out, x));
   Fp8Params p{};
   if (bias != nullptr) {
     check_tensor(bias, "bias", 1);

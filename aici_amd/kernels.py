@@ -350,8 +350,8 @@ def linear_fp8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor
                workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """out = x @ (weight * its scales).T (+ bias) (+ residual) for any number of rows of x [M, K], f16 or bf16: weight [N, K] float8_e4m3fn,
     weight_scale f32 [ceil(N / 128), ceil(K / 128)], one for each 128 x 128 of weight (`quantize_weight_fp8`).  The rows of x are rounded to
-    e4m3 in blocks of 128 columns, scaled by powers of two.  workspace: uint8, `linear_fp8_workspace_size` bytes; None: a buffer that the
-    library keeps per stream."""
+    e4m3 in blocks of 128 columns, scaled by powers of two.  out may lie over x, and be the residual.  workspace: uint8,
+    `linear_fp8_workspace_size` bytes; None: a buffer that the library keeps per stream."""
     if out is None:
         out = torch.empty((x.size(0), weight.size(0)), dtype=x.dtype, device=x.device)
     _native.linear_fp8(out, x, weight, weight_scale, bias, residual, workspace)

@@ -96,6 +96,22 @@ def test_strides_and_what_lies_around(device, m):
 
 
 @gpu
+@pytest.mark.parametrize("m,n,k", [(1, 4096, 4096), (2, 2048, 4096), (2, 4096, 1024), (5, 4096, 4096), (30, 2048, 2048), (200, 1024, 1024)])
+def test_out_over_x(device, m, n, k):
+    """The rows of x are whole until every workgroup has read them, whatever form the product takes."""
+    x, w, scale, _ = operands(11, m, n, k, torch.bfloat16, device)
+    need = K.linear_fp8_workspace_size(x, w)
+    for first in (0, 8 * (m == 1)):  # the same place, or one that starts inside x
+        for store in (None, torch.full((need,), 255, dtype=torch.uint8, device=device)):
+            place = torch.zeros((first + m * max(n, k),), dtype=x.dtype, device=device)
+            over, out = place[:m * k].view(m, k), place[first:first + m * n].view(m, n)
+            over.copy_(x)
+            check(K.linear_fp8(over, w, scale, out=out, workspace=store), x, w, scale)
+            with pytest.raises(HipAttnError, match="workspace has 16 bytes"):
+                K.linear_fp8(over, w, scale, out=out, workspace=torch.empty((16,), dtype=torch.uint8, device=device))
+
+
+@gpu
 def test_values_at_the_ends(device):
     """Zeros, the smallest and largest numbers of the types, blocks whose largest value is on the border between two scales, ties."""
     for dtype in (torch.bfloat16, torch.float16):
