@@ -342,8 +342,9 @@ __global__ __launch_bounds__(GN *GM *KG * 64) void fp8_tile_kernel(const Fp8Para
   }
   const uint32_t ring_lds = lds_address(ring);
   const char *sbase = uniform_base(reinterpret_cast<const char *>(p.xs + m0));
-  // The block of the u-th stage of a round (see `turned`; without its division here).
-  const int turn = nst > 0 ? turned(0, n0, nst) : 0;
+  // The block of the u-th stage of a round (see `turned`; without its division here).  A strip's tiles of W that read the same rows of x at once read
+  // the same blocks of them where there are many such rows (us, 4096 x 28672 x 4096: 523, 505 so; 600 rows: 107.6, 109.3, so not with few).
+  const int turn = nst > 0 ? turned(0, p.tiles_m >= 4 ? strip * 4 * BN : n0, nst) : 0;
   auto block_of = [&](int round, int u) {
     const int t = min(round * KG + u, nst - 1) + turn;
     return stage0 + (t < nst ? t : t - nst);
@@ -571,7 +572,7 @@ struct Fp8Plan {
 //   up to 64        4096 x 4096 16: 11.8, 32: 12.8, 64: 17.3, 128: 22.0; 6144 x 4096 18.9, 13.9, 17.8, 22.2; 28672 x 4096 50.7, 38.1, 27.6, 25.5
 //   up to 128       6144 x 4096 64: 22.3, 128: 29.8; 28672 x 4096 46.2, 36.8
 // Beyond 128 rows workgroups of 256 x 256, 2.25 us a stage (of whose 4100 cycles the matrix pipe is busy 2048; LDS 18 %, no bank conflicts.  Refilling each
-// part of a stage's place as soon as it has been read, with two more barriers, 4096 x 28672 x 4096: 502 -> 661 us), or of 128 x 128, two to a compute unit, 1.2 a stage and 1.37 where there are two; ranges of k
+// part of a stage's place as soon as it has been read, with two more barriers, took a third longer), or of 128 x 128, two to a compute unit, 1.2 a stage and 1.37 where there are two; ranges of k
 // of workgroups of their own cost a launch and their sums' way through memory (4096 x 14336, 301 rows: one range 134, two 81, four 52).
 // apart: out does not lie over x.
 Fp8Plan plan_fp8(int64_t M, int N, int K, bool apart) {
