@@ -231,6 +231,96 @@ def test_workspace_capture_and_streams(device):
     assert all(torch.equal(o, eager) for o in outs)
 
 
+def crowd(heads, nodes, priors):
+    """The trees and others beside them, so many that a compute unit has more than one workgroup whatever the columns of one."""
+    hq, hkv, _ = heads
+    nodes, priors = list(nodes), list(priors)
+    while (sum(nodes) * hq // hkv // 16 + len(nodes)) * hkv <= 300 or (max(nodes) * hq // hkv + 15) // 16 * len(nodes) * hkv <= 300:
+        nodes.append(20 + 13 * len(nodes) % 41)
+        priors.append(7 * len(nodes) % 90)
+    return nodes, priors
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads", HEADS)
+@pytest.mark.parametrize("bs", [8, 16, 32])
+def test_attention_of_a_crowd(device, heads, bs, dtype):
+    """More trees than compute units take at once: columns of a context share its keys."""
+    c = Case(29, *crowd(heads, [1, 24, 64, 7, 70, 0, 33], [45, 700, 0, 1, 333, 17, 64]), heads, bs, dtype, device)
+    out = K.paged_attention_tree(*c.args())
+    c.check(out)
+    assert torch.equal(out, K.paged_attention_tree(*c.args()))
+
+
+@gpu
+@pytest.mark.parametrize("heads", [(32, 8, 128), (16, 2, 64)])
+@pytest.mark.parametrize("nodes,priors", [([3] * 300, list(range(300))), ([1, 2] * 200, [0, 5] * 200), ([70, 1] + [5] * 320, [900, 0] + [40] * 320),
+                                          ([40] * 9, [600] * 9), ([33], [20000])])
+def test_bounds_beyond_what_there_is(device, heads, nodes, priors):
+    """Many sequences, and bounds of rows and keys that a captured step would have: larger than any."""
+    c = Case(31, nodes, priors, heads, 16, torch.bfloat16, device)
+    c.check(K.paged_attention_tree(*c.args()))
+    args = c.args()
+    args[9] = torch.cat([args[9], torch.full((c.T, 3), -1, dtype=torch.int64, device=device)], 1)
+    args[6], args[7] = 200, c.max_k + 30000
+    args[3] = torch.cat([args[3], torch.full((len(nodes), 30000 // 16 + 1), 1 << 30, dtype=torch.int32, device=device)], 1)
+    c.check(K.paged_attention_tree(*args))
+
+
+@gpu
+@pytest.mark.parametrize("heads", [(32, 8, 128), (12, 4, 112), (8, 2, 256)])
+def test_bounds_below_what_there_is(device, heads):
+    """Rows beyond the bound are left out or computed; those of sequences that it allows for are whole."""
+    nodes, priors = crowd(heads, [9, 30, 16], [100, 40, 333])
+    for some in (3, len(nodes)):
+        c = Case(37, nodes[:some], priors[:some], heads, 16, torch.float16, device)
+        args = c.args()
+        args[6] = 25
+        out = torch.full_like(args[0], 3.0)
+        K.paged_attention_tree(*args, out=out)
+        whole = K.paged_attention_tree(*c.args())
+        for s, n in enumerate(c.nodes):
+            rows = slice(c.cu[s], c.cu[s + 1])
+            left = (out[rows] == 3.0).flatten(1).all(1)
+            assert n > 25 or not bool(left.any())
+            err = (out[rows][~left].double() - whole[rows][~left].double()).abs()
+            # (both within u (A + |out|) and little more, and A and |out| are at most the values' 5: 2 x 10 eps / 2, twice that allowed)
+            assert not bool((err > 20 * torch.finfo(c.dtype).eps).any())
+
+
+@gpu
+@pytest.mark.parametrize("bs", [8, 16])
+@pytest.mark.parametrize("odd", [float("nan"), float("inf"), -float("inf")])
+def test_values_that_are_not_finite_in_a_crowd(device, odd, bs):
+    heads = (16, 8, 64)
+    c = Case(41, *crowd(heads, [20, 64], [33, 129]), heads, bs, torch.float16, device)
+    rng = random.Random(3)
+    for s, n in enumerate(c.nodes):
+        for j in rng.sample(range(n), n // 4):  # of the tree's keys and values: rows that do not see them are as they were
+            c.values[s][c.ctx[s] - n + j] = odd
+            if j % 2:
+                c.keys[s][c.ctx[s] - n + j] = odd
+    c.fill()
+    c.check(K.paged_attention_tree(*c.args()))
+
+
+@gpu
+def test_offsets_beyond_32_bits_in_a_crowd(device):
+    heads = (8, 8, 128)
+    c = Case(43, *crowd(heads, [70, 20], [70, 5]), heads, 16, torch.bfloat16, device)
+    args = c.args()
+    small_k, small_v = args[1], args[2]
+    blocks = small_k.size(0)
+    far = (1 << 32) // (8 * 128 * 16) + 100 + blocks
+    args[1] = torch.empty((far,) + small_k.shape[1:], dtype=c.dtype, device=device)
+    args[2] = torch.empty((far,) + small_v.shape[1:], dtype=c.dtype, device=device)
+    args[1][far - blocks:] = small_k
+    args[2][far - blocks:] = small_v
+    args[3] = torch.where(args[3] < blocks, args[3] + (far - blocks), args[3])
+    c.check(K.paged_attention_tree(*args))
+
+
 @gpu
 @pytest.mark.parametrize("nodes", [[1], [24], [64], [65, 1, 0, 200], [1024], [3] * 100])
 def test_tree_rows(device, nodes):
