@@ -32,7 +32,7 @@ constexpr int kBlock = 128;  // columns (and rows of W) that share a scale; byte
 
 struct Fp8Params {
   const void *x, *bias, *residual;
-  const uint8_t *w, *xq;  // xq [M, KB * 128]
+  const uint8_t *w, *xq;  // xq [KB, M, 128]: a tile's rows end to end (us, 4096 x 28672 x 4096: 499 row by row, 488 so)
   const float *ws;
   float *xs;  // [KB, Mp]
   void *out;
@@ -81,7 +81,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const Fp8Params p) {
   if (k < p.K) raw = *reinterpret_cast<const uint4 *>(static_cast<const T *>(p.x) + (int64_t)m * p.ldx + k);
   float scale;
   const uint2 q = round_run<T>(raw, scale);
-  *reinterpret_cast<uint2 *>(const_cast<uint8_t *>(p.xq) + ((int64_t)m * p.KB + b) * kBlock + (i % 16) * 8) = q;
+  *reinterpret_cast<uint2 *>(const_cast<uint8_t *>(p.xq) + ((int64_t)b * p.M + m) * kBlock + (i % 16) * 8) = q;
   if (i % 16 == 0) p.xs[(int64_t)b * p.Mp + m] = scale;
 }
 
@@ -196,8 +196,8 @@ __global__ __launch_bounds__(WAVES * 64) void fp8_few_kernel(const Fp8Params p) 
     wbase[i] = uniform_base(reinterpret_cast<const char *>(p.w) + (int64_t)first * p.ldw);
     woff[i] = (uint32_t)(min(n0 + i * 8 + row8, p.N - 1) - first) * (uint32_t)p.ldw;
     const int xfirst = min(i * 8, p.M - 1);
-    xbase[i] = uniform_base(reinterpret_cast<const char *>(p.xq) + (int64_t)xfirst * p.KB * kBlock);
-    xoff[i] = (uint32_t)(min(i * 8 + row8, p.M - 1) - xfirst) * (uint32_t)(p.KB * kBlock) + run;
+    xbase[i] = uniform_base(reinterpret_cast<const char *>(p.xq) + (int64_t)xfirst * kBlock);
+    xoff[i] = (uint32_t)(min(i * 8 + row8, p.M - 1) - xfirst) * kBlock + run;
   }
   const uint32_t ring_lds = lds_address(ring);
   auto ask = [&](int slot, int st) {
@@ -205,7 +205,7 @@ __global__ __launch_bounds__(WAVES * 64) void fp8_few_kernel(const Fp8Params p) 
     const uint32_t to = ring_lds + slot * kStage;
     if constexpr (!HELD) {
 #pragma unroll
-      for (int i = 0; i < 2; i++) copy_1k(to + 2048 + i * 1024, xbase[i] + (int64_t)b * kBlock, xoff[i]);
+      for (int i = 0; i < 2; i++) copy_1k(to + 2048 + i * 1024, xbase[i] + (int64_t)b * p.M * kBlock, xoff[i]);
       copy_256(to + 4096, uniform_base(reinterpret_cast<const char *>(p.xs + (int64_t)b * p.Mp)), lane * 4);
     }
 #pragma unroll
@@ -337,8 +337,8 @@ __global__ __launch_bounds__(GN *GM *KG * 64) void fp8_tile_kernel(const Fp8Para
   for (int i = 0; i < kCopiesX; i++) {
     const int r = (wave + i * WAVES) % kAllX % (BM / 8) * 8, in_tile = r + row8;
     const int first = min(m0 + r, p.M - 1), rows_on = min(m0 + in_tile, p.M - 1) - first;
-    xbase[i] = uniform_base(reinterpret_cast<const char *>(p.xq) + (int64_t)first * p.KB * kBlock);
-    xoff[i] = (uint32_t)rows_on * (uint32_t)(p.KB * kBlock) + ((lane & 7) ^ (row8 & 7)) * 16;
+    xbase[i] = uniform_base(reinterpret_cast<const char *>(p.xq) + (int64_t)first * kBlock);
+    xoff[i] = (uint32_t)rows_on * kBlock + ((lane & 7) ^ (row8 & 7)) * 16;
   }
   const uint32_t ring_lds = lds_address(ring);
   const char *sbase = uniform_base(reinterpret_cast<const char *>(p.xs + m0));
@@ -354,7 +354,7 @@ __global__ __launch_bounds__(GN *GM *KG * 64) void fp8_tile_kernel(const Fp8Para
     const uint32_t to = ring_lds + slot * kRoundBytes;
     if (c < kCopiesX) {
       const int i = (wave + c * WAVES) % kAllX, u = i / (BM / 8);
-      copy_1k(to + u * kStageBytes + (BN + i % (BM / 8) * 8) * kBlock, xbase[c] + (int64_t)block_of(round, u) * kBlock, xoff[c]);
+      copy_1k(to + u * kStageBytes + (BN + i % (BM / 8) * 8) * kBlock, xbase[c] + (int64_t)block_of(round, u) * p.M * kBlock, xoff[c]);
     } else if (c < kCopiesX + kCopiesW) {
       c -= kCopiesX;
       const int i = (wave + c * WAVES) % kAllW, u = i / (BN / 8);
@@ -397,6 +397,7 @@ __global__ __launch_bounds__(GN *GM *KG * 64) void fp8_tile_kernel(const Fp8Para
     if (!MORE && KG > 1 && st * KG + group >= nst) return;  // (the last round)
     const char *wrows = stage + wn * WN * 16 * kBlock, *xrows = stage + BN * kBlock;
     const float *scales = reinterpret_cast<const float *>(stage + (BN + BM) * kBlock);
+    const float sw_next = ws[block_of(st + 1, group)];  // (here: the next round's barrier waits for all of them)
     i32x8_t xf[WM];
     float s[WM];
 #pragma unroll
@@ -443,7 +444,7 @@ __global__ __launch_bounds__(GN *GM *KG * 64) void fp8_tile_kernel(const Fp8Para
       }
       __builtin_amdgcn_sched_barrier(0);
     }
-    sw = ws[block_of(st + 1, group)];
+    sw = sw_next;
   };
   int st = 0;
   for (; st + S - 1 < rounds; st++) take(st, std::true_type{});
@@ -566,13 +567,15 @@ struct Fp8Plan {
   int Mp;
 };
 
-// What bounds the tiles is what a compute unit gets from L2, some 30 to 40 bytes a nanosecond with 64 to 96 KB on their way, whoever else asks:
+// What bounds the tiles up to 128 rows is what a compute unit gets into LDS, some 30 to 40 bytes a nanosecond with 64 to 96 KB on their way:
 // narrow tiles of W give every unit work, wide ones copy x less often.  us with the rows' launch, in rows of W per workgroup:
 //   up to 32 rows   4096 x 4096 16: 10.2, 32: 11.2, 128: 17.9; 6144 x 4096 14.8, 12.1, 18.4; 4096 x 14336 20.5, 24.7, 49.7; 28672 x 4096 42.9, 29.4, 24.6
 //   up to 64        4096 x 4096 16: 11.8, 32: 12.8, 64: 17.3, 128: 22.0; 6144 x 4096 18.9, 13.9, 17.8, 22.2; 28672 x 4096 50.7, 38.1, 27.6, 25.5
 //   up to 128       6144 x 4096 64: 22.3, 128: 29.8; 28672 x 4096 46.2, 36.8
-// Beyond 128 rows workgroups of 256 x 256, 2.25 us a stage (of whose 4100 cycles the matrix pipe is busy 2048; LDS 18 %, no bank conflicts.  Refilling each
-// part of a stage's place as soon as it has been read, with two more barriers, took a third longer), or of 128 x 128, two to a compute unit, 1.2 a stage and 1.37 where there are two; ranges of k
+// Beyond 128 rows workgroups of 256 x 256, 2.1 us a stage, of whose some 4100 cycles the matrix pipe is busy 2048 (us, 4096 x 28672 x 4096: 485; with no
+// copies but the first stages' 402, which is what products, additions and reads of LDS take of each other; LDS 18 %, no bank conflicts; reading a stage's
+// first rows among the last products of the one before, 482; refilling parts of a stage's place as soon as they have been read, with two more barriers,
+// a third longer), or of 128 x 128, two to a compute unit, 1.2 a stage and 1.37 where there are two; ranges of k
 // of workgroups of their own cost a launch and their sums' way through memory (4096 x 14336, 301 rows: one range 134, two 81, four 52).
 // apart: out does not lie over x.
 Fp8Plan plan_fp8(int64_t M, int N, int K, bool apart) {
