@@ -139,6 +139,7 @@ char *hipattn_mha_varlen_fwd_paged_window_workspace_size(int64_t total_q, int nu
  * positions are hipattn_tree_rows').  Every row sees the keys in front of the tree, and of the tree's keys those that its mask names:
  * tree_mask int64 [total_q, words], words * 64 >= max_seqlen_q, rows may lie apart: bit j % 64 of word j / 64 for the key of the sequence's j-th
  * row; bits from n on are not looked at.  Any mask will do, a tree's or not; a causal one gives hipattn_mha_varlen_fwd_paged's result.
+ * max_seqlen_q (or total_q, if that is less) times the heads of a kv group below 2^22.
  * A row that sees nothing is zero.  What a row does not see of its tree has no say in its result, NaN and infinities among them.
  * q/out [total_q, Hq, d] f16 or bf16, d 64, 80, 96, 112, 128 or 256; caches, block_tables and the other arguments as for
  * hipattn_mha_varlen_fwd_paged; rows and keys beyond max_seqlen_q and max_seqlen_k may be left out, rows of no sequence are left as they are.
