@@ -4,10 +4,10 @@
 //   out[i] = sum_t p[t] v[t] / sum_t p[t],  p[t] = 2^(log2(e) scale q[i].k[t] - m) where t < ctx - n or bit t - (ctx - n) of mask[i] is set, else 0
 //
 // The rows of a tree with the query heads of a kv group are columns of the decode kernel's products (paged_decode.h), 16 to a tile and two tiles to a
-// wavefront (one with heads of 256): 32 tokens' keys and values in registers go through both.  Up to that many columns, and where there is little work, a
-// workgroup's eight wavefronts take pairs of runs of their own, straight from the cache (tree_few_kernel); else wavefronts with different columns read
-// the same pairs from LDS, so that a context is read once for 128 columns (tree_many_kernel).  The parts of a long context go to several workgroups, whose
-// results a second launch adds up.
+// wavefront (one with heads of 256): 32 tokens' keys and values in registers go through both.  Up to that many columns, where there is little work, and
+// where values do not lie on 16-byte boundaries, a workgroup's eight wavefronts take pairs of runs of their own, straight from the cache
+// (tree_few_kernel); else wavefronts with different columns read the same pairs from LDS, so that a context is read once for 128 columns
+// (tree_many_kernel).  The parts of a long context go to several workgroups, whose results a second launch adds up.
 //
 // A tree is memory-bound in theory up to some 300 columns (its products per byte of the cache).  Only pairs that reach into the tree look at the mask.
 //
@@ -674,8 +674,10 @@ TreePlan plan_tree(const PrefillParams &p, int most_parts) {
     pl.num_parts = (int)((pairs + pl.part_pairs - 1) / pl.part_pairs);
     return pl;
   }
-  pl.cw = cols <= (p.d > 128 ? 16 : 32) ? 0 : 4;
-  pl.tiles = p.d > 128 || cols <= 16 || (cols > 32 && cols <= 64) ? 1 : 2;
+  // Values go into LDS in pieces of 16 bytes; where blocks or heads of the cache do not keep to such boundaries every wavefront reads its own, by 8.
+  const bool shares = p.vc_block % 8 == 0 && p.vc_head % 8 == 0;
+  pl.cw = !shares || cols <= (p.d > 128 ? 16 : 32) ? 0 : 4;
+  pl.tiles = p.d > 128 || cols <= 16 || (pl.cw > 0 && cols > 32 && cols <= 64) ? 1 : 2;
   const int64_t groups = groups_of(16 * pl.tiles * std::max(pl.cw, 1));
   // Parts for two workgroups to a compute unit, or one where there are few sequences, whose lengths differ less: what a workgroup takes before its first
   // keys are there is some 8 us.  us, for one / two / four / eight: 2 trees of 40 rows over up to 8000 keys, 32 / 8 x 128 38 / 49 / - / -; 12
