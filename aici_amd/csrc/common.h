@@ -125,6 +125,27 @@ inline bool apart(const hipattn_tensor *a, const hipattn_tensor *b) {
   return numel(a) == 0 || numel(b) == 0 || end(a) <= static_cast<const char *>(b->data) || end(b) <= static_cast<const char *>(a->data);
 }
 
+// Whether two tensors may have bytes in common.  What lies between the rows (of the first dimension) of one is free for the other where the rows of both
+// lie as far apart, as column ranges of one wider matrix do; else what lies between them counts as theirs.
+inline bool may_share(const hipattn_tensor *a, const hipattn_tensor *b) {
+  struct Span {
+    int64_t at, lo, hi, row, pitch;  // bytes; of the whole, and of a row (none of whose strides is negative)
+  };
+  auto span = [](const hipattn_tensor *t) {
+    const int64_t size = dtype_size(t->dtype), at = (int64_t)reinterpret_cast<uintptr_t>(t->data);
+    int64_t row = 1;
+    for (int i = 1; i < t->ndim; i++) row += (t->sizes[i] - 1) * t->strides[i];
+    const int64_t pitch = t->ndim > 0 ? t->strides[0] * size : 0, reach = t->ndim > 0 ? (t->sizes[0] - 1) * pitch : 0;
+    return Span{at, at + (reach < 0 ? reach : 0), at + (reach > 0 ? reach : 0) + row * size, row * size, pitch};
+  };
+  if (numel(a) == 0 || numel(b) == 0) return false;
+  const Span sa = span(a), sb = span(b);
+  if (sa.hi <= sb.lo || sb.hi <= sa.lo) return false;
+  if (sa.pitch <= 0 || sa.pitch != sb.pitch) return true;
+  const int64_t off = (sb.at - sa.at) % sa.pitch, within = off < 0 ? off + sa.pitch : off;  // where b's rows start in a's
+  return within < sa.row || within + sb.row > sa.pitch;
+}
+
 inline void check_contiguous(const hipattn_tensor *t, const char *name) {
   HA_CHECK(numel(t) == 0 || is_contiguous(t), "%s must be contiguous", name);
 }

@@ -18,7 +18,6 @@
 #include "device_types.h"
 #include "workspace.h"
 
-#include <algorithm>
 #include <type_traits>
 
 // The copies set M0, and say so; the compiler reports that it is a reserved register.
@@ -682,19 +681,6 @@ void launch_fp8(const Fp8Params &p, const Fp8Plan &pl, hipStream_t stream) {
   }
 }
 
-// Whether two matrices of 16-bit elements with contiguous rows have bytes in common (what lies between rows counts as theirs).
-bool meet(const hipattn_tensor *a, const hipattn_tensor *b) {
-  auto ends = [](const hipattn_tensor *t, const char *&lo, const char *&hi) {
-    const int64_t last = (t->sizes[0] - 1) * t->strides[0];
-    lo = static_cast<const char *>(t->data) + 2 * std::min<int64_t>(last, 0);
-    hi = static_cast<const char *>(t->data) + 2 * (std::max<int64_t>(last, 0) + t->sizes[1]);
-  };
-  const char *a0, *a1, *b0, *b1;
-  ends(a, a0, a1);
-  ends(b, b0, b1);
-  return a0 < b1 && b0 < a1;
-}
-
 bool at_multiple(const void *p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
 void linear_fp8_impl(hipattn_tensor *out, const hipattn_tensor *x, const hipattn_tensor *weight, const hipattn_tensor *scale,
@@ -735,13 +721,16 @@ void linear_fp8_impl(hipattn_tensor *out, const hipattn_tensor *x, const hipattn
            "%s: rows of x and weight must start on 16-byte boundaries", op);
   HA_CHECK((M == 1 || out->strides[0] % 4 == 0) && at_multiple(out->data, 8), "%s: rows of out must start on 8-byte boundaries", op);
   HA_CHECK(weight->strides[0] >= 0 && weight->strides[0] < (1 << 28), "%s: rows of weight lie too far apart", op);
-  const Fp8Plan pl = plan_fp8(M, (int)N, (int)K, !meet(out, x));
+  HA_CHECK(!may_share(out, weight), "%s: out lies over weight", op);
+  HA_CHECK(!may_share(out, scale), "%s: out lies over weight_scale", op);
+  const Fp8Plan pl = plan_fp8(M, (int)N, (int)K, !may_share(out, x));
   Fp8Params p{};
   if (bias != nullptr) {
     check_tensor(bias, "bias", 1);
     HA_CHECK(bias->dtype == dt && bias->sizes[0] == N && bias->strides[0] == 1 && at_multiple(bias->data, 8),
              "%s: bias must be %lld contiguous %s on an 8-byte boundary", op, (long long)N, dtype_name(dt));
     check_data(bias, "bias");
+    HA_CHECK(!may_share(out, bias), "%s: out lies over bias", op);
     p.bias = bias->data;
   }
   if (residual != nullptr) {
@@ -751,6 +740,8 @@ void linear_fp8_impl(hipattn_tensor *out, const hipattn_tensor *x, const hipattn
     HA_CHECK((M == 1 || residual->strides[0] % 4 == 0) && at_multiple(residual->data, 8), "%s: rows of residual must start on 8-byte boundaries",
              op);
     check_data(residual, "residual");
+    HA_CHECK((out->data == residual->data && (M == 1 || out->strides[0] == residual->strides[0])) || !may_share(out, residual),
+             "%s: out lies over part of residual", op);
     p.residual = residual->data;
     p.ldr = residual->strides[0];
   }

@@ -1,0 +1,57 @@
+"""Outputs that lie over inputs are refused where they are not named as places for them, and column ranges of one wider matrix beside each other are not
+such.  The checks come before anything asks for a device: host memory stands in for the GPU's."""
+import pytest
+import torch
+
+from aici_amd._lib import HipAttnError, call
+from aici_amd.kernels import _desc
+
+
+def desc(t):
+    return _desc(t, device=False)
+
+
+def linear(out, x, w, scale, bias=None, residual=None):
+    call("hipattn_linear_fp8", desc(out), desc(x), desc(w), desc(scale), desc(bias), desc(residual), None, None)
+
+
+def accepted(run):
+    """Whether the arguments pass (without a device the call then ends where it asks for one)."""
+    if torch.cuda.is_available():
+        pytest.skip("host memory, which only a machine without a GPU may be handed")
+    try:
+        run()
+    except HipAttnError as e:
+        return "lies over" not in str(e) and "must" not in str(e)
+    return True
+
+
+@pytest.mark.parametrize("m", [1, 2, 20, 300])
+def test_linear_fp8(m):
+    n, k = 272, 256
+    store = torch.zeros((1 << 20,), dtype=torch.bfloat16)
+    x = torch.zeros((m, k), dtype=torch.bfloat16)
+    out = store[:m * n].view(m, n)
+    raw = store.view(torch.uint8)
+    w, scale, bias = torch.zeros((n, k), dtype=torch.uint8).view(torch.float8_e4m3fn), torch.ones((3, 2)), torch.zeros((n,), dtype=torch.bfloat16)
+    with pytest.raises(HipAttnError, match="out lies over weight"):
+        linear(out, x, raw[:n * k].view(torch.float8_e4m3fn).view(n, k), scale)
+    with pytest.raises(HipAttnError, match="out lies over weight"):  # its last rows
+        last = 2 * m * n - 16
+        linear(out, x, raw[last:last + n * k].view(torch.float8_e4m3fn).view(n, k), scale)
+    with pytest.raises(HipAttnError, match="out lies over weight_scale"):
+        linear(out, x, w, raw[16:16 + 24].view(torch.float32).view(3, 2))
+    with pytest.raises(HipAttnError, match="out lies over bias"):
+        linear(out, x, w, scale, bias=out[0])
+    for first in (4, (m - 1) * n + 4):  # some of it, or another row's
+        with pytest.raises(HipAttnError, match="out lies over part of residual"):
+            linear(out, x, w, scale, residual=store[first:first + m * n].view(m, n))
+    if m > 1:
+        with pytest.raises(HipAttnError, match="out lies over part of residual"):
+            linear(out, x, w, scale, residual=out[:1].expand(m, n))
+        with pytest.raises(HipAttnError, match="out lies over part of residual"):
+            linear(out, x, w, scale, residual=store[:2 * m * n].view(m, 2 * n)[:, :n])
+    assert accepted(lambda: linear(out, x, w, scale, bias=bias, residual=out))
+    wide = store[:m * (2 * n + k)].view(m, 2 * n + k)
+    assert accepted(lambda: linear(wide[:, :n], wide[:, 2 * n:], w, scale, bias=bias, residual=wide[:, n:2 * n]))
+    assert accepted(lambda: linear(store[:m * n].view(m, n), store[:m * k].view(m, k), w, scale, bias=bias))
