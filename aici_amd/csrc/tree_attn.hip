@@ -769,6 +769,16 @@ void paged_attention_tree_impl(const hipattn_tensor *q, const hipattn_tensor *ke
   check_data(mask, "tree_mask");
   HA_CHECK((reinterpret_cast<uintptr_t>(mask->data) & 7) == 0, "%s: tree_mask must be 8-byte aligned", op);
   HA_CHECK(pp.table_cols > 0, "%s: block_tables has no columns", op);
+  // A workgroup has all that it reads of q before it writes, and nobody else reads those heads of those rows.
+  HA_CHECK((out->data == q->data && (pp.total_q == 1 || out->strides[0] == q->strides[0]) && (pp.Hq == 1 || out->strides[1] == q->strides[1])) ||
+               !may_share(out, q),
+           "%s: out lies over part of q", op);
+  const struct {
+    const hipattn_tensor *t;
+    const char *name;
+  } others[] = {{key_cache, "key_cache"}, {value_cache, "value_cache"}, {block_tables, "block_tables"}, {cu_q, "cu_seqlens_q"},
+                {context_lens, "context_lens"}, {mask, "tree_mask"}};
+  for (const auto &o : others) HA_CHECK(!may_share(out, o.t), "%s: out lies over %s", op, o.name);
   const int possible = tree_held_parts(pp.total_q, pp.Hq, pp.d);
   char *given = nullptr;
   if (workspace && possible > 1) {

@@ -143,6 +143,7 @@ char *hipattn_mha_varlen_fwd_paged_window_workspace_size(int64_t total_q, int nu
  * A row that sees nothing is zero.  What a row does not see of its tree has no say in its result, NaN and infinities among them.
  * q/out [total_q, Hq, d] f16 or bf16, d 64, 80, 96, 112, 128 or 256; caches, block_tables and the other arguments as for
  * hipattn_mha_varlen_fwd_paged; rows and keys beyond max_seqlen_q and max_seqlen_k may be left out, rows of no sequence are left as they are.
+ * out may be q itself; over any other part of q, or of another operand, it is refused.
  * Contexts are dealt out to several workgroups where few would leave compute units idle, by way of workspace: u8, 256-byte aligned,
  * hipattn_paged_attention_tree_workspace_size bytes (at most 128 MiB), not shared by calls that overlap, replays of captured ones included.
  * NULL: a buffer of 128 MiB that the library allocates once per stream; under capture, on hipStreamPerThread and without that memory contexts

@@ -48,3 +48,19 @@ def test_values_apart_lengths(device, nodes, priors, pads):
     args = c.args()
     args[2] = apart(args[2], *pads, first=8)
     c.check(K.paged_attention_tree(*args))
+
+
+@pytest.mark.parametrize("nodes,priors", [([24], [1500]), ([200, 3], [100, 9000]), ([40] * 9, [600] * 9), ([1, 24, 64, 7, 70, 0, 33], [45, 700, 0, 1, 333, 17, 64])])
+@pytest.mark.parametrize("many", [False, True])
+def test_out_over_q(device, nodes, priors, many):
+    """out is q itself, and lies beside q in rows of one wider matrix: the bits of a place of its own."""
+    heads = (32, 8, 128)
+    c = Case(59, *(crowd(heads, nodes, priors) if many else (nodes, priors)), heads, 16, torch.bfloat16, device)
+    args = c.args()
+    want = K.paged_attention_tree(*args)
+    c.check(want)
+    wide = torch.zeros((c.T, 2, 32, 128), dtype=c.dtype, device=device)
+    wide[:, 0] = args[0]
+    beside = K.paged_attention_tree(wide[:, 0], *args[1:], out=wide[:, 1])
+    assert torch.equal(beside, want) and torch.equal(wide[:, 0], args[0])
+    assert torch.equal(K.paged_attention_tree(*args, out=args[0]), want)

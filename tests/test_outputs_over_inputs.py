@@ -55,3 +55,29 @@ def test_linear_fp8(m):
     wide = store[:m * (2 * n + k)].view(m, 2 * n + k)
     assert accepted(lambda: linear(wide[:, :n], wide[:, 2 * n:], w, scale, bias=bias, residual=wide[:, n:2 * n]))
     assert accepted(lambda: linear(store[:m * n].view(m, n), store[:m * k].view(m, k), w, scale, bias=bias))
+
+
+def tree(out, q, kc, vc, tables, cu, ctx, mask):
+    call("hipattn_paged_attention_tree", desc(q), desc(kc), desc(vc), desc(tables), desc(cu), desc(ctx), 4, 40, 0.1, desc(mask), desc(out), None, None)
+
+
+def test_paged_attention_tree():
+    T, hq, hkv, d, bs, blocks = 8, 4, 2, 64, 16, 6
+    store = torch.zeros((1 << 16,), dtype=torch.float16)
+    out, elements = store[:T * hq * d].view(T, hq, d), T * hq * d
+    good = {"q": torch.zeros((T, hq, d), dtype=torch.float16), "kc": torch.zeros((blocks, hkv, d // 8, bs, 8), dtype=torch.float16),
+            "vc": torch.zeros((blocks, hkv, d, bs), dtype=torch.float16), "tables": torch.zeros((2, 3), dtype=torch.int32),
+            "cu": torch.tensor([0, 4, 8], dtype=torch.int32), "ctx": torch.tensor([40, 9], dtype=torch.int32), "mask": torch.zeros((T, 1), dtype=torch.int64)}
+    for name, operand in (("q", "q"), ("kc", "key_cache"), ("vc", "value_cache"), ("tables", "block_tables"), ("cu", "cu_seqlens_q"),
+                          ("ctx", "context_lens"), ("mask", "tree_mask")):
+        t = good[name]
+        for first in (16, 2 * elements - 16):
+            place = store.view(torch.uint8)[first:first + t.numel() * t.element_size()].view(t.dtype).view(t.shape)
+            with pytest.raises(HipAttnError, match=f"out lies over (part of )?{operand}"):
+                tree(out, **{**good, name: place})
+    with pytest.raises(HipAttnError, match="out lies over part of q"):  # its heads in another order
+        tree(out, **{**good, "q": store[:elements].view(hq, T, d).transpose(0, 1)})
+    assert accepted(lambda: tree(out, **good))
+    assert accepted(lambda: tree(out, **{**good, "q": out}))
+    wide = store[:2 * elements].view(T, 2, hq, d)
+    assert accepted(lambda: tree(wide[:, 1], **{**good, "q": wide[:, 0]}))
