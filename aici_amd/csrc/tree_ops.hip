@@ -296,7 +296,8 @@ void tree_accept_impl(const hipattn_tensor *tokens, const hipattn_tensor *parent
     HA_CHECK(key_ptrs->sizes[0] <= 65535, "%s: at most 65535 layers, got %lld", op, (long long)key_ptrs->sizes[0]);
     check_index_tensor(slots, "slot_mapping", 1);
     HA_CHECK(slots->sizes[0] == p.T, "%s: %lld slots for %d rows", op, (long long)slots->sizes[0], p.T);
-    HA_CHECK(apart(slots, lens) && apart(slots, path) && apart(slots, next), "%s: an output lies over an input", op);
+    for (const hipattn_tensor *in : {slots, key_ptrs, value_ptrs})
+      HA_CHECK(apart(in, lens) && apart(in, path) && apart(in, next), "%s: an output lies over an input", op);
     p.g = cache_geometry(key0, value0, op);
     elt = dtype_size(key0->dtype);
     HA_CHECK((reinterpret_cast<uintptr_t>(key0->data) & 15) == 0 && p.g.k_block_stride % p.g.x == 0 && p.g.k_head_stride % p.g.x == 0,

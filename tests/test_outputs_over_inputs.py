@@ -81,3 +81,19 @@ def test_paged_attention_tree():
     assert accepted(lambda: tree(out, **{**good, "q": out}))
     wide = store[:2 * elements].view(T, 2, hq, d)
     assert accepted(lambda: tree(wide[:, 1], **{**good, "q": wide[:, 0]}))
+
+
+def test_tree_accept():
+    kc, vc = torch.zeros((4, 2, 8, 16, 8), dtype=torch.float16), torch.zeros((4, 2, 64, 16), dtype=torch.float16)
+    i32 = [torch.zeros((4,), dtype=torch.int32) for _ in range(3)]
+    cu, slots, ptrs = torch.tensor([0, 4], dtype=torch.int32), torch.zeros((4,), dtype=torch.int32), torch.zeros((2,), dtype=torch.int64)
+    one, path = torch.zeros((1,), dtype=torch.int32), torch.zeros((1, 4), dtype=torch.int32)
+
+    def accept(lens=one, path=path, following=torch.zeros((1,), dtype=torch.int32)):
+        call("hipattn_tree_accept", *map(desc, i32), desc(cu), 4, desc(slots), desc(ptrs), desc(ptrs.clone()), desc(kc), desc(vc), desc(lens), desc(path),
+             desc(following), None)
+
+    for kw in ({"lens": ptrs.view(torch.int32)[1:2]}, {"path": ptrs.view(torch.int32).view(1, 4)}, {"following": ptrs.view(torch.int32)[3:]}):
+        with pytest.raises(HipAttnError, match="an output lies over an input"):
+            accept(**kw)
+    assert accepted(accept)
