@@ -156,24 +156,24 @@ class Llama:
         return (not isinstance(weight, Fp8Weight) and x.size(0) <= kernels.RMS_NORM_LINEAR_MAX_ROWS and self.skinny_linear and self.fused_norm
                 and kernels.rms_norm_linear_takes(x, norm_weight, weight))
 
-    def _proj(self, x: torch.Tensor, weight: Union[torch.Tensor, Fp8Weight]) -> torch.Tensor:
+    def _proj(self, x: torch.Tensor, weight: Union[torch.Tensor, Fp8Weight], fp8_workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
         """x @ weight.T (llama.rs:81-83, 210).  A vocabulary's rows with more than 64 sequences stay with the library where the kernel reads
         them front to back (columns no multiple of 2048, rows none of 256), and with long rows from 97 sequences on.  us, library / C ABI:
         128256 x 4096 32 rows 197 / 161, 64 rows 209 / 176, 128 rows 233 / 219; 64 / 96 / 128 rows 65536 x 5120 118 / 115, 122 / 140, 126 / 150,
         65536 x 3072 77 / 70, 81 / 85, 84 / 91, 151936 x 4096 260 / 253, 268 / 287, 278 / 296, 131072 x 8192 0.91, 0.95, 1.05 of the library's.
         49 to 64 rows: 0.65 to 1.06 of it, 0.87 on average."""
         if isinstance(weight, Fp8Weight):
-            return kernels.linear_fp8(x, weight.data, weight.scale)
+            return kernels.linear_fp8(x, weight.data, weight.scale, workspace=fp8_workspace)
         rows, (n, k) = x.size(0), weight.shape
         if self.skinny_linear and kernels.linear_takes(x, weight) and (
                 rows <= 64 or n < 65536 or (n % 256 == 0 and k % 2048 == 0 and (k <= 4096 or (k <= 8192 and rows <= 96)))):
             return kernels.linear(x, weight)
         return x @ weight.t()
 
-    def _gate_up_silu(self, h: torch.Tensor, weight: Union[torch.Tensor, Fp8Weight]) -> torch.Tensor:
+    def _gate_up_silu(self, h: torch.Tensor, weight: Union[torch.Tensor, Fp8Weight], fp8_workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
         """silu(h @ gate.T) * (h @ up.T) (llama.rs:135-142), weight = the gate rows and then the up rows."""
         if isinstance(weight, Fp8Weight):
-            gu = kernels.linear_fp8(h, weight.data, weight.scale)
+            gu = kernels.linear_fp8(h, weight.data, weight.scale, workspace=fp8_workspace)
         elif self.skinny_linear and kernels.linear_takes(h, weight) and weight.size(0) % 32 == 0:
             return kernels.linear_silu_and_mul(h, weight)
         else:
@@ -182,14 +182,15 @@ class Llama:
         kernels.silu_and_mul(act, gu)
         return act
 
-    def _proj_add_norm(self, y: torch.Tensor, weight: Union[torch.Tensor, Fp8Weight], x: torch.Tensor, norm_weight: torch.Tensor, behind=None):
+    def _proj_add_norm(self, y: torch.Tensor, weight: Union[torch.Tensor, Fp8Weight], x: torch.Tensor, norm_weight: torch.Tensor, behind=None,
+                       fp8_workspace: Optional[torch.Tensor] = None):
         """x' = y @ weight.T + x (llama.rs:96 + 166, 143 + 173) and the RMS norm of x' that follows it (:169, :165 of the
         next block, :207), or None where the projection `behind` normalises its rows itself.  Few rows: the C ABI's kernel,
         which splits the inner dimension over the device and finishes the rows -- residual and norm -- in the launch that adds
         the parts up; else a library GEMM and one launch for the addition and the norm (742 x 4096: 6.3 us, two launches 5.4
         and 6.2).  The same bits either way as far as the norm goes."""
         if isinstance(weight, Fp8Weight):
-            x = kernels.linear_fp8(y, weight.data, weight.scale, residual=x)
+            x = kernels.linear_fp8(y, weight.data, weight.scale, residual=x, workspace=fp8_workspace)
             if behind is not None and self._norm_in_proj(x, norm_weight, behind):
                 return x, None
             return x, self._rms(x, norm_weight)
@@ -216,15 +217,28 @@ class Llama:
         return window_workspace_size(batch_info, cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim, cfg.dtype,
                                      cfg.sliding_window - 1, cfg.attention_sinks)
 
+    def fp8_workspace_size(self, batch_info: BatchInfo) -> int:
+        """Bytes of a workspace for what `forward` of batches of these shapes projects with weights of 8 bits; 0 without such weights."""
+        rows = batch_info.tokens.numel()
+        weights = {(rows, *w.data.shape): w for layer in self.layers for w in layer.values() if isinstance(w, Fp8Weight)}
+        if isinstance(self.lm_head, Fp8Weight):
+            weights[(batch_info.logit_idxs.numel(), *self.lm_head.data.shape)] = self.lm_head
+        some = self.ln_f[:1]  # (of the projections' type; their rows' number is all that counts)
+        return max((kernels.linear_fp8_workspace_size(some.expand(m, k), w.data) for (m, _, k), w in weights.items()), default=0)
+
     def forward(self, batch_info: BatchInfo, caches: List[Tuple[torch.Tensor, torch.Tensor]],
-                paged_prefill: bool = False, fused: bool = False, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+                paged_prefill: bool = False, fused: bool = False, workspace: Optional[torch.Tensor] = None,
+                fp8_workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
         """batch_info on the device; caches[layer] = (key_cache, value_cache), updated in place.
         paged_prefill: multi-token rows read their context through block tables (no gather copy).
         fused: q, k, v stay views of the fused projection's output (the kernels honour the row stride) and
         rotary + cache scatter are one launch, or part of the projection's -- four or five launches fewer per layer, the same
         bits.
         workspace: uint8, `workspace_size` bytes, of a model with a window or a batch of trees: a captured step's attention is then the eager one and lies in no memory of the
-        library's."""
+        library's.  fp8_workspace: uint8, `fp8_workspace_size` bytes, on a 256-byte boundary, the same for the projections with weights of 8 bits, which
+        need no eager call on the capture's stream then.  Without it, and for what has no workspace here (projections with weights of 16 bits, decode
+        rows without a window), steps captured on one stream share that stream's scratch memory: their replays, and eager calls on that
+        stream, must not overlap."""
         cfg = self.cfg
         Hq, Hkv, d = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
         window = {} if cfg.sliding_window is None else {"window_size_left": cfg.sliding_window - 1, "sink_tokens": cfg.attention_sinks}
@@ -245,7 +259,7 @@ class Llama:
             elif h is None:
                 qkv = kernels.rms_norm_linear(x, layer["rms_1"], cfg.rms_norm_eps, layer["qkv"])
             else:
-                qkv = self._proj(h, layer["qkv"])                               # :81-83
+                qkv = self._proj(h, layer["qkv"], fp8_workspace)                # :81-83
             if fused:
                 q, k, v = qkv.split([Hq * d, Hkv * d, Hkv * d], dim=1)
                 v = v.view(T, Hkv, d)
@@ -257,17 +271,17 @@ class Llama:
                 q, k, v = (t.contiguous() for t in qkv.split([Hq * d, Hkv * d, Hkv * d], dim=1))
                 q, k = self.rotary.forward(batch_info.positions, q, k)          # :85 (in place on the copies)
                 y = varlen_attn(q, k, v.reshape(T, Hkv, d), batch_info, kc, vc, paged_prefill=paged_prefill, **window)  # :93
-            x, h = self._proj_add_norm(y, layer["o"], x, layer["rms_2"], layer["gate_up"])  # :96, :166, :169
+            x, h = self._proj_add_norm(y, layer["o"], x, layer["rms_2"], layer["gate_up"], fp8_workspace)  # :96, :166, :169
             if h is None:
                 act = kernels.rms_norm_linear(x, layer["rms_2"], cfg.rms_norm_eps, layer["gate_up"], silu_and_mul=True)
             else:
-                act = self._gate_up_silu(h, layer["gate_up"])                   # :135-142
+                act = self._gate_up_silu(h, layer["gate_up"], fp8_workspace)    # :135-142
             # the norm behind the block is the next block's first one, or the model's last (:165, :207)
             behind = self.layers[li + 1] if li + 1 < len(self.layers) else {"rms_1": self.ln_f, "qkv": None}
-            x, h = self._proj_add_norm(act, layer["down"], x, behind["rms_1"], behind["qkv"])  # :143, :173
+            x, h = self._proj_add_norm(act, layer["down"], x, behind["rms_1"], behind["qkv"], fp8_workspace)  # :143, :173
         x0 = h
         sel = _rows(x0, batch_info.logit_idxs)                                  # :209 extract_positions
-        return self._proj(sel, self.lm_head)                                    # :210
+        return self._proj(sel, self.lm_head, fp8_workspace)                     # :210
 
 
 @dataclass
