@@ -265,6 +265,8 @@ class BatchInfo:
 
         if self.multi_block_tables is None or self.q_multi == 0:
             raise ValueError("trees are multi-token entries whose slots follow their blocks in order: the batch has none")
+        if parents.shape != (self.q_multi,):
+            raise ValueError(f"{parents.numel()} parents for {self.q_multi} rows of multi-token entries")
         rows = kernels.tree_rows(parents, self.seqlens_q, self.multi_context_lens, self.max_seqlen_q)
         positions = self.positions.clone()
         positions[:self.q_multi] = rows.positions
