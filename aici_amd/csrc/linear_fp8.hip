@@ -3,6 +3,7 @@
 //
 //   e[m, b] = the least integer with max |x[m, block b]| <= 448 2^e (at least -126);  q[m, k] = x[m, k] 2^-e rounded to e4m3, ties to even
 //   y[m, n] = T( sum over blocks b of 2^e[m, b] ws[n / 128, b] (sum over k in b of q[m, k] w[n, k])  + bias[n] ) (+ residual[m, n], rounded again)
+//   (the product of the two scales comes first, in fp32: it has to be a finite number, and a normal one for the sums to keep all their bits)
 //
 // The scales of x are powers of two, so that scaling is exact and what is rounded is x itself; the largest of a block lands in (224, 448], and e4m3
 // has the same relative steps there as below.  Sums of a block are the matrix pipe's, the sum over blocks is one fp32 FMA per block.
@@ -571,7 +572,7 @@ struct Fp8Plan {
 //   up to 32 rows   4096 x 4096 16: 10.2, 32: 11.2, 128: 17.9; 6144 x 4096 14.8, 12.1, 18.4; 4096 x 14336 20.5, 24.7, 49.7; 28672 x 4096 42.9, 29.4, 24.6
 //   up to 64        4096 x 4096 16: 11.8, 32: 12.8, 64: 17.3, 128: 22.0; 6144 x 4096 18.9, 13.9, 17.8, 22.2; 28672 x 4096 50.7, 38.1, 27.6, 25.5
 //   up to 128       6144 x 4096 64: 22.3, 128: 29.8; 28672 x 4096 46.2, 36.8
-// Beyond 128 rows workgroups of 256 x 256, 2.1 us a stage, of whose some 4100 cycles the matrix pipe is busy 2048 (us, 4096 x 28672 x 4096: 485; with no
+// Beyond 128 rows workgroups of 256 x 256, 2.1 us a stage (the choice below counts 2.25, from before the rounded rows lay block by block), of whose some 4100 cycles the matrix pipe is busy 2048 (us, 4096 x 28672 x 4096: 485; with no
 // copies but the first stages' 402, which is what products, additions and reads of LDS take of each other; LDS 18 %, no bank conflicts; reading a stage's
 // first rows among the last products of the one before, 482; refilling parts of a stage's place as soon as they have been read, with two more barriers,
 // a third longer), or of 128 x 128, two to a compute unit, 1.2 a stage and 1.37 where there are two; ranges of k

@@ -52,6 +52,8 @@ __device__ __forceinline__ int tree_pairs(const TreeParams &p, int ctx) {
 
 // Bits j .. j + 63 of a row's mask; bits in front of the tree are set, those behind its n rows are not.  Two words are read whatever they are needed
 // for: a condition in front of each makes every one of them a wait (us, 1 tree of 24 rows over 1500 keys, 32 / 8 x 128: 21.5 -> 19.2 with the merge below).
+// Compiled, the two of a call still stand behind one condition, that there are rows left, and are waited for there, with all loads in front of them: once for
+// each tile in a pair that reaches into the tree, twice where a lane's tokens are of both runs.
 __device__ __forceinline__ unsigned long long tree_bits(const unsigned long long *row, int words, int n, int j) {
   const int w = j >> 6, s = j & 63, last = words - 1;
   unsigned long long lo = row[min(max(w, 0), last)], hi = row[min(max(w + 1, 0), last)];
@@ -674,7 +676,12 @@ TreePlan plan_tree(const PrefillParams &p, int most_parts) {
     pl.num_parts = (int)((pairs + pl.part_pairs - 1) / pl.part_pairs);
     return pl;
   }
-  // Values go into LDS in pieces of 16 bytes; where blocks or heads of the cache do not keep to such boundaries every wavefront reads its own, by 8.
+  // Values go into LDS in pieces of 16 bytes; where blocks or heads of the cache do not keep to such boundaries every wavefront reads its own, by 8 (us, 64
+  // trees over 1000 to 15000 keys, 32 / 8 x 128, blocks apart by a multiple of 16 bytes / of 8: 8 rows 365 / 365, 24 rows, 96 columns, 380 / 571, as 32 columns
+  // at a time read the keys).
+  // Up to 32 columns as well, which the other form would do in less time over long contexts: us, own pairs / shared ones, 64 trees of 5, 6, 8 rows over 1000
+  // to 15000 keys, 32 / 8 x 128 364 / 325, 365 / 326, 365 / 328; 16 of 8 124 / 113; 64 of 30 over 1000 to 8000, 32 / 32 x 80 543 / 525; 8 of 5 over 500
+  // to 8000 43.6 / 43.6.
   const bool shares = p.vc_block % 8 == 0 && p.vc_head % 8 == 0;
   pl.cw = !shares || cols <= (p.d > 128 ? 16 : 32) ? 0 : 4;
   pl.tiles = p.d > 128 || cols <= 16 || (pl.cw > 0 && cols > 32 && cols <= 64) ? 1 : 2;

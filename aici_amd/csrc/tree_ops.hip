@@ -95,10 +95,11 @@ struct TreeAcceptParams {
 };
 
 // One workgroup per (sequence, layer): each finds the way for itself, the first of a sequence's says it.  A token's values lie in a cache line of
-// their own with those of its neighbours for every element of d, and its keys 256 bytes apart, so that what is touched of a few tokens is every line of
-// their blocks, some 64 KB for each block that a way leaves or enters: 64 trees of 16 to 61 rows, 8 heads of 128, 32 layers move 33 MB and touch
-// some 500, in 106 us (among other work 157; one token after the other, not eight at a time, 175).  Half rows of V read at a time and neighbours written
-// together changed nothing: it is the lines.
+// their own with those of its neighbours for every element of d, and its keys 256 bytes apart, so that what is touched of a few tokens is every line of V in
+// their blocks and half of K's: 64 trees of 16 to 61 rows, 8 heads of 128, 32 layers move 33 MB and touch 271 to 279 (lines of 128 bytes, counted from
+// their slots; 211 to 219 in sectors of 32), 57 to 59 us at a large copy's rate.  The kernel takes 106 to 114 by itself, the call 144 to 157 among other work (one
+// token after the other, not eight at a time, 175): it is not the lines but the waits.  The caches' addresses come out of memory, so loads and stores
+// are flat ones, each load stands behind a condition, and compiled each is waited for by itself; K's eight go by way of scratch memory.
 constexpr int kBatch = 8;
 template <typename E>
 __global__ __launch_bounds__(256) void tree_accept_kernel(TreeAcceptParams p) {
@@ -171,7 +172,7 @@ __global__ __launch_bounds__(256) void tree_accept_kernel(TreeAcceptParams p) {
     }
     __syncthreads();
     const int moves = s_moves;
-    // All that a batch reads is asked for before anything is written: a row of the way comes from one that no earlier row of it goes to.
+    // All that a batch reads is read before anything is written: a row of the way comes from one that no earlier row of it goes to.
     for (int i = tid; i < items; i += 256) {
       if (i < key_items) {
         const int head = i / runs;

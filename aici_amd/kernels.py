@@ -126,7 +126,7 @@ def paged_attention_tree(q: torch.Tensor, key_cache: torch.Tensor, value_cache: 
     """Attention of trees of drafted tokens over the paged cache.  q [Tq,Hq,d], block_tables, seqlens_q and context_lens as for
     `flash_attn_varlen_paged` (the rows' own keys are the last of the context); a row sees every key in front of its tree and, of the tree's
     keys, those that tree_mask int64 [Tq, words] names: bit j % 64 of word j / 64 for the sequence's j-th row (`tree_rows`).  A row that sees
-    nothing is zero.  workspace: uint8, `paged_attention_tree_workspace_size` bytes, for calls that are captured and for those that must not
+    nothing is zero.  out may be q.  workspace: uint8, `paged_attention_tree_workspace_size` bytes, for calls that are captured and for those that must not
     allocate; None: a buffer that the library keeps per stream, and under capture none, which takes longer for few long contexts."""
     if out is None:
         out = torch.empty_like(q)
