@@ -125,25 +125,35 @@ inline bool apart(const hipattn_tensor *a, const hipattn_tensor *b) {
   return numel(a) == 0 || numel(b) == 0 || end(a) <= static_cast<const char *>(b->data) || end(b) <= static_cast<const char *>(a->data);
 }
 
-// Whether two tensors may have bytes in common.  What lies between the rows (of the first dimension) of one is free for the other where the rows of both
-// lie as far apart, as column ranges of one wider matrix do; else what lies between them counts as theirs.
+// Whether two tensors may have bytes in common.  What lies between the rows (or heads) of one is free for the other where both have theirs as far apart,
+// as column ranges of one wider matrix do; else what lies between them counts as theirs.
 inline bool may_share(const hipattn_tensor *a, const hipattn_tensor *b) {
   struct Span {
-    int64_t at, lo, hi, row, pitch;  // bytes; of the whole, and of a row (none of whose strides is negative)
+    int64_t lo, hi;  // bytes from the first element on, hi past the end
   };
-  auto span = [](const hipattn_tensor *t) {
-    const int64_t size = dtype_size(t->dtype), at = (int64_t)reinterpret_cast<uintptr_t>(t->data);
-    int64_t row = 1;
-    for (int i = 1; i < t->ndim; i++) row += (t->sizes[i] - 1) * t->strides[i];
-    const int64_t pitch = t->ndim > 0 ? t->strides[0] * size : 0, reach = t->ndim > 0 ? (t->sizes[0] - 1) * pitch : 0;
-    return Span{at, at + (reach < 0 ? reach : 0), at + (reach > 0 ? reach : 0) + row * size, row * size, pitch};
+  auto span = [](const hipattn_tensor *t, int dim) {  // of the dimensions from `dim` on
+    Span s{0, 1};
+    for (int i = dim; i < t->ndim; i++) (t->strides[i] < 0 ? s.lo : s.hi) += (t->sizes[i] - 1) * t->strides[i];
+    const int64_t size = dtype_size(t->dtype);
+    return Span{s.lo * size, s.hi * size};
   };
+  auto pitch = [](const hipattn_tensor *t, int dim) { return t->strides[dim] * dtype_size(t->dtype); };
   if (numel(a) == 0 || numel(b) == 0) return false;
-  const Span sa = span(a), sb = span(b);
-  if (sa.hi <= sb.lo || sb.hi <= sa.lo) return false;
-  if (sa.pitch <= 0 || sa.pitch != sb.pitch) return true;
-  const int64_t off = (sb.at - sa.at) % sa.pitch, within = off < 0 ? off + sa.pitch : off;  // where b's rows start in a's
-  return within < sa.row || within + sb.row > sa.pitch;
+  const Span whole_a = span(a, 0), whole_b = span(b, 0);
+  const int64_t off = (int64_t)reinterpret_cast<uintptr_t>(b->data) - (int64_t)reinterpret_cast<uintptr_t>(a->data);
+  if (whole_a.hi <= off + whole_b.lo || off + whole_b.hi <= whole_a.lo) return false;
+  for (int i = 0; i < a->ndim && i < b->ndim; i++) {
+    // modulo a step that both have, and that divides the steps outside it, either is what lies inside
+    const int64_t step = pitch(a, i);
+    bool divides = step > 0 && step == pitch(b, i);
+    for (const hipattn_tensor *t : {a, b})
+      for (int o = 0; o < i && divides; o++) divides = t->sizes[o] == 1 || pitch(t, o) % step == 0;
+    const Span in_a = span(a, i + 1), in_b = span(b, i + 1);
+    if (!divides || in_a.lo < 0 || in_b.lo < 0) continue;
+    const int64_t within = (off % step + step) % step;  // where b's begins in a's
+    if (within >= in_a.hi && within + in_b.hi <= step) return false;
+  }
+  return true;
 }
 
 inline void check_contiguous(const hipattn_tensor *t, const char *name) {

@@ -81,6 +81,11 @@ def test_paged_attention_tree():
     assert accepted(lambda: tree(out, **{**good, "q": out}))
     wide = store[:2 * elements].view(T, 2, hq, d)
     assert accepted(lambda: tree(wide[:, 1], **{**good, "q": wide[:, 0]}))
+    heads = store[:3 * elements].view(T, hq, 3, d)  # every head's q beside its k and v
+    assert accepted(lambda: tree(heads[:, :, 2], **{**good, "q": heads[:, :, 0]}))
+    assert accepted(lambda: tree(heads[:, :, 0], **{**good, "q": heads[:, :, 2]}))
+    with pytest.raises(HipAttnError, match="out lies over part of q"):
+        tree(store[32:32 + 3 * elements].view(T, hq, 3, d)[:, :, 0], **{**good, "q": heads[:, :, 0]})
 
 
 def test_tree_accept():
