@@ -585,6 +585,9 @@ class CacheList:
                     raise HipAttnError(f"CacheList: expected GPU tensors of one device, got one on {t.device}")
                 if t.dtype != self.key_caches[0].dtype or t.size() != first.size() or t.stride() != first.stride() or t.data_ptr() % 16 != 0:
                     raise HipAttnError("CacheList: the layers' caches must have one type, one shape and the same strides, and start on 16-byte boundaries")
+        # (layers that share a cache have it once in the list: two moves of the same rows at a time would take from each other what they have moved)
+        if self.key_caches[0].numel() > 0 and len({t.data_ptr() for t in self.key_caches + self.value_caches}) < 2 * len(self.key_caches):
+            raise HipAttnError("CacheList: the same cache twice")
         device = self.key_caches[0].device
         self.key_ptrs = torch.tensor([t.data_ptr() for t in self.key_caches], dtype=torch.int64).to(device)
         self.value_ptrs = torch.tensor([t.data_ptr() for t in self.value_caches], dtype=torch.int64).to(device)

@@ -169,8 +169,8 @@ char *hipattn_tree_rows(const hipattn_tensor *parents, const hipattn_tensor *seq
  * path int32 [R, max_seqlen_q]: the rows, counted in the tree, -1 behind the last; next int32 [R]: what was chosen at the last of them, -1 without
  * rows.  max_seqlen_q at most 1024; rows beyond it are left out.
  * With slot_mapping [T] (int32 or int64, -1: none), key_cache_ptrs and value_cache_ptrs (int64 [layers] on the device: the caches of every
- * layer, each like key0 and value0 in type, sizes and strides) the keys and values of the way's k-th row are moved to the slot of the tree's
- * k-th row, so that the sequence's first context_lens - n + lens keys are those of its tokens.  Rows may not share slots.  All five NULL: nothing
+ * layer, each like key0 and value0 in type, sizes and strides, and none of them twice) the keys and values of the way's k-th row are moved to the
+ * slot of the tree's k-th row, so that the sequence's first context_lens - n + lens keys are those of its tokens.  Rows may not share slots.  All five NULL: nothing
  * is moved.  At most 65535 sequences and layers. */
 char *hipattn_tree_accept(const hipattn_tensor *tokens, const hipattn_tensor *parents, const hipattn_tensor *chosen,
                           const hipattn_tensor *seqlens_q, int max_seqlen_q, const hipattn_tensor *slot_mapping,
